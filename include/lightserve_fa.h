@@ -447,6 +447,103 @@ typedef struct {
   int32_t reserved;
 } lsfa_greedy_args;
 
+/* 8-bit paged KV cache: append (quantise on write) and read back. No
+ * counterpart in the reference, whose caches hold the model's own type
+ * (engine/config.py:5-7).
+ *   k, v         rows [tokens, heads_kv, head_dim] of the given dtype (read by
+ *                the append, written by the read), head-dim stride 1
+ *   k_cache,     e4m3 codes [num_blocks, block_size, heads_kv, head_dim], byte
+ *   v_cache      strides, head-dim stride 1
+ *   kv_scales    exponents [num_blocks, heads_kv, block_size, 2], contiguous:
+ *                the row in block i, slot j of head h stands for code *
+ *                2^(e - 127) with e = kv_scales[i][h][j][0] for K, [1] for V.
+ *                The append writes the least e in 1..254 with max |x| <=
+ *                448 * 2^(e - 127) over the row's finite values; codes round
+ *                to nearest even, infinities and NaN become NaN, and where 256
+ *                * 2^(e - 127) does not fit dtype magnitudes stop at 240 of it.
+ *   block_tables int32 [batch, max_blocks_per_seq]
+ *   cu_seqlens   int32 [batch + 1]: sequence b's rows are cu_seqlens[b] ..
+ *                cu_seqlens[b + 1] - 1; NULL (append only): one row each
+ *   seq_lens     int32 [batch] (append only): cached tokens with the appended
+ *                ones; row i of a sequence's n goes to position seq_lens[b] - n
+ *                + i. The read takes positions 0, 1, ...
+ * Rows of no sequence, before position 0 or in no block (table entries outside
+ * [0, num_blocks)) are not stored; the read writes zeros for them. Two rows of
+ * one append must not go to the same slot. */
+typedef struct {
+  void* k;
+  void* v;
+  void* k_cache;
+  void* v_cache;
+  uint8_t* kv_scales;
+  const int32_t* block_tables;
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens;
+  int64_t k_stride[2];         /* token, head */
+  int64_t v_stride[2];
+  int64_t k_cache_stride[3];   /* block, slot, head */
+  int64_t v_cache_stride[3];
+  int64_t block_table_stride;
+  int32_t dtype;               /* of k and v */
+  int32_t batch;
+  int32_t tokens;
+  int32_t heads_kv;
+  int32_t head_dim;            /* multiple of 16, at most 128 */
+  int32_t block_size;          /* power of two, at least 16 */
+  int32_t num_blocks;
+  int32_t max_blocks_per_seq;
+} lsfa_kv_cache_args;
+
+/* Attention over a paged KV cache of 8 or 16 bits, with a sliding window and
+ * sinks or without. No counterpart in the reference (see lsfa_decode_args).
+ *   q, o         [tokens, heads_q, head_dim], head-dim stride 1
+ *   k_cache,     of q's dtype with kv_scales NULL, else 8-bit as in
+ *   v_cache      lsfa_kv_cache_args; [num_blocks, block_size, heads_kv, head_dim]
+ *   cu_seqlens_q int32 [batch + 1], or NULL: one query per sequence
+ *   seq_lens     int32 [batch]: cached tokens with the queries' own; clamped to
+ *                max_seq_len and max_blocks_per_seq * block_size
+ *   lse          fp32, token and head strides, or NULL
+ * Query i of a sequence's n sits at position p = seq_lens[b] - n + i and sees
+ * keys j <= p (all keys with causal = 0), with window > 0 only j > p - window
+ * or j < sinks. Block ids outside [0, num_blocks) read as zeros. Rows of q
+ * behind the last sequence are not computed. workspace:
+ * lsfa_window_workspace_size() bytes, 256-byte aligned. */
+typedef struct {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  void* o;
+  float* lse;
+  const uint8_t* kv_scales;
+  const int32_t* cu_seqlens_q;
+  const int32_t* seq_lens;
+  const int32_t* block_tables;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t q_stride[2];         /* token, head */
+  int64_t k_stride[3];         /* block, slot, head */
+  int64_t v_stride[3];
+  int64_t o_stride[2];
+  int64_t lse_stride[2];       /* token, head */
+  int64_t block_table_stride;
+  int32_t dtype;               /* of q and o: bf16 or fp16 */
+  int32_t batch;
+  int32_t tokens;              /* rows of q */
+  int32_t heads_q;
+  int32_t heads_kv;
+  int32_t head_dim;            /* multiple of 8 (8-bit caches: of 16), at most 128 */
+  int32_t block_size;          /* power of two, at least 16 */
+  int32_t num_blocks;
+  int32_t max_blocks_per_seq;
+  int32_t max_seqlen_q;        /* bound of a sequence's queries */
+  int32_t max_seq_len;         /* bound of seq_lens */
+  int32_t causal;
+  int32_t window;              /* 0: none; needs causal */
+  int32_t sinks;
+  float sm_scale;
+  int32_t reserved;
+} lsfa_window_args;
+
 /* ABI version of the loaded library (LSFA_ABI_VERSION). */
 int lsfa_abi_version(void);
 
@@ -515,6 +612,25 @@ int lsfa_decode_workspace_size(const lsfa_decode_args* args, uint64_t* bytes);
  * seq_lens[b] cached tokens (and lse if requested). No reference
  * counterpart (see lsfa_decode_args). */
 int lsfa_decode(const lsfa_decode_args* args, void* stream);
+
+/* Host-only validation of 8-bit cache arguments; never touches the GPU. */
+int lsfa_kv_append_check(const lsfa_kv_cache_args* args);
+int lsfa_kv_read_check(const lsfa_kv_cache_args* args);
+
+/* Quantises new K/V rows into an 8-bit paged cache, and reads cached rows back
+ * (see lsfa_kv_cache_args); one launch each. */
+int lsfa_kv_append(const lsfa_kv_cache_args* args, void* stream);
+int lsfa_kv_read(const lsfa_kv_cache_args* args, void* stream);
+
+/* Host-only validation of windowed paged attention; never touches the GPU. */
+int lsfa_window_check(const lsfa_window_args* args);
+
+/* Workspace bytes lsfa_window needs (partial results); no GPU work. */
+int lsfa_window_workspace_size(const lsfa_window_args* args, uint64_t* bytes);
+
+/* Attention over a paged cache of 8 or 16 bits with an optional window and
+ * sinks (see lsfa_window_args). Deterministic. */
+int lsfa_window(const lsfa_window_args* args, void* stream);
 
 /* Host-only validation of RoPE arguments; never touches the GPU. */
 int lsfa_rope_check(const lsfa_rope_args* args);

@@ -34,7 +34,9 @@ EXPORTED_SYMBOLS = ("lsfa_abi_version", "lsfa_last_error", "lsfa_fwd_check", "ls
                     "lsfa_capture_id", "lsfa_gemv_check", "lsfa_gemv_workspace_size", "lsfa_gemv",
                     "lsfa_gemv_group_check", "lsfa_gemv_group_workspace_size", "lsfa_gemv_group",
                     "lsfa_gemm_group_check", "lsfa_gemm_group_workspace_size", "lsfa_gemm_group",
-                    "lsfa_greedy_check", "lsfa_greedy")
+                    "lsfa_greedy_check", "lsfa_greedy",
+                    "lsfa_kv_append_check", "lsfa_kv_append", "lsfa_kv_read_check", "lsfa_kv_read",
+                    "lsfa_window_check", "lsfa_window_workspace_size", "lsfa_window")
 
 _i64x4 = ctypes.c_int64 * 4
 _i64x3 = ctypes.c_int64 * 3
@@ -177,6 +179,37 @@ class RmsNormArgs(ctypes.Structure):
     ]
 
 
+class KvCacheArgs(ctypes.Structure):
+    """Mirror of lsfa_kv_cache_args."""
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_cache", ctypes.c_void_p), ("v_cache", ctypes.c_void_p),
+        ("kv_scales", ctypes.c_void_p), ("block_tables", ctypes.c_void_p), ("seq_lens", ctypes.c_void_p),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("k_stride", _i64x2), ("v_stride", _i64x2), ("k_cache_stride", _i64x3), ("v_cache_stride", _i64x3),
+        ("block_table_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("batch", ctypes.c_int32), ("tokens", ctypes.c_int32), ("heads_kv", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("block_size", ctypes.c_int32), ("num_blocks", ctypes.c_int32),
+        ("max_blocks_per_seq", ctypes.c_int32),
+    ]
+
+
+class WindowArgs(ctypes.Structure):
+    """Mirror of lsfa_window_args."""
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k_cache", ctypes.c_void_p), ("v_cache", ctypes.c_void_p), ("o", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p), ("kv_scales", ctypes.c_void_p), ("cu_seqlens_q", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p), ("block_tables", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
+        ("q_stride", _i64x2), ("k_stride", _i64x3), ("v_stride", _i64x3), ("o_stride", _i64x2), ("lse_stride", _i64x2),
+        ("block_table_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("batch", ctypes.c_int32), ("tokens", ctypes.c_int32), ("heads_q", ctypes.c_int32),
+        ("heads_kv", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("block_size", ctypes.c_int32),
+        ("num_blocks", ctypes.c_int32), ("max_blocks_per_seq", ctypes.c_int32), ("max_seqlen_q", ctypes.c_int32),
+        ("max_seq_len", ctypes.c_int32), ("causal", ctypes.c_int32), ("window", ctypes.c_int32),
+        ("sinks", ctypes.c_int32), ("sm_scale", ctypes.c_float), ("reserved", ctypes.c_int32),
+    ]
+
+
 # Packed forms of the argument structs: filling one from Python costs a call
 # per field and per stride array (7.8 us for lsfa_fwd_args), packing the same
 # fields in one call and copying the bytes 2.7 us. "=" is the structs' own
@@ -185,7 +218,8 @@ class RmsNormArgs(ctypes.Structure):
 _PACK = {cls: struct.Struct(fmt) for cls, fmt in (
     (FwdArgs, "=5Q19q2Q8ifi"), (BwdArgs, "=10QQ35q2Q8ifi"), (DecodeArgs, "=8QQ17q9if"),
     (PrefillPagedArgs, "=8Q13q10ifi"), (GemvGroupArgs, "=3QqQq4Q4Q4q4q4i4i3Q2qfi"),
-    (RmsNormArgs, "=5Q4q3if"), (RopeArgs, "=6Q9q8i4Q7qQq2i"))}
+    (RmsNormArgs, "=5Q4q3if"), (RopeArgs, "=6Q9q8i4Q7qQq2i"),
+    (KvCacheArgs, "=8Q11q8i"), (WindowArgs, "=11Q13q14ifi"))}
 
 
 def pack(cls, *fields):
@@ -239,7 +273,8 @@ def load():
                              ("lsfa_rmsnorm_check", RmsNormArgs), ("lsfa_prefill_paged_check", PrefillPagedArgs),
                              ("lsfa_gemv_check", GemvArgs), ("lsfa_gemv_group_check", GemvGroupArgs),
                              ("lsfa_gemm_group_check", GemvGroupArgs),
-                             ("lsfa_greedy_check", GreedyArgs)):
+                             ("lsfa_greedy_check", GreedyArgs), ("lsfa_kv_append_check", KvCacheArgs),
+                             ("lsfa_kv_read_check", KvCacheArgs), ("lsfa_window_check", WindowArgs)):
             fn = getattr(lib, name)
             fn.restype = ctypes.c_int
             fn.argtypes = [ctypes.POINTER(struct)]
@@ -248,7 +283,8 @@ def load():
                              ("lsfa_rope", RopeArgs), ("lsfa_rmsnorm", RmsNormArgs),
                              ("lsfa_prefill_paged", PrefillPagedArgs), ("lsfa_gemv", GemvArgs),
                              ("lsfa_gemv_group", GemvGroupArgs), ("lsfa_gemm_group", GemvGroupArgs),
-                             ("lsfa_greedy", GreedyArgs)):
+                             ("lsfa_greedy", GreedyArgs), ("lsfa_kv_append", KvCacheArgs),
+                             ("lsfa_kv_read", KvCacheArgs), ("lsfa_window", WindowArgs)):
             fn = getattr(lib, name)
             fn.restype = ctypes.c_int
             fn.argtypes = [ctypes.POINTER(struct), ctypes.c_void_p]
@@ -268,6 +304,8 @@ def load():
         lib.lsfa_gemv_workspace_size.argtypes = [ctypes.POINTER(GemvArgs), ctypes.POINTER(ctypes.c_uint64)]
         lib.lsfa_decode_workspace_size.restype = ctypes.c_int
         lib.lsfa_decode_workspace_size.argtypes = [ctypes.POINTER(DecodeArgs), ctypes.POINTER(ctypes.c_uint64)]
+        lib.lsfa_window_workspace_size.restype = ctypes.c_int
+        lib.lsfa_window_workspace_size.argtypes = [ctypes.POINTER(WindowArgs), ctypes.POINTER(ctypes.c_uint64)]
         version = lib.lsfa_abi_version()
         if version != ABI_VERSION:
             raise RuntimeError(f"{_LIB_NAME} has ABI version {version}, expected {ABI_VERSION}")
@@ -407,6 +445,43 @@ def greedy_check(args):
 
 def greedy(args, stream):
     _raise_on(load().lsfa_greedy(ctypes.byref(args), stream), "lsfa_greedy")
+
+
+def kv_append_check(args):
+    """Host-only validation (no GPU access); returns (status, message)."""
+    rc = load().lsfa_kv_append_check(ctypes.byref(args))
+    return rc, load().lsfa_last_error().decode(errors="replace")
+
+
+def kv_append(args, stream):
+    _raise_on(load().lsfa_kv_append(ctypes.byref(args), stream), "lsfa_kv_append")
+
+
+def kv_read_check(args):
+    """Host-only validation (no GPU access); returns (status, message)."""
+    rc = load().lsfa_kv_read_check(ctypes.byref(args))
+    return rc, load().lsfa_last_error().decode(errors="replace")
+
+
+def kv_read(args, stream):
+    _raise_on(load().lsfa_kv_read(ctypes.byref(args), stream), "lsfa_kv_read")
+
+
+def window_check(args):
+    """Host-only validation (no GPU access); returns (status, message)."""
+    rc = load().lsfa_window_check(ctypes.byref(args))
+    return rc, load().lsfa_last_error().decode(errors="replace")
+
+
+def window_workspace_size(args):
+    """Bytes of device workspace lsfa_window needs (host only; 0 when no sequence is shared out)."""
+    n = ctypes.c_uint64(0)
+    _raise_on(load().lsfa_window_workspace_size(ctypes.byref(args), ctypes.byref(n)), "lsfa_window_workspace_size")
+    return n.value
+
+
+def window(args, stream):
+    _raise_on(load().lsfa_window(ctypes.byref(args), stream), "lsfa_window")
 
 
 def rope_check(args):

@@ -20,6 +20,10 @@ hipError_t bwd_mfma(const BwdParams& p, bool is_bf16, int dp, bool causal, int p
 hipError_t fwd_f32(const FwdParams& p, int dp, bool causal, bool varlen, float scale, hipStream_t s);
 hipError_t bwd_f32(const BwdParams& p, int dp, bool causal, hipStream_t s);
 hipError_t decode_gqa(const DecodeParams& p, bool is_bf16, int dp, hipStream_t s);
+hipError_t kv_cache_move(const KvCacheParams& p, int dtype, bool append, hipStream_t s);
+int window_runs(int B, int Hkv, int G, int max_n, long long max_keys);
+uint64_t window_part_bytes(int B, int Hkv, int G, int max_n, int D, int runs);
+hipError_t window_attention(const WindowParams& p, bool is_bf16, hipStream_t s);
 hipError_t rope_inplace(const RopeParams& p, int dtype, hipStream_t s);
 hipError_t add_rmsnorm(const NormParams& p, int dtype, bool vec, hipStream_t s);
 hipError_t gemv(const GemvParams& p, bool is_bf16, hipStream_t s);
@@ -669,6 +673,185 @@ int lsfa_prefill_paged_check(const lsfa_prefill_paged_args* a) {
   if (a->block_table_stride < a->max_blocks_per_seq)
     return fail(LSFA_ERR_INVALID, "block_table_stride %lld is below max_blocks_per_seq %d",
                 (long long)a->block_table_stride, a->max_blocks_per_seq);
+  return ok();
+}
+
+// What an 8-bit cache and its block tables must be for the kernels of
+// fa_kvq.hip and fa_window.hip: blocks of 16 slots or more, rows of whole 16-byte
+// pieces, 16 slots of one block within 32-bit byte offsets.
+static int check_paged(int head_dim, int dim_multiple, int block_size, int max_blocks, const int64_t* ks, const int64_t* vs,
+                       int elements_per_16, int64_t table_stride) {
+  if (head_dim < dim_multiple || head_dim > 128 || head_dim % dim_multiple != 0)
+    return fail(LSFA_ERR_UNSUPPORTED, "head_dim must be a multiple of %d in %d..128 (got %d)", dim_multiple, dim_multiple, head_dim);
+  if (block_size < 16 || log2_exact(block_size) < 0)
+    return fail(LSFA_ERR_UNSUPPORTED, "block_size must be a power of two of at least 16 (got %d)", block_size);
+  if ((long long)max_blocks * block_size > (1LL << 30))
+    return fail(LSFA_ERR_UNSUPPORTED, "max_blocks_per_seq * block_size exceeds 2^30");
+  for (int i = 0; i < 3; ++i)
+    if (ks[i] % elements_per_16 != 0 || vs[i] % elements_per_16 != 0)
+      return fail(LSFA_ERR_UNSUPPORTED, "k_cache/v_cache strides must be multiples of 16 bytes");
+  if (ks[1] < 0 || ks[1] > (1LL << 22) || vs[1] < 0 || vs[1] > (1LL << 22))
+    return fail(LSFA_ERR_UNSUPPORTED, "cache slot strides must lie in 0..2^22 elements");
+  if (table_stride < max_blocks)
+    return fail(LSFA_ERR_INVALID, "block_table_stride %lld is below max_blocks_per_seq %d", (long long)table_stride, max_blocks);
+  return LSFA_OK;
+}
+
+static int check_kv_cache(const lsfa_kv_cache_args* a, bool append) {
+  if (a == nullptr) return fail(LSFA_ERR_INVALID, "args is NULL");
+  if (a->dtype != LSFA_DTYPE_FP32 && a->dtype != LSFA_DTYPE_FP16 && a->dtype != LSFA_DTYPE_BF16)
+    return fail(LSFA_ERR_INVALID, "unknown dtype %d", a->dtype);
+  if (a->batch < 0 || a->tokens < 0 || a->heads_kv <= 0 || a->num_blocks < 0 || a->max_blocks_per_seq < 0)
+    return fail(LSFA_ERR_INVALID, "negative size or no heads (batch=%d tokens=%d heads_kv=%d num_blocks=%d "
+                "max_blocks_per_seq=%d)", a->batch, a->tokens, a->heads_kv, a->num_blocks, a->max_blocks_per_seq);
+  int rc = check_paged(a->head_dim, 16, a->block_size, a->max_blocks_per_seq, a->k_cache_stride, a->v_cache_stride, 16,
+                       a->block_table_stride);
+  if (rc) return rc;
+  if ((long long)a->tokens * a->heads_kv > INT32_MAX) return fail(LSFA_ERR_UNSUPPORTED, "more than 2^31 rows in one call");
+  if (a->tokens == 0) return ok();
+  if (!a->k || !a->v || (a->num_blocks > 0 && (!a->kv_scales || !a->k_cache || !a->v_cache)))
+    return fail(LSFA_ERR_INVALID, "k, v, k_cache, v_cache and kv_scales must be non-NULL");
+  if (a->batch > 0 && (!a->block_tables || (append ? !a->seq_lens : !a->cu_seqlens)))
+    return fail(LSFA_ERR_INVALID, append ? "block_tables and seq_lens must be non-NULL" : "block_tables and cu_seqlens must be non-NULL");
+  if (append && !a->cu_seqlens && a->tokens != a->batch)
+    return fail(LSFA_ERR_INVALID, "%d rows for %d sequences without cu_seqlens", a->tokens, a->batch);
+  if (!append && !a->cu_seqlens) return fail(LSFA_ERR_INVALID, "cu_seqlens must be non-NULL");
+  const int per16 = a->dtype == LSFA_DTYPE_FP32 ? 4 : 8;
+  for (int i = 0; i < 2; ++i)
+    if (a->k_stride[i] % per16 != 0 || a->v_stride[i] % per16 != 0)
+      return fail(LSFA_ERR_UNSUPPORTED, "k/v strides must be multiples of 16 bytes");
+  if (!aligned16(a->k) || !aligned16(a->v) || !aligned16(a->k_cache) || !aligned16(a->v_cache) ||
+      (reinterpret_cast<uintptr_t>(a->kv_scales) & 7u) != 0)
+    return fail(LSFA_ERR_UNSUPPORTED, "k, v, k_cache and v_cache must be 16-byte aligned, kv_scales 8-byte");
+  return ok();
+}
+
+int lsfa_kv_append_check(const lsfa_kv_cache_args* a) { return check_kv_cache(a, true); }
+int lsfa_kv_read_check(const lsfa_kv_cache_args* a) { return check_kv_cache(a, false); }
+
+static int run_kv_cache(const lsfa_kv_cache_args* a, bool append, void* stream) {
+  const int rc = check_kv_cache(a, append);
+  if (rc) return rc;
+  if (a->tokens == 0) return ok();
+  lsfa::KvCacheParams p;
+  memset(&p, 0, sizeof(p));
+  p.k = a->k; p.v = a->v;
+  p.kc = static_cast<uint8_t*>(a->k_cache); p.vc = static_cast<uint8_t*>(a->v_cache); p.scales = a->kv_scales;
+  p.block_tables = a->block_tables; p.seq_lens = a->seq_lens; p.cu = a->cu_seqlens;
+  for (int i = 0; i < 2; ++i) p.sk[i] = a->k_stride[i], p.sv[i] = a->v_stride[i];
+  for (int i = 0; i < 3; ++i) p.skc[i] = a->k_cache_stride[i], p.svc[i] = a->v_cache_stride[i];
+  p.sbt = a->block_table_stride;
+  p.tokens = a->tokens; p.B = a->batch; p.Hkv = a->heads_kv; p.D = a->head_dim;
+  p.block_shift = log2_exact(a->block_size);
+  p.max_blocks = a->max_blocks_per_seq;
+  p.num_blocks = a->num_blocks;
+  hipError_t e = lsfa::kv_cache_move(p, a->dtype, append, reinterpret_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(LSFA_ERR_LAUNCH, "8-bit cache launch failed: %s", hipGetErrorString(e));
+  return ok();
+}
+int lsfa_kv_append(const lsfa_kv_cache_args* a, void* stream) { return run_kv_cache(a, true, stream); }
+int lsfa_kv_read(const lsfa_kv_cache_args* a, void* stream) { return run_kv_cache(a, false, stream); }
+
+// Checks all but the workspace.
+static int check_window(const lsfa_window_args* a) {
+  if (a == nullptr) return fail(LSFA_ERR_INVALID, "args is NULL");
+  if (a->dtype != LSFA_DTYPE_FP16 && a->dtype != LSFA_DTYPE_BF16)
+    return fail(a->dtype == LSFA_DTYPE_FP32 ? LSFA_ERR_UNSUPPORTED : LSFA_ERR_INVALID,
+                "windowed paged attention supports bf16 and fp16 (dtype %d)", a->dtype);
+  if (a->batch < 0 || a->tokens < 0 || a->heads_q <= 0 || a->heads_kv <= 0 || a->num_blocks < 0 ||
+      a->max_blocks_per_seq < 0 || a->max_seqlen_q < 0 || a->max_seq_len < 0)
+    return fail(LSFA_ERR_INVALID, "negative size or no heads (batch=%d tokens=%d heads_q=%d heads_kv=%d num_blocks=%d "
+                "max_blocks_per_seq=%d max_seqlen_q=%d max_seq_len=%d)", a->batch, a->tokens, a->heads_q, a->heads_kv,
+                a->num_blocks, a->max_blocks_per_seq, a->max_seqlen_q, a->max_seq_len);
+  if (a->heads_q % a->heads_kv != 0)
+    return fail(LSFA_ERR_INVALID, "heads_q (%d) is not a multiple of heads_kv (%d)", a->heads_q, a->heads_kv);
+  if (a->window < 0 || a->sinks < 0 || a->sinks > (1 << 30) || (a->window > 0 && !a->causal) || (a->sinks > 0 && a->window == 0))
+    return fail(LSFA_ERR_INVALID, "window (%d) and sinks (%d) must not be negative, a window is causal, sinks need a window",
+                a->window, a->sinks);
+  if (!std::isfinite(a->sm_scale)) return fail(LSFA_ERR_INVALID, "sm_scale is not finite");
+  const bool q8 = a->kv_scales != nullptr;
+  int rc = check_paged(a->head_dim, q8 ? 16 : 8, a->block_size, a->max_blocks_per_seq, a->k_stride, a->v_stride, q8 ? 16 : 8,
+                       a->block_table_stride);
+  if (rc) return rc;
+  if (a->batch > 65535 || (long long)a->heads_q * std::max(a->max_seqlen_q, 1) > (1LL << 30))
+    return fail(LSFA_ERR_UNSUPPORTED, "more than 65535 sequences or 2^30 rows of one sequence in one call");
+  if (a->batch == 0 || a->tokens == 0 || a->max_seqlen_q == 0) return ok();
+  if (!a->q || !a->o || !a->block_tables || !a->seq_lens || ((!a->k_cache || !a->v_cache) && a->num_blocks > 0))
+    return fail(LSFA_ERR_INVALID, "q, k_cache, v_cache, o, block_tables and seq_lens must be non-NULL");
+  if (!a->cu_seqlens_q && (a->max_seqlen_q != 1 || a->tokens != a->batch))
+    return fail(LSFA_ERR_INVALID, "without cu_seqlens_q every sequence has one query");
+  for (int i = 0; i < 2; ++i)
+    if (a->q_stride[i] % 8 != 0 || a->o_stride[i] % 8 != 0)
+      return fail(LSFA_ERR_UNSUPPORTED, "q/o strides must be multiples of 8 elements");
+  if (!aligned16(a->q) || !aligned16(a->o) || !aligned16(a->k_cache) || !aligned16(a->v_cache) ||
+      (reinterpret_cast<uintptr_t>(a->kv_scales) & 7u) != 0)
+    return fail(LSFA_ERR_UNSUPPORTED, "q, o, k_cache and v_cache must be 16-byte aligned, kv_scales 8-byte");
+  return LSFA_OK;
+}
+
+static int window_run_count(const lsfa_window_args* a) {
+  const long long keys = std::min<long long>(a->max_seq_len, (long long)a->max_blocks_per_seq * a->block_size);
+  const long long seen = a->window > 0 ? std::min(keys, (long long)a->window + a->max_seqlen_q + a->sinks + 96) : keys;
+  return lsfa::window_runs(a->batch, a->heads_kv, a->heads_q / a->heads_kv, a->max_seqlen_q, seen);
+}
+static uint64_t window_bytes(const lsfa_window_args* a) {
+  if (a->batch == 0 || a->tokens == 0 || a->max_seqlen_q == 0) return 0;
+  return align256(lsfa::window_part_bytes(a->batch, a->heads_kv, a->heads_q / a->heads_kv, a->max_seqlen_q, a->head_dim,
+                                          window_run_count(a)));
+}
+
+int lsfa_window_check(const lsfa_window_args* a) {
+  const int rc = check_window(a);
+  if (rc) return rc;
+  const uint64_t need = window_bytes(a);
+  if (need > 0) {
+    if (!a->workspace) return fail(LSFA_ERR_INVALID, "workspace must be non-NULL");
+    if (a->workspace_bytes < need)
+      return fail(LSFA_ERR_INVALID, "workspace_bytes %llu is below the %llu bytes lsfa_window_workspace_size asks for",
+                  (unsigned long long)a->workspace_bytes, (unsigned long long)need);
+    if ((reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0)
+      return fail(LSFA_ERR_INVALID, "workspace is not 256-byte aligned");
+  }
+  return ok();
+}
+
+int lsfa_window_workspace_size(const lsfa_window_args* a, uint64_t* bytes) {
+  if (bytes == nullptr) return fail(LSFA_ERR_INVALID, "bytes is NULL");
+  const int rc = check_window(a);
+  if (rc) return rc;
+  *bytes = window_bytes(a);
+  return ok();
+}
+
+int lsfa_window(const lsfa_window_args* a, void* stream) {
+  const int rc = lsfa_window_check(a);
+  if (rc) return rc;
+  if (a->batch == 0 || a->tokens == 0 || a->max_seqlen_q == 0) return ok();
+  lsfa::WindowParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = a->q; p.kc = a->k_cache; p.vc = a->v_cache; p.o = a->o; p.lse = a->lse; p.scales = a->kv_scales;
+  p.cu_q = a->cu_seqlens_q; p.seq_lens = a->seq_lens; p.block_tables = a->block_tables;
+  p.part = static_cast<float*>(a->workspace);
+  p.sqt = a->q_stride[0]; p.sqh = a->q_stride[1];
+  p.skb = a->k_stride[0]; p.sks = a->k_stride[1]; p.skh = a->k_stride[2];
+  p.svb = a->v_stride[0]; p.svs = a->v_stride[1]; p.svh = a->v_stride[2];
+  p.sot = a->o_stride[0]; p.soh = a->o_stride[1];
+  p.slt = a->lse_stride[0]; p.slh = a->lse_stride[1];
+  p.sbt = a->block_table_stride;
+  p.B = a->batch; p.Hq = a->heads_q; p.Hkv = a->heads_kv; p.D = a->head_dim;
+  p.block_shift = log2_exact(a->block_size);
+  p.max_blocks = a->max_blocks_per_seq;
+  p.num_blocks = a->num_blocks;
+  p.tokens = a->tokens;
+  p.max_n = a->max_seqlen_q;
+  p.max_seq_len = a->max_seq_len;
+  p.causal = a->causal != 0;
+  p.window = a->window;
+  p.sinks = a->sinks;
+  p.runs = window_run_count(a);
+  p.scale_log2 = a->sm_scale * 1.4426950408889634f;
+  hipError_t e = lsfa::window_attention(p, a->dtype == LSFA_DTYPE_BF16, reinterpret_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(LSFA_ERR_LAUNCH, "windowed paged attention launch failed: %s", hipGetErrorString(e));
   return ok();
 }
 

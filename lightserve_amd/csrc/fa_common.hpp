@@ -106,6 +106,16 @@ __device__ __forceinline__ float half_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// All-reduce across the four 16-lane quarters of a wave.
+__device__ __forceinline__ float quarter_max(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float quarter_sum(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // 16-byte segment swizzle of LDS tiles stored [rows][DP]. Rows r..r+15 read
@@ -313,6 +323,54 @@ struct RopeParams {
   int block_size, max_blocks;
 };
 
+// Append to and read from an 8-bit paged KV cache (fa_kvq.hip). k/v: packed
+// rows [tokens, Hkv, D] (element strides token, head); kc/vc: e4m3 codes
+// (byte strides block, slot, head); scales: exponents [num_blocks, Hkv,
+// block_size, 2]. cu [B + 1] gives each sequence's rows (null: one row each).
+struct KvCacheParams {
+  void* k;
+  void* v;
+  uint8_t* kc;
+  uint8_t* vc;
+  uint8_t* scales;
+  const int32_t* block_tables;
+  const int32_t* seq_lens;
+  const int32_t* cu;
+  int64_t sk[2], sv[2];
+  int64_t skc[3], svc[3];
+  int64_t sbt;
+  int tokens, B, Hkv, D;
+  int block_shift, max_blocks, num_blocks;
+};
+
+// Attention over a paged KV cache of 8 or 16 bits with an optional window and
+// sinks (fa_window.hip); strides in elements.
+struct WindowParams {
+  const void* q;       // [tokens, Hq, D]
+  const void* kc;      // [num_blocks, block_size, Hkv, D]
+  const void* vc;
+  void* o;             // [tokens, Hq, D]
+  float* lse;          // or null
+  const uint8_t* scales;  // exponents of 8-bit caches [num_blocks, Hkv, block_size, 2], or null
+  const int32_t* cu_q;    // [B + 1], or null: one query per sequence
+  const int32_t* seq_lens;
+  const int32_t* block_tables;
+  float* part;            // partial results
+  int64_t sqt, sqh;       // token, head strides
+  int64_t skb, sks, skh;  // block, slot, head
+  int64_t svb, svs, svh;
+  int64_t sot, soh;
+  int64_t slt, slh;
+  int64_t sbt;
+  int B, Hq, Hkv, D;
+  int block_shift, max_blocks, num_blocks;
+  int tokens;              // rows of q and o
+  int max_n, max_seq_len;  // bounds of a sequence's queries and keys
+  int causal, window, sinks;
+  int runs;
+  float scale_log2;        // sm_scale * log2(e)
+};
+
 // Fused residual add + RMSNorm over rows of a [rows, cols] matrix (column
 // stride 1, row strides in elements). residual and residual_out may be null.
 struct NormParams {
@@ -446,6 +504,25 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, LDS_AS void* ds
 }
 __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rs, LDS_AS void* dst, int voff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, dst, 4, voff, 0, 0, 0);
+}
+__device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t rs, int voff) {
+  return __builtin_amdgcn_raw_buffer_load_b128(rs, voff, 0, 0);
+}
+__device__ __forceinline__ u32x2 load8b(__amdgpu_buffer_rsrc_t rs, int voff) {
+  return __builtin_amdgcn_raw_buffer_load_b64(rs, voff, 0, 0);
+}
+template <int W>
+__device__ __forceinline__ void load_words(__amdgpu_buffer_rsrc_t rs, int voff, uint32_t (&w)[W]) {
+  static_assert(W == 1 || W == 2 || W == 4, "4, 8 or 16 bytes");
+  if constexpr (W == 1) {
+    w[0] = __builtin_amdgcn_raw_buffer_load_b32(rs, voff, 0, 0);
+  } else if constexpr (W == 2) {
+    const u32x2 v = load8b(rs, voff);
+    w[0] = v[0], w[1] = v[1];
+  } else {
+    const u32x4 v = load16(rs, voff);
+    w[0] = v[0], w[1] = v[1], w[2] = v[2], w[3] = v[3];
+  }
 }
 __device__ __forceinline__ void store16(u32x4 v, __amdgpu_buffer_rsrc_t rs, int voff) {
   __builtin_amdgcn_raw_buffer_store_b128(v, rs, voff, 0, 0);

@@ -34,6 +34,19 @@ aligned: chunk query i of n sits at position seq_lens_k[b] - n + i. Returns
 o like q (and lse fp32 [heads_q, total_q] when asked); block_size must be a
 power of two of at least 16. One launch of the forward kernel with its K/V
 tiles gathered through the block tables.
+
+Both calls take three more keyword arguments:
+
+    kv_scales=None   the caches are 8-bit ones (quantized_kv_cache.py) with these scales
+    window=None      sliding window: a query at position p sees keys j > p - window ...
+    sinks=0          ... and the sequence's first `sinks` keys (attention sinks)
+
+A window is causal and counts the query's own token. Blocks that hold only keys
+which no query of the call sees are not read, so their table entries may be
+anything (an engine can give those blocks back). These calls need a
+power-of-two block_size of at least 16 (any heads_q / heads_kv) and, over 8-bit
+caches, a head_dim that is a multiple of 16. A query that sees no key gets o = 0
+and lse = -inf.
 """
 import math
 
@@ -41,6 +54,72 @@ import torch
 
 from .. import _lib
 from .flash_attention import SPLIT_MAX_TILES, SPLIT_MIN_KEYS
+from .quantized_kv_cache import check_quantized
+
+
+def _windowed(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens, max_seqlen_q, max_seq_len, causal, sm_scale,
+              return_lse, kv_scales, window, sinks):
+    """Attention over an 8-bit cache or under a window (lsfa_window); the lse is [tokens, heads_q]."""
+    assert q.dim() == 3, "q must be [tokens, heads_q, head_dim]"
+    assert q.dtype in (torch.float16, torch.bfloat16), "windowed paged attention supports bf16 and fp16"
+    if kv_scales is not None:
+        check_quantized(k_cache, v_cache, kv_scales)
+    else:
+        assert k_cache.dim() == 4 and v_cache.shape == k_cache.shape, \
+            "k_cache and v_cache must both be [num_blocks, block_size, heads_kv, head_dim]"
+        assert q.dtype == k_cache.dtype == v_cache.dtype, "q, k_cache and v_cache must share a dtype (or give kv_scales)"
+        assert k_cache.stride(3) == 1 and v_cache.stride(3) == 1, "the caches' head-dim stride must be 1"
+    T, Hq, D = q.shape
+    num_blocks, block_size, Hkv, _ = k_cache.shape
+    assert D == k_cache.shape[3], "head_dim of q and of the caches differ"
+    assert Hq % Hkv == 0, "heads_q must be a multiple of heads_kv"
+    assert block_tables.dim() == 2 and block_tables.dtype == seq_lens.dtype == torch.int32, \
+        "block_tables [batch, max_blocks] and the sequence lengths must be int32"
+    B = block_tables.shape[0]
+    assert seq_lens.shape == (B,), "the sequence lengths must be [batch]"
+    tensors = [("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables), ("seq_lens", seq_lens)]
+    if cu_seqlens_q is None:
+        assert T == B, "block_tables must be [batch, max_blocks]"
+    else:
+        assert cu_seqlens_q.dtype == torch.int32 and cu_seqlens_q.shape == (B + 1,), "cu_seqlens_q must be int32 [batch + 1]"
+        tensors.append(("cu_seqlens_q", cu_seqlens_q))
+    if kv_scales is not None:
+        tensors.append(("kv_scales", kv_scales))
+    for name, t in tensors:
+        assert t.is_cuda and t.device == q.device, f"{name} must be a GPU tensor on q's device"
+    if window is None:
+        assert sinks == 0, "sinks need a window"
+    else:
+        assert window >= 1 and sinks >= 0, "window must be at least 1 and sinks not negative"
+        assert causal, "a window is causal"
+    scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    q_ = q if (q.stride(-1) == 1 and all(s % 8 == 0 for s in q.stride()[:2]) and q.data_ptr() % 16 == 0) \
+        else q.contiguous()
+    bt = block_tables if block_tables.stride(1) == 1 else block_tables.contiguous()
+    sl = seq_lens.contiguous()
+    cu = cu_seqlens_q.contiguous() if cu_seqlens_q is not None else None
+    o = torch.empty(T, Hq, D, device=q.device, dtype=q.dtype)
+    lse = torch.empty(T, Hq, device=q.device, dtype=torch.float32) if return_lse and cu is None else \
+        torch.empty(Hq, T, device=q.device, dtype=torch.float32).t() if return_lse else None
+    if T > 0:
+        keys = min(int(max_seq_len), bt.shape[1] * block_size)
+        args = _lib.pack(
+            _lib.WindowArgs, q_.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(),
+            lse.data_ptr() if return_lse else 0, kv_scales.data_ptr() if kv_scales is not None else 0,
+            cu.data_ptr() if cu is not None else 0, sl.data_ptr(), bt.data_ptr(), 0, 0,  # the workspace follows
+            *q_.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3], *o.stride()[:2],
+            *(lse.stride() if return_lse else (0, 0)), bt.stride(0), _lib.TORCH_TO_LSFA[q.dtype], B, T, Hq, Hkv, D,
+            block_size, num_blocks, bt.shape[1], int(max_seqlen_q), keys, bool(causal),
+            # a window or sinks past the longest sequence say no more than its length
+            0 if window is None else min(int(window), keys + 1), min(int(sinks), keys), scale, 0)
+        nbytes = _lib.window_workspace_size(args)
+        ws = None
+        if nbytes > 0:
+            ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)  # 512-byte aligned blocks
+            args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+        with _lib.device_guard(q.device):
+            _lib.window(args, _lib.current_stream(q.device))
+    return (o, lse) if return_lse else o
 
 
 def _check(q, k_cache, v_cache, block_tables, seq_lens):
@@ -61,7 +140,12 @@ def _check(q, k_cache, v_cache, block_tables, seq_lens):
 
 
 def paged_attention_decode(q, k_cache, v_cache, block_tables, seq_lens, *, max_seq_len=None, sm_scale=None,
-                           return_lse=False):
+                           return_lse=False, kv_scales=None, window=None, sinks=0):
+    if kv_scales is not None or window is not None or sinks != 0:
+        if max_seq_len is None:
+            max_seq_len = int(seq_lens.max().item()) if seq_lens.numel() > 0 else 0
+        return _windowed(q, k_cache, v_cache, block_tables, None, seq_lens, 1, max_seq_len, True, sm_scale, return_lse,
+                         kv_scales, window, sinks)
     _check(q, k_cache, v_cache, block_tables, seq_lens)
     B, Hq, D = q.shape
     num_blocks, block_size, Hkv, _ = k_cache.shape
@@ -91,7 +175,14 @@ def paged_attention_decode(q, k_cache, v_cache, block_tables, seq_lens, *, max_s
 
 
 def paged_prefill(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens_k, *, max_seqlen_q=None, causal=True,
-                  sm_scale=None, return_lse=False):
+                  sm_scale=None, return_lse=False, kv_scales=None, window=None, sinks=0):
+    if kv_scales is not None or window is not None or sinks != 0:
+        if max_seqlen_q is None:
+            max_seqlen_q = int((cu_seqlens_q[1:] - cu_seqlens_q[:-1]).max().item()) if cu_seqlens_q.numel() > 1 else 0
+        most = block_tables.shape[-1] * k_cache.shape[1]
+        got = _windowed(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens_k, max_seqlen_q, most, causal, sm_scale,
+                        return_lse, kv_scales, window, sinks)
+        return (got[0], got[1].t()) if return_lse else got
     assert q.dim() == 3, "q must be packed [total_q, heads_q, head_dim]"
     assert k_cache.dim() == 4 and v_cache.shape == k_cache.shape, \
         "k_cache and v_cache must be [num_blocks, block_size, heads_kv, head_dim] of one shape"

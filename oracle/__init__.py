@@ -12,6 +12,8 @@ Contents
                 tiled forward/backward loops, varlen/GQA, paged-KV decode,
                 paged-KV chunked prefill,
                 and a pure-Python loop version for tiny inputs.
+  paged8.py     the 8-bit paged cache (quantised rows by search over e4m3's
+                values) and paged attention with a window and sinks.
   model.py      the reference's model forward in plain torch (RoPE tables and
                 rotation, RMSNorm, the fused add + RMSNorm's semantics,
                 reference_llama_forward, with GQA).
@@ -30,6 +32,8 @@ How each function is pinned (tests/test_oracle.py):
                         chunks), a block permutation, and the chunking
                         invariant (chunk-by-chunk prefill equals one causal
                         pass); a planted top-left mask fails it.
+  paged8.*              torch's float8 cast, hand-built rows and caches, the dense
+                        closed form under an explicit mask (tests/test_oracle_paged8.py).
   model.apply_rope      RoPE as an element-by-element rotation (tests/test_oracle_model.py).
   model.add_rmsnorm_reference  h and out written out by hand per element
                         (pure-Python sums), with and without the residual; unit

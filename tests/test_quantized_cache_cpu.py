@@ -1,0 +1,189 @@
+"""What the calls on 8-bit caches and under a window refuse, without a GPU: the C ABI's own checks, then the Python entry points'."""
+import ctypes
+
+import pytest
+import torch
+
+from lightserve_amd import _lib
+from lightserve_amd.kernels.paged_attention import paged_attention_decode, paged_prefill
+from lightserve_amd.kernels.quantized_kv_cache import kv_cache_append, kv_cache_read, quantized_kv_cache
+
+P = 1 << 20  # stands for a device address: the checks read nothing there
+
+
+def _kv(**kw):
+    a = _lib.KvCacheArgs(k=P, v=P, k_cache=P, v_cache=P, kv_scales=P, block_tables=P, seq_lens=P, cu_seqlens=P,
+                         k_stride=(1024, 128), v_stride=(1024, 128), k_cache_stride=(16384, 1024, 128),
+                         v_cache_stride=(16384, 1024, 128), block_table_stride=10, dtype=_lib.DTYPE_BF16, batch=3, tokens=20,
+                         heads_kv=8, head_dim=128, block_size=16, num_blocks=30, max_blocks_per_seq=10)
+    for name, value in kw.items():
+        setattr(a, name, value)
+    return a
+
+
+def _win(**kw):
+    a = _lib.WindowArgs(q=P, k_cache=P, v_cache=P, o=P, lse=P, kv_scales=P, cu_seqlens_q=P, seq_lens=P, block_tables=P,
+                        workspace=P, workspace_bytes=1 << 40, q_stride=(4096, 128), k_stride=(16384, 1024, 128),
+                        v_stride=(16384, 1024, 128), o_stride=(4096, 128), lse_stride=(32, 1), block_table_stride=10,
+                        dtype=_lib.DTYPE_BF16, batch=3, tokens=20, heads_q=32, heads_kv=8, head_dim=128, block_size=16,
+                        num_blocks=30, max_blocks_per_seq=10, max_seqlen_q=12, max_seq_len=160, causal=1, window=50, sinks=4,
+                        sm_scale=0.1)
+    for name, value in kw.items():
+        setattr(a, name, value)
+    return a
+
+
+BOTH = [(dict(head_dim=72), -2, "multiple of 16"), (dict(head_dim=144), -2, "multiple of 16"), (dict(head_dim=0), -2, "multiple"),
+        (dict(block_size=8), -2, "power of two"), (dict(block_size=48), -2, "power of two"), (dict(num_blocks=-1), -1, "negative"),
+        (dict(batch=-1), -1, "negative"), (dict(tokens=-1), -1, "negative"), (dict(heads_kv=0), -1, "no heads"),
+        (dict(dtype=7), -1, "dtype"), (dict(block_table_stride=9), -1, "block_table_stride"), (dict(k_cache=None), -1, "non-NULL"),
+        (dict(v_cache=P + 8), -2, "aligned"), (dict(kv_scales=P + 4), -2, "aligned"), (dict(block_tables=None), -1, "non-NULL"),
+        (dict(max_blocks_per_seq=1 << 27, block_table_stride=1 << 27), -2, "2^30")]
+
+
+@pytest.mark.parametrize("change,status,word", BOTH + [
+    (dict(k_cache_stride=(16384, 1032, 128)), -2, "16 bytes"), (dict(v_cache_stride=(16384, 1 << 23, 128)), -2, "slot strides"),
+    (dict(k=None), -1, "non-NULL"), (dict(v=P + 2), -2, "aligned"), (dict(k_stride=(1028, 128)), -2, "16 bytes"),
+    (dict(tokens=1 << 30), -2, "rows"), (dict(kv_scales=None), -1, "non-NULL")])
+def test_cache_refusals(built_library, change, status, word):
+    for check in (_lib.kv_append_check, _lib.kv_read_check):
+        assert check(_kv())[0] == 0
+        rc, msg = check(_kv(**change))
+        assert rc == status and word in msg, (rc, msg)
+
+
+def test_cache_refusals_of_one_call(built_library):
+    rc, msg = _lib.kv_append_check(_kv(cu_seqlens=None))
+    assert rc == -1 and "20 rows for 3 sequences" in msg
+    assert _lib.kv_append_check(_kv(cu_seqlens=None, tokens=3))[0] == 0
+    assert _lib.kv_append_check(_kv(seq_lens=None))[0] == -1 and _lib.kv_read_check(_kv(seq_lens=None))[0] == 0
+    assert _lib.kv_read_check(_kv(cu_seqlens=None))[0] == -1
+    for check in (_lib.kv_append_check, _lib.kv_read_check):
+        assert check(_kv(tokens=0, k=None, v=None))[0] == 0
+        assert check(_kv(num_blocks=0, k_cache=None, v_cache=None, kv_scales=None))[0] == 0
+        assert check(_kv(dtype=_lib.DTYPE_FP32, k_stride=(1028, 132), v_stride=(1028, 132)))[0] == 0  # 16 bytes of fp32
+    assert _lib.load().lsfa_kv_append_check(None) == -1 and _lib.load().lsfa_kv_read_check(None) == -1
+    assert _lib.load().lsfa_kv_append(None, None) == -1 and _lib.load().lsfa_kv_read(None, None) == -1
+
+
+@pytest.mark.parametrize("change,status,word", BOTH + [
+    (dict(k_stride=(16384, 1032, 128)), -2, "16 bytes"), (dict(v_stride=(16384, 1 << 23, 128)), -2, "slot strides"),
+    (dict(dtype=_lib.DTYPE_FP32), -2, "bf16 and fp16"), (dict(heads_q=33), -1, "multiple of heads_kv"),
+    (dict(window=-1), -1, "window"), (dict(sinks=-1), -1, "sinks"), (dict(window=0), -1, "sinks need a window"),
+    (dict(causal=0), -1, "causal"), (dict(sm_scale=float("inf")), -1, "finite"), (dict(sm_scale=float("nan")), -1, "finite"),
+    (dict(q=None), -1, "non-NULL"), (dict(o=None), -1, "non-NULL"), (dict(seq_lens=None), -1, "non-NULL"),
+    (dict(cu_seqlens_q=None), -1, "one query"), (dict(q_stride=(4100, 128)), -2, "multiples of 8"), (dict(o=P + 8), -2, "aligned"),
+    (dict(max_seq_len=-1), -1, "negative"), (dict(max_seqlen_q=-1), -1, "negative"), (dict(batch=70000), -2, "65535"),
+    (dict(max_seqlen_q=1 << 26), -2, "2^30"), (dict(workspace=None), -1, "workspace"), (dict(workspace=P + 16), -1, "aligned"),
+    (dict(workspace_bytes=16), -1, "below")])
+def test_window_refusals(built_library, change, status, word):
+    assert _lib.window_check(_win()) == (0, "")
+    rc, msg = _lib.window_check(_win(**change))
+    assert rc == status and word in msg, (rc, msg)
+
+
+def test_window_sizes(built_library):
+    """Head dims that 16-bit caches allow; nothing to do; workspaces of sizes that are refused elsewhere."""
+    assert _lib.window_check(_win(kv_scales=None, head_dim=72))[0] == 0
+    assert _lib.window_check(_win(kv_scales=None, head_dim=60))[0] == -2
+    for nothing in (dict(batch=0), dict(tokens=0), dict(max_seqlen_q=0)):
+        assert _lib.window_check(_win(workspace=None, q=None, **nothing))[0] == 0
+        assert _lib.window_workspace_size(_win(**nothing)) == 0
+    assert _lib.window_workspace_size(_win()) > 0
+    assert _lib.load().lsfa_window_check(None) == -1 and _lib.load().lsfa_window(None, None) == -1
+    n = ctypes.c_uint64(5)
+    assert _lib.load().lsfa_window_workspace_size(None, ctypes.byref(n)) == -1
+    assert _lib.load().lsfa_window_workspace_size(ctypes.byref(_win()), None) == -1
+    for bad in (dict(heads_kv=0), dict(block_size=0), dict(head_dim=0), dict(max_seqlen_q=-3)):
+        with pytest.raises(RuntimeError):
+            _lib.window_workspace_size(_win(**bad))
+
+
+def test_struct_sizes_match_the_header(built_library, tmp_path):
+    import os
+    import shutil
+    import subprocess
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no host C compiler")
+    include = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "include")
+    src = tmp_path / "t.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "lightserve_fa.h"\n'
+                   'int main(void){printf("%zu %zu %zu %zu %zu\\n", sizeof(lsfa_kv_cache_args), offsetof(lsfa_kv_cache_args, dtype),'
+                   ' sizeof(lsfa_window_args), offsetof(lsfa_window_args, dtype), offsetof(lsfa_window_args, sm_scale)); return 0;}\n')
+    subprocess.run([cc, "-I", include, str(src), "-o", str(tmp_path / "t")], check=True)
+    got = [int(x) for x in subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [ctypes.sizeof(_lib.KvCacheArgs), _lib.KvCacheArgs.dtype.offset, ctypes.sizeof(_lib.WindowArgs),
+                   _lib.WindowArgs.dtype.offset, _lib.WindowArgs.sm_scale.offset]
+
+
+def _tensors():
+    kc, vc, sc = quantized_kv_cache(4, 16, 2, 64, device="cpu")
+    return kc, vc, sc, torch.zeros(2, 2, dtype=torch.int32), torch.ones(2, dtype=torch.int32), torch.arange(3, dtype=torch.int32)
+
+
+def test_an_empty_cache():
+    kc, vc, sc, *_ = _tensors()
+    assert kc.dtype == vc.dtype == torch.float8_e4m3fn and kc.shape == vc.shape == (4, 16, 2, 64)
+    assert sc.dtype == torch.uint8 and sc.shape == (4, 2, 16, 2) and (kc.view(torch.uint8) == 0).all()
+    assert kc.data_ptr() != vc.data_ptr()
+
+
+def test_python_refusals_of_the_cache():
+    kc, vc, sc, bt, sl, cu = _tensors()
+    rows = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    for args, word in (((rows, rows, kc, vc, sc, bt, sl), "GPU tensor"),
+                       ((rows, rows[:1], kc, vc, sc, bt, sl), "tokens, heads_kv"),
+                       ((rows, rows.float(), kc, vc, sc, bt, sl), "tokens, heads_kv"),
+                       ((rows.long(), rows.long(), kc, vc, sc, bt, sl), "unsupported dtype"),
+                       ((rows, rows, kc.view(torch.uint8), vc, sc, bt, sl), "float8_e4m3fn"),
+                       ((rows, rows, kc, vc[:2], sc, bt, sl), "must both be"),
+                       ((rows, rows, kc, vc, sc.transpose(1, 2).contiguous(), bt, sl), "kv_scales"),
+                       ((rows, rows, kc, vc, sc.int(), bt, sl), "kv_scales"),
+                       ((rows, rows, kc, vc, sc, bt.long(), sl), "block_tables")):
+        with pytest.raises(AssertionError, match=word):
+            kv_cache_append(*args)
+    with pytest.raises(AssertionError, match="GPU tensor"):
+        kv_cache_read(kc, vc, sc, bt, cu)
+    with pytest.raises(AssertionError, match="kv_scales"):
+        kv_cache_read(kc, vc, sc[:3], bt, cu)
+
+
+def test_python_refusals_of_the_attention():
+    kc, vc, sc, bt, sl, cu = _tensors()
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+    half = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
+
+    def decode(q=q, k=kc, v=vc, bt=bt, sl=sl, **kw):
+        return paged_attention_decode(q, k, v, bt, sl, max_seq_len=16, **({"kv_scales": sc} | kw))
+
+    def chunk(q=q, k=kc, v=vc, bt=bt, cu=cu, sl=sl, **kw):
+        return paged_prefill(q, k, v, bt, cu, sl, max_seqlen_q=1, **({"kv_scales": sc} | kw))
+
+    for call in (decode, chunk):
+        for kw, word in ((dict(), "GPU tensor"), (dict(q=q.float()), "bf16 and fp16"), (dict(q=q[0]), "must be"),
+                         (dict(k=half, v=half), "float8_e4m3fn"), (dict(k=half, v=half, kv_scales=None, window=3), "GPU tensor"),
+                         (dict(k=half.half(), v=half.half(), kv_scales=None, window=3), "share a dtype"),
+                         (dict(kv_scales=sc[:2]), "kv_scales"), (dict(q=q[:, :3]), "multiple of heads_kv"),
+                         (dict(q=q[:, :, :32]), "head_dim"), (dict(bt=bt.long()), "int32"), (dict(sl=sl[:1]), "batch")):
+            with pytest.raises(AssertionError, match=word):
+                call(**kw)
+    with pytest.raises(AssertionError, match="cu_seqlens_q"):
+        chunk(cu=cu[:2])
+    with pytest.raises(AssertionError, match="batch"):
+        decode(q=torch.zeros(3, 4, 64, dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("kw,word", [(dict(sinks=1), "sinks need"), (dict(window=0), "at least 1"), (dict(window=-3), "at least 1"),
+                                     (dict(window=4, sinks=-1), "not negative")])
+def test_window_arguments(monkeypatch, kw, word):
+    """Checked after the tensors, so these stand on the GPU here in name."""
+    kc, vc, sc, bt, sl, cu = _tensors()
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+    with pytest.raises(AssertionError, match=word):
+        paged_attention_decode(q, kc, vc, bt, sl, max_seq_len=16, kv_scales=sc, **kw)
+    with pytest.raises(AssertionError, match=word):
+        paged_prefill(q, kc, vc, bt, cu, sl, max_seqlen_q=1, kv_scales=sc, **kw)
+    with pytest.raises(AssertionError, match="causal"):
+        paged_prefill(q, kc, vc, bt, cu, sl, max_seqlen_q=1, kv_scales=sc, causal=False, window=3)
