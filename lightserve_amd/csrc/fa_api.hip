@@ -21,9 +21,8 @@ hipError_t fwd_f32(const FwdParams& p, int dp, bool causal, bool varlen, float s
 hipError_t bwd_f32(const BwdParams& p, int dp, bool causal, hipStream_t s);
 hipError_t decode_gqa(const DecodeParams& p, bool is_bf16, int dp, hipStream_t s);
 hipError_t kv_cache_move(const KvCacheParams& p, int dtype, bool append, hipStream_t s);
-int window_runs(int B, int Hkv, int G, int max_n, long long max_keys);
-uint64_t window_part_bytes(int B, int Hkv, int G, int max_n, int D, int runs);
-hipError_t window_attention(const WindowParams& p, bool is_bf16, hipStream_t s);
+WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int max_n, long long max_keys, int window, int sinks);
+hipError_t window_attention(WindowParams p, const WindowPlan& w, bool is_bf16, hipStream_t s);
 hipError_t rope_inplace(const RopeParams& p, int dtype, hipStream_t s);
 hipError_t add_rmsnorm(const NormParams& p, int dtype, bool vec, hipStream_t s);
 hipError_t gemv(const GemvParams& p, bool is_bf16, hipStream_t s);
@@ -773,8 +772,9 @@ static int check_window(const lsfa_window_args* a) {
   int rc = check_paged(a->head_dim, q8 ? 16 : 8, a->block_size, a->max_blocks_per_seq, a->k_stride, a->v_stride, q8 ? 16 : 8,
                        a->block_table_stride);
   if (rc) return rc;
-  if (a->batch > 65535 || (long long)a->heads_q * std::max(a->max_seqlen_q, 1) > (1LL << 30))
-    return fail(LSFA_ERR_UNSUPPORTED, "more than 65535 sequences or 2^30 rows of one sequence in one call");
+  if (a->batch > 65535 || (long long)a->heads_q * std::max(a->max_seqlen_q, 1) > (1LL << 30) ||
+      (long long)a->heads_q * a->tokens > (1LL << 36) || (long long)a->heads_kv * a->batch > (1LL << 30))
+    return fail(LSFA_ERR_UNSUPPORTED, "more than 65535 sequences, 2^30 rows of one sequence or 2^36 rows in one call");
   if (a->batch == 0 || a->tokens == 0 || a->max_seqlen_q == 0) return ok();
   if (!a->q || !a->o || !a->block_tables || !a->seq_lens || ((!a->k_cache || !a->v_cache) && a->num_blocks > 0))
     return fail(LSFA_ERR_INVALID, "q, k_cache, v_cache, o, block_tables and seq_lens must be non-NULL");
@@ -789,21 +789,18 @@ static int check_window(const lsfa_window_args* a) {
   return LSFA_OK;
 }
 
-static int window_run_count(const lsfa_window_args* a) {
-  const long long keys = std::min<long long>(a->max_seq_len, (long long)a->max_blocks_per_seq * a->block_size);
-  const long long seen = a->window > 0 ? std::min(keys, (long long)a->window + a->max_seqlen_q + a->sinks + 96) : keys;
-  return lsfa::window_runs(a->batch, a->heads_kv, a->heads_q / a->heads_kv, a->max_seqlen_q, seen);
-}
-static uint64_t window_bytes(const lsfa_window_args* a) {
-  if (a->batch == 0 || a->tokens == 0 || a->max_seqlen_q == 0) return 0;
-  return align256(lsfa::window_part_bytes(a->batch, a->heads_kv, a->heads_q / a->heads_kv, a->max_seqlen_q, a->head_dim,
-                                          window_run_count(a)));
+static lsfa::WindowPlan plan_window(const lsfa_window_args* a) {
+  if (a->batch == 0 || a->tokens == 0 || a->max_seqlen_q == 0) return {};
+  return lsfa::window_plan(a->batch, a->tokens, a->heads_kv, a->heads_q / a->heads_kv, a->head_dim,
+                           std::min(a->max_seqlen_q, a->tokens),
+                           std::min<long long>(a->max_seq_len, (long long)a->max_blocks_per_seq * a->block_size), a->window,
+                           a->sinks);
 }
 
 int lsfa_window_check(const lsfa_window_args* a) {
   const int rc = check_window(a);
   if (rc) return rc;
-  const uint64_t need = window_bytes(a);
+  const uint64_t need = plan_window(a).part_bytes;
   if (need > 0) {
     if (!a->workspace) return fail(LSFA_ERR_INVALID, "workspace must be non-NULL");
     if (a->workspace_bytes < need)
@@ -819,7 +816,7 @@ int lsfa_window_workspace_size(const lsfa_window_args* a, uint64_t* bytes) {
   if (bytes == nullptr) return fail(LSFA_ERR_INVALID, "bytes is NULL");
   const int rc = check_window(a);
   if (rc) return rc;
-  *bytes = window_bytes(a);
+  *bytes = align256(plan_window(a).part_bytes);
   return ok();
 }
 
@@ -843,14 +840,14 @@ int lsfa_window(const lsfa_window_args* a, void* stream) {
   p.max_blocks = a->max_blocks_per_seq;
   p.num_blocks = a->num_blocks;
   p.tokens = a->tokens;
-  p.max_n = a->max_seqlen_q;
+  p.max_n = std::min(a->max_seqlen_q, a->tokens);
   p.max_seq_len = a->max_seq_len;
   p.causal = a->causal != 0;
   p.window = a->window;
   p.sinks = a->sinks;
-  p.runs = window_run_count(a);
   p.scale_log2 = a->sm_scale * 1.4426950408889634f;
-  hipError_t e = lsfa::window_attention(p, a->dtype == LSFA_DTYPE_BF16, reinterpret_cast<hipStream_t>(stream));
+  p.scale_abs = fmaxf(fabsf(p.scale_log2), 1e-30f);
+  hipError_t e = lsfa::window_attention(p, plan_window(a), a->dtype == LSFA_DTYPE_BF16, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(LSFA_ERR_LAUNCH, "windowed paged attention launch failed: %s", hipGetErrorString(e));
   return ok();
 }

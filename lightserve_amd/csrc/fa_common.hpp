@@ -367,8 +367,15 @@ struct WindowParams {
   int tokens;              // rows of q and o
   int max_n, max_seq_len;  // bounds of a sequence's queries and keys
   int causal, window, sinks;
-  int runs;
+  int runs, splits;        // WindowPlan's
   float scale_log2;        // sm_scale * log2(e)
+  float scale_abs;         // |scale_log2|, at least 1e-30
+};
+struct WindowPlan {
+  int runs;             // narrow kernel: runs that the key tiles are shared out over
+  int items, waves;     // wide kernel (items > 0): row tiles at most, waves of a workgroup
+  int splits;           // workgroups that an item's key tiles are shared out over
+  uint64_t part_bytes;  // partial results
 };
 
 // Fused residual add + RMSNorm over rows of a [rows, cols] matrix (column
@@ -510,6 +517,9 @@ __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t rs, int voff) {
 }
 __device__ __forceinline__ u32x2 load8b(__amdgpu_buffer_rsrc_t rs, int voff) {
   return __builtin_amdgcn_raw_buffer_load_b64(rs, voff, 0, 0);
+}
+__device__ __forceinline__ uint32_t load1(__amdgpu_buffer_rsrc_t rs, int voff) {
+  return (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rs, voff, 0, 0);
 }
 template <int W>
 __device__ __forceinline__ void load_words(__amdgpu_buffer_rsrc_t rs, int voff, uint32_t (&w)[W]) {

@@ -7,6 +7,7 @@
 // holds e4m3 codes and one power-of-two scale for each row (fa_kvq.hip).
 //
 // Few rows per KV head (decode, and chunks of a few tokens): the narrow kernel.
+// Many: the wide one, further down.
 // The path is bound by HBM, so it is built around bytes in flight, and each
 // byte of the cache is read once for all query heads that share it:
 //   rows       (token, query head of the KV head's group) pairs, 16 to a row
@@ -105,6 +106,7 @@ __device__ __forceinline__ int run_tiles(const WindowParams& p, int all) {
 }
 
 constexpr int kRowTile = 16;
+constexpr int kNarrowRows = 16;  // most rows of a sequence and KV head in the narrow kernel
 
 template <typename T, typename C, int DP>
 __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowParams p) {
@@ -441,6 +443,538 @@ __global__ __launch_bounds__(256) void fa_window_combine_kernel(const WindowPara
   }
 }
 
+// ---------------------------------------------------------------- wide kernel
+// Many rows per KV head (chunks of new tokens): a workgroup of NW waves takes
+// 32 NW (token, query head) rows of one sequence and KV head, wave w rows 32 w ..
+// 32 w + 31, so that every key tile brought into LDS serves the whole group of
+// query heads. Key tiles of 64 lie in LDS in q's type, K and V double-buffered;
+// 8-bit rows are loaded into registers one step ahead and written to LDS with
+// their scales applied (each value once per workgroup, where every wave would
+// convert it again on reading codes), 16-bit rows go there by direct loads.
+// Rows that none of the workgroup's queries sees read as zeros. S^T = K Q^T and
+// O^T += V^T P^T on v_mfma_f32_32x32x16 (fa_common.hpp has the lane layouts), the
+// scores of tile t + 1 beside the softmax of tile t.
+constexpr int kWideTile = 64;  // keys
+
+// Row tiles longest first (ranked_item) for up to 64 sequences, else in order.
+// The length that counts is that of a causal row without a window: under one, tiles are
+// about equally long and the order does not matter.
+template <int BM>
+__device__ __forceinline__ bool wide_item(const WindowParams& p, int item, int lane, int& b, int& rt) {
+  const int G = p.Hq / p.Hkv;
+  if (p.B <= 64) {
+    int tq = 0, nk = 0, off = 0;
+    if (lane < p.B) {
+      const KeyTiles t = key_tiles(p, lane);
+      tq = (int)(((int64_t)min(t.n, p.max_n) * G + BM - 1) / BM);
+      nk = t.seq;
+      off = nk - t.n;
+    }
+    auto above = [&](int x) -> int {
+      if (x < 0) return tq;
+      if (tq == 0 || nk <= kWideTile * x) return 0;
+      if (!p.causal) return tq;
+      const long long y = ((long long)kWideTile * x - off) * G;  // row tile t ends past key 64 x iff t >= y / BM
+      return y < 0 ? tq : 1 + (int)max(0LL, tq - 1 - y / BM);
+    };
+    int d;
+    b = ranked_item(p.B, item, lane, tq, nk > 0 ? (nk + kWideTile - 1) / kWideTile : 0, above, d);
+    if (b < 0) return false;
+    rt = __builtin_amdgcn_readlane(tq, b) - 1 - d;
+    return true;
+  }
+  int at = 0;
+  for (int j = 0; j < p.B; j += 64) {
+    const int mine = j + lane < p.B ? (int)(((int64_t)min(key_tiles(p, j + lane).n, p.max_n) * G + BM - 1) / BM) : 0;
+    const int upto = lanes_sum(mine);
+    const unsigned long long hit = __ballot(at + upto > item);
+    if (hit != 0) {
+      const int src = __builtin_ctzll(hit);
+      b = j + src;
+      rt = item - at - __builtin_amdgcn_readlane(upto - mine, src);
+      return true;
+    }
+    at += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+// A row tile's key tiles: `sink` of them from key 0 on, then those from tile
+// `first` on.
+struct WideSpan {
+  int sink, first, count;
+  int hi_max, lo_min;  // keys past hi_max, or before lo_min and no sinks, are seen by no row
+};
+template <int BM>
+__device__ __forceinline__ WideSpan wide_span(const WindowParams& p, const KeyTiles& kt, int rt) {
+  const int G = p.Hq / p.Hkv, rows = kt.n * G;
+  const int t0 = rt * BM / G, t1 = (min(rows, (rt + 1) * BM) - 1) / G;
+  WideSpan s;
+  s.hi_max = p.causal ? kt.seq - kt.n + t1 : kt.seq - 1;
+  s.lo_min = p.window > 0 ? kt.seq - kt.n + t0 - p.window + 1 : 0;
+  const int end = max(s.hi_max + 1, 0);
+  s.first = min(max(s.lo_min, 0), end) / kWideTile;
+  s.sink = p.window > 0 ? min((min(p.sinks, end) + kWideTile - 1) / kWideTile, s.first) : 0;
+  s.count = s.sink + (end + kWideTile - 1) / kWideTile - s.first;
+  return s;
+}
+// Tiles of one of an item's splits: an even share, at least kSplitLeast.
+constexpr int kSplitLeast = 3;
+__device__ __forceinline__ int split_share(int count, int splits) {
+  return max((count + splits - 1) / splits, kSplitLeast);
+}
+// Floats of one split's partial results: (offset, sum for O, sum for the lse, 0) of
+// each row, then O in the accumulators' own order, [wave][4-register group][lane].
+template <int BM, int DP> constexpr int kWidePart = BM * 4 + BM * DP;
+
+template <typename T> constexpr float kWideMaxLog2P = 64.0f;
+template <> constexpr float kWideMaxLog2P<_Float16> = 15.0f;
+
+template <typename T, typename C, int DP, int NW, bool LSE, bool SPLIT>
+__global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(const WindowParams p) {
+  using X8 = typename VecT<T>::x8;
+  using X4 = typename VecT<T>::x4;
+  constexpr bool Q8 = sizeof(C) == 1;
+  constexpr int EB = sizeof(C);
+  constexpr int BM = NW * 32, BN = kWideTile;
+  constexpr int TILE = BN * DP;            // elements of one K or V tile in LDS
+  constexpr int KSTEPS = DP / 16, DT = DP / 32, KB = BN / 32;
+  constexpr int RPW = BN / NW;             // tile rows that a wave loads: 8 or 16, in one cache block
+  constexpr int LPR = DP / 8;              // lanes per row, 8 elements each
+  constexpr int RPL = 64 / LPR;            // rows per load instruction
+  constexpr int NL = RPW / RPL;            // load instructions per wave and tile
+  static_assert(NL >= 1, "a wave loads whole instructions");
+
+  __shared__ __attribute__((aligned(1024))) T smem_raw[4 * TILE];  // K0 K1 V0 V1
+  LDS_AS char* smem = (LDS_AS char*)smem_raw;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hh = lane >> 5;
+  const int G = p.Hq / p.Hkv;
+  const int head = ranked_head(blockIdx.x % p.Hkv, p.Hkv);
+  int b, rt;
+  if (!wide_item<BM>(p, blockIdx.x / p.Hkv, lane, b, rt)) return;  // uniform, before any barrier
+  KeyTiles kt = key_tiles(p, b);
+  kt.seq = __builtin_amdgcn_readfirstlane(kt.seq);
+  kt.n = __builtin_amdgcn_readfirstlane(kt.n);
+  const int64_t tok0 = __builtin_amdgcn_readfirstlane(kt.tok0);
+  WideSpan sp = wide_span<BM>(p, kt, rt);
+  const int sink = __builtin_amdgcn_readfirstlane(sp.sink), first = __builtin_amdgcn_readfirstlane(sp.first);
+  const int hi_max = __builtin_amdgcn_readfirstlane(sp.hi_max), lo_min = __builtin_amdgcn_readfirstlane(sp.lo_min);
+  int t_lo = 0, t_hi = __builtin_amdgcn_readfirstlane(sp.count);
+  bool whole_item = true;
+  if constexpr (SPLIT) {
+    const int share = __builtin_amdgcn_readfirstlane(split_share(t_hi, p.splits));
+    whole_item = t_hi <= share;
+    t_lo = blockIdx.y * share;
+    if (blockIdx.y > 0 && t_lo >= t_hi) return;  // uniform, before any barrier
+    t_hi = min(t_hi, t_lo + share);
+  }
+  const int seq = kt.seq, nrows = min(kt.n, p.max_n) * G;
+  const int sinks = p.window > 0 ? p.sinks : 0;
+  const float sl2 = p.scale_abs;
+
+  // The lane's row and what it sees, and the same over the wave's rows.
+  const int r0 = rt * BM + wave * 32, r = r0 + l32, tok = r / G, hq = head * G + (r - tok * G);
+  const bool row_ok = r < nrows;
+  const int pos = p.causal ? seq - kt.n + tok : seq - 1;
+  const int hi = row_ok ? pos : -1, lo = p.window > 0 ? pos - p.window + 1 : 0;
+  const int w0 = seq - kt.n + r0 / G, w1 = seq - kt.n + (min(r0 + 32, nrows) - 1) / G;
+  const int whi_min = __builtin_amdgcn_readfirstlane(p.causal ? w0 : seq - 1);
+  const int whi_max = __builtin_amdgcn_readfirstlane(r0 >= nrows ? -1 : p.causal ? w1 : seq - 1);
+  const int wlo_min = __builtin_amdgcn_readfirstlane(p.window > 0 ? w0 - p.window + 1 : 0);
+  const int wlo_max = __builtin_amdgcn_readfirstlane(p.window > 0 ? w1 - p.window + 1 : 0);
+
+  X8 qreg[KSTEPS];
+#pragma unroll
+  for (int kk = 0; kk < KSTEPS; ++kk) {
+    const int col = 16 * kk + 8 * hh;
+    u32x4 raw = {0, 0, 0, 0};
+    if (row_ok && col < p.D) raw = ldg16((const T*)p.q + (tok0 + tok) * p.sqt + (int64_t)hq * p.sqh + col);
+    if (p.scale_log2 < 0.f) raw ^= 0x80008000u;
+    qreg[kk] = __builtin_bit_cast(X8, raw);
+  }
+
+  auto key_of = [&](int t) -> int { return (t < sink ? t : t - sink + first) * BN; };
+  const __attribute__((address_space(4))) int32_t* table =
+      (const __attribute__((address_space(4))) int32_t*)(p.block_tables + (int64_t)b * p.sbt);
+  // Cache block of the wave's rows of tile t (-1: none).
+  auto block_at = [&](int t) -> int {
+    const int key = key_of(t) + RPW * wave;
+    return t < t_hi && key < seq ? table[key >> p.block_shift] : -1;
+  };
+
+  // Loads. Lane offsets within the wave's RPW rows of a tile; 8-bit: row l / LPR,
+  // elements 8 (l % LPR) .. + 7; 16-bit: what the direct load's linear LDS order
+  // makes of the swizzled tile.
+  int krow[NL], kcol[NL];
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    krow[i] = i * RPL + lane / LPR;
+    const int seg = Q8 ? lane % LPR : (lane % LPR) ^ seg_swz<DP>(RPW * wave + krow[i]);
+    kcol[i] = 8 * seg;
+  }
+  auto offset = [&](int i, int64_t stride, int key0) -> int {
+    const int key = key0 + RPW * wave + krow[i];
+    const bool used = kcol[i] < p.D && key <= hi_max && (key >= lo_min || key < sinks);
+    return used ? (krow[i] * (int)stride + kcol[i]) * EB : (int)0x80000000;
+  };
+  auto rows_of = [&](const C* base, int64_t sb, int64_t ss, int64_t sh, int t, int blk) -> __amdgpu_buffer_rsrc_t {
+    const bool live = (unsigned)blk < (unsigned)p.num_blocks;
+    const int slot = (key_of(t) + RPW * wave) & ((1 << p.block_shift) - 1);
+    return tile_rsrc(base + (live ? (int64_t)blk * sb + (int64_t)slot * ss + (int64_t)head * sh : 0),
+                     live ? (int)(((RPW - 1) * ss + p.D) * EB) : 0);
+  };
+  struct Codes {
+    u32x2 w[NL];
+    uint32_t e[NL];
+  };
+  auto load_codes = [&](Codes& c, const C* base, int64_t sb, int64_t ss, int64_t sh, int t, int blk, int which) {
+    const __amdgpu_buffer_rsrc_t rs = rows_of(base, sb, ss, sh, t, blk);
+    const bool live = (unsigned)blk < (unsigned)p.num_blocks;
+    const int slot = (key_of(t) + RPW * wave) & ((1 << p.block_shift) - 1);
+    const uint8_t* sb8 = p.scales + (live ? ((((int64_t)blk * p.Hkv + head) << p.block_shift) + slot) * 2 : 0);
+    const __amdgpu_buffer_rsrc_t es = tile_rsrc(sb8, live ? 2 * RPW : 0);
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int vo = offset(i, ss, key_of(t));
+      c.w[i] = load8b(rs, vo);
+      c.e[i] = load1(es, vo < 0 ? vo : 2 * krow[i] + which);
+    }
+  };
+  auto write_codes = [&](const Codes& c, int buf) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const float s = __uint_as_float(c.e[i] << 23);
+      const u32x4 v = {codes2<false>(c.w[i][0], s, T()), codes2<true>(c.w[i][0], s, T()), codes2<false>(c.w[i][1], s, T()),
+                       codes2<true>(c.w[i][1], s, T())};
+      *(LDS_AS u32x4*)(smem + buf * TILE * 2 + swz_off<DP>(RPW * wave + krow[i], kcol[i]) * 2) = v;
+    }
+  };
+  auto load_direct = [&](const C* base, int64_t sb, int64_t ss, int64_t sh, int t, int blk, int buf) {
+    const __amdgpu_buffer_rsrc_t rs = rows_of(base, sb, ss, sh, t, blk);
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      dma16(rs, (LDS_AS void*)(smem + buf * TILE * 2 + (RPW * wave + i * RPL) * DP * 2), offset(i, ss, key_of(t)));
+  };
+  const C* K = (const C*)p.kc;
+  const C* V = (const C*)p.vc;
+
+  int koff[KSTEPS];
+#pragma unroll
+  for (int kk = 0; kk < KSTEPS; ++kk) koff[kk] = swz_off<DP>(l32, 16 * kk + 8 * hh) * 2;
+  const int tr_row = 4 * hh + ((lane & 15) >> 2);
+  const int tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  int voff[DT][2];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) {
+    voff[dt][0] = swz_off<DP>(tr_row, 32 * dt + tr_col) * 2;
+    voff[dt][1] = swz_off<DP>(tr_row + 8, 32 * dt + tr_col) * 2;
+  }
+
+  f32x16 acc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
+  float m_run = -1e30f, l_run = 0.f, l_lse = 0.f;
+  const float kTileSumMax = __builtin_exp2f(kWideMaxLog2P<T>);
+
+  // LDS operand reads run this many MFMAs ahead of the one that takes them.
+  constexpr int kReadAhead = 4;
+  auto scores = [&](int buf, f32x16* s) {
+    const LDS_AS char* Ks = smem + buf * TILE * 2;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) s[kb] = f32x16{};
+#pragma unroll
+    for (int kk = 0; kk < KSTEPS; ++kk)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const X8 a = *(const LDS_AS X8*)(Ks + kb * 32 * DP * 2 + koff[kk]);
+        s[kb] = mfma32(a, qreg[kk], s[kb]);
+      }
+    constexpr int NM = KSTEPS * KB;
+#pragma unroll
+    for (int i = 0; i < kReadAhead; ++i) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+#pragma unroll
+    for (int j = 0; j < NM; ++j) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (j + kReadAhead < NM) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+  };
+  auto mask = [&](int t, f32x16* s) {
+    const int key0 = key_of(t);
+    if (!(key0 + BN - 1 <= whi_min && (key0 >= wlo_max || key0 + BN - 1 < sinks))) {
+      asm volatile("" ::: "memory");  // stays a branch
+      const int up = hi - key0 - 4 * hh, dn = lo - key0 - 4 * hh, sk = sinks - key0 - 4 * hh;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int k = 32 * kb + 8 * (i >> 2) + (i & 3);
+          s[kb][i] = k <= up && (k >= dn || k < sk) ? s[kb][i] : -INFINITY;
+        }
+    }
+  };
+  auto sees = [&](int t) -> bool {
+    const int key0 = key_of(t);
+    return key0 <= whi_max && (key0 + BN - 1 >= wlo_min || key0 < sinks);
+  };
+  auto row_max = [&](const f32x16* s) -> float {
+    float mx = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+    mx = half_max(mx);
+    return mx == -INFINITY ? -INFINITY : mx * sl2;
+  };
+  // Exponentials with the current offset, rounded into the PV operands; x: the
+  // lane's part of the sum that normalises O (bf16: of the rounded p, so that
+  // the weights sum to one exactly; fp16: of the fp32 p), y: of the fp32 p.
+  auto softmax = [&](const f32x16* s, X8* pb) -> float2 {
+    constexpr bool kF16 = sizeof(T) == 2 && __is_same(T, _Float16);
+    const float neg_m = -m_run;
+    float rs[4] = {-0.f, -0.f, -0.f, -0.f}, re[4] = {-0.f, -0.f, -0.f, -0.f};
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      f32x16 e;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        e[i] = fast_exp2(fmaf(s[kb][i], sl2, neg_m));
+        if constexpr (LSE || kF16) re[i & 3] += e[i];
+      }
+      pb[2 * kb] = pack8<T>(e, 0);
+      pb[2 * kb + 1] = pack8<T>(e, 8);
+      if constexpr (!kF16) {
+        sum8_into(pb[2 * kb], rs);
+        sum8_into(pb[2 * kb + 1], rs);
+      }
+    }
+    float2 x;
+    x.y = (LSE || kF16) ? (re[0] + re[1]) + (re[2] + re[3]) : 0.f;
+    x.x = kF16 ? x.y : (rs[0] + rs[1]) + (rs[2] + rs[3]);
+    return x;
+  };
+  // The offset of a row is its first tile's maximum and rises only where p would
+  // come near the operands' range: then the tile's exponentials are taken again.
+  auto softmax_checked = [&](const f32x16* s, X8* pb) {
+    float2 ts = softmax(s, pb);
+    if (__builtin_amdgcn_ballot_w64(ts.x > kTileSumMax) != 0) {
+      const float mx = row_max(s);
+      if (__builtin_amdgcn_ballot_w64(mx > m_run) != 0) {
+        const float m_new = fmaxf(m_run, mx);
+        const float alpha = fast_exp2(m_run - m_new);
+        l_run *= alpha;
+        if constexpr (LSE) l_lse *= alpha;
+        m_run = m_new;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
+      }
+      ts = softmax(s, pb);
+    }
+    l_run += ts.x;
+    if constexpr (LSE) l_lse += ts.y;
+  };
+  auto pv = [&](int buf, const X8* pb) {
+    const LDS_AS char* Vs = smem + buf * TILE * 2;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int ks = 0; ks < 2 * KB; ++ks) {
+        const LDS_AS char* base = Vs + ks * 16 * DP * 2;
+        const X8 a = cat4<X8, X4>(lds_read_tr((const LDS_AS T*)(base + voff[dt][0])),
+                                  lds_read_tr((const LDS_AS T*)(base + voff[dt][1])));
+        acc[dt] = mfma32(a, pb[ks], acc[dt]);
+      }
+    constexpr int NM = DT * 2 * KB;
+#pragma unroll
+    for (int i = 0; i < kReadAhead; ++i) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+    for (int j = 0; j < NM; ++j) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (j + kReadAhead < NM) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+  };
+
+  // K of tile t lies in buffer t & 1, V in 2 + (t & 1) (counted from t_lo on).
+  // Step t needs K(t + 1), V(t) and scores(t); it brings K(t + 2) and V(t + 1) to LDS.
+  Codes kc, vc;
+  int b1 = block_at(t_lo + 1), b2 = block_at(t_lo + 2), b3 = block_at(t_lo + 3);
+  {
+    const int bl = block_at(t_lo);
+    if constexpr (Q8) {
+      Codes k1;
+      load_codes(kc, K, p.skb, p.sks, p.skh, t_lo, bl, 0);
+      load_codes(k1, K, p.skb, p.sks, p.skh, t_lo + 1, b1, 0);
+      load_codes(vc, V, p.svb, p.svs, p.svh, t_lo, bl, 1);
+      write_codes(kc, 0);
+      load_codes(kc, K, p.skb, p.sks, p.skh, t_lo + 2, b2, 0);
+      write_codes(k1, 1);
+      write_codes(vc, 2);
+      load_codes(vc, V, p.svb, p.svs, p.svh, t_lo + 1, b1, 1);
+    } else {
+      load_direct(K, p.skb, p.sks, p.skh, t_lo, bl, 0);
+      load_direct(K, p.skb, p.sks, p.skh, t_lo + 1, b1, 1);
+      load_direct(V, p.svb, p.svs, p.svh, t_lo, bl, 2);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+  }
+  __syncthreads();
+  f32x16 s0[KB], s1[KB];
+  if (t_lo < t_hi && sees(t_lo)) {
+    scores(0, s0);
+    mask(t_lo, s0);
+    m_run = fmaxf(row_max(s0), -1e30f);
+  }
+  __syncthreads();  // K buffer 0 is refilled by the first step
+  auto step = [&](int t, int par, f32x16* cur, f32x16* nxt) {
+    if constexpr (Q8) {
+      write_codes(kc, par);
+      write_codes(vc, 2 + (par ^ 1));
+      load_codes(kc, K, p.skb, p.sks, p.skh, t + 3, b3, 0);
+      load_codes(vc, V, p.svb, p.svs, p.svh, t + 2, b2, 1);
+    } else {
+      load_direct(K, p.skb, p.sks, p.skh, t + 2, b2, par);
+      load_direct(V, p.svb, p.svs, p.svh, t + 1, b1, 2 + (par ^ 1));
+    }
+    if (t + 1 < t_hi && sees(t + 1)) {
+      scores(par ^ 1, nxt);
+      mask(t + 1, nxt);
+    }
+    if (sees(t)) {
+      X8 pb[2 * KB];
+      softmax_checked(cur, pb);
+      pv(2 + par, pb);
+    }
+    if constexpr (!Q8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    b1 = b2, b2 = b3, b3 = block_at(t + 4);
+    __syncthreads();
+  };
+  int t = t_lo;
+  for (; t + 1 < t_hi; t += 2) {
+    step(t, 0, s0, s1);
+    step(t + 1, 1, s1, s0);
+  }
+  if (t < t_hi) step(t, 0, s0, s1);
+
+  const float lt = half_sum(l_run), le = half_sum(l_lse);
+  if constexpr (SPLIT) {
+    if (!whole_item) {
+      float* part = p.part + ((int64_t)blockIdx.x * p.splits + blockIdx.y) * kWidePart<BM, DP>;
+      if (hh == 0) *(f32x4*)(part + (wave * 32 + l32) * 4) = f32x4{m_run, lt, le, 0.f};
+      f32x4* po = (f32x4*)(part + BM * 4) + wave * DT * 4 * 64 + lane;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          po[(dt * 4 + g) * 64] = f32x4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+      return;
+    }
+  }
+  // O leaves through LDS (the tiles' buffers are free after the last barrier):
+  // each wave stages its 32 rows and stores whole ones.
+  const float inv = lt == 0.f ? 0.f : 1.f / lt;
+  {
+    constexpr int BLK = 32 * DP * 2;
+    static_assert(NW * BLK <= 4 * TILE * 2, "O staging fits in the K/V buffers");
+    LDS_AS char* wb = smem + wave * BLK;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        X4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (T)(acc[dt][4 * g + e] * inv);
+        *(LDS_AS X4*)(wb + swz_off<DP>(l32, 32 * dt + 8 * g + 4 * hh) * 2) = v;
+      }
+#pragma unroll
+    for (int c = 0; c < BLK / 1024; ++c) {
+      const int byte = c * 1024 + lane * 16;
+      const int row = byte / (DP * 2), seg = (byte % (DP * 2)) / 16;
+      const X8 v = *(const LDS_AS X8*)(wb + row * DP * 2 + ((seg ^ seg_swz<DP>(row)) << 4));
+      const int rr = r0 + row, tk = rr / G, h = head * G + (rr - tk * G);
+      if (rr < nrows && seg * 8 < p.D) *(X8*)((T*)p.o + (tok0 + tk) * p.sot + (int64_t)h * p.soh + seg * 8) = v;
+    }
+  }
+  if constexpr (LSE) {
+    if (row_ok && hh == 0 && p.lse != nullptr)
+      p.lse[(tok0 + tok) * p.slt + (int64_t)hq * p.slh] = le == 0.f ? -INFINITY : (m_run + __log2f(le)) * kWinLn2;
+  }
+}
+
+// Merges the key splits of fa_window_wide_kernel<..., SPLIT>: workgroup (item,
+// dt) combines 32 channels of the item's rows in the accumulators' order.
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void fa_window_wide_combine_kernel(const WindowParams p) {
+  using X4 = typename VecT<T>::x4;
+  constexpr int BM = NW * 32, DT = DP / 32;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, dt = blockIdx.y;
+  const int l32 = lane & 31, hh = lane >> 5, G = p.Hq / p.Hkv;
+  const int head = ranked_head(blockIdx.x % p.Hkv, p.Hkv);
+  int b, rt;
+  if (!wide_item<BM>(p, blockIdx.x / p.Hkv, lane, b, rt)) return;
+  const KeyTiles kt = key_tiles(p, b);
+  const int count = wide_span<BM>(p, kt, rt).count, share = split_share(count, p.splits);
+  if (count <= share) return;  // already in o
+  const int n = (count + share - 1) / share;
+  const int r = rt * BM + wave * 32 + l32, nrows = min(kt.n, p.max_n) * G;
+  float M = -1e30f, L = 0.f, E = 0.f;
+  f32x4 O[4] = {};
+  for (int i = 0; i < n; ++i) {
+    const float* part = p.part + ((int64_t)blockIdx.x * p.splits + i) * kWidePart<BM, DP>;
+    const f32x4 st = *(const f32x4*)(part + (wave * 32 + l32) * 4);
+    const f32x4* po = (const f32x4*)(part + BM * 4) + (wave * DT + dt) * 4 * 64 + lane;
+    const float m = fmaxf(M, st[0]), a = fast_exp2(M - m), w = fast_exp2(st[0] - m);
+    L = a * L + w * st[1];
+    E = a * E + w * st[2];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) O[g] = a * O[g] + w * po[g * 64];
+    M = m;
+  }
+  if (r >= nrows) return;
+  const int tok = r / G, hq = head * G + (r - tok * G);
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  T* o = (T*)p.o + ((int64_t)kt.tok0 + tok) * p.sot + (int64_t)hq * p.soh;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int d = 32 * dt + 8 * g + 4 * hh;
+    X4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (T)(O[g][e] * inv);
+    if (d < p.D) *(X4*)(o + d) = v;
+  }
+  if (dt == 0 && hh == 0 && p.lse != nullptr)
+    p.lse[((int64_t)kt.tok0 + tok) * p.slt + (int64_t)hq * p.slh] = E == 0.f ? -INFINITY : (M + __log2f(E)) * kWinLn2;
+}
+
+// ------------------------------------------------------------------- launches
+// How a launch goes, from what the host knows (sizes and bounds, not lengths).
+WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int max_n, long long max_keys, int window, int sinks) {
+  WindowPlan w = {};
+  const int dp = D <= 64 ? 64 : 128;
+  const long long rows = (long long)max_n * G;
+  const long long seen = window > 0 ? std::min(max_keys, (long long)window + max_n + sinks + 96) : max_keys;
+  if (rows <= kNarrowRows) {
+    const long long tiles = (rows + kRowTile - 1) / kRowTile * Hkv;
+    const long long most = std::max(1LL, ((seen + 31) / 32 * B + 3) / 4);
+    w.runs = (int)std::min(std::max(1LL, 1024 / tiles), most);
+    if (w.runs > 1) w.part_bytes = (uint64_t)tiles * 2 * w.runs * kRowTile * (dp + 4) * 4;
+    return w;
+  }
+  auto items = [&](int bm) {
+    return Hkv * std::min((long long)tokens * G / bm + B, (rows + bm - 1) / bm * B);
+  };
+  w.waves = items(256) >= 256 ? 8 : 4;
+  w.items = (int)items(w.waves * 32);
+  w.splits = 1;
+  if (w.waves == 4) {
+    const long long tiles = (std::min(seen, (long long)(window > 0 ? window + sinks + 32 * 4 / G + 128 : seen)) + 63) / 64;
+    w.splits = (int)std::max(1LL, std::min(512 / std::max(1, w.items), (int)(tiles / kSplitLeast)) * 1LL);
+    if (w.splits > 1) w.part_bytes = (uint64_t)w.items * w.splits * (128 * 4 + 128 * dp) * 4;
+  }
+  return w;
+}
+
 template <typename T, typename C, int DP>
 static hipError_t launch_narrow(const WindowParams& p, hipStream_t s) {
   const int G = p.Hq / p.Hkv, tiles = (p.max_n * G + kRowTile - 1) / kRowTile;
@@ -450,30 +984,39 @@ static hipError_t launch_narrow(const WindowParams& p, hipStream_t s) {
   hipLaunchKernelGGL((fa_window_combine_kernel<T, DP>), dim3(p.Hkv * tiles, p.B), dim3(256), 0, s, p);
   return hipGetLastError();
 }
+template <typename T, typename C, int DP>
+static hipError_t launch_wide(const WindowParams& p, const WindowPlan& w, hipStream_t s) {
+  if (w.splits > 1) {
+    hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 4, true, true>), dim3(w.items, w.splits), dim3(256), 0, s, p);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((fa_window_wide_combine_kernel<T, DP, 4>), dim3(w.items, DP / 32), dim3(256), 0, s, p);
+    return hipGetLastError();
+  }
+  if (w.waves == 8) {
+    if (p.lse != nullptr) hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 8, true, false>), dim3(w.items), dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 8, false, false>), dim3(w.items), dim3(512), 0, s, p);
+  } else {
+    if (p.lse != nullptr) hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 4, true, false>), dim3(w.items), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 4, false, false>), dim3(w.items), dim3(256), 0, s, p);
+  }
+  return hipGetLastError();
+}
+template <typename T, typename C, int DP>
+static hipError_t launch_window(const WindowParams& p, const WindowPlan& w, hipStream_t s) {
+  return w.items > 0 ? launch_wide<T, C, DP>(p, w, s) : launch_narrow<T, C, DP>(p, s);
+}
 template <typename T>
-static hipError_t dispatch_narrow(const WindowParams& p, hipStream_t s) {
-  if (p.scales != nullptr) return p.D <= 64 ? launch_narrow<T, uint8_t, 64>(p, s) : launch_narrow<T, uint8_t, 128>(p, s);
-  return p.D <= 64 ? launch_narrow<T, T, 64>(p, s) : launch_narrow<T, T, 128>(p, s);
-}
-
-// Runs that the key tiles of a launch are shared out over (per KV head and row
-// tile): as many as fill the GPU, no more than there can be for the longest
-// sequences.
-int window_runs(int B, int Hkv, int G, int max_n, long long max_keys) {
-  const long long tiles = (long long)Hkv * (((long long)max_n * G + kRowTile - 1) / kRowTile);
-  const long long fill = std::max(1LL, 1024 / std::max(1LL, tiles));
-  const long long most = std::max(1LL, ((max_keys + 31) / 32 * B + 3) / 4);
-  return (int)std::min(std::max(fill, std::min<long long>(B, 64)), most);
-}
-uint64_t window_part_bytes(int B, int Hkv, int G, int max_n, int D, int runs) {
-  if (runs <= 1) return 0;
-  const uint64_t tiles = (uint64_t)Hkv * (((uint64_t)max_n * G + kRowTile - 1) / kRowTile);
-  return tiles * 2 * runs * kRowTile * ((D <= 64 ? 64 : 128) + 4) * 4;
+static hipError_t dispatch_window(const WindowParams& p, const WindowPlan& w, hipStream_t s) {
+  if (p.scales != nullptr) return p.D <= 64 ? launch_window<T, uint8_t, 64>(p, w, s) : launch_window<T, uint8_t, 128>(p, w, s);
+  return p.D <= 64 ? launch_window<T, T, 64>(p, w, s) : launch_window<T, T, 128>(p, w, s);
 }
 
 // Host entry used by the C ABI layer (arguments already validated).
-hipError_t window_attention(const WindowParams& p, bool is_bf16, hipStream_t s) {
-  return is_bf16 ? dispatch_narrow<__bf16>(p, s) : dispatch_narrow<_Float16>(p, s);
+hipError_t window_attention(WindowParams p, const WindowPlan& w, bool is_bf16, hipStream_t s) {
+  p.runs = w.runs;
+  p.splits = w.splits;
+  return is_bf16 ? dispatch_window<__bf16>(p, w, s) : dispatch_window<_Float16>(p, w, s);
 }
 
 }  // namespace lsfa
