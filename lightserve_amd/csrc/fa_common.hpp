@@ -518,8 +518,8 @@ __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t rs, int voff) {
 __device__ __forceinline__ u32x2 load8b(__amdgpu_buffer_rsrc_t rs, int voff) {
   return __builtin_amdgcn_raw_buffer_load_b64(rs, voff, 0, 0);
 }
-__device__ __forceinline__ uint32_t load1(__amdgpu_buffer_rsrc_t rs, int voff) {
-  return (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rs, voff, 0, 0);
+__device__ __forceinline__ uint32_t load2(__amdgpu_buffer_rsrc_t rs, int voff) {
+  return (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rs, voff, 0, 0);
 }
 template <int W>
 __device__ __forceinline__ void load_words(__amdgpu_buffer_rsrc_t rs, int voff, uint32_t (&w)[W]) {

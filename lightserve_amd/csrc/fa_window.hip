@@ -605,20 +605,15 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
     return t < t_hi && key < seq ? table[key >> p.block_shift] : -1;
   };
 
-  // Loads. Lane offsets within the wave's RPW rows of a tile; 8-bit: row l / LPR,
-  // elements 8 (l % LPR) .. + 7; 16-bit: what the direct load's linear LDS order
-  // makes of the swizzled tile.
-  int krow[NL], kcol[NL];
-#pragma unroll
-  for (int i = 0; i < NL; ++i) {
-    krow[i] = i * RPL + lane / LPR;
-    const int seg = Q8 ? lane % LPR : (lane % LPR) ^ seg_swz<DP>(RPW * wave + krow[i]);
-    kcol[i] = 8 * seg;
-  }
+  // Loads of the wave's RPW rows of a tile, 8 elements a lane. 8-bit: row (l / LPR)
+  // NL + i in instruction i, so that a lane's rows have adjacent scales; 16-bit: what
+  // the direct load's linear LDS order makes of the swizzled tile.
+  auto row_at = [&](int i) -> int { return Q8 ? lane / LPR * NL + i : i * RPL + lane / LPR; };
   auto offset = [&](int i, int64_t stride, int key0) -> int {
-    const int key = key0 + RPW * wave + krow[i];
-    const bool used = kcol[i] < p.D && key <= hi_max && (key >= lo_min || key < sinks);
-    return used ? (krow[i] * (int)stride + kcol[i]) * EB : (int)0x80000000;
+    const int row = row_at(i), key = key0 + RPW * wave + row;
+    const int col = 8 * (Q8 ? lane % LPR : (lane % LPR) ^ seg_swz<DP>(RPW * wave + row));
+    const bool used = col < p.D && key <= hi_max && (key >= lo_min || key < sinks);
+    return used ? (row * (int)stride + col) * EB : (int)0x80000000;
   };
   auto rows_of = [&](const C* base, int64_t sb, int64_t ss, int64_t sh, int t, int blk) -> __amdgpu_buffer_rsrc_t {
     const bool live = (unsigned)blk < (unsigned)p.num_blocks;
@@ -626,30 +621,35 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
     return tile_rsrc(base + (live ? (int64_t)blk * sb + (int64_t)slot * ss + (int64_t)head * sh : 0),
                      live ? (int)(((RPW - 1) * ss + p.D) * EB) : 0);
   };
+  constexpr int EW = NL == 4 ? 2 : 1;  // words of a lane's scales (K and V of NL rows)
   struct Codes {
     u32x2 w[NL];
-    uint32_t e[NL];
+    uint32_t e[EW];
   };
-  auto load_codes = [&](Codes& c, const C* base, int64_t sb, int64_t ss, int64_t sh, int t, int blk, int which) {
+  auto load_codes = [&](Codes& c, const C* base, int64_t sb, int64_t ss, int64_t sh, int t, int blk) {
     const __amdgpu_buffer_rsrc_t rs = rows_of(base, sb, ss, sh, t, blk);
     const bool live = (unsigned)blk < (unsigned)p.num_blocks;
     const int slot = (key_of(t) + RPW * wave) & ((1 << p.block_shift) - 1);
     const uint8_t* sb8 = p.scales + (live ? ((((int64_t)blk * p.Hkv + head) << p.block_shift) + slot) * 2 : 0);
     const __amdgpu_buffer_rsrc_t es = tile_rsrc(sb8, live ? 2 * RPW : 0);
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int vo = offset(i, ss, key_of(t));
-      c.w[i] = load8b(rs, vo);
-      c.e[i] = load1(es, vo < 0 ? vo : 2 * krow[i] + which);
-    }
+    for (int i = 0; i < NL; ++i) c.w[i] = load8b(rs, offset(i, ss, key_of(t)));
+    if constexpr (NL == 1) c.e[0] = load2(es, 2 * row_at(0));
+    else load_words<EW>(es, 2 * row_at(0), c.e);
   };
-  auto write_codes = [&](const Codes& c, int buf) {
+  // (A row that no query sees has codes of zero here, but its scale may be anything:
+  // infinity, which 255 stands for, would make NaN of them.)
+  int woff = swz_off<DP>(RPW * wave + row_at(0), 8 * (lane % LPR)) * 2;
+  auto write_codes = [&](const Codes& c, int buf, int which) {
+    asm volatile("" : "+v"(woff));
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const float s = __uint_as_float(c.e[i] << 23);
+      const uint32_t e = c.e[i / 2] >> (16 * (i & 1) + 8 * which) << 23;
+      const float s = fminf(__uint_as_float(e & 0x7f800000u), 0x1p127f);
       const u32x4 v = {codes2<false>(c.w[i][0], s, T()), codes2<true>(c.w[i][0], s, T()), codes2<false>(c.w[i][1], s, T()),
                        codes2<true>(c.w[i][1], s, T())};
-      *(LDS_AS u32x4*)(smem + buf * TILE * 2 + swz_off<DP>(RPW * wave + krow[i], kcol[i]) * 2) = v;
+      // row + i: the row and its swizzle (swz_off) differ from the first one's in whole bits
+      *(LDS_AS u32x4*)(smem + buf * TILE * 2 + (woff ^ (i * (DP == 128 ? 0x140 : 0x80)))) = v;
     }
   };
   auto load_direct = [&](const C* base, int64_t sb, int64_t ss, int64_t sh, int t, int blk, int buf) {
@@ -661,17 +661,14 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
   const C* K = (const C*)p.kc;
   const C* V = (const C*)p.vc;
 
-  int koff[KSTEPS];
-#pragma unroll
-  for (int kk = 0; kk < KSTEPS; ++kk) koff[kk] = swz_off<DP>(l32, 16 * kk + 8 * hh) * 2;
+  // LDS offsets of the operands: the segment index of a column step differs from
+  // the first one's by an xor of whole bits (swz_off), so one register each does
+  // for all of them; taken through an empty asm in every step, or the compiler
+  // hoists all 14 results out of the loop and spills.
+  int koff = swz_off<DP>(l32, 8 * hh) * 2;
   const int tr_row = 4 * hh + ((lane & 15) >> 2);
   const int tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-  int voff[DT][2];
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) {
-    voff[dt][0] = swz_off<DP>(tr_row, 32 * dt + tr_col) * 2;
-    voff[dt][1] = swz_off<DP>(tr_row + 8, 32 * dt + tr_col) * 2;
-  }
+  int voff0 = swz_off<DP>(tr_row, tr_col) * 2, voff1 = swz_off<DP>(tr_row + 8, tr_col) * 2;
 
   f32x16 acc[DT];
 #pragma unroll
@@ -683,13 +680,14 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
   constexpr int kReadAhead = 4;
   auto scores = [&](int buf, f32x16* s) {
     const LDS_AS char* Ks = smem + buf * TILE * 2;
+    asm volatile("" : "+v"(koff));
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) s[kb] = f32x16{};
 #pragma unroll
     for (int kk = 0; kk < KSTEPS; ++kk)
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
-        const X8 a = *(const LDS_AS X8*)(Ks + kb * 32 * DP * 2 + koff[kk]);
+        const X8 a = *(const LDS_AS X8*)(Ks + kb * 32 * DP * 2 + (koff ^ (kk << 5)));
         s[kb] = mfma32(a, qreg[kk], s[kb]);
       }
     constexpr int NM = KSTEPS * KB;
@@ -777,13 +775,14 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
   };
   auto pv = [&](int buf, const X8* pb) {
     const LDS_AS char* Vs = smem + buf * TILE * 2;
+    asm volatile("" : "+v"(voff0), "+v"(voff1));
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int ks = 0; ks < 2 * KB; ++ks) {
         const LDS_AS char* base = Vs + ks * 16 * DP * 2;
-        const X8 a = cat4<X8, X4>(lds_read_tr((const LDS_AS T*)(base + voff[dt][0])),
-                                  lds_read_tr((const LDS_AS T*)(base + voff[dt][1])));
+        const X8 a = cat4<X8, X4>(lds_read_tr((const LDS_AS T*)(base + (voff0 ^ (dt << 6)))),
+                                  lds_read_tr((const LDS_AS T*)(base + (voff1 ^ (dt << 6)))));
         acc[dt] = mfma32(a, pb[ks], acc[dt]);
       }
     constexpr int NM = DT * 2 * KB;
@@ -804,14 +803,14 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
     const int bl = block_at(t_lo);
     if constexpr (Q8) {
       Codes k1;
-      load_codes(kc, K, p.skb, p.sks, p.skh, t_lo, bl, 0);
-      load_codes(k1, K, p.skb, p.sks, p.skh, t_lo + 1, b1, 0);
-      load_codes(vc, V, p.svb, p.svs, p.svh, t_lo, bl, 1);
-      write_codes(kc, 0);
-      load_codes(kc, K, p.skb, p.sks, p.skh, t_lo + 2, b2, 0);
-      write_codes(k1, 1);
-      write_codes(vc, 2);
-      load_codes(vc, V, p.svb, p.svs, p.svh, t_lo + 1, b1, 1);
+      load_codes(kc, K, p.skb, p.sks, p.skh, t_lo, bl);
+      load_codes(k1, K, p.skb, p.sks, p.skh, t_lo + 1, b1);
+      load_codes(vc, V, p.svb, p.svs, p.svh, t_lo, bl);
+      write_codes(kc, 0, 0);
+      load_codes(kc, K, p.skb, p.sks, p.skh, t_lo + 2, b2);
+      write_codes(k1, 1, 0);
+      write_codes(vc, 2, 1);
+      load_codes(vc, V, p.svb, p.svs, p.svh, t_lo + 1, b1);
     } else {
       load_direct(K, p.skb, p.sks, p.skh, t_lo, bl, 0);
       load_direct(K, p.skb, p.sks, p.skh, t_lo + 1, b1, 1);
@@ -829,10 +828,10 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
   __syncthreads();  // K buffer 0 is refilled by the first step
   auto step = [&](int t, int par, f32x16* cur, f32x16* nxt) {
     if constexpr (Q8) {
-      write_codes(kc, par);
-      write_codes(vc, 2 + (par ^ 1));
-      load_codes(kc, K, p.skb, p.sks, p.skh, t + 3, b3, 0);
-      load_codes(vc, V, p.svb, p.svs, p.svh, t + 2, b2, 1);
+      write_codes(kc, par, 0);
+      write_codes(vc, 2 + (par ^ 1), 1);
+      load_codes(kc, K, p.skb, p.sks, p.skh, t + 3, b3);
+      load_codes(vc, V, p.svb, p.svs, p.svh, t + 2, b2);
     } else {
       load_direct(K, p.skb, p.sks, p.skh, t + 2, b2, par);
       load_direct(V, p.svb, p.svs, p.svh, t + 1, b1, 2 + (par ^ 1));
