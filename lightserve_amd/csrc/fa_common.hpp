@@ -372,7 +372,7 @@ struct WindowParams {
   float scale_abs;         // |scale_log2|, at least 1e-30
 };
 struct WindowPlan {
-  int runs;             // narrow kernel: runs that the key tiles are shared out over
+  int runs, columns;    // narrow kernel: runs that the key tiles are shared out over, column blocks of 16 rows
   int items, waves;     // wide kernel (items > 0): row tiles at most, waves of a workgroup
   int splits;           // workgroups that an item's key tiles are shared out over
   uint64_t part_bytes;  // partial results

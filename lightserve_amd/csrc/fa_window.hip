@@ -10,7 +10,7 @@
 // Many: the wide one, further down.
 // The path is bound by HBM, so it is built around bytes in flight, and each
 // byte of the cache is read once for all query heads that share it:
-//   rows       (token, query head of the KV head's group) pairs, 16 to a row
+//   rows       (token, query head of the KV head's group) pairs, 16 or 32 to a row
 //              tile, are the columns of S^T = K Q^T and of O^T += V^T P^T on
 //              v_mfma_f32_16x16x32.
 //   key tiles  of 32 keys: two pieces of 16 that each lie in one cache block,
@@ -105,15 +105,33 @@ __device__ __forceinline__ int run_tiles(const WindowParams& p, int all) {
   return max((all + p.runs - 1) / p.runs, 4);
 }
 
-constexpr int kRowTile = 16;
-constexpr int kNarrowRows = 16;  // most rows of a sequence and KV head in the narrow kernel
+// Channels d .. d + 3 of row r of a sequence and KV head from the sums over its keys
+// (offset M in log2 units), and its lse with channel 0.
+template <typename T>
+__device__ __forceinline__ void store_row(const WindowParams& p, int64_t tok0, int r, int G, int head, int d, float M, float L,
+                                          float E, const f32x4& O) {
+  const int tok = r / G, h = head * G + (r - tok * G);
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  if (d < p.D) {
+    typename VecT<T>::x4 out;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = (T)(O[e] * inv);
+    *(typename VecT<T>::x4*)((T*)p.o + (tok0 + tok) * p.sot + (int64_t)h * p.soh + d) = out;
+  }
+  if (d == 0 && p.lse != nullptr)
+    p.lse[(tok0 + tok) * p.slt + (int64_t)h * p.slh] = E == 0.f ? -INFINITY : (M + __log2f(E)) * kWinLn2;
+}
 
-template <typename T, typename C, int DP>
+constexpr int kRowTile = 16;  // rows of a column block; a row tile has one or two
+
+// NC column blocks of 16 rows share the tile's K and V operands.
+template <typename T, typename C, int DP, int NC>
 __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowParams p) {
   using X8 = typename VecT<T>::x8;
   constexpr bool Q8 = sizeof(C) == 1;
   constexpr int EB = sizeof(C);           // bytes of a cached element
   constexpr int NW = 4;
+  constexpr int RT = kRowTile * NC;       // rows of a row tile
   constexpr int KK = DP / 32;             // MFMAs of S per 16 keys
   constexpr int KD = DP * EB / 64;        // 16-byte loads of K per lane and piece
   constexpr int VJ = DP / 16;             // channels per lane, MFMAs of O
@@ -121,7 +139,7 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
   constexpr float kThreshold = 8.0f;      // log2 units
 
   __shared__ float st_o[NW][kRowTile][DP];
-  __shared__ float st_m[NW][kRowTile], st_l[NW][kRowTile], st_e[NW][kRowTile];
+  __shared__ float st_m[NW][RT], st_l[NW][RT], st_e[NW][RT];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -158,6 +176,7 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
   const uint32_t vo = c * VJ < p.D ? (uint32_t)(4 * g * (int)p.svs * EB + c * VJ * EB) : kOut;
   const uint32_t vstep = vo == kOut ? 0 : (uint32_t)((int)p.svs * EB);
   const int kbytes = (15 * (int)p.sks + p.D) * EB, vbytes = (15 * (int)p.svs + p.D) * EB;
+  const int sinks = p.window > 0 ? p.sinks : 0;
 
   for (; b < p.B && at < end; ++b) {
     const KeyTiles kt = key_tiles(p, b);
@@ -167,44 +186,53 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
     const int sink = __builtin_amdgcn_readfirstlane(kt.sink), first = __builtin_amdgcn_readfirstlane(kt.first);
     const int ta = max(start - at, 0), tb = min(count, end - at);
     at += count;
-    const int nrows = n * G - rt * kRowTile;  // of this row tile
+    const int nrows = n * G - rt * RT;  // of this row tile
     if (nrows <= 0) continue;
     const int64_t tok0 = __builtin_amdgcn_readfirstlane(kt.tok0);
 
-    // The lane's row, and the keys that it sees.
-    const int r = rt * kRowTile + c, tok = r / G, hq = head * G + (r - tok * G);
-    const bool row_ok = c < nrows;
-    const int pos = p.causal ? seq - n + tok : seq - 1;
-    const int hi = row_ok ? pos : -1, lo = p.window > 0 ? pos - p.window + 1 : 0;
-    // The same of the tile's first and last rows.
-    const int t0 = rt * kRowTile / G, t1 = (rt * kRowTile + min(nrows, kRowTile) - 1) / G;
-    const int hi_min = p.causal ? seq - n + t0 : seq - 1, hi_max = p.causal ? seq - n + t1 : seq - 1;
-    const int lo_min = p.window > 0 ? hi_min - p.window + 1 : 0, lo_max = p.window > 0 ? hi_max - p.window + 1 : 0;
-    const int sinks = p.window > 0 ? p.sinks : 0;
-
-    // Q as the B operand of S^T: elements g D/4 + 8 kk .. + 7 of row c.
-    X8 qr[KK];
+    // The lane's rows, and the keys that they see.
+    int hi[NC], lo[NC];
+    X8 qr[NC][KK];  // Q as the B operand of S^T: elements g D/4 + 8 kk .. + 7 of row c
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      const int d = g * (DP / 4) + 8 * kk;
-      u32x4 raw = {0, 0, 0, 0};
-      if (row_ok && d < p.D) raw = ldg16((const T*)p.q + (tok0 + tok) * p.sqt + (int64_t)hq * p.sqh + d);
-      qr[kk] = __builtin_bit_cast(X8, raw);
+    for (int x = 0; x < NC; ++x) {
+      const int r = rt * RT + 16 * x + c, tok = r / G, hq = head * G + (r - tok * G);
+      const bool row_ok = 16 * x + c < nrows;
+      const int pos = p.causal ? seq - n + tok : seq - 1;
+      hi[x] = row_ok ? pos : -1;
+      lo[x] = p.window > 0 ? pos - p.window + 1 : 0;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const int d = g * (DP / 4) + 8 * kk;
+        u32x4 raw = {0, 0, 0, 0};
+        if (row_ok && d < p.D) raw = ldg16((const T*)p.q + (tok0 + tok) * p.sqt + (int64_t)hq * p.sqh + d);
+        qr[x][kk] = __builtin_bit_cast(X8, raw);
+      }
     }
+    // The same of the tile's first and last rows.
+    const int t0 = rt * RT / G, t1 = (rt * RT + min(nrows, RT) - 1) / G;
+    const int hi_min = __builtin_amdgcn_readfirstlane(p.causal ? seq - n + t0 : seq - 1);
+    const int hi_max = __builtin_amdgcn_readfirstlane(p.causal ? seq - n + t1 : seq - 1);
+    const int lo_min = p.window > 0 ? hi_min - p.window + 1 : 0, lo_max = p.window > 0 ? hi_max - p.window + 1 : 0;
 
+    // Of the run's tiles ta .. tb - 1 of this sequence those that the row tile sees,
+    // u = 0 .. nt - 1: n1 with sinks (numbered by their keys) from tile ta on, then
+    // those of its own window, keys from 32 (f2 + u) on.
+    const int own = sink + (max(lo_min, 0) >> 5) - first, a2 = max(ta, own);
+    const int n1 = max(min(min(tb, own), (min(sinks, seq) + 31) >> 5) - ta, 0);
+    const int nt = n1 + max(min(tb, sink + ((hi_max + 32) >> 5) - first) - a2, 0), f2 = first + a2 - sink - n1;
     const __attribute__((address_space(4))) int32_t* table =
         (const __attribute__((address_space(4))) int32_t*)(p.block_tables + (int64_t)b * p.sbt);
-    auto key_of = [&](int t) -> int { return (t < sink ? t : t - sink + first) * 32; };
-    auto block_at = [&](int t, int piece) -> int {
-      const int key = key_of(t) + 16 * piece;
-      return t < tb && key < seq ? table[key >> p.block_shift] : -1;
+    auto key_of = [&](int u) -> int { return (u < n1 ? ta + u : f2 + u) * 32; };
+    auto block_at = [&](int u, int piece) -> int {
+      const int key = key_of(u) + 16 * piece;
+      return u < nt && key < seq ? table[key >> p.block_shift] : -1;
     };
     u32x4 kr[2][KD];
     uint32_t vr[2][4][VW];
     u32x2 sc[2];
-    auto load_k = [&](int t, int blk, int piece) {
+    auto load_k = [&](int u, int blk, int piece) {
       const bool live = (unsigned)blk < (unsigned)p.num_blocks;
-      const int slot = (key_of(t) + 16 * piece) & ((1 << p.block_shift) - 1);
+      const int slot = (key_of(u) + 16 * piece) & ((1 << p.block_shift) - 1);
       const C* base = (const C*)p.kc + (live ? (int64_t)blk * p.skb + (int64_t)slot * p.sks + (int64_t)head * p.skh : 0);
       const __amdgpu_buffer_rsrc_t rs = tile_rsrc(base, live ? kbytes : 0);
 #pragma unroll
@@ -213,42 +241,47 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
         kr[piece][i] = load16(rs, (int)o);
       }
     };
-    auto load_s = [&](int t, int blk, int piece) {
+    auto load_s = [&](int u, int blk, int piece) {
       if constexpr (Q8) {
         const bool live = (unsigned)blk < (unsigned)p.num_blocks;
-        const int slot = (key_of(t) + 16 * piece) & ((1 << p.block_shift) - 1);
+        const int slot = (key_of(u) + 16 * piece) & ((1 << p.block_shift) - 1);
         const uint8_t* base = p.scales + (live ? ((((int64_t)blk * p.Hkv + head) << p.block_shift) + slot) * 2 : 0);
         sc[piece] = load8b(tile_rsrc(base, live ? 32 : 0), 8 * g);
       }
     };
-    auto load_v = [&](int t, int blk, int piece) {
+    auto load_v = [&](int u, int blk, int piece) {
       const bool live = (unsigned)blk < (unsigned)p.num_blocks;
-      const int slot = (key_of(t) + 16 * piece) & ((1 << p.block_shift) - 1);
+      const int slot = (key_of(u) + 16 * piece) & ((1 << p.block_shift) - 1);
       const C* base = (const C*)p.vc + (live ? (int64_t)blk * p.svb + (int64_t)slot * p.svs + (int64_t)head * p.svh : 0);
       const __amdgpu_buffer_rsrc_t rs = tile_rsrc(base, live ? vbytes : 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) load_words<VW>(rs, (int)(vo + i * vstep), vr[piece][i]);
     };
 
-    f32x4 acc[VJ];
-#pragma unroll
-    for (int j = 0; j < VJ; ++j) acc[j] = f32x4{};
+    f32x4 acc[NC][VJ];
     // l_run: sum of the rounded p (normalises O: the weights of the V rows then
     // sum to one exactly); l_lse: of the fp32 p (the logsumexp).
-    float m_run = -1e30f, l_run = 0.f, l_lse = 0.f;
+    float m_run[NC], l_run[NC], l_lse[NC];
+#pragma unroll
+    for (int x = 0; x < NC; ++x) {
+      m_run[x] = -1e30f, l_run[x] = 0.f, l_lse[x] = 0.f;
+#pragma unroll
+      for (int j = 0; j < VJ; ++j) acc[x][j] = f32x4{};
+    }
 
-    int t = ta + wave;
-    int b0 = block_at(t, 0), b1 = block_at(t, 1);
-    load_k(t, b0, 0), load_k(t, b1, 1);
-    load_s(t, b0, 0), load_s(t, b1, 1);
-    load_v(t, b0, 0), load_v(t, b1, 1);
-    b0 = block_at(t + NW, 0), b1 = block_at(t + NW, 1);
-    for (; t < tb; t += NW) {
-      const int tn = t + NW, key0 = key_of(t);
-      f32x4 s[2];
+    int u = wave;
+    int b0 = block_at(u, 0), b1 = block_at(u, 1);
+    load_k(u, b0, 0), load_k(u, b1, 1);
+    load_s(u, b0, 0), load_s(u, b1, 1);
+    load_v(u, b0, 0), load_v(u, b1, 1);
+    b0 = block_at(u + NW, 0), b1 = block_at(u + NW, 1);
+    for (; u < nt; u += NW) {
+      const int un = u + NW, key0 = key_of(u);
+      f32x4 s[NC][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        s[h] = f32x4{};
+#pragma unroll
+        for (int x = 0; x < NC; ++x) s[x][h] = f32x4{};
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
           u32x4 a;
@@ -258,10 +291,11 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
           } else {
             a = kr[h][kk];
           }
-          s[h] = mfma16(__builtin_bit_cast(X8, a), qr[kk], s[h]);
+#pragma unroll
+          for (int x = 0; x < NC; ++x) s[x][h] = mfma16(__builtin_bit_cast(X8, a), qr[x][kk], s[x][h]);
         }
       }
-      load_k(tn, b0, 0), load_k(tn, b1, 1);
+      load_k(un, b0, 0), load_k(un, b1, 1);
 
       // Scores in log2 units, masked to -inf where the row does not see the key.
       float vs[2][4];
@@ -269,17 +303,18 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+          float ks = p.scale_log2;
+          vs[h][i] = 1.f;
           if constexpr (Q8) {
             const uint32_t w = sc[h][i >> 1];
             const uint32_t ke = (i & 1) ? w << 7 : w << 23, ve = (i & 1) ? w >> 1 : w << 15;
-            s[h][i] *= __uint_as_float(ke & 0x7f800000u) * p.scale_log2;
+            ks *= __uint_as_float(ke & 0x7f800000u);
             vs[h][i] = __uint_as_float(ve & 0x7f800000u);
-          } else {
-            s[h][i] *= p.scale_log2;
-            vs[h][i] = 1.f;
           }
+#pragma unroll
+          for (int x = 0; x < NC; ++x) s[x][h][i] *= ks;
         }
-      load_s(tn, b0, 0), load_s(tn, b1, 1);
+      load_s(un, b0, 0), load_s(un, b1, 1);
       const bool whole = key0 + 31 <= hi_min && (key0 >= lo_max || key0 + 31 < sinks);
       if (!whole) {
 #pragma unroll
@@ -287,7 +322,9 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int key = key0 + 16 * h + 4 * g + i;
-            if (!(key <= hi && (key >= lo || key < sinks))) s[h][i] = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < NC; ++x)
+              if (!(key <= hi[x] && (key >= lo[x] || key < sinks))) s[x][h][i] = -INFINITY;
             // Rows of V that no query sees are not read as numbers (0 * NaN is NaN).
             const bool used = key <= hi_max && (key >= lo_min || key < sinks);
             if (!used) vs[h][i] = 1.f;
@@ -295,32 +332,36 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
             for (int w = 0; w < VW; ++w) vr[h][i][w] = used ? vr[h][i][w] : 0u;
           }
       }
-      float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-      mx = quarter_max(mx);
-      if (__builtin_amdgcn_ballot_w64(mx > m_run + kThreshold) != 0) {
-        const float m_new = fmaxf(m_run, mx);
-        const float alpha = fast_exp2(m_run - m_new);
-        l_run *= alpha;
-        l_lse *= alpha;
-        m_run = m_new;
+      X8 pb[NC];
 #pragma unroll
-        for (int j = 0; j < VJ; ++j) acc[j] *= alpha;
-      }
-      X8 pb;
+      for (int x = 0; x < NC; ++x) {
+        const f32x4 s0 = s[x][0], s1 = s[x][1];
+        float mx = fmaxf(fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s0[2], s0[3])), fmaxf(fmaxf(s1[0], s1[1]), fmaxf(s1[2], s1[3])));
+        mx = quarter_max(mx);
+        if (__builtin_amdgcn_ballot_w64(mx > m_run[x] + kThreshold) != 0) {
+          const float m_new = fmaxf(m_run[x], mx);
+          const float alpha = fast_exp2(m_run[x] - m_new);
+          l_run[x] *= alpha;
+          l_lse[x] *= alpha;
+          m_run[x] = m_new;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = fast_exp2(s[h][i] - m_run);
-          l_lse += e;
-          pb[4 * h + i] = (T)e;
+          for (int j = 0; j < VJ; ++j) acc[x][j] *= alpha;
         }
-      float rs[4] = {0.f, 0.f, 0.f, 0.f};
-      sum8_into(pb, rs);
-      l_run += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e = fast_exp2(s[x][h][i] - m_run[x]);
+            l_lse[x] += e;
+            pb[x][4 * h + i] = (T)e;
+          }
+        float rs[4] = {0.f, 0.f, 0.f, 0.f};
+        sum8_into(pb[x], rs);
+        l_run[x] += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+      }
 
       // Channel (D/16) c + j of the 8 keys, two keys to a word.
-      uint32_t x[2][4][VJ / 2];  // words of two adjacent channels of one key
+      uint32_t v2[2][4][VJ / 2];  // words of two adjacent channels of one key
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -328,81 +369,80 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
 #pragma unroll
           for (int w = 0; w < VJ / 2; ++w) {
             if constexpr (Q8)
-              x[h][i][w] = (w & 1) ? codes2<true>(vr[h][i][w / 2], vs[h][i], T()) : codes2<false>(vr[h][i][w / 2], vs[h][i], T());
+              v2[h][i][w] = (w & 1) ? codes2<true>(vr[h][i][w / 2], vs[h][i], T()) : codes2<false>(vr[h][i][w / 2], vs[h][i], T());
             else
-              x[h][i][w] = vr[h][i][w];
+              v2[h][i][w] = vr[h][i][w];
           }
 #pragma unroll
       for (int j = 0; j < VJ; ++j) {
         const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
         u32x4 a;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) a[k] = __builtin_amdgcn_perm(x[k / 2][2 * (k & 1) + 1][j / 2], x[k / 2][2 * (k & 1)][j / 2], sel);
-        acc[j] = mfma16(__builtin_bit_cast(X8, a), pb, acc[j]);
+        for (int k = 0; k < 4; ++k) a[k] = __builtin_amdgcn_perm(v2[k / 2][2 * (k & 1) + 1][j / 2], v2[k / 2][2 * (k & 1)][j / 2], sel);
+#pragma unroll
+        for (int x = 0; x < NC; ++x) acc[x][j] = mfma16(__builtin_bit_cast(X8, a), pb[x], acc[x][j]);
       }
-      load_v(tn, b0, 0), load_v(tn, b1, 1);
-      b0 = block_at(tn + NW, 0), b1 = block_at(tn + NW, 1);
+      load_v(un, b0, 0), load_v(un, b1, 1);
+      b0 = block_at(un + NW, 0), b1 = block_at(un + NW, 1);
     }
 
-    // Merge the waves. A wave without a tile has m = -1e30 and sums of zero.
-    const float lt = quarter_sum(l_run), le = quarter_sum(l_lse);
-    if (g == 0) {
-      st_m[wave][c] = m_run;
-      st_l[wave][c] = lt;
-      st_e[wave][c] = le;
+    // Merge the waves, a column block at a time. A wave without a tile has m = -1e30
+    // and sums of zero.
+#pragma unroll
+    for (int x = 0; x < NC; ++x) {
+      const float lt = quarter_sum(l_run[x]), le = quarter_sum(l_lse[x]);
+      if (g == 0) {
+        st_m[wave][16 * x + c] = m_run[x];
+        st_l[wave][16 * x + c] = lt;
+        st_e[wave][16 * x + c] = le;
+      }
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < VJ; ++j) st_o[wave][c][(4 * g + i) * VJ + j] = acc[j][i];
-    __syncthreads();
     const bool complete = ta == 0 && tb == count;
-    const int rows = min(nrows, kRowTile);
     const int64_t slot = (int64_t)blockIdx.x * 2 * p.runs + 2 * run + (ta == 0);
-    float* part = p.part + slot * (kRowTile * (DP + 4));
-    for (int idx = tid; idx < rows * (DP / 4); idx += 256) {
-      const int row = idx / (DP / 4), d = (idx - row * (DP / 4)) * 4;
-      float M = st_m[0][row];
+    float* part = p.part + slot * (RT * (DP + 4));
 #pragma unroll
-      for (int w = 1; w < NW; ++w) M = fmaxf(M, st_m[w][row]);
-      float L = 0.f, E = 0.f;
-      f32x4 O = {};
+    for (int x = 0; x < NC; ++x) {
 #pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const float a = fast_exp2(st_m[w][row] - M);
-        L += a * st_l[w][row];
-        E += a * st_e[w][row];
-        O += a * *(const f32x4*)&st_o[w][row][d];
-      }
-      if (complete) {
-        const int rr = rt * kRowTile + row, tk = rr / G, h = head * G + (rr - tk * G);
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        if (d < p.D) {
-          typename VecT<T>::x4 out;
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) out[e] = (T)(O[e] * inv);
-          *(typename VecT<T>::x4*)((T*)p.o + (tok0 + tk) * p.sot + (int64_t)h * p.soh + d) = out;
+        for (int j = 0; j < VJ; ++j) st_o[wave][c][(4 * g + i) * VJ + j] = acc[x][j][i];
+      __syncthreads();
+      for (int idx = tid; idx < min(nrows - 16 * x, kRowTile) * (DP / 4); idx += 256) {
+        const int row = idx / (DP / 4), d = (idx - row * (DP / 4)) * 4, rr = 16 * x + row;
+        float M = st_m[0][rr];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) M = fmaxf(M, st_m[w][rr]);
+        float L = 0.f, E = 0.f;
+        f32x4 O = {};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const float a = fast_exp2(st_m[w][rr] - M);
+          L += a * st_l[w][rr];
+          E += a * st_e[w][rr];
+          O += a * *(const f32x4*)&st_o[w][row][d];
         }
-        if (d == 0 && p.lse != nullptr)
-          p.lse[(tok0 + tk) * p.slt + (int64_t)h * p.slh] = E == 0.f ? -INFINITY : (M + __log2f(E)) * kWinLn2;
-      } else {
-        *(f32x4*)(part + row * DP + d) = O;
-        if (d == 0) *(f32x4*)(part + kRowTile * DP + 4 * row) = f32x4{M, L, E, 0.f};
+        if (complete) {
+          store_row<T>(p, tok0, rt * RT + rr, G, head, d, M, L, E, O);
+        } else {
+          *(f32x4*)(part + rr * DP + d) = O;
+          if (d == 0) *(f32x4*)(part + RT * DP + 4 * rr) = f32x4{M, L, E, 0.f};
+        }
       }
+      __syncthreads();  // the next merge reuses the arrays
     }
-    __syncthreads();  // the next sequence's merge reuses the arrays
   }
 }
 
 // Merges the partial results of a sequence's row tile that lies in several runs:
 // o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
-template <typename T, int DP>
+template <typename T, int DP, int NC>
 __global__ __launch_bounds__(256) void fa_window_combine_kernel(const WindowParams p) {
+  constexpr int RT = kRowTile * NC;
   const int tid = threadIdx.x, lane = tid & 63;
   const int head = blockIdx.x % p.Hkv, rt = blockIdx.x / p.Hkv, b = blockIdx.y;
   const int G = p.Hq / p.Hkv;
   const KeyTiles kt = key_tiles(p, b);
-  const int nrows = kt.n * G - rt * kRowTile;
+  const int nrows = kt.n * G - rt * RT;
   if (kt.count == 0 || nrows <= 0) return;
   int all = 0, at = 0;  // tiles of all sequences, tiles before b's
   for (int j = 0; j < p.B; j += 64) {
@@ -414,15 +454,14 @@ __global__ __launch_bounds__(256) void fa_window_combine_kernel(const WindowPara
   const int per = run_tiles(p, all);
   const int r0 = at / per, r1 = (at + kt.count - 1) / per;
   if (r0 == r1) return;  // already in o
-  const int64_t tok0 = kt.tok0;
-  const float* base = p.part + (int64_t)blockIdx.x * 2 * p.runs * (kRowTile * (DP + 4));
-  for (int idx = tid; idx < min(nrows, kRowTile) * (DP / 4); idx += 256) {
+  const float* base = p.part + (int64_t)blockIdx.x * 2 * p.runs * (RT * (DP + 4));
+  for (int idx = tid; idx < min(nrows, RT) * (DP / 4); idx += 256) {
     const int row = idx / (DP / 4), d = (idx - row * (DP / 4)) * 4;
     float M = -1e30f, L = 0.f, E = 0.f;
     f32x4 O = {};
     for (int r = r0; r <= r1; ++r) {
-      const float* part = base + (int64_t)(2 * r + (r == r0)) * (kRowTile * (DP + 4));
-      const f32x4 st = *(const f32x4*)(part + kRowTile * DP + 4 * row);
+      const float* part = base + (int64_t)(2 * r + (r == r0)) * (RT * (DP + 4));
+      const f32x4 st = *(const f32x4*)(part + RT * DP + 4 * row);
       const f32x4 o = *(const f32x4*)(part + row * DP + d);
       const float m = fmaxf(M, st[0]), a = fast_exp2(M - m), w = fast_exp2(st[0] - m);
       L = a * L + w * st[1];
@@ -430,16 +469,7 @@ __global__ __launch_bounds__(256) void fa_window_combine_kernel(const WindowPara
       O = a * O + w * o;
       M = m;
     }
-    const int rr = rt * kRowTile + row, tk = rr / G, h = head * G + (rr - tk * G);
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    if (d < p.D) {
-      typename VecT<T>::x4 out;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) out[e] = (T)(O[e] * inv);
-      *(typename VecT<T>::x4*)((T*)p.o + (tok0 + tk) * p.sot + (int64_t)h * p.soh + d) = out;
-    }
-    if (d == 0 && p.lse != nullptr)
-      p.lse[(tok0 + tk) * p.slt + (int64_t)h * p.slh] = E == 0.f ? -INFINITY : (M + __log2f(E)) * kWinLn2;
+    store_row<T>(p, kt.tok0, rt * RT + row, G, head, d, M, L, E, O);
   }
 }
 
@@ -947,6 +977,9 @@ __global__ __launch_bounds__(NW * 64) void fa_window_wide_combine_kernel(const W
 }
 
 // ------------------------------------------------------------------- launches
+constexpr long long kNarrowRows = 2048;  // most rows of a sequence and KV head in the narrow kernel
+constexpr long long kNarrowFill = 1024;  // its workgroups that fill the GPU, with one column block
+
 // How a launch goes, from what the host knows (sizes and bounds, not lengths).
 WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int max_n, long long max_keys, int window, int sinks) {
   WindowPlan w = {};
@@ -954,10 +987,12 @@ WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int max_n, long
   const long long rows = (long long)max_n * G;
   const long long seen = window > 0 ? std::min(max_keys, (long long)window + max_n + sinks + 96) : max_keys;
   if (rows <= kNarrowRows) {
-    const long long tiles = (rows + kRowTile - 1) / kRowTile * Hkv;
+    w.columns = rows > kRowTile ? 2 : 1;
+    const int rt = kRowTile * w.columns;
+    const long long tiles = (rows + rt - 1) / rt * Hkv;
     const long long most = std::max(1LL, ((seen + 31) / 32 * B + 3) / 4);
-    w.runs = (int)std::min(std::max(1LL, 1024 / tiles), most);
-    if (w.runs > 1) w.part_bytes = (uint64_t)tiles * 2 * w.runs * kRowTile * (dp + 4) * 4;
+    w.runs = (int)std::min(std::max({1LL, kNarrowFill / w.columns / tiles, std::min((long long)B, kNarrowFill / tiles)}), most);
+    if (w.runs > 1) w.part_bytes = (uint64_t)tiles * 2 * w.runs * rt * (dp + 4) * 4;
     return w;
   }
   auto items = [&](int bm) {
@@ -974,13 +1009,13 @@ WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int max_n, long
   return w;
 }
 
-template <typename T, typename C, int DP>
+template <typename T, typename C, int DP, int NC>
 static hipError_t launch_narrow(const WindowParams& p, hipStream_t s) {
-  const int G = p.Hq / p.Hkv, tiles = (p.max_n * G + kRowTile - 1) / kRowTile;
-  hipLaunchKernelGGL((fa_window_narrow_kernel<T, C, DP>), dim3(p.Hkv * tiles, p.runs), dim3(256), 0, s, p);
+  const int rt = kRowTile * NC, tiles = (p.max_n * (p.Hq / p.Hkv) + rt - 1) / rt;
+  hipLaunchKernelGGL((fa_window_narrow_kernel<T, C, DP, NC>), dim3(p.Hkv * tiles, p.runs), dim3(256), 0, s, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.runs == 1) return e;
-  hipLaunchKernelGGL((fa_window_combine_kernel<T, DP>), dim3(p.Hkv * tiles, p.B), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((fa_window_combine_kernel<T, DP, NC>), dim3(p.Hkv * tiles, p.B), dim3(256), 0, s, p);
   return hipGetLastError();
 }
 template <typename T, typename C, int DP>
@@ -1003,7 +1038,8 @@ static hipError_t launch_wide(const WindowParams& p, const WindowPlan& w, hipStr
 }
 template <typename T, typename C, int DP>
 static hipError_t launch_window(const WindowParams& p, const WindowPlan& w, hipStream_t s) {
-  return w.items > 0 ? launch_wide<T, C, DP>(p, w, s) : launch_narrow<T, C, DP>(p, s);
+  if (w.items > 0) return launch_wide<T, C, DP>(p, w, s);
+  return w.columns == 1 ? launch_narrow<T, C, DP, 1>(p, s) : launch_narrow<T, C, DP, 2>(p, s);
 }
 template <typename T>
 static hipError_t dispatch_window(const WindowParams& p, const WindowPlan& w, hipStream_t s) {
