@@ -507,7 +507,11 @@ typedef struct {
  * keys j <= p (all keys with causal = 0), with window > 0 only j > p - window
  * or j < sinks. Block ids outside [0, num_blocks) read as zeros. Rows of q
  * behind the last sequence are not computed. workspace:
- * lsfa_window_workspace_size() bytes, 256-byte aligned. */
+ * lsfa_window_workspace_size() bytes, 256-byte aligned (0 bytes: may be NULL);
+ * as the skinny GEMM's, its first LSFA_GEMV_COUNTER_BYTES hold int32 arrival
+ * counters that must be zero on entry and are zero again when the call is done,
+ * so calls in stream order (of either kind) can share one workspace; calls that
+ * may run at the same time need one each. */
 typedef struct {
   const void* q;
   const void* k_cache;

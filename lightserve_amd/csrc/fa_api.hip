@@ -691,6 +691,8 @@ static int check_paged(int head_dim, int dim_multiple, int block_size, int max_b
       return fail(LSFA_ERR_UNSUPPORTED, "k_cache/v_cache strides must be multiples of 16 bytes");
   if (ks[1] < 0 || ks[1] > (1LL << 22) || vs[1] < 0 || vs[1] > (1LL << 22))
     return fail(LSFA_ERR_UNSUPPORTED, "cache slot strides must lie in 0..2^22 elements");
+  if (ks[0] < 0 || ks[0] >= (1LL << 31) || vs[0] < 0 || vs[0] >= (1LL << 31))
+    return fail(LSFA_ERR_UNSUPPORTED, "cache block strides must lie in 0..2^31 - 1 elements");
   if (table_stride < max_blocks)
     return fail(LSFA_ERR_INVALID, "block_table_stride %lld is below max_blocks_per_seq %d", (long long)table_stride, max_blocks);
   return LSFA_OK;
@@ -828,7 +830,8 @@ int lsfa_window(const lsfa_window_args* a, void* stream) {
   memset(&p, 0, sizeof(p));
   p.q = a->q; p.kc = a->k_cache; p.vc = a->v_cache; p.o = a->o; p.lse = a->lse; p.scales = a->kv_scales;
   p.cu_q = a->cu_seqlens_q; p.seq_lens = a->seq_lens; p.block_tables = a->block_tables;
-  p.part = static_cast<float*>(a->workspace);
+  p.counters = static_cast<int*>(a->workspace);
+  p.part = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + LSFA_GEMV_COUNTER_BYTES);
   p.sqt = a->q_stride[0]; p.sqh = a->q_stride[1];
   p.skb = a->k_stride[0]; p.sks = a->k_stride[1]; p.skh = a->k_stride[2];
   p.svb = a->v_stride[0]; p.svs = a->v_stride[1]; p.svh = a->v_stride[2];

@@ -355,6 +355,7 @@ struct WindowParams {
   const int32_t* cu_q;    // [B + 1], or null: one query per sequence
   const int32_t* seq_lens;
   const int32_t* block_tables;
+  int* counters;          // arrivals (zero on entry and on exit), one per run
   float* part;            // partial results
   int64_t sqt, sqh;       // token, head strides
   int64_t skb, sks, skh;  // block, slot, head
@@ -375,7 +376,7 @@ struct WindowPlan {
   int runs, columns;    // narrow kernel: runs that the key tiles are shared out over, column blocks of 16 rows
   int items, waves;     // wide kernel (items > 0): row tiles at most, waves of a workgroup
   int splits;           // workgroups that an item's key tiles are shared out over
-  uint64_t part_bytes;  // partial results
+  uint64_t part_bytes;  // workspace: arrival counters and partial results, 0 where nothing is shared out
 };
 
 // Fused residual add + RMSNorm over rows of a [rows, cols] matrix (column
@@ -500,6 +501,11 @@ __device__ __forceinline__ u32x4 ldg16(const void* p) { return *(const u32x4*)p;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* base, int bytes) {
   const int n = __builtin_amdgcn_readfirstlane(bytes);
   return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, n > 0 ? n : 0, 0x00020000);
+}
+
+// The same over a size that is known to be neither negative nor in a vector register.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t piece_rsrc(const void* base, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, bytes, 0x00020000);
 }
 
 // Buffer accesses as device functions (the host compilation pass then

@@ -31,8 +31,8 @@
 // Work is shared out evenly whatever the lengths: the key tiles of all sequences
 // are numbered one after another and every workgroup takes an equal run of
 // them, which may end inside a sequence or hold several. A sequence that lies
-// in several runs leaves fp32 partial results that fa_window_combine_kernel
-// merges.
+// in several runs leaves fp32 partial results, which the last of them merges.
+#include "../../include/lightserve_fa.h"
 #include "fa_common.hpp"
 
 #include <algorithm>
@@ -57,28 +57,31 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w, float scale, _Float16) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
 }
 
-// Key tiles of 32 of a sequence: those with sinks that its window's tiles do
-// not hold, then the window's from `first` on.
+// A sequence's keys, queries and first row of q, and its key tiles of 32: those
+// with sinks that its window's tiles do not hold, then the window's from `first` on.
 struct KeyTiles {
-  int seq, n, tok0;  // cached tokens, queries, the first one's row
-  int sink, first;   // tiles of sinks ahead of the window's, the window's first tile
+  int seq, n, tok0;
+  int sink, first;
   int count;         // all of them; 1 where queries see no key, 0 without queries
 };
-__device__ __forceinline__ KeyTiles key_tiles(const WindowParams& p, int b) {
+__device__ __forceinline__ KeyTiles key_tiles_of(const WindowParams& p, int seq, int n, int tok0) {
   KeyTiles t;
-  t.tok0 = b, t.n = 1;
-  if (p.cu_q != nullptr) {  // (no row outside q, whatever the offsets)
-    t.tok0 = min(max(p.cu_q[b], 0), p.tokens);
-    t.n = max(min(p.cu_q[b + 1], p.tokens) - t.tok0, 0);
-  }
-  t.seq = min(max(p.seq_lens[b], 0), min(p.max_seq_len, p.max_blocks << p.block_shift));
+  t.seq = seq, t.n = n, t.tok0 = tok0;
   t.first = t.sink = 0;
   if (p.window > 0) {
-    t.first = max(t.seq - t.n - p.window + 1, 0) >> 5;
-    t.sink = min((min(p.sinks, t.seq) + 31) >> 5, t.first);
+    t.first = max(seq - n - p.window + 1, 0) >> 5;
+    t.sink = min((min(p.sinks, seq) + 31) >> 5, t.first);
   }
-  t.count = t.n > 0 ? max(t.sink + ((t.seq + 31) >> 5) - t.first, 1) : 0;
+  t.count = n > 0 ? max(t.sink + ((seq + 31) >> 5) - t.first, 1) : 0;
   return t;
+}
+__device__ __forceinline__ KeyTiles key_tiles(const WindowParams& p, int b) {
+  int n = 1, tok0 = b;
+  if (p.cu_q != nullptr) {  // (no row outside q, whatever the offsets)
+    tok0 = min(max(p.cu_q[b], 0), p.tokens);
+    n = max(min(p.cu_q[b + 1], p.tokens) - tok0, 0);
+  }
+  return key_tiles_of(p, min(max(p.seq_lens[b], 0), min(p.max_seq_len, p.max_blocks << p.block_shift)), n, tok0);
 }
 
 // Inclusive sum over the wave's lanes.
@@ -90,15 +93,6 @@ __device__ __forceinline__ int lanes_sum(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15, rows 1 and 3
   v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31, rows 2 and 3
   return v;
-}
-// Key tiles of all sequences.
-__device__ __forceinline__ int all_tiles(const WindowParams& p, int lane) {
-  int sum = 0;
-  for (int j = 0; j < p.B; j += 64) {
-    const int mine = j + lane < p.B ? key_tiles(p, j + lane).count : 0;
-    sum += __builtin_amdgcn_readlane(lanes_sum(mine), 63);
-  }
-  return sum;
 }
 // Tiles of a run: the tiles there are over the runs there are, no less than one for each wave.
 __device__ __forceinline__ int run_tiles(const WindowParams& p, int all) {
@@ -122,6 +116,19 @@ __device__ __forceinline__ void store_row(const WindowParams& p, int64_t tok0, i
     p.lse[(tok0 + tok) * p.slt + (int64_t)h * p.slh] = E == 0.f ? -INFINITY : (M + __log2f(E)) * kWinLn2;
 }
 
+// Four floats at device scope: written through to, and read from, where all XCDs see them.
+__device__ __forceinline__ void store_device(float* to, const f32x4& v) {
+  const u32x4 w = __builtin_bit_cast(u32x4, v);
+  __hip_atomic_store((uint64_t*)to, w[0] | (uint64_t)w[1] << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __hip_atomic_store((uint64_t*)to + 1, w[2] | (uint64_t)w[3] << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f32x4 load_device(const float* from) {
+  const uint64_t a = __hip_atomic_load((uint64_t*)from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const uint64_t b = __hip_atomic_load((uint64_t*)from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return f32x4{__uint_as_float((uint32_t)a), __uint_as_float((uint32_t)(a >> 32)), __uint_as_float((uint32_t)b),
+               __uint_as_float((uint32_t)(b >> 32))};
+}
+
 constexpr int kRowTile = 16;  // rows of a column block; a row tile has one or two
 
 // NC column blocks of 16 rows share the tile's K and V operands.
@@ -140,27 +147,41 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
 
   __shared__ float st_o[NW][kRowTile][DP];
   __shared__ float st_m[NW][RT], st_l[NW][RT], st_e[NW][RT];
+  __shared__ bool st_last;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, c = lane & 15;
-  const int head = blockIdx.x % p.Hkv, rt = blockIdx.x / p.Hkv;
-  const int run = blockIdx.y;
+  // Workgroups go to the XCDs round-robin, so with 8 heads an XCD would read one head
+  // only: with rows of 128 bytes every eighth line, which is two of its L2's sixteen
+  // channels. Heads are turned by one from run to run instead.
+  const int run = blockIdx.y, rt = blockIdx.x / p.Hkv, head = (blockIdx.x - rt * p.Hkv + run) % p.Hkv;
+  const int column = rt * p.Hkv + head;  // whose runs meet
   const int G = p.Hq / p.Hkv;
 
-  const int all = all_tiles(p, lane), per = run_tiles(p, all);
+  // The runs' tiles, this run's, the sequence that holds its first one, and the number of
+  // that sequence's first tile. (Up to 64 sequences lie in the lanes.)
+  KeyTiles mine = {};
+  if (lane < p.B) mine = key_tiles(p, lane);
+  int upto = lanes_sum(mine.count), all = __builtin_amdgcn_readlane(upto, 63);
+  for (int j = 64; j < p.B; j += 64) {
+    const int more = j + lane < p.B ? key_tiles(p, j + lane).count : 0;
+    all += __builtin_amdgcn_readlane(lanes_sum(more), 63);
+  }
+  const int per = run_tiles(p, all);
   if ((int64_t)run * per >= all) return;  // uniform, before any barrier
   const int start = run * per, end = min(all, start + per);
-  // The sequence that holds tile `start`, and its first tile's number.
-  int b = 0, at = 0;
+  int b = 0, at = 0, have = mine.count;
   for (int j = 0; j < p.B; j += 64) {
-    const int mine = j + lane < p.B ? key_tiles(p, j + lane).count : 0;
-    const int upto = lanes_sum(mine);
+    if (j > 0) {
+      have = j + lane < p.B ? key_tiles(p, j + lane).count : 0;
+      upto = lanes_sum(have);
+    }
     const unsigned long long hit = __ballot(at + upto > start);
     if (hit != 0) {
       const int src = __builtin_ctzll(hit);
       b = j + src;
-      at += __builtin_amdgcn_readlane(upto - mine, src);
+      at += __builtin_amdgcn_readlane(upto - have, src);
       break;
     }
     at += __builtin_amdgcn_readlane(upto, 63);
@@ -176,19 +197,33 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
   const uint32_t vo = c * VJ < p.D ? (uint32_t)(4 * g * (int)p.svs * EB + c * VJ * EB) : kOut;
   const uint32_t vstep = vo == kOut ? 0 : (uint32_t)((int)p.svs * EB);
   const int kbytes = (15 * (int)p.sks + p.D) * EB, vbytes = (15 * (int)p.svs + p.D) * EB;
+  // Byte strides of a block (below 2^32, so that a block's address is one 32 x 32-bit
+  // product) and of a slot, and where the head's rows of block 0 are.
+  const uint32_t kblock = (uint32_t)(p.skb * EB), vblock = (uint32_t)(p.svb * EB), sblock = (uint32_t)p.Hkv << (p.block_shift + 1);
+  const uint32_t kslot = (uint32_t)(p.sks * EB), vslot = (uint32_t)(p.svs * EB);
+  const char* kbase = (const char*)p.kc + (int64_t)head * p.skh * EB;
+  const char* vbase = (const char*)p.vc + (int64_t)head * p.svh * EB;
+  const char* sbase = (const char*)p.scales + ((int64_t)head << (p.block_shift + 1));
+  const int slot_mask = (1 << p.block_shift) - 1;
   const int sinks = p.window > 0 ? p.sinks : 0;
 
   for (; b < p.B && at < end; ++b) {
-    const KeyTiles kt = key_tiles(p, b);
-    const int count = __builtin_amdgcn_readfirstlane(kt.count);
+    KeyTiles kt;
+    if (p.B <= 64) {
+      kt = key_tiles_of(p, __builtin_amdgcn_readlane(mine.seq, b), __builtin_amdgcn_readlane(mine.n, b),
+                        __builtin_amdgcn_readlane(mine.tok0, b));
+    } else {
+      kt = key_tiles(p, b);
+      kt = key_tiles_of(p, __builtin_amdgcn_readfirstlane(kt.seq), __builtin_amdgcn_readfirstlane(kt.n),
+                        __builtin_amdgcn_readfirstlane(kt.tok0));
+    }
+    const int count = kt.count, seq = kt.seq, n = kt.n, sink = kt.sink, first = kt.first, head0 = at;
     if (count == 0) continue;
-    const int seq = __builtin_amdgcn_readfirstlane(kt.seq), n = __builtin_amdgcn_readfirstlane(kt.n);
-    const int sink = __builtin_amdgcn_readfirstlane(kt.sink), first = __builtin_amdgcn_readfirstlane(kt.first);
     const int ta = max(start - at, 0), tb = min(count, end - at);
     at += count;
     const int nrows = n * G - rt * RT;  // of this row tile
     if (nrows <= 0) continue;
-    const int64_t tok0 = __builtin_amdgcn_readfirstlane(kt.tok0);
+    const int64_t tok0 = kt.tok0;
 
     // The lane's rows, and the keys that they see.
     int hi[NC], lo[NC];
@@ -227,33 +262,31 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
       const int key = key_of(u) + 16 * piece;
       return u < nt && key < seq ? table[key >> p.block_shift] : -1;
     };
+    // A piece's block and slot; one that is not there has descriptors of no bytes.
+    struct Piece {
+      uint32_t blk, slot;
+      int live;  // all bits or none
+    };
+    auto piece_of = [&](int u, int blk, int piece) -> Piece {
+      const bool live = (unsigned)blk < (unsigned)p.num_blocks;
+      return {live ? (uint32_t)blk : 0u, (uint32_t)((key_of(u) + 16 * piece) & slot_mask), live ? -1 : 0};
+    };
     u32x4 kr[2][KD];
     uint32_t vr[2][4][VW];
     u32x2 sc[2];
-    auto load_k = [&](int u, int blk, int piece) {
-      const bool live = (unsigned)blk < (unsigned)p.num_blocks;
-      const int slot = (key_of(u) + 16 * piece) & ((1 << p.block_shift) - 1);
-      const C* base = (const C*)p.kc + (live ? (int64_t)blk * p.skb + (int64_t)slot * p.sks + (int64_t)head * p.skh : 0);
-      const __amdgpu_buffer_rsrc_t rs = tile_rsrc(base, live ? kbytes : 0);
+    auto load_k = [&](const Piece& c, int piece) {
+      const __amdgpu_buffer_rsrc_t rs = piece_rsrc(kbase + ((uint64_t)c.blk * kblock + (uint64_t)c.slot * kslot), kbytes & c.live);
 #pragma unroll
       for (int i = 0; i < KD; ++i) {
         const uint32_t o = ko[i];
         kr[piece][i] = load16(rs, (int)o);
       }
     };
-    auto load_s = [&](int u, int blk, int piece) {
-      if constexpr (Q8) {
-        const bool live = (unsigned)blk < (unsigned)p.num_blocks;
-        const int slot = (key_of(u) + 16 * piece) & ((1 << p.block_shift) - 1);
-        const uint8_t* base = p.scales + (live ? ((((int64_t)blk * p.Hkv + head) << p.block_shift) + slot) * 2 : 0);
-        sc[piece] = load8b(tile_rsrc(base, live ? 32 : 0), 8 * g);
-      }
+    auto load_s = [&](const Piece& c, int piece) {
+      if constexpr (Q8) sc[piece] = load8b(piece_rsrc(sbase + ((uint64_t)c.blk * sblock + c.slot * 2), 32 & c.live), 8 * g);
     };
-    auto load_v = [&](int u, int blk, int piece) {
-      const bool live = (unsigned)blk < (unsigned)p.num_blocks;
-      const int slot = (key_of(u) + 16 * piece) & ((1 << p.block_shift) - 1);
-      const C* base = (const C*)p.vc + (live ? (int64_t)blk * p.svb + (int64_t)slot * p.svs + (int64_t)head * p.svh : 0);
-      const __amdgpu_buffer_rsrc_t rs = tile_rsrc(base, live ? vbytes : 0);
+    auto load_v = [&](const Piece& c, int piece) {
+      const __amdgpu_buffer_rsrc_t rs = piece_rsrc(vbase + ((uint64_t)c.blk * vblock + (uint64_t)c.slot * vslot), vbytes & c.live);
 #pragma unroll
       for (int i = 0; i < 4; ++i) load_words<VW>(rs, (int)(vo + i * vstep), vr[piece][i]);
     };
@@ -271,12 +304,14 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
 
     int u = wave;
     int b0 = block_at(u, 0), b1 = block_at(u, 1);
-    load_k(u, b0, 0), load_k(u, b1, 1);
-    load_s(u, b0, 0), load_s(u, b1, 1);
-    load_v(u, b0, 0), load_v(u, b1, 1);
+    Piece c0 = piece_of(u, b0, 0), c1 = piece_of(u, b1, 1);
+    load_k(c0, 0), load_k(c1, 1);
+    load_s(c0, 0), load_s(c1, 1);
+    load_v(c0, 0), load_v(c1, 1);
     b0 = block_at(u + NW, 0), b1 = block_at(u + NW, 1);
     for (; u < nt; u += NW) {
       const int un = u + NW, key0 = key_of(u);
+      c0 = piece_of(un, b0, 0), c1 = piece_of(un, b1, 1);
       f32x4 s[NC][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -295,7 +330,8 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
           for (int x = 0; x < NC; ++x) s[x][h] = mfma16(__builtin_bit_cast(X8, a), qr[x][kk], s[x][h]);
         }
       }
-      load_k(un, b0, 0), load_k(un, b1, 1);
+      load_k(c0, 0), load_k(c1, 1);
+      b0 = block_at(un + NW, 0), b1 = block_at(un + NW, 1);
 
       // Scores in log2 units, masked to -inf where the row does not see the key.
       float vs[2][4];
@@ -314,7 +350,7 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
 #pragma unroll
           for (int x = 0; x < NC; ++x) s[x][h][i] *= ks;
         }
-      load_s(un, b0, 0), load_s(un, b1, 1);
+      load_s(c0, 0), load_s(c1, 1);
       const bool whole = key0 + 31 <= hi_min && (key0 >= lo_max || key0 + 31 < sinks);
       if (!whole) {
 #pragma unroll
@@ -382,8 +418,7 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
 #pragma unroll
         for (int x = 0; x < NC; ++x) acc[x][j] = mfma16(__builtin_bit_cast(X8, a), pb[x], acc[x][j]);
       }
-      load_v(un, b0, 0), load_v(un, b1, 1);
-      b0 = block_at(un + NW, 0), b1 = block_at(un + NW, 1);
+      load_v(c0, 0), load_v(c1, 1);
     }
 
     // Merge the waves, a column block at a time. A wave without a tile has m = -1e30
@@ -397,8 +432,13 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
         st_e[wave][16 * x + c] = le;
       }
     }
+    // A sequence within the run is done. Of one in several runs the partial sums go to
+    // the workspace, and the run that arrives last merges them. The handoff is that of
+    // the skinny GEMM (fa_gemv.hip): partials are device-scope atomic stores (written
+    // through past the XCD's L2), every wave waits for its own before the barrier ahead
+    // of the counter's add, and the last run reads them with device-scope loads.
     const bool complete = ta == 0 && tb == count;
-    const int64_t slot = (int64_t)blockIdx.x * 2 * p.runs + 2 * run + (ta == 0);
+    const int64_t slot = (int64_t)column * 2 * p.runs + 2 * run + (ta == 0);
     float* part = p.part + slot * (RT * (DP + 4));
 #pragma unroll
     for (int x = 0; x < NC; ++x) {
@@ -424,52 +464,76 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
         if (complete) {
           store_row<T>(p, tok0, rt * RT + rr, G, head, d, M, L, E, O);
         } else {
-          *(f32x4*)(part + rr * DP + d) = O;
-          if (d == 0) *(f32x4*)(part + RT * DP + 4 * rr) = f32x4{M, L, E, 0.f};
+          store_device(part + rr * DP + d, O);
+          if (d == 0) store_device(part + RT * DP + 4 * rr, f32x4{M, L, E, 0.f});
         }
       }
       __syncthreads();  // the next merge reuses the arrays
     }
-  }
-}
-
-// Merges the partial results of a sequence's row tile that lies in several runs:
-// o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
-template <typename T, int DP, int NC>
-__global__ __launch_bounds__(256) void fa_window_combine_kernel(const WindowParams p) {
-  constexpr int RT = kRowTile * NC;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int head = blockIdx.x % p.Hkv, rt = blockIdx.x / p.Hkv, b = blockIdx.y;
-  const int G = p.Hq / p.Hkv;
-  const KeyTiles kt = key_tiles(p, b);
-  const int nrows = kt.n * G - rt * RT;
-  if (kt.count == 0 || nrows <= 0) return;
-  int all = 0, at = 0;  // tiles of all sequences, tiles before b's
-  for (int j = 0; j < p.B; j += 64) {
-    const int mine = j + lane < p.B ? key_tiles(p, j + lane).count : 0;
-    const int upto = lanes_sum(mine);
-    if (j <= b && b < j + 64) at = all + __builtin_amdgcn_readlane(upto - mine, b - j);
-    all += __builtin_amdgcn_readlane(upto, 63);
-  }
-  const int per = run_tiles(p, all);
-  const int r0 = at / per, r1 = (at + kt.count - 1) / per;
-  if (r0 == r1) return;  // already in o
-  const float* base = p.part + (int64_t)blockIdx.x * 2 * p.runs * (RT * (DP + 4));
-  for (int idx = tid; idx < min(nrows, RT) * (DP / 4); idx += 256) {
-    const int row = idx / (DP / 4), d = (idx - row * (DP / 4)) * 4;
-    float M = -1e30f, L = 0.f, E = 0.f;
-    f32x4 O = {};
-    for (int r = r0; r <= r1; ++r) {
-      const float* part = base + (int64_t)(2 * r + (r == r0)) * (RT * (DP + 4));
-      const f32x4 st = *(const f32x4*)(part + RT * DP + 4 * row);
-      const f32x4 o = *(const f32x4*)(part + row * DP + d);
-      const float m = fmaxf(M, st[0]), a = fast_exp2(M - m), w = fast_exp2(st[0] - m);
-      L = a * L + w * st[1];
-      E = a * E + w * st[2];
-      O = a * O + w * o;
-      M = m;
+    if (complete) continue;
+    const int r0 = head0 / per, r1 = (head0 + count - 1) / per;  // the sequence's runs
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the partials have reached device scope
+    __syncthreads();
+    if (tid == 0) {
+      int* counter = p.counters + column * p.runs + r0;
+      const bool last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == r1 - r0;
+      if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      st_last = last;
     }
-    store_row<T>(p, kt.tok0, rt * RT + row, G, head, d, M, L, E, O);
+    __syncthreads();
+    if (!st_last) continue;
+    // o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the runs i, in order: groups
+    // of threads take every ng-th run, four at a time, and the groups meet in LDS.
+    const float* base = p.part + (int64_t)column * 2 * p.runs * (RT * (DP + 4));
+    const int items = min(nrows, RT) * (DP / 4), ng = max(256 / items, 1), grp = tid / items;
+    f32x4* meet = (f32x4*)&st_o[0][0][0];
+    for (int i0 = 0; i0 < items; i0 += 256) {
+      const int idx = i0 + (ng > 1 ? tid - grp * items : tid);
+      const int row = idx / (DP / 4), d = (idx - row * (DP / 4)) * 4;
+      float M = -1e30f, L = 0.f, E = 0.f;
+      f32x4 O = {};
+      if (idx < items && (ng == 1 || grp < ng)) {
+        constexpr int U = 4;
+        for (int r = r0 + (ng > 1 ? grp : 0); r <= r1; r += ng * U) {
+          f32x4 st[U], o[U];
+#pragma unroll
+          for (int k = 0; k < U; ++k) {
+            const int rk = min(r + k * ng, r1);
+            const float* from = base + (int64_t)(2 * rk + (rk == r0)) * (RT * (DP + 4));
+            st[k] = load_device(from + RT * DP + 4 * row);
+            o[k] = load_device(from + row * DP + d);
+          }
+#pragma unroll
+          for (int k = 0; k < U; ++k) {
+            if (r + k * ng > r1) break;
+            const float m = fmaxf(M, st[k][0]), a = fast_exp2(M - m), w = fast_exp2(st[k][0] - m);
+            L = a * L + w * st[k][1];
+            E = a * E + w * st[k][2];
+            O = a * O + w * o[k];
+            M = m;
+          }
+        }
+      }
+      if (ng > 1) {
+        if (grp < ng) {
+          meet[2 * tid] = f32x4{M, L, E, 0.f};
+          meet[2 * tid + 1] = O;
+        }
+        __syncthreads();
+        if (tid < items) {
+          for (int k = 1; k < ng; ++k) {
+            const f32x4 st = meet[2 * (tid + k * items)], o = meet[2 * (tid + k * items) + 1];
+            const float m = fmaxf(M, st[0]), a = fast_exp2(M - m), w = fast_exp2(st[0] - m);
+            L = a * L + w * st[1];
+            E = a * E + w * st[2];
+            O = a * O + w * o;
+            M = m;
+          }
+        }
+      }
+      if (tid < items && idx < items) store_row<T>(p, tok0, rt * RT + row, G, head, d, M, L, E, O);
+    }
+    __syncthreads();
   }
 }
 
@@ -529,6 +593,12 @@ __device__ __forceinline__ bool wide_item(const WindowParams& p, int item, int l
   return false;
 }
 
+// Its KV head: an XCD takes the same head of all row tiles of a sequence, which share
+// keys, and another one of the next sequence, so that it reads all channels of its L2.
+__device__ __forceinline__ int wide_head(const WindowParams& p, int b) {
+  return ranked_head((blockIdx.x + b) % p.Hkv, p.Hkv);
+}
+
 // A row tile's key tiles: `sink` of them from key 0 on, then those from tile
 // `first` on.
 struct WideSpan {
@@ -582,9 +652,9 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hh = lane >> 5;
   const int G = p.Hq / p.Hkv;
-  const int head = ranked_head(blockIdx.x % p.Hkv, p.Hkv);
   int b, rt;
   if (!wide_item<BM>(p, blockIdx.x / p.Hkv, lane, b, rt)) return;  // uniform, before any barrier
+  const int head = wide_head(p, b);
   KeyTiles kt = key_tiles(p, b);
   kt.seq = __builtin_amdgcn_readfirstlane(kt.seq);
   kt.n = __builtin_amdgcn_readfirstlane(kt.n);
@@ -939,9 +1009,9 @@ __global__ __launch_bounds__(NW * 64) void fa_window_wide_combine_kernel(const W
   constexpr int BM = NW * 32, DT = DP / 32;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, dt = blockIdx.y;
   const int l32 = lane & 31, hh = lane >> 5, G = p.Hq / p.Hkv;
-  const int head = ranked_head(blockIdx.x % p.Hkv, p.Hkv);
   int b, rt;
   if (!wide_item<BM>(p, blockIdx.x / p.Hkv, lane, b, rt)) return;
+  const int head = wide_head(p, b);
   const KeyTiles kt = key_tiles(p, b);
   const int count = wide_span<BM>(p, kt, rt).count, share = split_share(count, p.splits);
   if (count <= share) return;  // already in o
@@ -978,7 +1048,6 @@ __global__ __launch_bounds__(NW * 64) void fa_window_wide_combine_kernel(const W
 
 // ------------------------------------------------------------------- launches
 constexpr long long kNarrowRows = 2048;  // most rows of a sequence and KV head in the narrow kernel
-constexpr long long kNarrowFill = 1024;  // its workgroups that fill the GPU, with one column block
 
 // How a launch goes, from what the host knows (sizes and bounds, not lengths).
 WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int max_n, long long max_keys, int window, int sinks) {
@@ -990,9 +1059,12 @@ WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int max_n, long
     w.columns = rows > kRowTile ? 2 : 1;
     const int rt = kRowTile * w.columns;
     const long long tiles = (rows + rt - 1) / rt * Hkv;
+    // As many runs as workgroups are resident at once (by their registers): all start
+    // together and, their work being equal, end together.
+    const long long fill = 256 * (w.columns == 1 ? (dp == 64 ? 4 : 3) : (dp == 64 ? 3 : 2));
     const long long most = std::max(1LL, ((seen + 31) / 32 * B + 3) / 4);
-    w.runs = (int)std::min(std::max({1LL, kNarrowFill / w.columns / tiles, std::min((long long)B, kNarrowFill / tiles)}), most);
-    if (w.runs > 1) w.part_bytes = (uint64_t)tiles * 2 * w.runs * rt * (dp + 4) * 4;
+    w.runs = (int)std::min(std::max(fill / tiles, 1LL), most);
+    if (w.runs > 1) w.part_bytes = LSFA_GEMV_COUNTER_BYTES + (uint64_t)tiles * 2 * w.runs * rt * (dp + 4) * 4;
     return w;
   }
   auto items = [&](int bm) {
@@ -1004,7 +1076,7 @@ WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int max_n, long
   if (w.waves == 4) {
     const long long tiles = (std::min(seen, (long long)(window > 0 ? window + sinks + 32 * 4 / G + 128 : seen)) + 63) / 64;
     w.splits = (int)std::max(1LL, std::min(512 / std::max(1, w.items), (int)(tiles / kSplitLeast)) * 1LL);
-    if (w.splits > 1) w.part_bytes = (uint64_t)w.items * w.splits * (128 * 4 + 128 * dp) * 4;
+    if (w.splits > 1) w.part_bytes = LSFA_GEMV_COUNTER_BYTES + (uint64_t)w.items * w.splits * (128 * 4 + 128 * dp) * 4;
   }
   return w;
 }
@@ -1013,9 +1085,6 @@ template <typename T, typename C, int DP, int NC>
 static hipError_t launch_narrow(const WindowParams& p, hipStream_t s) {
   const int rt = kRowTile * NC, tiles = (p.max_n * (p.Hq / p.Hkv) + rt - 1) / rt;
   hipLaunchKernelGGL((fa_window_narrow_kernel<T, C, DP, NC>), dim3(p.Hkv * tiles, p.runs), dim3(256), 0, s, p);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.runs == 1) return e;
-  hipLaunchKernelGGL((fa_window_combine_kernel<T, DP, NC>), dim3(p.Hkv * tiles, p.B), dim3(256), 0, s, p);
   return hipGetLastError();
 }
 template <typename T, typename C, int DP>

@@ -55,6 +55,7 @@ import torch
 from .. import _lib
 from .flash_attention import SPLIT_MAX_TILES, SPLIT_MIN_KEYS
 from .quantized_kv_cache import check_quantized
+from .tiled_matmul import _workspace as stream_workspace
 
 
 def _windowed(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens, max_seqlen_q, max_seq_len, causal, sm_scale,
@@ -113,12 +114,12 @@ def _windowed(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens, max_seq
             # a window or sinks past the longest sequence say no more than its length
             0 if window is None else min(int(window), keys + 1), min(int(sinks), keys), scale, 0)
         nbytes = _lib.window_workspace_size(args)
-        ws = None
-        if nbytes > 0:
-            ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)  # 512-byte aligned blocks
-            args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
         with _lib.device_guard(q.device):
-            _lib.window(args, _lib.current_stream(q.device))
+            stream = _lib.current_stream(q.device)
+            if nbytes > 0:  # arrival counters, kept at zero from call to call, and partial results
+                ws = stream_workspace(q.device, stream, nbytes)
+                args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+            _lib.window(args, stream)
     return (o, lse) if return_lse else o
 
 
