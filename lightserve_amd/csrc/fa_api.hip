@@ -21,7 +21,7 @@ hipError_t fwd_f32(const FwdParams& p, int dp, bool causal, bool varlen, float s
 hipError_t bwd_f32(const BwdParams& p, int dp, bool causal, hipStream_t s);
 hipError_t decode_gqa(const DecodeParams& p, bool is_bf16, int dp, hipStream_t s);
 hipError_t kv_cache_move(const KvCacheParams& p, int dtype, bool append, hipStream_t s);
-WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int max_n, long long max_keys, int window, int sinks);
+WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int eb, int max_n, long long max_keys, int window, int sinks);
 hipError_t window_attention(WindowParams p, const WindowPlan& w, bool is_bf16, hipStream_t s);
 hipError_t rope_inplace(const RopeParams& p, int dtype, hipStream_t s);
 hipError_t add_rmsnorm(const NormParams& p, int dtype, bool vec, hipStream_t s);
@@ -794,7 +794,7 @@ static int check_window(const lsfa_window_args* a) {
 static lsfa::WindowPlan plan_window(const lsfa_window_args* a) {
   if (a->batch == 0 || a->tokens == 0 || a->max_seqlen_q == 0) return {};
   return lsfa::window_plan(a->batch, a->tokens, a->heads_kv, a->heads_q / a->heads_kv, a->head_dim,
-                           std::min(a->max_seqlen_q, a->tokens),
+                           a->kv_scales != nullptr ? 1 : 2, std::min(a->max_seqlen_q, a->tokens),
                            std::min<long long>(a->max_seq_len, (long long)a->max_blocks_per_seq * a->block_size), a->window,
                            a->sinks);
 }

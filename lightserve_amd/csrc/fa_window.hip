@@ -95,9 +95,37 @@ __device__ __forceinline__ int lanes_sum(int v) {
   return v;
 }
 // Tiles of a run: the tiles there are over the runs there are, no less than one for each wave.
-__device__ __forceinline__ int run_tiles(const WindowParams& p, int all) {
-  return max((all + p.runs - 1) / p.runs, 4);
+__device__ __forceinline__ int run_tiles(int all, int runs) {
+  return __builtin_amdgcn_readfirstlane(max((all + runs - 1) / runs, 4));
 }
+// From this many tiles a run on a launch is a long one: a workgroup then takes two or four
+// adjacent KV heads (a wave each, or two) for as many times fewer tiles, and runs meet in
+// fa_window_combine_kernel.
+constexpr int kLongRun = 16;
+__device__ __forceinline__ bool long_runs(const WindowParams& p, int all) {
+  return p.may_be_long && run_tiles(all, p.runs) >= kLongRun;
+}
+// KV heads of a workgroup in a launch of long runs.
+__device__ __forceinline__ int heads_per_group(const WindowParams& p) { return (p.Hkv & 3) == 0 ? 4 : (p.Hkv & 1) == 0 ? 2 : 1; }
+// Partial result of run r of a row tile and KV head: O of part_rows rows, then (offset,
+// sum for O, sum for the lse, 0) of each. A run has two: the end of a sequence and,
+// first_run, the beginning of one.
+template <int DP>
+__device__ __forceinline__ float* part_of(const WindowParams& p, int rt, int head, int runs, int r, bool first_run) {
+  return p.part + (((int64_t)rt * p.Hkv + head) * 2 * runs + 2 * r + first_run) * (p.part_rows * (DP + 4));
+}
+// Sums over the keys of one row (offset M in log2 units) taking in those of others.
+struct RowSums {
+  float M = -1e30f, L = 0.f, E = 0.f;
+  f32x4 O = {};
+  __device__ __forceinline__ void take(const f32x4& st, const f32x4& o) {
+    const float m = fmaxf(M, st[0]), a = fast_exp2(M - m), w = fast_exp2(st[0] - m);
+    L = a * L + w * st[1];
+    E = a * E + w * st[2];
+    O = a * O + w * o;
+    M = m;
+  }
+};
 
 // Channels d .. d + 3 of row r of a sequence and KV head from the sums over its keys
 // (offset M in log2 units), and its lse with channel 0.
@@ -131,9 +159,14 @@ __device__ __forceinline__ f32x4 load_device(const float* from) {
 
 constexpr int kRowTile = 16;  // rows of a column block; a row tile has one or two
 
+// What the narrow kernel's registers allow: tiles of K and V in flight per wave, and
+// workgroups (4 waves) per CU.
+constexpr int narrow_depth(int eb, int dp, int nc) { return eb * dp * nc >= 512 ? 1 : 2; }
+constexpr int narrow_occupancy(int eb, int dp, int nc) { return nc == 2 || eb * dp >= 256 ? 2 : (eb * dp >= 128 ? 3 : 4); }
+
 // NC column blocks of 16 rows share the tile's K and V operands.
 template <typename T, typename C, int DP, int NC>
-__global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowParams p) {
+__global__ __launch_bounds__(256, narrow_occupancy(sizeof(C), DP, NC)) void fa_window_narrow_kernel(const WindowParams p) {
   using X8 = typename VecT<T>::x8;
   constexpr bool Q8 = sizeof(C) == 1;
   constexpr int EB = sizeof(C);           // bytes of a cached element
@@ -143,20 +176,18 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
   constexpr int KD = DP * EB / 64;        // 16-byte loads of K per lane and piece
   constexpr int VJ = DP / 16;             // channels per lane, MFMAs of O
   constexpr int VW = VJ * EB / 4;         // 32-bit words of V per lane and key
+  constexpr int DEPTH = narrow_depth(EB, DP, NC);
+  constexpr int QS = DP + 8;              // elements between rows of Q in LDS (8: the 16 lanes' rows on other banks)
   constexpr float kThreshold = 8.0f;      // log2 units
 
   __shared__ float st_o[NW][kRowTile][DP];
+  __shared__ __attribute__((aligned(16))) T st_q[NW][RT * QS];  // of each head
   __shared__ float st_m[NW][RT], st_l[NW][RT], st_e[NW][RT];
   __shared__ bool st_last;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, c = lane & 15;
-  // Workgroups go to the XCDs round-robin, so with 8 heads an XCD would read one head
-  // only: with rows of 128 bytes every eighth line, which is two of its L2's sixteen
-  // channels. Heads are turned by one from run to run instead.
-  const int run = blockIdx.y, rt = blockIdx.x / p.Hkv, head = (blockIdx.x - rt * p.Hkv + run) % p.Hkv;
-  const int column = rt * p.Hkv + head;  // whose runs meet
   const int G = p.Hq / p.Hkv;
 
   // The runs' tiles, this run's, the sequence that holds its first one, and the number of
@@ -168,7 +199,19 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
     const int more = j + lane < p.B ? key_tiles(p, j + lane).count : 0;
     all += __builtin_amdgcn_readlane(lanes_sum(more), 63);
   }
-  const int per = run_tiles(p, all);
+  // Adjacent heads' rows of a token are adjacent in the cache: read by one workgroup
+  // they are asked for together, in pieces of 2 or 4 rows (512 bytes at head dim 128 and 8
+  // bits) where one head's alone reach HBM as 128-byte ones (64 sequences of 8192 tokens,
+  // 8 KV heads: XXX us). Few tiles stay shared out over the waves of one head, which end
+  // sooner.
+  const bool deferred = long_runs(p, all);
+  const int hw = deferred ? heads_per_group(p) : 1;
+  const int groups = p.Hkv / hw, columns = gridDim.x / hw, runs = p.runs * hw, nk = NW / hw;  // nk: waves that share a head's tiles
+  const int id = blockIdx.y * gridDim.x + blockIdx.x;
+  const int run = __builtin_amdgcn_readfirstlane(id / columns), column = id - run * columns;
+  const int rt = __builtin_amdgcn_readfirstlane(column / groups), head_0 = (column - rt * groups) * hw;
+  const int wave_k = wave / hw, head = head_0 + wave - wave_k * hw;
+  const int per = run_tiles(all, runs);
   if ((int64_t)run * per >= all) return;  // uniform, before any barrier
   const int start = run * per, end = min(all, start + per);
   int b = 0, at = 0, have = mine.count;
@@ -191,7 +234,7 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
   uint32_t ko[KD];
 #pragma unroll
   for (int i = 0; i < KD; ++i) {
-    const int byte = g * (DP * EB / 4) + 16 * i;
+    const int byte = 64 * i + 16 * g;  // a load takes 64 bytes of each of the 16 rows
     ko[i] = byte < p.D * EB ? (uint32_t)(c * (int)p.sks * EB + byte) : kOut;
   }
   const uint32_t vo = c * VJ < p.D ? (uint32_t)(4 * g * (int)p.svs * EB + c * VJ * EB) : kOut;
@@ -221,27 +264,26 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
     if (count == 0) continue;
     const int ta = max(start - at, 0), tb = min(count, end - at);
     at += count;
-    const int nrows = n * G - rt * RT;  // of this row tile
+    const int nrows = min(n, p.max_n) * G - rt * RT;  // of this row tile
     if (nrows <= 0) continue;
     const int64_t tok0 = kt.tok0;
 
-    // The lane's rows, and the keys that they see.
+    // Q, the B operand of S^T, to LDS: kept in registers it would cost the waves that
+    // keep the loads of K and V in flight.
+    for (int i = tid; i < hw * RT * (DP / 8); i += 256) {
+      const int hs = i / (RT * (DP / 8)), row = i / (DP / 8) % RT, d = i % (DP / 8) * 8, r = rt * RT + row, tok = r / G;
+      u32x4 raw = {0, 0, 0, 0};
+      if (row < nrows && d < p.D)
+        raw = ldg16((const T*)p.q + (tok0 + tok) * p.sqt + (int64_t)((head_0 + hs) * G + (r - tok * G)) * p.sqh + d);
+      *(u32x4*)(st_q[hs] + row * QS + d) = raw;
+    }
+    // The lane's rows see keys lo .. hi.
     int hi[NC], lo[NC];
-    X8 qr[NC][KK];  // Q as the B operand of S^T: elements g D/4 + 8 kk .. + 7 of row c
 #pragma unroll
     for (int x = 0; x < NC; ++x) {
-      const int r = rt * RT + 16 * x + c, tok = r / G, hq = head * G + (r - tok * G);
-      const bool row_ok = 16 * x + c < nrows;
-      const int pos = p.causal ? seq - n + tok : seq - 1;
-      hi[x] = row_ok ? pos : -1;
+      const int pos = p.causal ? seq - n + (rt * RT + 16 * x + c) / G : seq - 1;
+      hi[x] = 16 * x + c < nrows ? pos : -1;
       lo[x] = p.window > 0 ? pos - p.window + 1 : 0;
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        const int d = g * (DP / 4) + 8 * kk;
-        u32x4 raw = {0, 0, 0, 0};
-        if (row_ok && d < p.D) raw = ldg16((const T*)p.q + (tok0 + tok) * p.sqt + (int64_t)hq * p.sqh + d);
-        qr[x][kk] = __builtin_bit_cast(X8, raw);
-      }
     }
     // The same of the tile's first and last rows.
     const int t0 = rt * RT / G, t1 = (rt * RT + min(nrows, RT) - 1) / G;
@@ -271,24 +313,27 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
       const bool live = (unsigned)blk < (unsigned)p.num_blocks;
       return {live ? (uint32_t)blk : 0u, (uint32_t)((key_of(u) + 16 * piece) & slot_mask), live ? -1 : 0};
     };
-    u32x4 kr[2][KD];
-    uint32_t vr[2][4][VW];
-    u32x2 sc[2];
-    auto load_k = [&](const Piece& c, int piece) {
+    // One tile of a wave in flight or in use.
+    struct Tile {
+      u32x4 k[2][KD];
+      uint32_t v[2][4][VW];
+      u32x2 sc[2];
+    };
+    auto load_k = [&](Tile& t, const Piece& c, int piece) {
       const __amdgpu_buffer_rsrc_t rs = piece_rsrc(kbase + ((uint64_t)c.blk * kblock + (uint64_t)c.slot * kslot), kbytes & c.live);
 #pragma unroll
       for (int i = 0; i < KD; ++i) {
         const uint32_t o = ko[i];
-        kr[piece][i] = load16(rs, (int)o);
+        t.k[piece][i] = load16(rs, (int)o);
       }
     };
-    auto load_s = [&](const Piece& c, int piece) {
-      if constexpr (Q8) sc[piece] = load8b(piece_rsrc(sbase + ((uint64_t)c.blk * sblock + c.slot * 2), 32 & c.live), 8 * g);
+    auto load_s = [&](Tile& t, const Piece& c, int piece) {
+      if constexpr (Q8) t.sc[piece] = load8b(piece_rsrc(sbase + ((uint64_t)c.blk * sblock + c.slot * 2), 32 & c.live), 8 * g);
     };
-    auto load_v = [&](const Piece& c, int piece) {
+    auto load_v = [&](Tile& t, const Piece& c, int piece) {
       const __amdgpu_buffer_rsrc_t rs = piece_rsrc(vbase + ((uint64_t)c.blk * vblock + (uint64_t)c.slot * vslot), vbytes & c.live);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) load_words<VW>(rs, (int)(vo + i * vstep), vr[piece][i]);
+      for (int i = 0; i < 4; ++i) load_words<VW>(rs, (int)(vo + i * vstep), t.v[piece][i]);
     };
 
     f32x4 acc[NC][VJ];
@@ -302,36 +347,49 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
       for (int j = 0; j < VJ; ++j) acc[x][j] = f32x4{};
     }
 
-    int u = wave;
-    int b0 = block_at(u, 0), b1 = block_at(u, 1);
-    Piece c0 = piece_of(u, b0, 0), c1 = piece_of(u, b1, 1);
-    load_k(c0, 0), load_k(c1, 1);
-    load_s(c0, 0), load_s(c1, 1);
-    load_v(c0, 0), load_v(c1, 1);
-    b0 = block_at(u + NW, 0), b1 = block_at(u + NW, 1);
-    for (; u < nt; u += NW) {
-      const int un = u + NW, key0 = key_of(u);
-      c0 = piece_of(un, b0, 0), c1 = piece_of(un, b1, 1);
+    // Blocks of the tile after those that the loads below are for.
+    int b0 = block_at(wave_k, 0), b1 = block_at(wave_k, 1);
+    const T* my_q = st_q[head - head_0];
+    Tile tiles[DEPTH];
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) {
+      const int u = wave_k + i * nk;
+      const Piece c0 = piece_of(u, b0, 0), c1 = piece_of(u, b1, 1);
+      b0 = block_at(u + nk, 0), b1 = block_at(u + nk, 1);
+      load_k(tiles[i], c0, 0), load_k(tiles[i], c1, 1);
+      load_s(tiles[i], c0, 0), load_s(tiles[i], c1, 1);
+      load_v(tiles[i], c0, 0), load_v(tiles[i], c1, 1);
+    }
+    __syncthreads();  // Q is in LDS
+    // Tile u, whose registers take tile u + DEPTH nk as they become free.
+    auto use = [&](Tile& t, int u) {
+      const int un = u + DEPTH * nk, key0 = key_of(u);
+      const Piece c0 = piece_of(un, b0, 0), c1 = piece_of(un, b1, 1);
       f32x4 s[NC][2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int x = 0; x < NC; ++x) s[x][0] = s[x][1] = f32x4{};
 #pragma unroll
-        for (int x = 0; x < NC; ++x) s[x][h] = f32x4{};
+      for (int kk = 0; kk < KK; ++kk) {
+        X8 qr[NC];  // elements d .. d + 7 of row c, as ko has K's
+        const int d = Q8 ? 64 * (kk / 2) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g;
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
+        for (int x = 0; x < NC; ++x) qr[x] = *(const X8*)(my_q + (16 * x + c) * QS + d);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
           u32x4 a;
           if constexpr (Q8) {
-            const uint32_t w0 = kr[h][kk / 2][2 * (kk & 1)], w1 = kr[h][kk / 2][2 * (kk & 1) + 1];
+            const uint32_t w0 = t.k[h][kk / 2][2 * (kk & 1)], w1 = t.k[h][kk / 2][2 * (kk & 1) + 1];
             a = u32x4{codes2<false>(w0, 1.f, T()), codes2<true>(w0, 1.f, T()), codes2<false>(w1, 1.f, T()), codes2<true>(w1, 1.f, T())};
           } else {
-            a = kr[h][kk];
+            a = t.k[h][kk];
           }
 #pragma unroll
-          for (int x = 0; x < NC; ++x) s[x][h] = mfma16(__builtin_bit_cast(X8, a), qr[x][kk], s[x][h]);
+          for (int x = 0; x < NC; ++x) s[x][h] = mfma16(__builtin_bit_cast(X8, a), qr[x], s[x][h]);
         }
       }
-      load_k(c0, 0), load_k(c1, 1);
-      b0 = block_at(un + NW, 0), b1 = block_at(un + NW, 1);
+      load_k(t, c0, 0), load_k(t, c1, 1);
+      b0 = block_at(un + nk, 0), b1 = block_at(un + nk, 1);
+      __builtin_amdgcn_sched_barrier(0);
 
       // Scores in log2 units, masked to -inf where the row does not see the key.
       float vs[2][4];
@@ -342,7 +400,7 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
           float ks = p.scale_log2;
           vs[h][i] = 1.f;
           if constexpr (Q8) {
-            const uint32_t w = sc[h][i >> 1];
+            const uint32_t w = t.sc[h][i >> 1];
             const uint32_t ke = (i & 1) ? w << 7 : w << 23, ve = (i & 1) ? w >> 1 : w << 15;
             ks *= __uint_as_float(ke & 0x7f800000u);
             vs[h][i] = __uint_as_float(ve & 0x7f800000u);
@@ -350,7 +408,7 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
 #pragma unroll
           for (int x = 0; x < NC; ++x) s[x][h][i] *= ks;
         }
-      load_s(c0, 0), load_s(c1, 1);
+      load_s(t, c0, 0), load_s(t, c1, 1);
       const bool whole = key0 + 31 <= hi_min && (key0 >= lo_max || key0 + 31 < sinks);
       if (!whole) {
 #pragma unroll
@@ -365,7 +423,7 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
             const bool used = key <= hi_max && (key >= lo_min || key < sinks);
             if (!used) vs[h][i] = 1.f;
 #pragma unroll
-            for (int w = 0; w < VW; ++w) vr[h][i][w] = used ? vr[h][i][w] : 0u;
+            for (int w = 0; w < VW; ++w) t.v[h][i][w] = used ? t.v[h][i][w] : 0u;
           }
       }
       X8 pb[NC];
@@ -396,29 +454,40 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
         l_run[x] += (rs[0] + rs[1]) + (rs[2] + rs[3]);
       }
 
-      // Channel (D/16) c + j of the 8 keys, two keys to a word.
-      uint32_t v2[2][4][VJ / 2];  // words of two adjacent channels of one key
+      __builtin_amdgcn_sched_barrier(0);
+      // Channels (D/16) c + 2 w and + 1 of the 8 keys: converted (8 bits), then two keys to
+      // a word.
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int w = 0; w < VJ / 2; ++w) {
+        uint32_t v2[2][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int w = 0; w < VJ / 2; ++w) {
+          for (int i = 0; i < 4; ++i) {
             if constexpr (Q8)
-              v2[h][i][w] = (w & 1) ? codes2<true>(vr[h][i][w / 2], vs[h][i], T()) : codes2<false>(vr[h][i][w / 2], vs[h][i], T());
+              v2[h][i] = (w & 1) ? codes2<true>(t.v[h][i][w / 2], vs[h][i], T()) : codes2<false>(t.v[h][i][w / 2], vs[h][i], T());
             else
-              v2[h][i][w] = vr[h][i][w];
+              v2[h][i] = t.v[h][i][w];
           }
 #pragma unroll
-      for (int j = 0; j < VJ; ++j) {
-        const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
-        u32x4 a;
+        for (int odd = 0; odd < 2; ++odd) {
+          u32x4 a;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) a[k] = __builtin_amdgcn_perm(v2[k / 2][2 * (k & 1) + 1][j / 2], v2[k / 2][2 * (k & 1)][j / 2], sel);
+          for (int k = 0; k < 4; ++k)
+            a[k] = __builtin_amdgcn_perm(v2[k / 2][2 * (k & 1) + 1], v2[k / 2][2 * (k & 1)], odd ? 0x07060302u : 0x05040100u);
 #pragma unroll
-        for (int x = 0; x < NC; ++x) acc[x][j] = mfma16(__builtin_bit_cast(X8, a), pb[x], acc[x][j]);
+          for (int x = 0; x < NC; ++x) acc[x][2 * w + odd] = mfma16(__builtin_bit_cast(X8, a), pb[x], acc[x][2 * w + odd]);
+        }
+        if (w & 1) __builtin_amdgcn_sched_barrier(0);
       }
-      load_v(c0, 0), load_v(c1, 1);
+      load_v(t, c0, 0), load_v(t, c1, 1);
+    };
+    for (int u = wave_k; u < nt; u += DEPTH * nk) {
+      use(tiles[0], u);
+      if constexpr (DEPTH == 2) {
+        if (u + nk >= nt) break;
+        use(tiles[1], u + nk);
+      }
     }
 
     // Merge the waves, a column block at a time. A wave without a tile has m = -1e30
@@ -433,13 +502,14 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
       }
     }
     // A sequence within the run is done. Of one in several runs the partial sums go to
-    // the workspace, and the run that arrives last merges them. The handoff is that of
-    // the skinny GEMM (fa_gemv.hip): partials are device-scope atomic stores (written
-    // through past the XCD's L2), every wave waits for its own before the barrier ahead
-    // of the counter's add, and the last run reads them with device-scope loads.
+    // the workspace. Long runs leave them for the combine kernel (waiting for the
+    // stores and the counter at the end of every run took 20 us of 129 over 64 windows of
+    // 4096 tokens, the kernel 5); of short ones, whose launches are a few microseconds, the
+    // run that arrives last merges them. That handoff is the skinny GEMM's (fa_gemv.hip):
+    // partials are device-scope atomic stores (written through past the XCD's L2),
+    // every wave waits for its own before the barrier ahead of the counter's add, and
+    // the last run reads them with device-scope loads.
     const bool complete = ta == 0 && tb == count;
-    const int64_t slot = (int64_t)column * 2 * p.runs + 2 * run + (ta == 0);
-    float* part = p.part + slot * (RT * (DP + 4));
 #pragma unroll
     for (int x = 0; x < NC; ++x) {
 #pragma unroll
@@ -447,51 +517,54 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
 #pragma unroll
         for (int j = 0; j < VJ; ++j) st_o[wave][c][(4 * g + i) * VJ + j] = acc[x][j][i];
       __syncthreads();
-      for (int idx = tid; idx < min(nrows - 16 * x, kRowTile) * (DP / 4); idx += 256) {
-        const int row = idx / (DP / 4), d = (idx - row * (DP / 4)) * 4, rr = 16 * x + row;
-        float M = st_m[0][rr];
-#pragma unroll
-        for (int w = 1; w < NW; ++w) M = fmaxf(M, st_m[w][rr]);
+      const int items = min(nrows - 16 * x, kRowTile) * (DP / 4);
+      for (int idx = tid; idx < items * hw; idx += 256) {
+        const int hs = idx / items, row = (idx - hs * items) / (DP / 4), d = (idx - hs * items) % (DP / 4) * 4, rr = 16 * x + row;
+        float M = st_m[hs][rr];
+        for (int w = hs + hw; w < NW; w += hw) M = fmaxf(M, st_m[w][rr]);
         float L = 0.f, E = 0.f;
         f32x4 O = {};
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
+        for (int w = hs; w < NW; w += hw) {
           const float a = fast_exp2(st_m[w][rr] - M);
           L += a * st_l[w][rr];
           E += a * st_e[w][rr];
           O += a * *(const f32x4*)&st_o[w][row][d];
         }
         if (complete) {
-          store_row<T>(p, tok0, rt * RT + rr, G, head, d, M, L, E, O);
+          store_row<T>(p, tok0, rt * RT + rr, G, head_0 + hs, d, M, L, E, O);
         } else {
-          store_device(part + rr * DP + d, O);
-          if (d == 0) store_device(part + RT * DP + 4 * rr, f32x4{M, L, E, 0.f});
+          float* part = part_of<DP>(p, rt, head_0 + hs, runs, run, ta == 0);
+          const f32x4 st = {M, L, E, 0.f};
+          if (deferred) {
+            *(f32x4*)(part + rr * DP + d) = O;
+            if (d == 0) *(f32x4*)(part + p.part_rows * DP + 4 * rr) = st;
+          } else {
+            store_device(part + rr * DP + d, O);
+            if (d == 0) store_device(part + p.part_rows * DP + 4 * rr, st);
+          }
         }
       }
       __syncthreads();  // the next merge reuses the arrays
     }
-    if (complete) continue;
+    if (complete || deferred) continue;
     const int r0 = head0 / per, r1 = (head0 + count - 1) / per;  // the sequence's runs
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the partials have reached device scope
     __syncthreads();
     if (tid == 0) {
-      int* counter = p.counters + column * p.runs + r0;
+      int* counter = p.counters + column * runs + r0;
       const bool last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == r1 - r0;
       if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       st_last = last;
     }
     __syncthreads();
     if (!st_last) continue;
-    // o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the runs i, in order: groups
-    // of threads take every ng-th run, four at a time, and the groups meet in LDS.
-    const float* base = p.part + (int64_t)column * 2 * p.runs * (RT * (DP + 4));
+    // (one head a workgroup here) Groups of threads take every ng-th run, four at a time,
+    // and meet in LDS.
     const int items = min(nrows, RT) * (DP / 4), ng = max(256 / items, 1), grp = tid / items;
     f32x4* meet = (f32x4*)&st_o[0][0][0];
     for (int i0 = 0; i0 < items; i0 += 256) {
-      const int idx = i0 + (ng > 1 ? tid - grp * items : tid);
-      const int row = idx / (DP / 4), d = (idx - row * (DP / 4)) * 4;
-      float M = -1e30f, L = 0.f, E = 0.f;
-      f32x4 O = {};
+      const int idx = i0 + (ng > 1 ? tid - grp * items : tid), row = idx / (DP / 4), d = idx % (DP / 4) * 4;
+      RowSums sum;
       if (idx < items && (ng == 1 || grp < ng)) {
         constexpr int U = 4;
         for (int r = r0 + (ng > 1 ? grp : 0); r <= r1; r += ng * U) {
@@ -499,41 +572,72 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
 #pragma unroll
           for (int k = 0; k < U; ++k) {
             const int rk = min(r + k * ng, r1);
-            const float* from = base + (int64_t)(2 * rk + (rk == r0)) * (RT * (DP + 4));
-            st[k] = load_device(from + RT * DP + 4 * row);
+            const float* from = part_of<DP>(p, rt, head, runs, rk, rk == r0);
+            st[k] = load_device(from + p.part_rows * DP + 4 * row);
             o[k] = load_device(from + row * DP + d);
           }
 #pragma unroll
-          for (int k = 0; k < U; ++k) {
-            if (r + k * ng > r1) break;
-            const float m = fmaxf(M, st[k][0]), a = fast_exp2(M - m), w = fast_exp2(st[k][0] - m);
-            L = a * L + w * st[k][1];
-            E = a * E + w * st[k][2];
-            O = a * O + w * o[k];
-            M = m;
-          }
+          for (int k = 0; k < U; ++k)
+            if (r + k * ng <= r1) sum.take(st[k], o[k]);
         }
       }
       if (ng > 1) {
         if (grp < ng) {
-          meet[2 * tid] = f32x4{M, L, E, 0.f};
-          meet[2 * tid + 1] = O;
+          meet[2 * tid] = f32x4{sum.M, sum.L, sum.E, 0.f};
+          meet[2 * tid + 1] = sum.O;
         }
         __syncthreads();
-        if (tid < items) {
-          for (int k = 1; k < ng; ++k) {
-            const f32x4 st = meet[2 * (tid + k * items)], o = meet[2 * (tid + k * items) + 1];
-            const float m = fmaxf(M, st[0]), a = fast_exp2(M - m), w = fast_exp2(st[0] - m);
-            L = a * L + w * st[1];
-            E = a * E + w * st[2];
-            O = a * O + w * o;
-            M = m;
-          }
-        }
+        if (tid < items)
+          for (int k = 1; k < ng; ++k) sum.take(meet[2 * (tid + k * items)], meet[2 * (tid + k * items) + 1]);
       }
-      if (tid < items && idx < items) store_row<T>(p, tok0, rt * RT + row, G, head, d, M, L, E, O);
+      if (idx < items && (ng == 1 || tid < items)) store_row<T>(p, tok0, rt * RT + row, G, head, d, sum.M, sum.L, sum.E, sum.O);
     }
     __syncthreads();
+  }
+}
+
+// Merges the partial results of long runs: one workgroup for a sequence, KV head and row tile.
+template <typename T, int DP, int NC>
+__global__ __launch_bounds__(256) void fa_window_combine_kernel(const WindowParams p) {
+  constexpr int RT = kRowTile * NC;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int head = blockIdx.x % p.Hkv, rt = blockIdx.x / p.Hkv, b = blockIdx.y;
+  const int G = p.Hq / p.Hkv;
+  int all = 0, at = 0, tok0 = 0, count = 0, nrows = 0;  // tiles of all sequences, tiles before b's; b's
+  for (int j = 0; j < p.B; j += 64) {
+    KeyTiles mine = {};
+    if (j + lane < p.B) mine = key_tiles(p, j + lane);
+    const int upto = lanes_sum(mine.count);
+    if (j <= b && b < j + 64) {
+      at = all + __builtin_amdgcn_readlane(upto - mine.count, b - j);
+      count = __builtin_amdgcn_readlane(mine.count, b - j);
+      tok0 = __builtin_amdgcn_readlane(mine.tok0, b - j);
+      nrows = min(min(__builtin_amdgcn_readlane(mine.n, b - j), p.max_n) * G - rt * RT, RT);
+    }
+    all += __builtin_amdgcn_readlane(upto, 63);
+  }
+  if (!long_runs(p, all) || count == 0 || nrows <= 0) return;
+  const int runs = p.runs * heads_per_group(p), per = run_tiles(all, runs);
+  const int r0 = at / per, r1 = (at + count - 1) / per;
+  if (r0 == r1) return;  // already in o
+  for (int idx = tid; idx < nrows * (DP / 4); idx += 256) {
+    const int row = idx / (DP / 4), d = idx % (DP / 4) * 4;
+    RowSums sum;
+    constexpr int U = 8;
+    for (int r = r0; r <= r1; r += U) {
+      f32x4 st[U], o[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int rk = min(r + k, r1);
+        const float* from = part_of<DP>(p, rt, head, runs, rk, rk == r0);
+        st[k] = *(const f32x4*)(from + p.part_rows * DP + 4 * row);
+        o[k] = *(const f32x4*)(from + row * DP + d);
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (r + k <= r1) sum.take(st[k], o[k]);
+    }
+    store_row<T>(p, tok0, rt * RT + row, G, head, d, sum.M, sum.L, sum.E, sum.O);
   }
 }
 
@@ -1050,7 +1154,7 @@ __global__ __launch_bounds__(NW * 64) void fa_window_wide_combine_kernel(const W
 constexpr long long kNarrowRows = 2048;  // most rows of a sequence and KV head in the narrow kernel
 
 // How a launch goes, from what the host knows (sizes and bounds, not lengths).
-WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int max_n, long long max_keys, int window, int sinks) {
+WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int eb, int max_n, long long max_keys, int window, int sinks) {
   WindowPlan w = {};
   const int dp = D <= 64 ? 64 : 128;
   const long long rows = (long long)max_n * G;
@@ -1058,13 +1162,16 @@ WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int max_n, long
   if (rows <= kNarrowRows) {
     w.columns = rows > kRowTile ? 2 : 1;
     const int rt = kRowTile * w.columns;
+    w.part_rows = (int)std::min<long long>(rows, rt);
     const long long tiles = (rows + rt - 1) / rt * Hkv;
     // As many runs as workgroups are resident at once (by their registers): all start
     // together and, their work being equal, end together.
-    const long long fill = 256 * (w.columns == 1 ? (dp == 64 ? 4 : 3) : (dp == 64 ? 3 : 2));
+    const long long fill = 256 * narrow_occupancy(eb, dp, w.columns);
     const long long most = std::max(1LL, ((seen + 31) / 32 * B + 3) / 4);
     w.runs = (int)std::min(std::max(fill / tiles, 1LL), most);
-    if (w.runs > 1) w.part_bytes = LSFA_GEMV_COUNTER_BYTES + (uint64_t)tiles * 2 * w.runs * rt * (dp + 4) * 4;
+    w.may_be_long = w.runs > 1 && (seen + 31) / 32 * B >= (long long)w.runs * (kLongRun - 1);
+    if (w.runs > 1)  // (long runs are up to four times as many)
+      w.part_bytes = LSFA_GEMV_COUNTER_BYTES + (uint64_t)tiles * 2 * w.runs * (w.may_be_long ? 4 : 1) * w.part_rows * (dp + 4) * 4;
     return w;
   }
   auto items = [&](int bm) {
@@ -1082,9 +1189,12 @@ WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int max_n, long
 }
 
 template <typename T, typename C, int DP, int NC>
-static hipError_t launch_narrow(const WindowParams& p, hipStream_t s) {
+static hipError_t launch_narrow(const WindowParams& p, const WindowPlan& w, hipStream_t s) {
   const int rt = kRowTile * NC, tiles = (p.max_n * (p.Hq / p.Hkv) + rt - 1) / rt;
   hipLaunchKernelGGL((fa_window_narrow_kernel<T, C, DP, NC>), dim3(p.Hkv * tiles, p.runs), dim3(256), 0, s, p);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !w.may_be_long) return e;
+  hipLaunchKernelGGL((fa_window_combine_kernel<T, DP, NC>), dim3(p.Hkv * tiles, p.B), dim3(256), 0, s, p);
   return hipGetLastError();
 }
 template <typename T, typename C, int DP>
@@ -1108,7 +1218,7 @@ static hipError_t launch_wide(const WindowParams& p, const WindowPlan& w, hipStr
 template <typename T, typename C, int DP>
 static hipError_t launch_window(const WindowParams& p, const WindowPlan& w, hipStream_t s) {
   if (w.items > 0) return launch_wide<T, C, DP>(p, w, s);
-  return w.columns == 1 ? launch_narrow<T, C, DP, 1>(p, s) : launch_narrow<T, C, DP, 2>(p, s);
+  return w.columns == 1 ? launch_narrow<T, C, DP, 1>(p, w, s) : launch_narrow<T, C, DP, 2>(p, w, s);
 }
 template <typename T>
 static hipError_t dispatch_window(const WindowParams& p, const WindowPlan& w, hipStream_t s) {
@@ -1119,6 +1229,8 @@ static hipError_t dispatch_window(const WindowParams& p, const WindowPlan& w, hi
 // Host entry used by the C ABI layer (arguments already validated).
 hipError_t window_attention(WindowParams p, const WindowPlan& w, bool is_bf16, hipStream_t s) {
   p.runs = w.runs;
+  p.part_rows = w.part_rows;
+  p.may_be_long = w.may_be_long;
   p.splits = w.splits;
   return is_bf16 ? dispatch_window<__bf16>(p, w, s) : dispatch_window<_Float16>(p, w, s);
 }
