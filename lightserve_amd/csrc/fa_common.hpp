@@ -368,14 +368,14 @@ struct WindowParams {
   int tokens;              // rows of q and o
   int max_n, max_seq_len;  // bounds of a sequence's queries and keys
   int causal, window, sinks;
-  int runs, part_rows, splits, may_be_long;  // WindowPlan's
+  int runs, long_run, part_rows, splits;  // WindowPlan's
   float scale_log2;        // sm_scale * log2(e)
   float scale_abs;         // |scale_log2|, at least 1e-30
 };
 struct WindowPlan {
   int runs, columns;    // narrow kernel: runs that the key tiles are shared out over, column blocks of 16 rows
   int part_rows;        // rows of a partial result
-  bool may_be_long;     // whether runs can be long ones (fa_window.hip)
+  int long_run;         // tiles from which runs are long ones (fa_window.hip), 0 where none can be
   int items, waves;     // wide kernel (items > 0): row tiles at most, waves of a workgroup
   int splits;           // workgroups that an item's key tiles are shared out over
   uint64_t part_bytes;  // workspace: arrival counters and partial results, 0 where nothing is shared out

@@ -98,12 +98,11 @@ __device__ __forceinline__ int lanes_sum(int v) {
 __device__ __forceinline__ int run_tiles(int all, int runs) {
   return __builtin_amdgcn_readfirstlane(max((all + runs - 1) / runs, 4));
 }
-// From this many tiles a run on a launch is a long one: a workgroup then takes two or four
-// adjacent KV heads (a wave each, or two) for as many times fewer tiles, and runs meet in
-// fa_window_combine_kernel.
-constexpr int kLongRun = 16;
+// Runs of at least long_run tiles (WindowPlan's, from what a partial result weighs) are long
+// ones: a workgroup then takes two or four adjacent KV heads (a wave each, or two) for as
+// many times fewer tiles, and runs meet in fa_window_combine_kernel.
 __device__ __forceinline__ bool long_runs(const WindowParams& p, int all) {
-  return p.may_be_long && run_tiles(all, p.runs) >= kLongRun;
+  return p.long_run > 0 && run_tiles(all, p.runs) >= p.long_run;
 }
 // KV heads of a workgroup in a launch of long runs.
 __device__ __forceinline__ int heads_per_group(const WindowParams& p) { return (p.Hkv & 3) == 0 ? 4 : (p.Hkv & 1) == 0 ? 2 : 1; }
@@ -159,14 +158,9 @@ __device__ __forceinline__ f32x4 load_device(const float* from) {
 
 constexpr int kRowTile = 16;  // rows of a column block; a row tile has one or two
 
-// What the narrow kernel's registers allow: tiles of K and V in flight per wave, and
-// workgroups (4 waves) per CU.
-constexpr int narrow_depth(int eb, int dp, int nc) { return eb * dp * nc >= 512 ? 1 : 2; }
-constexpr int narrow_occupancy(int eb, int dp, int nc) { return nc == 2 || eb * dp >= 256 ? 2 : (eb * dp >= 128 ? 3 : 4); }
-
 // NC column blocks of 16 rows share the tile's K and V operands.
 template <typename T, typename C, int DP, int NC>
-__global__ __launch_bounds__(256, narrow_occupancy(sizeof(C), DP, NC)) void fa_window_narrow_kernel(const WindowParams p) {
+__global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowParams p) {
   using X8 = typename VecT<T>::x8;
   constexpr bool Q8 = sizeof(C) == 1;
   constexpr int EB = sizeof(C);           // bytes of a cached element
@@ -176,7 +170,6 @@ __global__ __launch_bounds__(256, narrow_occupancy(sizeof(C), DP, NC)) void fa_w
   constexpr int KD = DP * EB / 64;        // 16-byte loads of K per lane and piece
   constexpr int VJ = DP / 16;             // channels per lane, MFMAs of O
   constexpr int VW = VJ * EB / 4;         // 32-bit words of V per lane and key
-  constexpr int DEPTH = narrow_depth(EB, DP, NC);
   constexpr int QS = DP + 8;              // elements between rows of Q in LDS (8: the 16 lanes' rows on other banks)
   constexpr float kThreshold = 8.0f;      // log2 units
 
@@ -347,24 +340,19 @@ __global__ __launch_bounds__(256, narrow_occupancy(sizeof(C), DP, NC)) void fa_w
       for (int j = 0; j < VJ; ++j) acc[x][j] = f32x4{};
     }
 
-    // Blocks of the tile after those that the loads below are for.
-    int b0 = block_at(wave_k, 0), b1 = block_at(wave_k, 1);
     const T* my_q = st_q[head - head_0];
-    Tile tiles[DEPTH];
-#pragma unroll
-    for (int i = 0; i < DEPTH; ++i) {
-      const int u = wave_k + i * nk;
-      const Piece c0 = piece_of(u, b0, 0), c1 = piece_of(u, b1, 1);
-      b0 = block_at(u + nk, 0), b1 = block_at(u + nk, 1);
-      load_k(tiles[i], c0, 0), load_k(tiles[i], c1, 1);
-      load_s(tiles[i], c0, 0), load_s(tiles[i], c1, 1);
-      load_v(tiles[i], c0, 0), load_v(tiles[i], c1, 1);
-    }
+    int b0 = block_at(wave_k, 0), b1 = block_at(wave_k, 1);
+    Piece c0 = piece_of(wave_k, b0, 0), c1 = piece_of(wave_k, b1, 1);
+    b0 = block_at(wave_k + nk, 0), b1 = block_at(wave_k + nk, 1);
+    Tile t;
+    load_k(t, c0, 0), load_k(t, c1, 1);
+    load_s(t, c0, 0), load_s(t, c1, 1);
+    load_v(t, c0, 0), load_v(t, c1, 1);
     __syncthreads();  // Q is in LDS
-    // Tile u, whose registers take tile u + DEPTH nk as they become free.
-    auto use = [&](Tile& t, int u) {
-      const int un = u + DEPTH * nk, key0 = key_of(u);
-      const Piece c0 = piece_of(un, b0, 0), c1 = piece_of(un, b1, 1);
+    // Registers of tile u take the wave's next one as they become free.
+    for (int u = wave_k; u < nt; u += nk) {
+      const int un = u + nk, key0 = key_of(u);
+      c0 = piece_of(un, b0, 0), c1 = piece_of(un, b1, 1);
       f32x4 s[NC][2];
 #pragma unroll
       for (int x = 0; x < NC; ++x) s[x][0] = s[x][1] = f32x4{};
@@ -481,13 +469,6 @@ __global__ __launch_bounds__(256, narrow_occupancy(sizeof(C), DP, NC)) void fa_w
         if (w & 1) __builtin_amdgcn_sched_barrier(0);
       }
       load_v(t, c0, 0), load_v(t, c1, 1);
-    };
-    for (int u = wave_k; u < nt; u += DEPTH * nk) {
-      use(tiles[0], u);
-      if constexpr (DEPTH == 2) {
-        if (u + nk >= nt) break;
-        use(tiles[1], u + nk);
-      }
     }
 
     // Merge the waves, a column block at a time. A wave without a tile has m = -1e30
@@ -596,10 +577,12 @@ __global__ __launch_bounds__(256, narrow_occupancy(sizeof(C), DP, NC)) void fa_w
   }
 }
 
-// Merges the partial results of long runs: one workgroup for a sequence, KV head and row tile.
+// Merges the partial results of long runs: a workgroup takes 32 channels of a sequence, KV
+// head and row tile; groups of threads take every ng-th run and meet in LDS.
 template <typename T, int DP, int NC>
 __global__ __launch_bounds__(256) void fa_window_combine_kernel(const WindowParams p) {
   constexpr int RT = kRowTile * NC;
+  __shared__ f32x4 meet[512];
   const int tid = threadIdx.x, lane = tid & 63;
   const int head = blockIdx.x % p.Hkv, rt = blockIdx.x / p.Hkv, b = blockIdx.y;
   const int G = p.Hq / p.Hkv;
@@ -620,25 +603,31 @@ __global__ __launch_bounds__(256) void fa_window_combine_kernel(const WindowPara
   const int runs = p.runs * heads_per_group(p), per = run_tiles(all, runs);
   const int r0 = at / per, r1 = (at + count - 1) / per;
   if (r0 == r1) return;  // already in o
-  for (int idx = tid; idx < nrows * (DP / 4); idx += 256) {
-    const int row = idx / (DP / 4), d = idx % (DP / 4) * 4;
-    RowSums sum;
+  const int items = nrows * 8, ng = 256 / items, grp = tid / items, idx = tid - grp * items;  // (nrows <= 32)
+  const int row = idx / 8, d = blockIdx.z * 32 + idx % 8 * 4;
+  RowSums sum;
+  if (grp < ng) {
     constexpr int U = 8;
-    for (int r = r0; r <= r1; r += U) {
+    for (int r = r0 + grp; r <= r1; r += ng * U) {
       f32x4 st[U], o[U];
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        const int rk = min(r + k, r1);
+        const int rk = min(r + k * ng, r1);
         const float* from = part_of<DP>(p, rt, head, runs, rk, rk == r0);
         st[k] = *(const f32x4*)(from + p.part_rows * DP + 4 * row);
         o[k] = *(const f32x4*)(from + row * DP + d);
       }
 #pragma unroll
       for (int k = 0; k < U; ++k)
-        if (r + k <= r1) sum.take(st[k], o[k]);
+        if (r + k * ng <= r1) sum.take(st[k], o[k]);
     }
-    store_row<T>(p, tok0, rt * RT + row, G, head, d, sum.M, sum.L, sum.E, sum.O);
+    meet[2 * tid] = f32x4{sum.M, sum.L, sum.E, 0.f};
+    meet[2 * tid + 1] = sum.O;
   }
+  __syncthreads();
+  if (grp > 0) return;
+  for (int k = 1; k < min(ng, r1 - r0 + 1); ++k) sum.take(meet[2 * (tid + k * items)], meet[2 * (tid + k * items) + 1]);
+  store_row<T>(p, tok0, rt * RT + row, G, head, d, sum.M, sum.L, sum.E, sum.O);
 }
 
 // ---------------------------------------------------------------- wide kernel
@@ -1151,7 +1140,7 @@ __global__ __launch_bounds__(NW * 64) void fa_window_wide_combine_kernel(const W
 }
 
 // ------------------------------------------------------------------- launches
-constexpr long long kNarrowRows = 2048;  // most rows of a sequence and KV head in the narrow kernel
+constexpr long long kNarrowRows = 32;  // most rows of a sequence and KV head in the narrow kernel
 
 // How a launch goes, from what the host knows (sizes and bounds, not lengths).
 WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int eb, int max_n, long long max_keys, int window, int sinks) {
@@ -1164,14 +1153,18 @@ WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int eb, int max
     const int rt = kRowTile * w.columns;
     w.part_rows = (int)std::min<long long>(rows, rt);
     const long long tiles = (rows + rt - 1) / rt * Hkv;
-    // As many runs as workgroups are resident at once (by their registers): all start
-    // together and, their work being equal, end together.
-    const long long fill = 256 * narrow_occupancy(eb, dp, w.columns);
+    // Two workgroups a CU, all resident at once: all start together and, their work being
+    // equal, end together. Three of them, which the registers would allow, start and merge
+    // more runs (64 windows of 4096 tokens 117 -> 123 us, 64 sequences of 8192 206 -> 217).
     const long long most = std::max(1LL, ((seen + 31) / 32 * B + 3) / 4);
-    w.runs = (int)std::min(std::max(fill / tiles, 1LL), most);
-    w.may_be_long = w.runs > 1 && (seen + 31) / 32 * B >= (long long)w.runs * (kLongRun - 1);
+    w.runs = (int)std::min(std::max(512 / tiles, 1LL), most);
+    // A long run's partial result, written and read, is to be less than an eighth of the
+    // keys and values that its waves read, and a workgroup to have 16 tiles.
+    const int tile_bytes = 64 * dp * eb, part_bytes = w.part_rows * (dp + 4) * 4;
+    w.long_run = std::max(16, 4 * 16 * part_bytes / tile_bytes);
+    if (w.runs == 1 || (seen + 31) / 32 * B <= (long long)w.runs * (w.long_run - 1)) w.long_run = 0;
     if (w.runs > 1)  // (long runs are up to four times as many)
-      w.part_bytes = LSFA_GEMV_COUNTER_BYTES + (uint64_t)tiles * 2 * w.runs * (w.may_be_long ? 4 : 1) * w.part_rows * (dp + 4) * 4;
+      w.part_bytes = LSFA_GEMV_COUNTER_BYTES + (uint64_t)tiles * 2 * w.runs * (w.long_run > 0 ? 4 : 1) * part_bytes;
     return w;
   }
   auto items = [&](int bm) {
@@ -1193,8 +1186,8 @@ static hipError_t launch_narrow(const WindowParams& p, const WindowPlan& w, hipS
   const int rt = kRowTile * NC, tiles = (p.max_n * (p.Hq / p.Hkv) + rt - 1) / rt;
   hipLaunchKernelGGL((fa_window_narrow_kernel<T, C, DP, NC>), dim3(p.Hkv * tiles, p.runs), dim3(256), 0, s, p);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || !w.may_be_long) return e;
-  hipLaunchKernelGGL((fa_window_combine_kernel<T, DP, NC>), dim3(p.Hkv * tiles, p.B), dim3(256), 0, s, p);
+  if (e != hipSuccess || w.long_run == 0) return e;
+  hipLaunchKernelGGL((fa_window_combine_kernel<T, DP, NC>), dim3(p.Hkv * tiles, p.B, DP / 32), dim3(256), 0, s, p);
   return hipGetLastError();
 }
 template <typename T, typename C, int DP>
@@ -1230,7 +1223,7 @@ static hipError_t dispatch_window(const WindowParams& p, const WindowPlan& w, hi
 hipError_t window_attention(WindowParams p, const WindowPlan& w, bool is_bf16, hipStream_t s) {
   p.runs = w.runs;
   p.part_rows = w.part_rows;
-  p.may_be_long = w.may_be_long;
+  p.long_run = w.long_run;
   p.splits = w.splits;
   return is_bf16 ? dispatch_window<__bf16>(p, w, s) : dispatch_window<_Float16>(p, w, s);
 }
