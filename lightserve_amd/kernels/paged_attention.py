@@ -54,70 +54,81 @@ import torch
 
 from .. import _lib
 from .flash_attention import SPLIT_MAX_TILES, SPLIT_MIN_KEYS
-from .quantized_kv_cache import check_quantized
+from .quantized_kv_cache import check_device, check_quantized
 from .tiled_matmul import _workspace as stream_workspace
 
 
 def _windowed(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens, max_seqlen_q, max_seq_len, causal, sm_scale,
               return_lse, kv_scales, window, sinks):
     """Attention over an 8-bit cache or under a window (lsfa_window); the lse is [tokens, heads_q]."""
-    assert q.dim() == 3, "q must be [tokens, heads_q, head_dim]"
-    assert q.dtype in (torch.float16, torch.bfloat16), "windowed paged attention supports bf16 and fp16"
+    rows, dtype = q.shape, q.dtype
+    assert len(rows) == 3, "q must be [tokens, heads_q, head_dim]"
+    assert dtype == torch.bfloat16 or dtype == torch.float16, "windowed paged attention supports bf16 and fp16"
     if kv_scales is not None:
-        check_quantized(k_cache, v_cache, kv_scales)
+        shape = check_quantized(k_cache, v_cache, kv_scales)
     else:
-        assert k_cache.dim() == 4 and v_cache.shape == k_cache.shape, \
+        shape = k_cache.shape
+        assert len(shape) == 4 and v_cache.shape == shape, \
             "k_cache and v_cache must both be [num_blocks, block_size, heads_kv, head_dim]"
-        assert q.dtype == k_cache.dtype == v_cache.dtype, "q, k_cache and v_cache must share a dtype (or give kv_scales)"
+        assert dtype == k_cache.dtype == v_cache.dtype, "q, k_cache and v_cache must share a dtype (or give kv_scales)"
         assert k_cache.stride(3) == 1 and v_cache.stride(3) == 1, "the caches' head-dim stride must be 1"
-    T, Hq, D = q.shape
-    num_blocks, block_size, Hkv, _ = k_cache.shape
-    assert D == k_cache.shape[3], "head_dim of q and of the caches differ"
+    T, Hq, D = rows
+    num_blocks, block_size, Hkv, _ = shape
+    assert D == shape[3], "head_dim of q and of the caches differ"
     assert Hq % Hkv == 0, "heads_q must be a multiple of heads_kv"
-    assert block_tables.dim() == 2 and block_tables.dtype == seq_lens.dtype == torch.int32, \
+    assert block_tables.dim() == 2 and block_tables.dtype == torch.int32 and seq_lens.dtype == torch.int32, \
         "block_tables [batch, max_blocks] and the sequence lengths must be int32"
-    B = block_tables.shape[0]
+    B, max_blocks = block_tables.shape
     assert seq_lens.shape == (B,), "the sequence lengths must be [batch]"
-    tensors = [("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables), ("seq_lens", seq_lens)]
     if cu_seqlens_q is None:
         assert T == B, "block_tables must be [batch, max_blocks]"
     else:
         assert cu_seqlens_q.dtype == torch.int32 and cu_seqlens_q.shape == (B + 1,), "cu_seqlens_q must be int32 [batch + 1]"
-        tensors.append(("cu_seqlens_q", cu_seqlens_q))
-    if kv_scales is not None:
-        tensors.append(("kv_scales", kv_scales))
-    for name, t in tensors:
-        assert t.is_cuda and t.device == q.device, f"{name} must be a GPU tensor on q's device"
+    on = q.get_device()
+    if not (on >= 0 and on == k_cache.get_device() == v_cache.get_device() == block_tables.get_device()
+            == seq_lens.get_device() and (cu_seqlens_q is None or cu_seqlens_q.get_device() == on)
+            and (kv_scales is None or kv_scales.get_device() == on)):
+        check_device((("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables),
+                      ("seq_lens", seq_lens), *((("cu_seqlens_q", cu_seqlens_q),) if cu_seqlens_q is not None else ()),
+                      *((("kv_scales", kv_scales),) if kv_scales is not None else ())))
     if window is None:
         assert sinks == 0, "sinks need a window"
     else:
         assert window >= 1 and sinks >= 0, "window must be at least 1 and sinks not negative"
         assert causal, "a window is causal"
     scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
-    q_ = q if (q.stride(-1) == 1 and all(s % 8 == 0 for s in q.stride()[:2]) and q.data_ptr() % 16 == 0) \
-        else q.contiguous()
+    qs = q.stride()
+    if qs[2] != 1 or qs[0] % 8 != 0 or qs[1] % 8 != 0 or q.data_ptr() % 16 != 0:
+        q = q.contiguous()
+        qs = q.stride()
     bt = block_tables if block_tables.stride(1) == 1 else block_tables.contiguous()
     sl = seq_lens.contiguous()
     cu = cu_seqlens_q.contiguous() if cu_seqlens_q is not None else None
-    o = torch.empty(T, Hq, D, device=q.device, dtype=q.dtype)
-    lse = torch.empty(T, Hq, device=q.device, dtype=torch.float32) if return_lse and cu is None else \
-        torch.empty(Hq, T, device=q.device, dtype=torch.float32).t() if return_lse else None
+    device = q.device
+    o = torch.empty(rows, device=device, dtype=dtype)
+    lse, ls = None, (0, 0)
+    if return_lse:
+        lse = torch.empty((T, Hq) if cu is None else (Hq, T), device=device, dtype=torch.float32)
+        if cu is not None:
+            lse = lse.t()
+        ls = lse.stride()
     if T > 0:
-        keys = min(int(max_seq_len), bt.shape[1] * block_size)
+        keys = min(int(max_seq_len), max_blocks * block_size)
+        ks, vs = k_cache.stride(), v_cache.stride()
         args = _lib.pack(
-            _lib.WindowArgs, q_.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(),
+            _lib.WindowArgs, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(),
             lse.data_ptr() if return_lse else 0, kv_scales.data_ptr() if kv_scales is not None else 0,
             cu.data_ptr() if cu is not None else 0, sl.data_ptr(), bt.data_ptr(), 0, 0,  # the workspace follows
-            *q_.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3], *o.stride()[:2],
-            *(lse.stride() if return_lse else (0, 0)), bt.stride(0), _lib.TORCH_TO_LSFA[q.dtype], B, T, Hq, Hkv, D,
-            block_size, num_blocks, bt.shape[1], int(max_seqlen_q), keys, bool(causal),
+            qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], Hq * D, D, ls[0], ls[1], bt.stride(0),
+            _lib.TORCH_TO_LSFA[dtype], B, T, Hq, Hkv, D, block_size, num_blocks, max_blocks, int(max_seqlen_q), keys,
+            bool(causal),
             # a window or sinks past the longest sequence say no more than its length
             0 if window is None else min(int(window), keys + 1), min(int(sinks), keys), scale, 0)
         nbytes = _lib.window_workspace_size(args)
-        with _lib.device_guard(q.device):
-            stream = _lib.current_stream(q.device)
+        with _lib.device_guard(device):
+            stream = _lib.current_stream(device)
             if nbytes > 0:  # arrival counters, kept at zero from call to call, and partial results
-                ws = stream_workspace(q.device, stream, nbytes)
+                ws = stream_workspace(device, stream, nbytes)
                 args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
             _lib.window(args, stream)
     return (o, lse) if return_lse else o

@@ -47,77 +47,97 @@ def quantized_kv_cache(num_blocks, block_size, heads_kv, head_dim, device="cuda"
     return k_cache, v_cache, torch.ones(num_blocks, heads_kv, block_size, 2, dtype=torch.uint8, device=device)
 
 
+_E4M3, _U8, _I32 = torch.float8_e4m3fn, torch.uint8, torch.int32
+
+
 def check_quantized(k_cache, v_cache, kv_scales):
-    """What a cache must be, for the calls here and for the attention over it."""
-    assert k_cache.dtype == v_cache.dtype == torch.float8_e4m3fn, "an 8-bit cache holds float8_e4m3fn"
-    assert k_cache.dim() == 4 and v_cache.shape == k_cache.shape, \
+    """What a cache must be, for the calls here and for the attention over it; its shape."""
+    shape = k_cache.shape
+    assert k_cache.dtype == _E4M3 and v_cache.dtype == _E4M3, "an 8-bit cache holds float8_e4m3fn"
+    assert len(shape) == 4 and v_cache.shape == shape, \
         "k_cache and v_cache must both be [num_blocks, block_size, heads_kv, head_dim]"
-    n, bs, h, _ = k_cache.shape
-    assert kv_scales.dtype == torch.uint8 and kv_scales.shape == (n, h, bs, 2) and kv_scales.is_contiguous(), \
+    n, bs, h, _ = shape
+    assert kv_scales.dtype == _U8 and kv_scales.shape == (n, h, bs, 2) and kv_scales.is_contiguous(), \
         "kv_scales must be contiguous uint8 [num_blocks, heads_kv, block_size, 2]"
     assert k_cache.stride(3) == 1 and v_cache.stride(3) == 1, "the caches' head-dim stride must be 1"
+    return shape
 
 
-def _check(k_cache, v_cache, kv_scales, block_tables, others):
-    check_quantized(k_cache, v_cache, kv_scales)
-    assert block_tables.dtype == torch.int32 and block_tables.dim() == 2, "block_tables must be int32 [batch, max_blocks]"
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("kv_scales", kv_scales), ("block_tables", block_tables),
-                    *others):
-        assert t.is_cuda and t.device == k_cache.device, f"{name} must be a GPU tensor on the cache's device"
+def check_device(named):
+    """All of these ((name, tensor), ...) on one GPU."""
+    for name, t in named:
+        assert t.is_cuda and t.device == named[0][1].device, f"{name} must be a GPU tensor on {named[0][0]}'s device"
 
 
-def _args(k, v, k_cache, v_cache, kv_scales, block_tables, seq_lens, cu_seqlens):
-    num_blocks, block_size, heads, dim = k_cache.shape
-    return _lib.pack(
+def _launch(call, k, v, k_cache, v_cache, kv_scales, shape, block_tables, seq_lens, cu_seqlens):
+    """The launch of one of the two calls on checked arguments; k and v are contiguous in head_dim."""
+    bt = block_tables if block_tables.stride(1) == 1 else block_tables.contiguous()
+    kc, vc = k_cache.stride(), v_cache.stride()
+    ks, vs = k.stride(), v.stride()
+    rows, max_blocks = bt.shape
+    args = _lib.pack(
         _lib.KvCacheArgs, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(),
-        block_tables.data_ptr(), seq_lens.data_ptr() if seq_lens is not None else 0,
-        cu_seqlens.data_ptr() if cu_seqlens is not None else 0, *k.stride()[:2], *v.stride()[:2],
-        *k_cache.stride()[:3], *v_cache.stride()[:3], block_tables.stride(0), _lib.TORCH_TO_LSFA[k.dtype],
-        block_tables.shape[0], k.shape[0], heads, dim, block_size, num_blocks, block_tables.shape[1])
+        bt.data_ptr(), seq_lens.data_ptr() if seq_lens is not None else 0,
+        cu_seqlens.data_ptr() if cu_seqlens is not None else 0, ks[0], ks[1], vs[0], vs[1], kc[0], kc[1], kc[2], vc[0],
+        vc[1], vc[2], bt.stride(0), _lib.TORCH_TO_LSFA[k.dtype], rows, k.shape[0], shape[2], shape[3], shape[1], shape[0],
+        max_blocks)
+    device = k.device
+    with _lib.device_guard(device):
+        call(args, _lib.current_stream(device))
 
 
 def _addressable(t):
+    s0, s1, s2 = t.stride()
     per16 = 16 // t.element_size()
-    return t.stride(2) == 1 and t.stride(0) % per16 == 0 and t.stride(1) % per16 == 0 and t.data_ptr() % 16 == 0
+    return s2 == 1 and s0 % per16 == 0 and s1 % per16 == 0 and t.data_ptr() % 16 == 0
 
 
 def kv_cache_append(k, v, k_cache, v_cache, kv_scales, block_tables, seq_lens, cu_seqlens=None):
-    assert k.dim() == 3 and v.shape == k.shape and v.dtype == k.dtype, "k and v must both be [tokens, heads_kv, head_dim]"
+    rows = k.shape
+    assert len(rows) == 3 and v.shape == rows and v.dtype == k.dtype, "k and v must both be [tokens, heads_kv, head_dim]"
     assert k.dtype in _lib.TORCH_TO_LSFA, f"unsupported dtype {k.dtype}"
-    offsets = () if cu_seqlens is None else (("cu_seqlens", cu_seqlens),)
-    _check(k_cache, v_cache, kv_scales, block_tables, (("k", k), ("v", v), ("seq_lens", seq_lens), *offsets))
-    assert k.shape[1:] == k_cache.shape[2:], "heads_kv / head_dim of k and of the caches differ"
+    shape = check_quantized(k_cache, v_cache, kv_scales)
+    assert block_tables.dtype == _I32 and block_tables.dim() == 2, "block_tables must be int32 [batch, max_blocks]"
+    on = k_cache.get_device()
+    if not (on >= 0 and on == v_cache.get_device() == kv_scales.get_device() == block_tables.get_device()
+            == k.get_device() == v.get_device() == seq_lens.get_device()
+            and (cu_seqlens is None or cu_seqlens.get_device() == on)):
+        check_device((("k_cache", k_cache), ("v_cache", v_cache), ("kv_scales", kv_scales), ("block_tables", block_tables),
+                      ("k", k), ("v", v), ("seq_lens", seq_lens),
+                      *((("cu_seqlens", cu_seqlens),) if cu_seqlens is not None else ())))
+    assert rows[1:] == shape[2:], "heads_kv / head_dim of k and of the caches differ"
     batch = block_tables.shape[0]
-    assert seq_lens.dtype == torch.int32 and seq_lens.shape == (batch,), "seq_lens must be int32 [batch]"
+    assert seq_lens.dtype == _I32 and seq_lens.shape == (batch,), "seq_lens must be int32 [batch]"
     if cu_seqlens is None:
-        assert k.shape[0] == batch, "without cu_seqlens k and v hold one row per sequence"
+        assert rows[0] == batch, "without cu_seqlens k and v hold one row per sequence"
     else:
-        assert cu_seqlens.dtype == torch.int32 and cu_seqlens.shape == (batch + 1,), "cu_seqlens must be int32 [batch + 1]"
+        assert cu_seqlens.dtype == _I32 and cu_seqlens.shape == (batch + 1,), "cu_seqlens must be int32 [batch + 1]"
         cu_seqlens = cu_seqlens.contiguous()
-    if k.shape[0] == 0:
+    if rows[0] == 0:
         return
-    k, v = (t if _addressable(t) else t.contiguous() for t in (k, v))
-    bt = block_tables if block_tables.stride(1) == 1 else block_tables.contiguous()
-    sl = seq_lens.contiguous()
-    args = _args(k, v, k_cache, v_cache, kv_scales, bt, sl, cu_seqlens)
-    with _lib.device_guard(k.device):
-        _lib.kv_append(args, _lib.current_stream(k.device))
+    if not _addressable(k):
+        k = k.contiguous()
+    if not _addressable(v):
+        v = v.contiguous()
+    _launch(_lib.kv_append, k, v, k_cache, v_cache, kv_scales, shape, block_tables, seq_lens.contiguous(), cu_seqlens)
 
 
 def kv_cache_read(k_cache, v_cache, kv_scales, block_tables, cu_seqlens, *, total=None, dtype=torch.bfloat16):
-    _check(k_cache, v_cache, kv_scales, block_tables, (("cu_seqlens", cu_seqlens),))
+    shape = check_quantized(k_cache, v_cache, kv_scales)
+    assert block_tables.dtype == _I32 and block_tables.dim() == 2, "block_tables must be int32 [batch, max_blocks]"
+    on = k_cache.get_device()
+    if not (on >= 0 and on == v_cache.get_device() == kv_scales.get_device() == block_tables.get_device()
+            == cu_seqlens.get_device()):
+        check_device((("k_cache", k_cache), ("v_cache", v_cache), ("kv_scales", kv_scales), ("block_tables", block_tables),
+                      ("cu_seqlens", cu_seqlens)))
     assert dtype in _lib.TORCH_TO_LSFA, f"unsupported dtype {dtype}"
     batch = block_tables.shape[0]
-    assert cu_seqlens.dtype == torch.int32 and cu_seqlens.shape == (batch + 1,), "cu_seqlens must be int32 [batch + 1]"
+    assert cu_seqlens.dtype == _I32 and cu_seqlens.shape == (batch + 1,), "cu_seqlens must be int32 [batch + 1]"
     if total is None:
         total = int(cu_seqlens[-1].item())
     assert total >= 0, "total must not be negative"
-    k, v = (torch.empty(total, *k_cache.shape[2:], dtype=dtype, device=k_cache.device) for _ in range(2))
-    if k.numel() == 0:
-        return k, v
-    bt = block_tables if block_tables.stride(1) == 1 else block_tables.contiguous()
-    cu = cu_seqlens.contiguous()
-    args = _args(k, v, k_cache, v_cache, kv_scales, bt, None, cu)
-    with _lib.device_guard(k.device):
-        _lib.kv_read(args, _lib.current_stream(k.device))
+    k = torch.empty((total, shape[2], shape[3]), dtype=dtype, device=k_cache.device)
+    v = torch.empty_like(k)
+    if total > 0:
+        _launch(_lib.kv_read, k, v, k_cache, v_cache, kv_scales, shape, block_tables, None, cu_seqlens.contiguous())
     return k, v
