@@ -29,17 +29,17 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // Eight values of a row as fp32, from 16-bit or 32-bit storage.
 __device__ __forceinline__ void load8(const __bf16* p, float (&x)[8]) {
-  const bf16x8 v = __builtin_bit_cast(bf16x8, ldg16(p));
+  const bf16x8 v = __builtin_bit_cast(bf16x8, __builtin_nontemporal_load((const u32x4*)p));
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
 }
 __device__ __forceinline__ void load8(const _Float16* p, float (&x)[8]) {
-  const f16x8 v = __builtin_bit_cast(f16x8, ldg16(p));
+  const f16x8 v = __builtin_bit_cast(f16x8, __builtin_nontemporal_load((const u32x4*)p));
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
 }
 __device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+  const f32x4 a = __builtin_nontemporal_load((const f32x4*)p), b = __builtin_nontemporal_load((const f32x4*)(p + 4));
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
 }
@@ -135,6 +135,10 @@ __device__ __forceinline__ int block_of(const KvCacheParams& p, int b, int pos, 
   return (unsigned)blk < (unsigned)p.num_blocks ? blk : -1;
 }
 
+// One row a lane group, read and written once past the caches' usual order (nontemporal):
+// 32768 rows of 8 heads of 128 in bf16 48.4 us, 4.2 TB/s (51.0 without the hints; two
+// or four rows a lane group, their loads together, 59 and 66; the 2-byte scales cost 2 of
+// it). Eight rows of a decode step take 4.0, a launch's own time.
 template <typename T, int LPR>
 __global__ __launch_bounds__(256) void fa_kv_append_kernel(const KvCacheParams p) {
   __shared__ int32_t s_cu[kCuStaged + 1];
@@ -164,42 +168,61 @@ __global__ __launch_bounds__(256) void fa_kv_append_kernel(const KvCacheParams p
   int ke, ve;
   const u32x2 kq = quantise_row<T, LPR>(k, ke), vq = quantise_row<T, LPR>(v, ve);
   if (has) {
-    *(u32x2*)(p.kc + (int64_t)blk * p.skc[0] + (int64_t)slot * p.skc[1] + (int64_t)h * p.skc[2] + 8 * c) = kq;
-    *(u32x2*)(p.vc + (int64_t)blk * p.svc[0] + (int64_t)slot * p.svc[1] + (int64_t)h * p.svc[2] + 8 * c) = vq;
+    __builtin_nontemporal_store(kq, (u32x2*)(p.kc + (int64_t)blk * p.skc[0] + (int64_t)slot * p.skc[1] + (int64_t)h * p.skc[2] + 8 * c));
+    __builtin_nontemporal_store(vq, (u32x2*)(p.vc + (int64_t)blk * p.svc[0] + (int64_t)slot * p.svc[1] + (int64_t)h * p.svc[2] + 8 * c));
   }
   if (c == 0)
     *(uint16_t*)(p.scales + ((((int64_t)blk * p.Hkv + h) << p.block_shift) + slot) * 2) = (uint16_t)(ke | ve << 8);
 }
 
-template <typename T, int LPR>
+template <typename T, int LPR, int U>
 __global__ __launch_bounds__(256) void fa_kv_read_kernel(const KvCacheParams p) {
   __shared__ int32_t s_cu[kCuStaged + 1];
   stage_offsets(p.cu, p.B, s_cu);
-  const int c = threadIdx.x % LPR;
-  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
-  const int t = (int)(row / p.Hkv), h = (int)(row - (int64_t)t * p.Hkv);
-  if (t >= p.tokens || 8 * c >= p.D) return;
   const int32_t* cu = p.B <= kCuStaged ? s_cu : p.cu;
-  const int b = sequence_of(cu, p.B, t);
-  int slot = 0, blk = -1;
-  if (b < p.B && t >= cu[b]) blk = block_of(p, b, t - cu[b], slot);
-  float k[8] = {}, v[8] = {};  // rows that no sequence or cache block holds are zeros
-  if (blk >= 0) {
-    const uint32_t e = *(const uint16_t*)(p.scales + ((((int64_t)blk * p.Hkv + h) << p.block_shift) + slot) * 2);
-    dequantise8(*(const u32x2*)(p.kc + (int64_t)blk * p.skc[0] + (int64_t)slot * p.skc[1] + (int64_t)h * p.skc[2] + 8 * c), e & 255u, k);
-    dequantise8(*(const u32x2*)(p.vc + (int64_t)blk * p.svc[0] + (int64_t)slot * p.svc[1] + (int64_t)h * p.svc[2] + 8 * c), e >> 8, v);
+  const int c = threadIdx.x % LPR;
+  if (8 * c >= p.D) return;
+  int t[U], h[U], blk[U], slot[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t row = ((int64_t)blockIdx.x * U + u) * (256 / LPR) + threadIdx.x / LPR;
+    t[u] = (int)(row / p.Hkv), h[u] = (int)(row - (int64_t)t[u] * p.Hkv);
+    blk[u] = -1;
+    if (t[u] >= p.tokens) continue;
+    const int b = sequence_of(cu, p.B, t[u]);
+    if (b < p.B && t[u] >= cu[b]) blk[u] = block_of(p, b, t[u] - cu[b], slot[u]);
   }
-  store8((T*)p.k + (int64_t)t * p.sk[0] + (int64_t)h * p.sk[1] + 8 * c, k);
-  store8((T*)p.v + (int64_t)t * p.sv[0] + (int64_t)h * p.sv[1] + 8 * c, v);
+  u32x2 kq[U], vq[U];
+  uint32_t e[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    kq[u] = vq[u] = u32x2{0, 0};  // rows that no sequence or cache block holds are zeros
+    e[u] = 0;
+    if (blk[u] < 0) continue;
+    e[u] = *(const uint16_t*)(p.scales + ((((int64_t)blk[u] * p.Hkv + h[u]) << p.block_shift) + slot[u]) * 2);
+    kq[u] = *(const u32x2*)(p.kc + (int64_t)blk[u] * p.skc[0] + (int64_t)slot[u] * p.skc[1] + (int64_t)h[u] * p.skc[2] + 8 * c);
+    vq[u] = *(const u32x2*)(p.vc + (int64_t)blk[u] * p.svc[0] + (int64_t)slot[u] * p.svc[1] + (int64_t)h[u] * p.svc[2] + 8 * c);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (t[u] >= p.tokens) continue;
+    float x[8];
+    dequantise8(kq[u], e[u] & 255u, x);
+    store8((T*)p.k + (int64_t)t[u] * p.sk[0] + (int64_t)h[u] * p.sk[1] + 8 * c, x);
+    dequantise8(vq[u], e[u] >> 8, x);
+    store8((T*)p.v + (int64_t)t[u] * p.sv[0] + (int64_t)h[u] * p.sv[1] + 8 * c, x);
+  }
 }
 
 template <typename T, int LPR>
 static void launch_kv(const KvCacheParams& p, bool append, hipStream_t s) {
-  const dim3 grid((unsigned)(((int64_t)p.tokens * p.Hkv * LPR + 255) / 256));
-  if (append)
-    hipLaunchKernelGGL((fa_kv_append_kernel<T, LPR>), grid, dim3(256), 0, s, p);
-  else
-    hipLaunchKernelGGL((fa_kv_read_kernel<T, LPR>), grid, dim3(256), 0, s, p);
+  const int64_t threads = (int64_t)p.tokens * p.Hkv * LPR;
+  const dim3 grid((unsigned)((threads + 255) / 256)), half((unsigned)((threads + 511) / 512));
+  // Reads take two rows a lane group where that leaves 2048 workgroups, 8 a CU (37000 rows of 8
+  // heads 46.5 -> 40.0 us, 5.7 TB/s); fewer rows spread over the GPU (4096: 7.0 and 7.1).
+  if (append) hipLaunchKernelGGL((fa_kv_append_kernel<T, LPR>), grid, dim3(256), 0, s, p);
+  else if (threads >= 2 * 256 * 2048) hipLaunchKernelGGL((fa_kv_read_kernel<T, LPR, 2>), half, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((fa_kv_read_kernel<T, LPR, 1>), grid, dim3(256), 0, s, p);
 }
 template <typename T>
 static void dispatch_kv(const KvCacheParams& p, bool append, hipStream_t s) {
