@@ -643,20 +643,19 @@ __global__ __launch_bounds__(256) void fa_window_combine_kernel(const WindowPara
 // scores of tile t + 1 beside the softmax of tile t.
 constexpr int kWideTile = 64;  // keys
 
-// Row tiles longest first (ranked_item) for up to 64 sequences, else in order.
-// The length that counts is that of a causal row without a window: under one, tiles are
-// about equally long and the order does not matter.
+// The sequence (with its key tiles) and row tile of an item; false past the last. Row
+// tiles go longest first (ranked_item) where their lengths differ: up to 64 sequences
+// without a window. Else they go in order, the last of a sequence first.
 template <int BM>
-__device__ __forceinline__ bool wide_item(const WindowParams& p, int item, int lane, int& b, int& rt) {
+__device__ __forceinline__ bool wide_item(const WindowParams& p, int item, int lane, int& b, int& rt, KeyTiles& kt) {
   const int G = p.Hq / p.Hkv;
-  if (p.B <= 64) {
-    int tq = 0, nk = 0, off = 0;
-    if (lane < p.B) {
-      const KeyTiles t = key_tiles(p, lane);
-      tq = (int)(((int64_t)min(t.n, p.max_n) * G + BM - 1) / BM);
-      nk = t.seq;
-      off = nk - t.n;
-    }
+  auto tiles_of = [&](const KeyTiles& t) -> int { return (int)(((int64_t)min(t.n, p.max_n) * G + BM - 1) / BM); };
+  KeyTiles mine = {};
+  if (lane < p.B) mine = key_tiles(p, lane);
+  int tq = tiles_of(mine);
+  bool found = false;
+  if (p.B > 1 && p.B <= 64 && p.window == 0) {
+    const int nk = mine.seq, off = nk - mine.n;
     auto above = [&](int x) -> int {
       if (x < 0) return tq;
       if (tq == 0 || nk <= kWideTile * x) return 0;
@@ -666,24 +665,32 @@ __device__ __forceinline__ bool wide_item(const WindowParams& p, int item, int l
     };
     int d;
     b = ranked_item(p.B, item, lane, tq, nk > 0 ? (nk + kWideTile - 1) / kWideTile : 0, above, d);
-    if (b < 0) return false;
-    rt = __builtin_amdgcn_readlane(tq, b) - 1 - d;
-    return true;
-  }
-  int at = 0;
-  for (int j = 0; j < p.B; j += 64) {
-    const int mine = j + lane < p.B ? (int)(((int64_t)min(key_tiles(p, j + lane).n, p.max_n) * G + BM - 1) / BM) : 0;
-    const int upto = lanes_sum(mine);
-    const unsigned long long hit = __ballot(at + upto > item);
-    if (hit != 0) {
-      const int src = __builtin_ctzll(hit);
-      b = j + src;
-      rt = item - at - __builtin_amdgcn_readlane(upto - mine, src);
-      return true;
+    found = b >= 0;
+    if (found) rt = __builtin_amdgcn_readlane(tq, b) - 1 - d;
+  } else {
+    int at = 0;
+    for (int j = 0; j < p.B && !found; j += 64) {
+      if (j > 0) {
+        mine = {};
+        if (j + lane < p.B) mine = key_tiles(p, j + lane);
+        tq = tiles_of(mine);
+      }
+      const int upto = lanes_sum(tq);
+      const unsigned long long hit = __ballot(at + upto > item);
+      if (hit != 0) {
+        const int src = __builtin_ctzll(hit);
+        b = j + src;
+        rt = at + __builtin_amdgcn_readlane(upto, src) - 1 - item;
+        found = true;
+      }
+      at += __builtin_amdgcn_readlane(upto, 63);
     }
-    at += __builtin_amdgcn_readlane(upto, 63);
   }
-  return false;
+  if (!found) return false;
+  const int src = b & 63;
+  kt = key_tiles_of(p, __builtin_amdgcn_readlane(mine.seq, src), __builtin_amdgcn_readlane(mine.n, src),
+                    __builtin_amdgcn_readlane(mine.tok0, src));
+  return true;
 }
 
 // Its KV head: an XCD takes the same head of all row tiles of a sequence, which share
@@ -746,12 +753,10 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
   const int l32 = lane & 31, hh = lane >> 5;
   const int G = p.Hq / p.Hkv;
   int b, rt;
-  if (!wide_item<BM>(p, blockIdx.x / p.Hkv, lane, b, rt)) return;  // uniform, before any barrier
+  KeyTiles kt;
+  if (!wide_item<BM>(p, blockIdx.x / p.Hkv, lane, b, rt, kt)) return;  // uniform, before any barrier
   const int head = wide_head(p, b);
-  KeyTiles kt = key_tiles(p, b);
-  kt.seq = __builtin_amdgcn_readfirstlane(kt.seq);
-  kt.n = __builtin_amdgcn_readfirstlane(kt.n);
-  const int64_t tok0 = __builtin_amdgcn_readfirstlane(kt.tok0);
+  const int64_t tok0 = kt.tok0;
   WideSpan sp = wide_span<BM>(p, kt, rt);
   const int sink = __builtin_amdgcn_readfirstlane(sp.sink), first = __builtin_amdgcn_readfirstlane(sp.first);
   const int hi_max = __builtin_amdgcn_readfirstlane(sp.hi_max), lo_min = __builtin_amdgcn_readfirstlane(sp.lo_min);
@@ -780,15 +785,6 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
   const int wlo_max = __builtin_amdgcn_readfirstlane(p.window > 0 ? w1 - p.window + 1 : 0);
 
   X8 qreg[KSTEPS];
-#pragma unroll
-  for (int kk = 0; kk < KSTEPS; ++kk) {
-    const int col = 16 * kk + 8 * hh;
-    u32x4 raw = {0, 0, 0, 0};
-    if (row_ok && col < p.D) raw = ldg16((const T*)p.q + (tok0 + tok) * p.sqt + (int64_t)hq * p.sqh + col);
-    if (p.scale_log2 < 0.f) raw ^= 0x80008000u;
-    qreg[kk] = __builtin_bit_cast(X8, raw);
-  }
-
   auto key_of = [&](int t) -> int { return (t < sink ? t : t - sink + first) * BN; };
   const __attribute__((address_space(4))) int32_t* table =
       (const __attribute__((address_space(4))) int32_t*)(p.block_tables + (int64_t)b * p.sbt);
@@ -990,6 +986,16 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
 
   // K of tile t lies in buffer t & 1, V in 2 + (t & 1) (counted from t_lo on).
   // Step t needs K(t + 1), V(t) and scores(t); it brings K(t + 2) and V(t + 1) to LDS.
+  auto load_q = [&]() {  // the B operand of S^T: row l32, columns 16 kk + 8 hh .. + 7
+#pragma unroll
+    for (int kk = 0; kk < KSTEPS; ++kk) {
+      const int col = 16 * kk + 8 * hh;
+      u32x4 raw = {0, 0, 0, 0};
+      if (row_ok && col < p.D) raw = ldg16((const T*)p.q + (tok0 + tok) * p.sqt + (int64_t)hq * p.sqh + col);
+      if (p.scale_log2 < 0.f) raw ^= 0x80008000u;
+      qreg[kk] = __builtin_bit_cast(X8, raw);
+    }
+  };
   Codes kc, vc;
   int b1 = block_at(t_lo + 1), b2 = block_at(t_lo + 2), b3 = block_at(t_lo + 3);
   {
@@ -999,6 +1005,7 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
       load_codes(kc, K, p.skb, p.sks, p.skh, t_lo, bl);
       load_codes(k1, K, p.skb, p.sks, p.skh, t_lo + 1, b1);
       load_codes(vc, V, p.svb, p.svs, p.svh, t_lo, bl);
+      load_q();
       write_codes(kc, 0, 0);
       load_codes(kc, K, p.skb, p.sks, p.skh, t_lo + 2, b2);
       write_codes(k1, 1, 0);
@@ -1008,6 +1015,7 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
       load_direct(K, p.skb, p.sks, p.skh, t_lo, bl, 0);
       load_direct(K, p.skb, p.sks, p.skh, t_lo + 1, b1, 1);
       load_direct(V, p.svb, p.svs, p.svh, t_lo, bl, 2);
+      load_q();
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
   }
@@ -1103,9 +1111,9 @@ __global__ __launch_bounds__(NW * 64) void fa_window_wide_combine_kernel(const W
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, dt = blockIdx.y;
   const int l32 = lane & 31, hh = lane >> 5, G = p.Hq / p.Hkv;
   int b, rt;
-  if (!wide_item<BM>(p, blockIdx.x / p.Hkv, lane, b, rt)) return;
+  KeyTiles kt;
+  if (!wide_item<BM>(p, blockIdx.x / p.Hkv, lane, b, rt, kt)) return;
   const int head = wide_head(p, b);
-  const KeyTiles kt = key_tiles(p, b);
   const int count = wide_span<BM>(p, kt, rt).count, share = split_share(count, p.splits);
   if (count <= share) return;  // already in o
   const int n = (count + share - 1) / share;
