@@ -14,7 +14,10 @@ Two decode loops:
            and written into a paged cache ([num_blocks, block_size, Hkv, D],
            the engine's layout, engine/config.py:5-7), and attention is
            paged_attention_decode over the block tables. Static shapes, no
-           host synchronisation: one graph replay per step.
+           host synchronisation: one graph replay per step. --kv-e4m3 keeps
+           the cache in 8 bits (kv_cache_append after the rotation, half the
+           bytes that a step reads of it), --window W [--sinks S] attends to
+           the last W tokens and the first S only.
 
     python -m lightserve_amd.model.graph_decode [--mode full|kvcache|both] [--n-layers 4] ...
 
@@ -30,6 +33,7 @@ import torch
 import torch.nn.functional as F
 
 from ..kernels.paged_attention import paged_attention_decode, paged_prefill
+from ..kernels.quantized_kv_cache import kv_cache_append, quantized_kv_cache
 from ..kernels.rope import apply_rope_
 from ..kernels.fused_rmsnorm_residual import fused_add_rmsnorm
 from ..kernels.greedy import greedy_next_token
@@ -116,9 +120,13 @@ class KVCacheDecoder:
     State on the device: tokens [B] (the step's input), seq_lens [B] (tokens
     cached so far), k/v caches per layer and the block tables. step() issues
     only device work of static shape, so it can be captured and replayed;
-    prefill() caches a prompt chunk by chunk before the decode steps."""
+    prefill() caches a prompt chunk by chunk before the decode steps.
 
-    def __init__(self, weights, config, batch_size, block_size=16, device="cuda", shuffle_blocks=True, seed=0):
+    kv_e4m3 keeps K and V in 8 bits (quantized_kv_cache); window and sinks
+    limit what a token attends to (paged_attention.py)."""
+
+    def __init__(self, weights, config, batch_size, block_size=16, device="cuda", shuffle_blocks=True, seed=0, *,
+                 kv_e4m3=False, window=None, sinks=0):
         self.w, self.cfg, self.B = weights, config, batch_size
         nkv, hd = config.kv_heads, config.head_dim
         self.bs = block_size
@@ -128,11 +136,29 @@ class KVCacheDecoder:
             else torch.arange(n_blocks)
         self.block_tables = order.to(torch.int32).view(batch_size, self.max_blocks).to(device)
         shape = (n_blocks, block_size, nkv, hd)
-        self.k_cache = [torch.zeros(shape, dtype=config.dtype, device=device) for _ in weights.layers]
-        self.v_cache = [torch.zeros(shape, dtype=config.dtype, device=device) for _ in weights.layers]
+        self.kv_scales = [None for _ in weights.layers]
+        if kv_e4m3:
+            caches = [quantized_kv_cache(*shape, device=device) for _ in weights.layers]
+            self.k_cache, self.v_cache, self.kv_scales = ([c[i] for c in caches] for i in range(3))
+        else:
+            self.k_cache = [torch.zeros(shape, dtype=config.dtype, device=device) for _ in weights.layers]
+            self.v_cache = [torch.zeros(shape, dtype=config.dtype, device=device) for _ in weights.layers]
+        self.attention = dict(window=window, sinks=sinks)
         self.seq_lens = torch.zeros(batch_size, dtype=torch.int32, device=device)
         self.tokens = torch.full((batch_size,), SEED_TOKEN_ID, dtype=torch.long, device=device)
         self.cos, self.sin = precompute_rope(config, device)
+
+    def rotate_and_append(self, i, q, k, v, positions, lens, cu=None, **where):
+        """RoPE of q and k [B, n, heads, head_dim] in place and K/V into layer i's cache: one launch, or for an 8-bit
+        cache two. where: the slots or block_tables of apply_rope_; cu: the offsets of n > 1 rows a sequence."""
+        q4, k4, v4 = (x.transpose(1, 2) for x in (q, k, v))
+        if self.kv_scales[i] is None:
+            apply_rope_(q4, k4, self.cos, self.sin, positions=positions, v=v4, k_cache=self.k_cache[i],
+                        v_cache=self.v_cache[i], **where)
+        else:
+            apply_rope_(q4, k4, self.cos, self.sin, positions=positions)
+            kv_cache_append(k.flatten(0, 1), v.flatten(0, 1), self.k_cache[i], self.v_cache[i], self.kv_scales[i],
+                            self.block_tables, lens, cu)
 
     def step(self):
         """Logits [B, vocab] of the current tokens; appends their K/V."""
@@ -149,11 +175,10 @@ class KVCacheDecoder:
                 x_in, r_in, layer.input_layernorm_weight, cfg.rms_eps, (layer.q_proj, layer.k_proj, layer.v_proj))
             # RoPE at each sequence's position; the same launch stores the rotated k and v rows at the slot
             # its block table gives for that position
-            apply_rope_(q.view(B, nh, 1, hd), k.view(B, nkv, 1, hd), self.cos, self.sin, positions=pos,
-                        v=v.view(B, nkv, 1, hd), k_cache=self.k_cache[i], v_cache=self.v_cache[i],
-                        block_tables=self.block_tables)
+            self.rotate_and_append(i, q.view(B, 1, nh, hd), k.view(B, 1, nkv, hd), v.view(B, 1, nkv, hd), pos, lens,
+                                   block_tables=self.block_tables)
             o = paged_attention_decode(q.view(B, nh, hd), self.k_cache[i], self.v_cache[i], self.block_tables,
-                                       lens, max_seq_len=cfg.max_seq_len)
+                                       lens, max_seq_len=cfg.max_seq_len, kv_scales=self.kv_scales[i], **self.attention)
             (gate, up), residual = add_rmsnorm_matmul_shared_input(
                 matmul(o.view(B, nh * hd), layer.o_proj), residual, layer.post_attention_layernorm_weight,
                 cfg.rms_eps, (layer.gate_proj, layer.up_proj))
@@ -186,11 +211,10 @@ class KVCacheDecoder:
             for i, layer in enumerate(self.w.layers):
                 h, residual = add_norm(pending, residual, layer.input_layernorm_weight, cfg.rms_eps)
                 q, k, v = matmul_shared_input(h, (layer.q_proj, layer.k_proj, layer.v_proj))
-                apply_rope_(q.view(B, c, nh, hd).transpose(1, 2), k.view(B, c, nkv, hd).transpose(1, 2),
-                            self.cos, self.sin, positions=pos, v=v.view(B, c, nkv, hd).transpose(1, 2),
-                            k_cache=self.k_cache[i], v_cache=self.v_cache[i], slots=slot)
+                self.rotate_and_append(i, q.view(B, c, nh, hd), k.view(B, c, nkv, hd), v.view(B, c, nkv, hd), pos, lens, cu,
+                                       slots=slot)
                 o = paged_prefill(q.view(B * c, nh, hd), self.k_cache[i], self.v_cache[i], self.block_tables, cu, lens,
-                                  max_seqlen_q=c)
+                                  max_seqlen_q=c, kv_scales=self.kv_scales[i], **self.attention)
                 h2, residual = fused_add_rmsnorm(matmul(o.view(B * c, nh * hd), layer.o_proj), residual,
                                                  layer.post_attention_layernorm_weight, cfg.rms_eps)
                 gate, up = matmul_shared_input(h2, (layer.gate_proj, layer.up_proj))
@@ -218,7 +242,12 @@ def summarize(lat):
 def make_decoder(mode, weights, config, args):
     if mode == "full":
         return FullRecomputeDecoder(weights, config, args.batch_size)
-    return KVCacheDecoder(weights, config, args.batch_size, block_size=args.block_size)
+    return KVCacheDecoder(weights, config, args.batch_size, block_size=args.block_size, **cache_options(args))
+
+
+def cache_options(args):
+    """KVCacheDecoder's options among the command's."""
+    return dict(kv_e4m3=args.kv_e4m3, window=args.window, sinks=args.sinks)
 
 
 def step_fn(dec):
@@ -264,7 +293,7 @@ def prefill_main(args):
     weights = init_weights(config, device="cuda", seed=args.seed)
     prompt = torch.randint(0, config.vocab_size, (args.batch_size, P), generator=torch.Generator().manual_seed(1))
     prompt = prompt.cuda()
-    dec = KVCacheDecoder(weights, config, args.batch_size, block_size=args.block_size)
+    dec = KVCacheDecoder(weights, config, args.batch_size, block_size=args.block_size, **cache_options(args))
     lat = []
     for i in range(args.warmup_steps + args.num_steps):
         dec.seq_lens.zero_()
@@ -303,6 +332,9 @@ def main(argv=None):
                     help="instead of decode steps: time the chunked prefill of a P-token prompt per sequence "
                          "(max_seq_len is raised to fit it)")
     ap.add_argument("--chunk", type=int, default=512, help="prefill chunk size")
+    ap.add_argument("--kv-e4m3", action="store_true", help="8-bit KV cache (kvcache mode and --prefill)")
+    ap.add_argument("--window", type=int, default=None, metavar="W", help="sliding window of W tokens (as --kv-e4m3)")
+    ap.add_argument("--sinks", type=int, default=0, metavar="S", help="first tokens that stay visible under --window")
     args = ap.parse_args(argv)
     assert torch.cuda.is_available(), "needs a GPU"
     if args.prefill:

@@ -16,7 +16,8 @@ Contents
                 values) and paged attention with a window and sinks.
   model.py      the reference's model forward in plain torch (RoPE tables and
                 rotation, RMSNorm, the fused add + RMSNorm's semantics,
-                reference_llama_forward, with GQA).
+                reference_llama_forward, with GQA; the same in float64
+                under a window over given K/V rows).
 
 How each function is pinned (tests/test_oracle.py):
   attention_reference   pure-Python loops (golden fixtures under tests/golden),
@@ -38,6 +39,8 @@ How each function is pinned (tests/test_oracle.py):
   model.add_rmsnorm_reference  h and out written out by hand per element
                         (pure-Python sums), with and without the residual; unit
                         RMS with a unit weight (tests/test_oracle_model.py).
+  model.windowed_llama_forward   reference_llama_forward, and by what a planted
+                        window, sink or row changes (tests/test_oracle_model.py).
   model.reference_llama_forward  a pure-Python float64 one-layer forward.
 Every function has at least one check that a planted mistake (a dropped
 scale, a transposed operand, a wrong mask offset) fails.

@@ -94,3 +94,36 @@ def reference_llama_forward(weights, config, input_ids, causal=True):
         mlp = F.silu(F.linear(normed2, layer.gate_proj.t())) * F.linear(normed2, layer.up_proj.t())
         residual = residual + F.linear(mlp, layer.down_proj.t())
     return F.linear(rmsnorm(residual, weights.norm_weight, config.rms_eps), weights.lm_head.t())
+
+
+def windowed_llama_forward(weights, config, input_ids, window=None, sinks=0, held=None, rows=None):
+    """reference_llama_forward in float64 on the CPU, causal, with a sliding window and sinks. held: what a cache stands for
+    in place of K (rotated) and V, for each layer (k, v) [B, N, kv heads, head_dim]; rows, a list, is given the layers' own."""
+    B, N = input_ids.shape
+    hd, nh = config.head_dim, config.n_heads
+    nkv = config.n_kv_heads or nh
+    cv = lambda t: t.double().cpu()  # noqa: E731
+    cos, sin = (cv(t) for t in precompute_rope(hd, config.max_seq_len, config.rope_theta, config.dtype, "cpu"))
+    residual = F.embedding(input_ids.cpu(), cv(weights.embed_tokens))
+    p, j = torch.arange(N)[:, None], torch.arange(N)
+    seen = j <= p
+    if window is not None:
+        seen &= (j > p - window) | (j < sinks)
+    for i, layer in enumerate(weights.layers):
+        normed = rmsnorm(residual, cv(layer.input_layernorm_weight), config.rms_eps)
+        q = (normed @ cv(layer.q_proj)).view(B, N, nh, hd).transpose(1, 2)
+        k = (normed @ cv(layer.k_proj)).view(B, N, nkv, hd).transpose(1, 2)
+        v = (normed @ cv(layer.v_proj)).view(B, N, nkv, hd).transpose(1, 2)
+        q, k = apply_rope(q, k, cos, sin, N)
+        if rows is not None:
+            rows.append((k.transpose(1, 2), v.transpose(1, 2)))
+        if held is not None:
+            k, v = (t.transpose(1, 2) for t in held[i])
+        k, v = (t.repeat_interleave(nh // nkv, dim=1) for t in (k, v))
+        s = (q @ k.transpose(2, 3) / hd ** 0.5).masked_fill(~seen, float("-inf"))
+        attn = (s.softmax(-1) @ v).transpose(1, 2).reshape(B, N, nh * hd)
+        residual = residual + attn @ cv(layer.o_proj)
+        normed2 = rmsnorm(residual, cv(layer.post_attention_layernorm_weight), config.rms_eps)
+        mlp = F.silu(normed2 @ cv(layer.gate_proj)) * (normed2 @ cv(layer.up_proj))
+        residual = residual + mlp @ cv(layer.down_proj)
+    return rmsnorm(residual, cv(weights.norm_weight), config.rms_eps) @ cv(weights.lm_head)

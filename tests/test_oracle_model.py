@@ -157,3 +157,25 @@ def test_add_rmsnorm_reference_matches_loops(with_residual):
     # unit RMS before the weight
     ones, _ = om.add_rmsnorm_reference(x, r, torch.ones(5, dtype=torch.float64), 0.0)
     torch.testing.assert_close(ones.pow(2).mean(-1), torch.ones(3, dtype=torch.float64))
+
+
+def test_windowed_forward_without_a_window_is_the_reference_forward():
+    """windowed_llama_forward: the plain forward's logits in float32 weights, and sensitive to the window, the sinks and rows that stand in for K and V."""
+    from dataclasses import replace
+
+    from lightserve_amd.model.minimal_llama import TOY_CONFIG, init_weights
+    from oracle.model import reference_llama_forward, windowed_llama_forward
+    config = replace(TOY_CONFIG, n_kv_heads=2, dtype=torch.float32)
+    weights = init_weights(config, device="cpu", seed=0)
+    ids = torch.randint(0, config.vocab_size, (2, 24), generator=torch.Generator().manual_seed(1))
+    plain = windowed_llama_forward(weights, config, ids)
+    torch.testing.assert_close(plain, reference_llama_forward(weights, config, ids).double(), atol=1e-4, rtol=1e-4)
+    torch.testing.assert_close(windowed_llama_forward(weights, config, ids, window=24), plain, atol=1e-12, rtol=0)
+    last = windowed_llama_forward(weights, config, ids, window=8, sinks=2)
+    torch.testing.assert_close(last[:, :8], plain[:, :8], atol=1e-12, rtol=0)
+    rows = []
+    windowed_llama_forward(weights, config, ids, window=8, sinks=2, rows=rows)
+    torch.testing.assert_close(windowed_llama_forward(weights, config, ids, window=8, sinks=2, held=rows), last, atol=1e-12, rtol=0)
+    turned = [(k, v.flip(1)) for k, v in rows]
+    for other in (dict(window=9, sinks=2), dict(window=8, sinks=1), dict(window=8, sinks=2, held=turned)):
+        assert (windowed_llama_forward(weights, config, ids, **other) - last)[:, -1].abs().mean() > 1e-3
