@@ -156,10 +156,40 @@ __device__ __forceinline__ f32x4 load_device(const float* from) {
                __uint_as_float((uint32_t)(b >> 32))};
 }
 
+// 0 * infinity is NaN, so a row that does not see a key must not add that key's infinities
+// and NaN with its weight of zero. The narrow kernel takes such elements of V as zeros where
+// a mask cuts a tile for some of a chunk's rows and, if there were any (ordinary caches have
+// none), adds them to the rows that see their keys before the sums leave the registers; the
+// wide one takes the sums of a wave again, key by key, if they are not finite.
+// Ones in the elements of a word of V that are infinite or NaN (e4m3: NaN).
+template <typename T, bool Q8>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  if constexpr (Q8) return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
+  constexpr uint32_t e = __is_same(T, _Float16) ? 0x7c007c00u : 0x7f807f80u;  // exponents of ones
+  const uint32_t x = w & e;
+  return ((x & 0xffffu) == (e & 0xffffu) ? 0xffffu : 0u) | ((x & 0xffff0000u) == (e & 0xffff0000u) ? 0xffff0000u : 0u);
+}
+template <int N, typename A>
+__device__ __forceinline__ bool all_finite(const A (&acc)[N]) {
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(A) / 4); ++i) s = fmaf(acc[j][i], 0.f, s);
+  return s == 0.f;
+}
+// Element k of words of V, infinite or NaN, or zero.
+template <typename T, bool Q8>
+__device__ __forceinline__ float bad_value(const uint32_t* w, int k) {
+  if constexpr (Q8) return (w[k / 4] >> (8 * (k & 3)) & 0xff) != 0 ? __builtin_nanf("") : 0.f;
+  return (float)__builtin_bit_cast(T, (uint16_t)(w[k / 2] >> (16 * (k & 1))));
+}
+
 constexpr int kRowTile = 16;  // rows of a column block; a row tile has one or two
 
-// NC column blocks of 16 rows share the tile's K and V operands.
-template <typename T, typename C, int DP, int NC>
+// NC column blocks of 16 rows share the tile's K and V operands. ONE: of a decode step, whose
+// rows all see the same keys.
+template <typename T, typename C, int DP, int NC, bool ONE>
 __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowParams p) {
   using X8 = typename VecT<T>::x8;
   constexpr bool Q8 = sizeof(C) == 1;
@@ -340,6 +370,8 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
       for (int j = 0; j < VJ; ++j) acc[x][j] = f32x4{};
     }
 
+    auto whole = [&](int key0) -> bool { return key0 + 31 <= hi_min && (key0 >= lo_max || key0 + 31 < sinks); };
+    bool bad = false;  // V had infinities or NaN in a tile that the mask cuts
     const T* my_q = st_q[head - head_0];
     int b0 = block_at(wave_k, 0), b1 = block_at(wave_k, 1);
     Piece c0 = piece_of(wave_k, b0, 0), c1 = piece_of(wave_k, b1, 1);
@@ -397,8 +429,8 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
           for (int x = 0; x < NC; ++x) s[x][h][i] *= ks;
         }
       load_s(t, c0, 0), load_s(t, c1, 1);
-      const bool whole = key0 + 31 <= hi_min && (key0 >= lo_max || key0 + 31 < sinks);
-      if (!whole) {
+      if (!whole(key0)) {
+        uint32_t found = 0;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -411,8 +443,16 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
             const bool used = key <= hi_max && (key >= lo_min || key < sinks);
             if (!used) vs[h][i] = 1.f;
 #pragma unroll
-            for (int w = 0; w < VW; ++w) t.v[h][i][w] = used ? t.v[h][i][w] : 0u;
+            for (int w = 0; w < VW; ++w) {
+              t.v[h][i][w] = used ? t.v[h][i][w] : 0u;
+              if constexpr (!ONE) {
+                const uint32_t x = not_finite<T, Q8>(t.v[h][i][w]);
+                t.v[h][i][w] &= ~x;
+                found |= x;
+              }
+            }
           }
+        if (!ONE) bad |= __builtin_amdgcn_ballot_w64(found != 0) != 0;
       }
       X8 pb[NC];
 #pragma unroll
@@ -469,6 +509,34 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
         if (w & 1) __builtin_amdgcn_sched_barrier(0);
       }
       load_v(t, c0, 0), load_v(t, c1, 1);
+    }
+
+    if (!ONE && __builtin_expect(bad, 0)) {
+#pragma unroll 1
+      for (int u = wave_k; u < nt; u += nk) {
+        const int key0 = key_of(u);
+        if (whole(key0)) continue;
+#pragma unroll 1
+        for (int key = key0; key < key0 + 32; ++key) {
+          const int piece = (key - key0) >> 4;
+          const Piece at_key = piece_of(u, block_at(u, piece), piece);
+          const __amdgpu_buffer_rsrc_t rs =
+              piece_rsrc(vbase + ((uint64_t)at_key.blk * vblock + (uint64_t)(at_key.slot + (key & 15)) * vslot), (p.D * EB) & at_key.live);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {  // channels (4 g + i) VJ ..
+            uint32_t v[VW];
+            load_words<VW>(rs, (4 * g + i) * VJ < p.D ? (4 * g + i) * VJ * EB : (int)kOut, v);
+#pragma unroll
+            for (int w = 0; w < VW; ++w) v[w] &= not_finite<T, Q8>(v[w]);
+#pragma unroll
+            for (int x = 0; x < NC; ++x)
+              if (key <= hi[x] && (key >= lo[x] || key < sinks)) {
+#pragma unroll
+                for (int j = 0; j < VJ; ++j) acc[x][j][i] += bad_value<T, Q8>(v, j);
+              }
+          }
+        }
+      }
     }
 
     // Merge the waves, a column block at a time. A wave without a tile has m = -1e30
@@ -727,6 +795,15 @@ __device__ __forceinline__ int split_share(int count, int splits) {
 // each row, then O in the accumulators' own order, [wave][4-register group][lane].
 template <int BM, int DP> constexpr int kWidePart = BM * 4 + BM * DP;
 
+// The kernel's arguments, read again. What only the end needs is taken from here: kept in
+// scalar registers through the loop it would push the loop's own ones out of them, and the
+// loop's reads of LDS then all wait for each other.
+__device__ __forceinline__ const __attribute__((address_space(4))) WindowParams* arguments() {
+  auto a = (const __attribute__((address_space(4))) WindowParams*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  return a;
+}
+
 template <typename T> constexpr float kWideMaxLog2P = 64.0f;
 template <> constexpr float kWideMaxLog2P<_Float16> = 15.0f;
 
@@ -798,31 +875,38 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
   // NL + i in instruction i, so that a lane's rows have adjacent scales; 16-bit: what
   // the direct load's linear LDS order makes of the swizzled tile.
   auto row_at = [&](int i) -> int { return Q8 ? lane / LPR * NL + i : i * RPL + lane / LPR; };
-  auto offset = [&](int i, int64_t stride, int key0) -> int {
+  auto offset = [&](int i, uint32_t slot, int key0) -> int {
     const int row = row_at(i), key = key0 + RPW * wave + row;
     const int col = 8 * (Q8 ? lane % LPR : (lane % LPR) ^ seg_swz<DP>(RPW * wave + row));
     const bool used = col < p.D && key <= hi_max && (key >= lo_min || key < sinks);
-    return used ? (row * (int)stride + col) * EB : (int)0x80000000;
+    return used ? row * (int)slot + col * EB : (int)0x80000000;
   };
-  auto rows_of = [&](const C* base, int64_t sb, int64_t ss, int64_t sh, int t, int blk) -> __amdgpu_buffer_rsrc_t {
+  // The head's rows of block 0 and the byte strides (below 2^32) of a block and a slot.
+  struct Cache {
+    const char* base;
+    uint32_t block, slot;
+  };
+  const Cache K = {(const char*)p.kc + (int64_t)head * p.skh * EB, (uint32_t)(p.skb * EB), (uint32_t)(p.sks * EB)};
+  const Cache V = {(const char*)p.vc + (int64_t)head * p.svh * EB, (uint32_t)(p.svb * EB), (uint32_t)(p.svs * EB)};
+  auto rows_of = [&](const Cache& c, int t, int blk) -> __amdgpu_buffer_rsrc_t {
     const bool live = (unsigned)blk < (unsigned)p.num_blocks;
-    const int slot = (key_of(t) + RPW * wave) & ((1 << p.block_shift) - 1);
-    return tile_rsrc(base + (live ? (int64_t)blk * sb + (int64_t)slot * ss + (int64_t)head * sh : 0),
-                     live ? (int)(((RPW - 1) * ss + p.D) * EB) : 0);
+    const uint32_t slot = (key_of(t) + RPW * wave) & ((1 << p.block_shift) - 1);
+    return tile_rsrc(c.base + (live ? (uint64_t)blk * c.block + (uint64_t)slot * c.slot : 0),
+                     live ? (int)((RPW - 1) * c.slot + p.D * EB) : 0);
   };
   constexpr int EW = NL == 4 ? 2 : 1;  // words of a lane's scales (K and V of NL rows)
   struct Codes {
     u32x2 w[NL];
     uint32_t e[EW];
   };
-  auto load_codes = [&](Codes& c, const C* base, int64_t sb, int64_t ss, int64_t sh, int t, int blk) {
-    const __amdgpu_buffer_rsrc_t rs = rows_of(base, sb, ss, sh, t, blk);
+  auto load_codes = [&](Codes& c, const Cache& of, int t, int blk) {
+    const __amdgpu_buffer_rsrc_t rs = rows_of(of, t, blk);
     const bool live = (unsigned)blk < (unsigned)p.num_blocks;
     const int slot = (key_of(t) + RPW * wave) & ((1 << p.block_shift) - 1);
     const uint8_t* sb8 = p.scales + (live ? ((((int64_t)blk * p.Hkv + head) << p.block_shift) + slot) * 2 : 0);
     const __amdgpu_buffer_rsrc_t es = tile_rsrc(sb8, live ? 2 * RPW : 0);
 #pragma unroll
-    for (int i = 0; i < NL; ++i) c.w[i] = load8b(rs, offset(i, ss, key_of(t)));
+    for (int i = 0; i < NL; ++i) c.w[i] = load8b(rs, offset(i, of.slot, key_of(t)));
     if constexpr (NL == 1) c.e[0] = load2(es, 2 * row_at(0));
     else load_words<EW>(es, 2 * row_at(0), c.e);
   };
@@ -841,14 +925,12 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
       *(LDS_AS u32x4*)(smem + buf * TILE * 2 + (woff ^ (i * (DP == 128 ? 0x140 : 0x80)))) = v;
     }
   };
-  auto load_direct = [&](const C* base, int64_t sb, int64_t ss, int64_t sh, int t, int blk, int buf) {
-    const __amdgpu_buffer_rsrc_t rs = rows_of(base, sb, ss, sh, t, blk);
+  auto load_direct = [&](const Cache& of, int t, int blk, int buf) {
+    const __amdgpu_buffer_rsrc_t rs = rows_of(of, t, blk);
 #pragma unroll
     for (int i = 0; i < NL; ++i)
-      dma16(rs, (LDS_AS void*)(smem + buf * TILE * 2 + (RPW * wave + i * RPL) * DP * 2), offset(i, ss, key_of(t)));
+      dma16(rs, (LDS_AS void*)(smem + buf * TILE * 2 + (RPW * wave + i * RPL) * DP * 2), offset(i, of.slot, key_of(t)));
   };
-  const C* K = (const C*)p.kc;
-  const C* V = (const C*)p.vc;
 
   // LDS offsets of the operands: the segment index of a column step differs from
   // the first one's by an xor of whole bits (swz_off), so one register each does
@@ -1002,19 +1084,19 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
     const int bl = block_at(t_lo);
     if constexpr (Q8) {
       Codes k1;
-      load_codes(kc, K, p.skb, p.sks, p.skh, t_lo, bl);
-      load_codes(k1, K, p.skb, p.sks, p.skh, t_lo + 1, b1);
-      load_codes(vc, V, p.svb, p.svs, p.svh, t_lo, bl);
+      load_codes(kc, K, t_lo, bl);
+      load_codes(k1, K, t_lo + 1, b1);
+      load_codes(vc, V, t_lo, bl);
       load_q();
       write_codes(kc, 0, 0);
-      load_codes(kc, K, p.skb, p.sks, p.skh, t_lo + 2, b2);
+      load_codes(kc, K, t_lo + 2, b2);
       write_codes(k1, 1, 0);
       write_codes(vc, 2, 1);
-      load_codes(vc, V, p.svb, p.svs, p.svh, t_lo + 1, b1);
+      load_codes(vc, V, t_lo + 1, b1);
     } else {
-      load_direct(K, p.skb, p.sks, p.skh, t_lo, bl, 0);
-      load_direct(K, p.skb, p.sks, p.skh, t_lo + 1, b1, 1);
-      load_direct(V, p.svb, p.svs, p.svh, t_lo, bl, 2);
+      load_direct(K, t_lo, bl, 0);
+      load_direct(K, t_lo + 1, b1, 1);
+      load_direct(V, t_lo, bl, 2);
       load_q();
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
@@ -1031,11 +1113,11 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
     if constexpr (Q8) {
       write_codes(kc, par, 0);
       write_codes(vc, 2 + (par ^ 1), 1);
-      load_codes(kc, K, p.skb, p.sks, p.skh, t + 3, b3);
-      load_codes(vc, V, p.svb, p.svs, p.svh, t + 2, b2);
+      load_codes(kc, K, t + 3, b3);
+      load_codes(vc, V, t + 2, b2);
     } else {
-      load_direct(K, p.skb, p.sks, p.skh, t + 2, b2, par);
-      load_direct(V, p.svb, p.svs, p.svh, t + 1, b1, 2 + (par ^ 1));
+      load_direct(K, t + 2, b2, par);
+      load_direct(V, t + 1, b1, 2 + (par ^ 1));
     }
     if (t + 1 < t_hi && sees(t + 1)) {
       scores(par ^ 1, nxt);
@@ -1058,47 +1140,136 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
   if (t < t_hi) step(t, 0, s0, s1);
 
   const float lt = half_sum(l_run), le = half_sum(l_lse);
-  if constexpr (SPLIT) {
-    if (!whole_item) {
-      float* part = p.part + ((int64_t)blockIdx.x * p.splits + blockIdx.y) * kWidePart<BM, DP>;
-      if (hh == 0) *(f32x4*)(part + (wave * 32 + l32) * 4) = f32x4{m_run, lt, le, 0.f};
-      f32x4* po = (f32x4*)(part + BM * 4) + wave * DT * 4 * 64 + lane;
+  auto leave = [&]() {
+    const auto* q = arguments();
+    if constexpr (SPLIT) {
+      if (!whole_item) {
+        float* part = q->part + ((int64_t)blockIdx.x * q->splits + blockIdx.y) * kWidePart<BM, DP>;
+        if (hh == 0) *(f32x4*)(part + (wave * 32 + l32) * 4) = f32x4{m_run, lt, le, 0.f};
+        f32x4* po = (f32x4*)(part + BM * 4) + wave * DT * 4 * 64 + lane;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            po[(dt * 4 + g) * 64] = f32x4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+        return;
+      }
+    }
+    // O leaves through LDS (the tiles' buffers are free after the last barrier):
+    // each wave stages its 32 rows and stores whole ones.
+    const float inv = lt == 0.f ? 0.f : 1.f / lt;
+    {
+      constexpr int BLK = 32 * DP * 2;
+      static_assert(NW * BLK <= 4 * TILE * 2, "O staging fits in the K/V buffers");
+      LDS_AS char* wb = smem + wave * BLK;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          po[(dt * 4 + g) * 64] = f32x4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
-      return;
-    }
-  }
-  // O leaves through LDS (the tiles' buffers are free after the last barrier):
-  // each wave stages its 32 rows and stores whole ones.
-  const float inv = lt == 0.f ? 0.f : 1.f / lt;
-  {
-    constexpr int BLK = 32 * DP * 2;
-    static_assert(NW * BLK <= 4 * TILE * 2, "O staging fits in the K/V buffers");
-    LDS_AS char* wb = smem + wave * BLK;
+        for (int g = 0; g < 4; ++g) {
+          X4 v;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+          for (int e = 0; e < 4; ++e) v[e] = (T)(acc[dt][4 * g + e] * inv);
+          *(LDS_AS X4*)(wb + swz_off<DP>(l32, 32 * dt + 8 * g + 4 * hh) * 2) = v;
+        }
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        X4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (T)(acc[dt][4 * g + e] * inv);
-        *(LDS_AS X4*)(wb + swz_off<DP>(l32, 32 * dt + 8 * g + 4 * hh) * 2) = v;
+      for (int c = 0; c < BLK / 1024; ++c) {
+        const int byte = c * 1024 + lane * 16;
+        const int row = byte / (DP * 2), seg = (byte % (DP * 2)) / 16;
+        const X8 v = *(const LDS_AS X8*)(wb + row * DP * 2 + ((seg ^ seg_swz<DP>(row)) << 4));
+        const int rr = r0 + row, tk = rr / G, h = head * G + (rr - tk * G);
+        if (rr < nrows && seg * 8 < q->D) *(X8*)((T*)q->o + (tok0 + tk) * q->sot + (int64_t)h * q->soh + seg * 8) = v;
       }
-#pragma unroll
-    for (int c = 0; c < BLK / 1024; ++c) {
-      const int byte = c * 1024 + lane * 16;
-      const int row = byte / (DP * 2), seg = (byte % (DP * 2)) / 16;
-      const X8 v = *(const LDS_AS X8*)(wb + row * DP * 2 + ((seg ^ seg_swz<DP>(row)) << 4));
-      const int rr = r0 + row, tk = rr / G, h = head * G + (rr - tk * G);
-      if (rr < nrows && seg * 8 < p.D) *(X8*)((T*)p.o + (tok0 + tk) * p.sot + (int64_t)h * p.soh + seg * 8) = v;
     }
-  }
-  if constexpr (LSE) {
-    if (row_ok && hh == 0 && p.lse != nullptr)
-      p.lse[(tok0 + tok) * p.slt + (int64_t)hq * p.slh] = le == 0.f ? -INFINITY : (m_run + __log2f(le)) * kWinLn2;
+    if constexpr (LSE) {
+      if (row_ok && hh == 0 && q->lse != nullptr)
+        q->lse[(tok0 + tok) * q->slt + (int64_t)hq * q->slh] = le == 0.f ? -INFINITY : (m_run + __log2f(le)) * kWinLn2;
+    }
+  };
+  leave();
+
+  // Sums that are not finite while V has infinities or NaN in a tile that the mask cuts are
+  // taken again, key by key: a lane holds half of its row of q, and adds each key's V where
+  // the row sees it. (Looking for them in every such tile of the loop, before they are
+  // multiplied, made 111 us of 98 of windowed prompts of a 16-bit cache.)
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(!all_finite(acc)) != 0, 0)) {
+    auto row_of = [&](const Cache& c, int key, int blk) -> const C* {
+      return (const C*)(c.base + (uint64_t)blk * c.block + (uint64_t)(key & ((1 << p.block_shift) - 1)) * c.slot);
+    };
+    bool bad = false;
+#pragma unroll 1
+    for (int u = t_lo; u < t_hi; ++u) {
+      const int key0 = key_of(u), key = key0 + lane;
+      if (key0 + BN - 1 <= whi_min && (key0 >= wlo_max || key0 + BN - 1 < sinks)) continue;
+      // (whatever the tile holds: other waves may see more than this one)
+      const bool used = key <= hi_max && (key >= lo_min || key < sinks);
+      const int blk = used ? table[key >> p.block_shift] : -1;
+      if ((unsigned)blk >= (unsigned)p.num_blocks) continue;
+      const C* row = row_of(V, key, blk);
+#pragma unroll 1
+      for (int i = 0; i < p.D; i += 8) {
+        const u32x2 w = *(const u32x2*)(row + i);
+        bad |= (not_finite<T, Q8>(w[0]) | not_finite<T, Q8>(w[1])) != 0;
+        if constexpr (!Q8) {
+          const u32x2 w4 = *(const u32x2*)(row + i + 4);
+          bad |= (not_finite<T, Q8>(w4[0]) | not_finite<T, Q8>(w4[1])) != 0;
+        }
+      }
+    }
+    if (__builtin_amdgcn_ballot_w64(bad) != 0) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
+#pragma unroll 1
+      for (int i = 0; i < (t_hi - t_lo) * BN; ++i) {
+        const int key = key_of(t_lo + i / BN) + i % BN;
+        if (key > whi_max) continue;
+        const int blk = table[key >> p.block_shift];
+        if ((unsigned)blk >= (unsigned)p.num_blocks) continue;
+        float ks = 1.f, vs = 1.f;
+        if constexpr (Q8) {
+          const uint8_t* e = p.scales + ((((int64_t)blk * p.Hkv + head) << p.block_shift) + (key & ((1 << p.block_shift) - 1))) * 2;
+          ks = fminf(__uint_as_float((uint32_t)e[0] << 23), 0x1p127f);
+          vs = fminf(__uint_as_float((uint32_t)e[1] << 23), 0x1p127f);
+        }
+        const C* row = row_of(K, key, blk);
+        float s = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < KSTEPS; ++kk)
+          if (16 * kk + 8 * hh < p.D) {
+            X8 k8;
+            if constexpr (Q8) {
+              const u32x2 w = *(const u32x2*)(row + 16 * kk + 8 * hh);
+              k8 = __builtin_bit_cast(X8, u32x4{codes2<false>(w[0], ks, T()), codes2<true>(w[0], ks, T()), codes2<false>(w[1], ks, T()),
+                                                codes2<true>(w[1], ks, T())});
+            } else {
+              k8 = __builtin_bit_cast(X8, ldg16((const T*)row + 16 * kk + 8 * hh));
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s = fmaf((float)k8[e], (float)qreg[kk][e], s);
+          }
+        s = half_sum(s);
+        const float w = (float)(T)fast_exp2(fmaf(s, sl2, -m_run));
+        if (!(key <= hi && (key >= lo || key < sinks))) continue;
+        const C* vrow = row_of(V, key, blk);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int d = 32 * dt + 8 * g + 4 * hh;
+            if (d >= p.D) continue;
+            u32x2 v;
+            if constexpr (Q8) {
+              const uint32_t c = *(const uint32_t*)(vrow + d);
+              v = u32x2{codes2<false>(c, vs, T()), codes2<true>(c, vs, T())};
+            } else {
+              v = *(const u32x2*)(vrow + d);
+            }
+            const X4 v4 = __builtin_bit_cast(X4, v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[dt][4 * g + e] = fmaf(w, (float)v4[e], acc[dt][4 * g + e]);
+          }
+      }
+      leave();
+    }
   }
 }
 
@@ -1192,7 +1363,8 @@ WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int eb, int max
 template <typename T, typename C, int DP, int NC>
 static hipError_t launch_narrow(const WindowParams& p, const WindowPlan& w, hipStream_t s) {
   const int rt = kRowTile * NC, tiles = (p.max_n * (p.Hq / p.Hkv) + rt - 1) / rt;
-  hipLaunchKernelGGL((fa_window_narrow_kernel<T, C, DP, NC>), dim3(p.Hkv * tiles, p.runs), dim3(256), 0, s, p);
+  if (p.max_n == 1) hipLaunchKernelGGL((fa_window_narrow_kernel<T, C, DP, NC, true>), dim3(p.Hkv * tiles, p.runs), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((fa_window_narrow_kernel<T, C, DP, NC, false>), dim3(p.Hkv * tiles, p.runs), dim3(256), 0, s, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || w.long_run == 0) return e;
   hipLaunchKernelGGL((fa_window_combine_kernel<T, DP, NC>), dim3(p.Hkv * tiles, p.B, DP / 32), dim3(256), 0, s, p);

@@ -291,6 +291,116 @@ def test_nan_of_a_key_reaches_the_rows_that_see_it(gpu):
     assert torch.isfinite(o[0, :, :5]).all() and torch.isfinite(o[0, :, 6:]).all()
 
 
+@pytest.mark.parametrize("kind,bad", [("e4m3", math.nan), ("16 bit", math.nan), ("16 bit", math.inf), ("16 bit", -math.inf)])
+@pytest.mark.parametrize("n,heads,d", [(3, 4, 64), (6, 4, 128), (8, 8, 80), (40, 4, 64), (100, 2, 128), (200, 16, 64), (600, 32, 72)])
+def test_values_not_finite_reach_the_rows_that_see_them_alone(gpu, kind, bad, n, heads, d):
+    """V of a key that a chunk's later (or, at the window's start, earlier) queries do not see, in both kernels."""
+    print(f"case not finite {kind} {bad} n={n} heads={heads} d={d}", flush=True)
+    if kind == "e4m3" and d % 16 != 0:
+        d = 80
+    length, bs, dtype = n + 150, 16, torch.float16 if n == 40 else torch.bfloat16
+    table, pool = tables([length], bs, 54)
+    codes = cache8(pool, bs, 2, d, 55)
+    clean = paged8.cache_values(*codes)
+    q = _q(n, heads, d, dtype, 56)
+    at = [length - 2, length - n + 1, length - n - 40, 1, length - n - 58 + n // 2]
+    p = torch.arange(length - n, length)
+    for window, sinks in ((60, 2), (None, 0)):
+        if window is None and kind != "e4m3":
+            continue
+        kc, vc, sc = (t.clone() for t in codes)
+        if kind != "e4m3":
+            kc, vc, sc = clean[0].to(dtype), clean[1].to(dtype), None
+        for i, j in enumerate(at):
+            vc[table[0, j // bs], j % bs, :, 7 * i] = 127 if kind == "e4m3" else bad
+        dev = [t.cuda() if t is not None else None for t in (kc, vc, sc)]
+        if kind == "e4m3":
+            dev[:2] = [t.view(E4M3) for t in dev[:2]]
+        o, lse = paged_prefill(q.cuda(), dev[0], dev[1], table.cuda(), offsets([n]).cuda(),
+                               torch.tensor([length], dtype=torch.int32).cuda(), return_lse=True, kv_scales=dev[2],
+                               window=window, sinks=sinks)
+        o, ref = o.cpu(), paged8.window_reference(q, *clean, table, offsets([n]), [length], window, sinks)
+        for i, j in enumerate(at):
+            sees = (j <= p) & ((j > p - window) | (j < sinks) if window is not None else True)
+            got = o[:, :, 7 * i]
+            assert (torch.isnan(got[sees]).all() if math.isnan(bad) else (got[sees] == bad).all()), f"key {j}"
+            assert torch.isfinite(got[~sees]).all(), f"key {j}"
+            got[sees] = ref[0][:, :, 7 * i][sees].to(dtype)
+        _assert_close(o, lse.t(), ref, length, f"the others w={window}")
+
+
+# (kind, type, lengths from and to, sequences, heads, KV heads, head dim, queries, window, sinks): enough keys for every
+# workgroup to have a long run, whose partial results a launch of their own merges; one, two and four KV heads a
+# workgroup; one and two column blocks of rows; more sequences than lanes.
+LONG = [("e4m3", torch.bfloat16, 0, 8000, 20, 32, 8, 128, 1, None, 0), ("e4m3", torch.float16, 1500, 3500, 70, 8, 2, 64, 1, None, 0),
+        ("16 bit", torch.bfloat16, 15000, 25000, 6, 3, 3, 64, 1, 24000, 3), ("e4m3", torch.bfloat16, 2000, 3500, 70, 8, 4, 64, 1, 1500, 5),
+        ("16 bit", torch.float16, 20000, 30000, 5, 64, 8, 64, 3, 29000, 0), ("e4m3", torch.bfloat16, 0, 60000, 2, 64, 16, 80, 2, None, 0),
+        ("e4m3", torch.float16, 100, 20000, 9, 128, 16, 48, 4, 9000, 40)]
+
+
+@pytest.mark.parametrize("case", range(len(LONG)))
+def test_long_runs(gpu, case):
+    kind, dtype, least, most, batch, hq, hkv, d, new, window, sinks = LONG[case]
+    print(f"case long runs {LONG[case]}", flush=True)
+    g = torch.Generator().manual_seed(60 + case)
+    lens = torch.randint(least, most + 1, (batch,), generator=g).tolist()
+    lens[0] = most
+    if new == 1:
+        _decode(kind, dtype, lens, hq, hkv, d, 16, 70 + case, window, sinks, what=f"long runs {case}")
+    else:
+        n = [min(new - b % 2, m) for b, m in enumerate(lens)]
+        _chunk(kind, dtype, n, [m - k for m, k in zip(lens, n)], hq, hkv, d, 16, 70 + case, window, sinks, what=f"long runs {case}")
+
+
+@pytest.mark.parametrize("window", [None, 100])
+def test_chunks_of_many_sequences(gpu, window):
+    """More sequences than a wave has lanes, some without queries, in the wide kernel."""
+    print(f"case many chunks window={window}", flush=True)
+    g = torch.Generator().manual_seed(63)
+    new = [int(n) if b % 5 else 0 for b, n in enumerate(torch.randint(0, 90, (130,), generator=g))]
+    had = torch.randint(0, 300, (130,), generator=g).tolist()
+    _chunk("e4m3", torch.bfloat16, new, had, 8, 2, 64, 16, 64, window, 3 if window else 0, what=f"many chunks w={window}")
+
+
+def test_graph_follows_the_lengths(gpu):
+    """A captured step replayed after the lengths have changed: short runs, long ones, one sequence, none, and eager steps and
+    calls on another stream between and beside the replays."""
+    print("case graph lengths", flush=True)
+    B, hq, hkv, d, bs, most = 24, 32, 8, 128, 16, 4096
+    table, pool = tables([most] * B, bs, 65)
+    cache, _ = _cache("e4m3", torch.bfloat16, pool, bs, hkv, d, 66)
+    bt, q, sl = table.cuda(), _q(B, hq, d, torch.bfloat16, 67).cuda(), torch.full((B,), most, dtype=torch.int32).cuda()
+    lens = [[most] * B, [33] * B, [most] + [0] * (B - 1), [0] * B, [most - 100 * b for b in range(B)], [1] * B]
+
+    def step():
+        return paged_attention_decode(q, *cache[:2], bt, sl, max_seq_len=most, return_lse=True, kv_scales=cache[2])
+
+    want = []
+    for n in lens:
+        sl.copy_(torch.tensor(n, dtype=torch.int32))
+        want.append(step())
+    other = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    sl2 = torch.tensor(lens[4], dtype=torch.int32).cuda()
+    torch.cuda.synchronize()
+    for turn in range(2):
+        for i, n in enumerate(lens):
+            sl.copy_(torch.tensor(n, dtype=torch.int32))
+            with torch.cuda.stream(other):
+                beside = paged_attention_decode(q, *cache[:2], bt, sl2, max_seq_len=most, return_lse=True, kv_scales=cache[2])
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i])), f"turn {turn}: lengths {i}"
+            assert all(torch.equal(a, b) for a, b in zip(beside, want[4])), f"turn {turn}: beside lengths {i}"
+            assert all(torch.equal(a, b) for a, b in zip(step(), want[i])), f"turn {turn}: eager, lengths {i}"
+    for i, n in enumerate(lens[2:5]):
+        o, lse = want[2 + i]
+        none = torch.tensor(n) == 0
+        assert (o.cpu()[none] == 0).all() and (lse.cpu()[none] == -math.inf).all()
+
+
 def test_strided_inputs(gpu):
     """q inside a fused projection, caches of a wider allocation, a table with another column stride."""
     print("case strided", flush=True)
