@@ -84,6 +84,15 @@ __device__ __forceinline__ KeyTiles key_tiles(const WindowParams& p, int b) {
   return key_tiles_of(p, min(max(p.seq_lens[b], 0), min(p.max_seq_len, p.max_blocks << p.block_shift)), n, tok0);
 }
 
+// The kernel's arguments, read again. What only the beginning and the end of a run or item
+// need is taken from here: kept in scalar registers through the loop it would push the
+// loop's own ones out of them (the wide kernel's reads of LDS then all wait for each other).
+__device__ __forceinline__ const __attribute__((address_space(4))) WindowParams* arguments() {
+  auto a = (const __attribute__((address_space(4))) WindowParams*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  return a;
+}
+
 // Inclusive sum over the wave's lanes.
 __device__ __forceinline__ int lanes_sum(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
@@ -109,8 +118,8 @@ __device__ __forceinline__ int heads_per_group(const WindowParams& p) { return (
 // Partial result of run r of a row tile and KV head: O of part_rows rows, then (offset,
 // sum for O, sum for the lse, 0) of each. A run has two: the end of a sequence and,
 // first_run, the beginning of one.
-template <int DP>
-__device__ __forceinline__ float* part_of(const WindowParams& p, int rt, int head, int runs, int r, bool first_run) {
+template <int DP, typename P>
+__device__ __forceinline__ float* part_of(const P& p, int rt, int head, int runs, int r, bool first_run) {
   return p.part + (((int64_t)rt * p.Hkv + head) * 2 * runs + 2 * r + first_run) * (p.part_rows * (DP + 4));
 }
 // Sums over the keys of one row (offset M in log2 units) taking in those of others.
@@ -128,8 +137,8 @@ struct RowSums {
 
 // Channels d .. d + 3 of row r of a sequence and KV head from the sums over its keys
 // (offset M in log2 units), and its lse with channel 0.
-template <typename T>
-__device__ __forceinline__ void store_row(const WindowParams& p, int64_t tok0, int r, int G, int head, int d, float M, float L,
+template <typename T, typename P>
+__device__ __forceinline__ void store_row(const P& p, int64_t tok0, int r, int G, int head, int d, float M, float L,
                                           float E, const f32x4& O) {
   const int tok = r / G, h = head * G + (r - tok * G);
   const float inv = L == 0.f ? 0.f : 1.f / L;
@@ -293,11 +302,12 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
 
     // Q, the B operand of S^T, to LDS: kept in registers it would cost the waves that
     // keep the loads of K and V in flight.
+    const auto* args = arguments();
     for (int i = tid; i < hw * RT * (DP / 8); i += 256) {
       const int hs = i / (RT * (DP / 8)), row = i / (DP / 8) % RT, d = i % (DP / 8) * 8, r = rt * RT + row, tok = r / G;
       u32x4 raw = {0, 0, 0, 0};
-      if (row < nrows && d < p.D)
-        raw = ldg16((const T*)p.q + (tok0 + tok) * p.sqt + (int64_t)((head_0 + hs) * G + (r - tok * G)) * p.sqh + d);
+      if (row < nrows && d < args->D)
+        raw = ldg16((const T*)args->q + (tok0 + tok) * args->sqt + (int64_t)((head_0 + hs) * G + (r - tok * G)) * args->sqh + d);
       *(u32x4*)(st_q[hs] + row * QS + d) = raw;
     }
     // The lane's rows see keys lo .. hi.
@@ -559,6 +569,7 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
     // every wave waits for its own before the barrier ahead of the counter's add, and
     // the last run reads them with device-scope loads.
     const bool complete = ta == 0 && tb == count;
+    args = arguments();
 #pragma unroll
     for (int x = 0; x < NC; ++x) {
 #pragma unroll
@@ -580,16 +591,16 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
           O += a * *(const f32x4*)&st_o[w][row][d];
         }
         if (complete) {
-          store_row<T>(p, tok0, rt * RT + rr, G, head_0 + hs, d, M, L, E, O);
+          store_row<T>(*args, tok0, rt * RT + rr, G, head_0 + hs, d, M, L, E, O);
         } else {
-          float* part = part_of<DP>(p, rt, head_0 + hs, runs, run, ta == 0);
+          float* part = part_of<DP>(*args, rt, head_0 + hs, runs, run, ta == 0);
           const f32x4 st = {M, L, E, 0.f};
           if (deferred) {
             *(f32x4*)(part + rr * DP + d) = O;
-            if (d == 0) *(f32x4*)(part + p.part_rows * DP + 4 * rr) = st;
+            if (d == 0) *(f32x4*)(part + args->part_rows * DP + 4 * rr) = st;
           } else {
             store_device(part + rr * DP + d, O);
-            if (d == 0) store_device(part + p.part_rows * DP + 4 * rr, st);
+            if (d == 0) store_device(part + args->part_rows * DP + 4 * rr, st);
           }
         }
       }
@@ -600,7 +611,7 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the partials have reached device scope
     __syncthreads();
     if (tid == 0) {
-      int* counter = p.counters + column * runs + r0;
+      int* counter = args->counters + column * runs + r0;
       const bool last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == r1 - r0;
       if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       st_last = last;
@@ -621,8 +632,8 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
 #pragma unroll
           for (int k = 0; k < U; ++k) {
             const int rk = min(r + k * ng, r1);
-            const float* from = part_of<DP>(p, rt, head, runs, rk, rk == r0);
-            st[k] = load_device(from + p.part_rows * DP + 4 * row);
+            const float* from = part_of<DP>(*args, rt, head, runs, rk, rk == r0);
+            st[k] = load_device(from + args->part_rows * DP + 4 * row);
             o[k] = load_device(from + row * DP + d);
           }
 #pragma unroll
@@ -639,7 +650,7 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
         if (tid < items)
           for (int k = 1; k < ng; ++k) sum.take(meet[2 * (tid + k * items)], meet[2 * (tid + k * items) + 1]);
       }
-      if (idx < items && (ng == 1 || tid < items)) store_row<T>(p, tok0, rt * RT + row, G, head, d, sum.M, sum.L, sum.E, sum.O);
+      if (idx < items && (ng == 1 || tid < items)) store_row<T>(*args, tok0, rt * RT + row, G, head, d, sum.M, sum.L, sum.E, sum.O);
     }
     __syncthreads();
   }
@@ -794,15 +805,6 @@ __device__ __forceinline__ int split_share(int count, int splits) {
 // Floats of one split's partial results: (offset, sum for O, sum for the lse, 0) of
 // each row, then O in the accumulators' own order, [wave][4-register group][lane].
 template <int BM, int DP> constexpr int kWidePart = BM * 4 + BM * DP;
-
-// The kernel's arguments, read again. What only the end needs is taken from here: kept in
-// scalar registers through the loop it would push the loop's own ones out of them, and the
-// loop's reads of LDS then all wait for each other.
-__device__ __forceinline__ const __attribute__((address_space(4))) WindowParams* arguments() {
-  auto a = (const __attribute__((address_space(4))) WindowParams*)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(a));
-  return a;
-}
 
 template <typename T> constexpr float kWideMaxLog2P = 64.0f;
 template <> constexpr float kWideMaxLog2P<_Float16> = 15.0f;
