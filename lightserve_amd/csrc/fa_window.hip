@@ -8,11 +8,13 @@
 //
 // Few rows per KV head (decode, and chunks of a few tokens): the narrow kernel.
 // Many: the wide one, further down.
-// The path is bound by HBM, so it is built around bytes in flight, and each
-// byte of the cache is read once for all query heads that share it:
+// The narrow path is bound by HBM (64 sequences of 8192 tokens, 8 KV heads of 128, 8
+// bits: 207 us, 5.2 TB/s; 64 windows of 4096: 116 us, 4.7) or, for one sequence, by
+// latency (1500 tokens 12 us, 32768 30), so it is built around bytes in flight, and
+// each byte of the cache is read once for all query heads that share it:
 //   rows       (token, query head of the KV head's group) pairs, 16 or 32 to a row
 //              tile, are the columns of S^T = K Q^T and of O^T += V^T P^T on
-//              v_mfma_f32_16x16x32.
+//              v_mfma_f32_16x16x32. Q lies in LDS: registers hold loads in flight.
 //   key tiles  of 32 keys: two pieces of 16 that each lie in one cache block,
 //              so that a piece takes one buffer descriptor built from one
 //              block-table entry (scalar work); pieces past the sequence and
@@ -31,11 +33,14 @@
 // Work is shared out evenly whatever the lengths: the key tiles of all sequences
 // are numbered one after another and every workgroup takes an equal run of
 // them, which may end inside a sequence or hold several. A sequence that lies
-// in several runs leaves fp32 partial results, which the last of them merges.
+// in several runs leaves fp32 partial results: a second launch merges those of
+// long runs, the last run to arrive those of short ones, whose launches are a few
+// microseconds. Either way they are added in the runs' order, whichever ends first.
 #include "../../include/lightserve_fa.h"
 #include "fa_common.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace lsfa {
 
@@ -234,8 +239,8 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
   // Adjacent heads' rows of a token are adjacent in the cache: read by one workgroup
   // they are asked for together, in pieces of 2 or 4 rows (512 bytes at head dim 128 and 8
   // bits) where one head's alone reach HBM as 128-byte ones (64 sequences of 8192 tokens,
-  // 8 KV heads: XXX us). Few tiles stay shared out over the waves of one head, which end
-  // sooner.
+  // 8 KV heads: 210 us, 227 with a head each; 64 windows of 4096, 120 and 130). Few tiles
+  // stay shared out over the waves of one head, which end sooner.
   const bool deferred = long_runs(p, all);
   const int hw = deferred ? heads_per_group(p) : 1;
   const int groups = p.Hkv / hw, columns = gridDim.x / hw, runs = p.runs * hw, nk = NW / hw;  // nk: waves that share a head's tiles
@@ -656,11 +661,17 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
   }
 }
 
-// Merges the partial results of long runs: a workgroup takes 32 channels of a sequence, KV
-// head and row tile; groups of threads take every ng-th run and meet in LDS.
-template <typename T, int DP, int NC>
+// Merges the partial results of long runs: a workgroup takes CH channels of a sequence, KV
+// head and row tile; groups of threads take every ng-th run and meet in LDS. Bound by latency.
+// Many sequences lie in few runs each: two of them in flight a thread do, and 64 channels a
+// workgroup, where there are 256 of them or more (64 windows of 4096 tokens of 8 heads, 5 runs
+// each: 116 us in all, 32 channels 118, with eight runs in flight 121, which load what others
+// have). A long one lies in hundreds: eight in flight and 32 channels, for more groups
+// (32768 tokens: 30 us in all, 64 channels with two in flight 47).
+template <typename T, int DP, int NC, int CH>
 __global__ __launch_bounds__(256) void fa_window_combine_kernel(const WindowParams p) {
   constexpr int RT = kRowTile * NC;
+  static_assert(RT * CH / 4 <= 256, "a thread has at most one row's four channels");
   __shared__ f32x4 meet[512];
   const int tid = threadIdx.x, lane = tid & 63;
   const int head = blockIdx.x % p.Hkv, rt = blockIdx.x / p.Hkv, b = blockIdx.y;
@@ -682,11 +693,11 @@ __global__ __launch_bounds__(256) void fa_window_combine_kernel(const WindowPara
   const int runs = p.runs * heads_per_group(p), per = run_tiles(all, runs);
   const int r0 = at / per, r1 = (at + count - 1) / per;
   if (r0 == r1) return;  // already in o
-  const int items = nrows * 8, ng = 256 / items, grp = tid / items, idx = tid - grp * items;  // (nrows <= 32)
-  const int row = idx / 8, d = blockIdx.z * 32 + idx % 8 * 4;
+  const int items = nrows * (CH / 4), ng = 256 / items, grp = tid / items, idx = tid - grp * items;
+  const int row = idx / (CH / 4), d = blockIdx.z * CH + idx % (CH / 4) * 4;
   RowSums sum;
-  if (grp < ng) {
-    constexpr int U = 8;
+  auto merge = [&](auto in_flight) {
+    constexpr int U = decltype(in_flight)::value;
     for (int r = r0 + grp; r <= r1; r += ng * U) {
       f32x4 st[U], o[U];
 #pragma unroll
@@ -700,6 +711,10 @@ __global__ __launch_bounds__(256) void fa_window_combine_kernel(const WindowPara
       for (int k = 0; k < U; ++k)
         if (r + k * ng <= r1) sum.take(st[k], o[k]);
     }
+  };
+  if (grp < ng) {
+    if (r1 - r0 >= 4 * ng) merge(std::integral_constant<int, 8>());
+    else merge(std::integral_constant<int, 2>());
     meet[2 * tid] = f32x4{sum.M, sum.L, sum.E, 0.f};
     meet[2 * tid + 1] = sum.O;
   }
@@ -719,7 +734,10 @@ __global__ __launch_bounds__(256) void fa_window_combine_kernel(const WindowPara
 // convert it again on reading codes), 16-bit rows go there by direct loads.
 // Rows that none of the workgroup's queries sees read as zeros. S^T = K Q^T and
 // O^T += V^T P^T on v_mfma_f32_32x32x16 (fa_common.hpp has the lane layouts), the
-// scores of tile t + 1 beside the softmax of tile t.
+// scores of tile t + 1 beside the softmax of tile t. Bound by the matrix pipe and the
+// exponentials that share its issue slots (batched chunks of 8-bit prompts 327 us, 998 TFLOP/s,
+// where the card's large bf16 product reaches 1265), short ones by their steps' latency (2.7
+// us a tile of 64 keys, and 6 us before the first).
 constexpr int kWideTile = 64;  // keys
 
 // The sequence (with its key tiles) and row tile of an item; false past the last. Row
@@ -797,7 +815,9 @@ __device__ __forceinline__ WideSpan wide_span(const WindowParams& p, const KeyTi
   s.count = s.sink + (end + kWideTile - 1) / kWideTile - s.first;
   return s;
 }
-// Tiles of one of an item's splits: an even share, at least kSplitLeast.
+// Tiles of one of an item's splits: an even share, at least kSplitLeast (333 tokens under a
+// window of 1024: 29.2 us, 33.8 with 8; 64 tokens of 4 sequences of 16 bits: 16.3, 20.3 with
+// 8, 16.7 with 1).
 constexpr int kSplitLeast = 3;
 __device__ __forceinline__ int split_share(int count, int splits) {
   return max((count + splits - 1) / splits, kSplitLeast);
@@ -1321,7 +1341,9 @@ __global__ __launch_bounds__(NW * 64) void fa_window_wide_combine_kernel(const W
 }
 
 // ------------------------------------------------------------------- launches
-constexpr long long kNarrowRows = 32;  // most rows of a sequence and KV head in the narrow kernel
+// Most rows of a sequence and KV head in the narrow kernel: 16 chunks of 8 tokens, group 4 (32
+// rows), take 66 us there and 88 in the wide one, 4 chunks of 64 tokens (256 rows) 73 and 46.
+constexpr long long kNarrowRows = 32;
 
 // How a launch goes, from what the host knows (sizes and bounds, not lengths).
 WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int eb, int max_n, long long max_keys, int window, int sinks) {
@@ -1340,7 +1362,8 @@ WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int eb, int max
     const long long most = std::max(1LL, ((seen + 31) / 32 * B + 3) / 4);
     w.runs = (int)std::min(std::max(512 / tiles, 1LL), most);
     // A long run's partial result, written and read, is to be less than an eighth of the
-    // keys and values that its waves read, and a workgroup to have 16 tiles.
+    // keys and values that its waves read, and a workgroup to have 16 tiles. (Short runs
+    // only: 64 windows of 4096 tokens 127 us for 120, a batch of 32 of mixed lengths 77 for 75.)
     const int tile_bytes = 64 * dp * eb, part_bytes = w.part_rows * (dp + 4) * 4;
     w.long_run = std::max(16, 4 * 16 * part_bytes / tile_bytes);
     if (w.runs == 1 || (seen + 31) / 32 * B <= (long long)w.runs * (w.long_run - 1)) w.long_run = 0;
@@ -1351,8 +1374,13 @@ WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int eb, int max
   auto items = [&](int bm) {
     return Hkv * std::min((long long)tokens * G / bm + B, (rows + bm - 1) / bm * B);
   };
+  // Eight waves bring each key tile in once for 256 rows, four fill the chip with half as
+  // many: at 256 items (2048 tokens of 8 KV heads, group 4) 36.2 us and 40.4, and more
+  // of them 353 and 415; at 128 (1024 tokens) 69.4 and 62.5.
   w.waves = items(256) >= 256 ? 8 : 4;
   w.items = (int)items(w.waves * 32);
+  // Few items share their keys out over two workgroups a CU (4 chunks of 64 tokens after
+  // up to 4096: 46 us, 115 without; 256, 384, 640 and 768 workgroups took no less).
   w.splits = 1;
   if (w.waves == 4) {
     const long long tiles = (std::min(seen, (long long)(window > 0 ? window + sinks + 32 * 4 / G + 128 : seen)) + 63) / 64;
@@ -1369,7 +1397,11 @@ static hipError_t launch_narrow(const WindowParams& p, const WindowPlan& w, hipS
   else hipLaunchKernelGGL((fa_window_narrow_kernel<T, C, DP, NC, false>), dim3(p.Hkv * tiles, p.runs), dim3(256), 0, s, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || w.long_run == 0) return e;
-  hipLaunchKernelGGL((fa_window_combine_kernel<T, DP, NC>), dim3(p.Hkv * tiles, p.B, DP / 32), dim3(256), 0, s, p);
+  const dim3 parts(p.Hkv * tiles, p.B, DP / 32);
+  if (NC == 1 && (long long)parts.x * p.B * (DP / 64) >= 256)
+    hipLaunchKernelGGL((fa_window_combine_kernel<T, DP, NC, 64 / NC>), dim3(parts.x, p.B, DP / 64), dim3(256), 0, s, p);
+  else
+    hipLaunchKernelGGL((fa_window_combine_kernel<T, DP, NC, 32>), parts, dim3(256), 0, s, p);
   return hipGetLastError();
 }
 template <typename T, typename C, int DP>
