@@ -777,6 +777,11 @@ static int check_window(const lsfa_window_args* a) {
   if (a->batch > 65535 || (long long)a->heads_q * std::max(a->max_seqlen_q, 1) > (1LL << 30) ||
       (long long)a->heads_q * a->tokens > (1LL << 36) || (long long)a->heads_kv * a->batch > (1LL << 30))
     return fail(LSFA_ERR_UNSUPPORTED, "more than 65535 sequences, 2^30 rows of one sequence or 2^36 rows in one call");
+  // Positions and the numbers of all sequences' key tiles are 32-bit.
+  long long keys = std::min<long long>(a->max_seq_len, (long long)a->max_blocks_per_seq * a->block_size);
+  if (a->window > 0) keys = std::min(keys, (long long)a->window + a->sinks + a->max_seqlen_q + 96);
+  if (a->tokens > (1 << 30) || (keys + 63) / 32 * a->batch > (1LL << 30))
+    return fail(LSFA_ERR_UNSUPPORTED, "more than 2^30 tokens, or 2^30 tiles of 32 keys of all sequences (max_seq_len, or the window)");
   if (a->batch == 0 || a->tokens == 0 || a->max_seqlen_q == 0) return ok();
   if (!a->q || !a->o || !a->block_tables || !a->seq_lens || ((!a->k_cache || !a->v_cache) && a->num_blocks > 0))
     return fail(LSFA_ERR_INVALID, "q, k_cache, v_cache, o, block_tables and seq_lens must be non-NULL");
@@ -846,7 +851,7 @@ int lsfa_window(const lsfa_window_args* a, void* stream) {
   p.max_n = std::min(a->max_seqlen_q, a->tokens);
   p.max_seq_len = a->max_seq_len;
   p.causal = a->causal != 0;
-  p.window = a->window;
+  p.window = std::min(a->window, 1 << 30);  // (no position lies further back)
   p.sinks = a->sinks;
   p.scale_log2 = a->sm_scale * 1.4426950408889634f;
   p.scale_abs = fmaxf(fabsf(p.scale_log2), 1e-30f);

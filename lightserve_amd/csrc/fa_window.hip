@@ -1383,7 +1383,7 @@ WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int eb, int max
   // up to 4096: 46 us, 115 without; 256, 384, 640 and 768 workgroups took no less).
   w.splits = 1;
   if (w.waves == 4) {
-    const long long tiles = (std::min(seen, (long long)(window > 0 ? window + sinks + 32 * 4 / G + 128 : seen)) + 63) / 64;
+    const long long tiles = (std::min(seen, window > 0 ? (long long)window + sinks + 32 * 4 / G + 128 : seen) + 63) / 64;
     w.splits = (int)std::max(1LL, std::min(512 / std::max(1, w.items), (int)(tiles / kSplitLeast)) * 1LL);
     if (w.splits > 1) w.part_bytes = LSFA_GEMV_COUNTER_BYTES + (uint64_t)w.items * w.splits * (128 * 4 + 128 * dp) * 4;
   }

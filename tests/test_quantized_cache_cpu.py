@@ -100,6 +100,19 @@ def test_window_sizes(built_library):
             _lib.window_workspace_size(_win(**bad))
 
 
+def test_window_sizes_past_32_bits(built_library):
+    """Key tiles of all sequences, tokens and windows that positions of 32 bits would not hold."""
+    huge = dict(max_blocks_per_seq=1 << 26, block_table_stride=1 << 26, max_seq_len=1 << 30, window=0, sinks=0)
+    assert _lib.window_check(_win(**huge, batch=31, tokens=31, workspace_bytes=1 << 40)) == (0, "")
+    for change in (dict(batch=33, tokens=33), dict(batch=65535, tokens=65535)):
+        rc, msg = _lib.window_check(_win(**huge, **change))
+        assert rc == -2 and "tiles" in msg, (rc, msg)
+    rc, msg = _lib.window_check(_win(tokens=(1 << 30) + 1, heads_q=1, heads_kv=1))
+    assert rc == -2 and "tokens" in msg, (rc, msg)
+    assert _lib.window_check(_win(**{**huge, "window": 4096}, batch=65535, tokens=65535)) == (0, "")
+    assert _lib.window_check(_win(window=2 ** 31 - 1, workspace_bytes=1 << 40)) == (0, "")
+
+
 def test_struct_sizes_match_the_header(built_library, tmp_path):
     import os
     import shutil

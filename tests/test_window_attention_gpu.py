@@ -12,6 +12,7 @@ import math
 import pytest
 import torch
 
+from lightserve_amd import _lib
 from lightserve_amd.kernels.paged_attention import paged_attention_decode, paged_prefill
 from lightserve_amd.kernels.quantized_kv_cache import kv_cache_append, quantized_kv_cache
 from oracle import paged8
@@ -360,6 +361,30 @@ def test_chunks_of_many_sequences(gpu, window):
     new = [int(n) if b % 5 else 0 for b, n in enumerate(torch.randint(0, 90, (130,), generator=g))]
     had = torch.randint(0, 300, (130,), generator=g).tolist()
     _chunk("e4m3", torch.bfloat16, new, had, 8, 2, 64, 16, 64, window, 3 if window else 0, what=f"many chunks w={window}")
+
+
+def test_window_past_every_position(gpu, monkeypatch):
+    """The largest window that the C argument holds sees what a window of the sequence's length does."""
+    print("case largest window", flush=True)
+    lens = [90, 700]
+    table, pool = tables(lens, 16, 68)
+    cache, _ = _cache("e4m3", torch.bfloat16, pool, 16, 2, 64, 69)
+    q = _q(120, 4, 64, torch.bfloat16, 70).cuda()
+    launch, sizes = _lib.window, []
+
+    def largest(args, stream):
+        sizes.append(args.window)
+        args.window = 2 ** 31 - 1
+        launch(args, stream)
+
+    def calls():
+        sl = torch.tensor(lens, dtype=torch.int32).cuda()
+        return [paged_prefill(q, *cache[:2], table.cuda(), offsets([n, 120 - n]).cuda(), sl, kv_scales=cache[2], window=800, sinks=0)
+                for n in (2, 60)] + [paged_attention_decode(q[:2], *cache[:2], table.cuda(), sl, kv_scales=cache[2], window=800)]
+
+    want = calls()
+    monkeypatch.setattr(_lib, "window", largest)
+    assert all(torch.equal(a, b) for a, b in zip(calls(), want)) and len(sizes) == 3
 
 
 def test_graph_follows_the_lengths(gpu):
