@@ -46,7 +46,8 @@ which no query of the call sees are not read, so their table entries may be
 anything (an engine can give those blocks back). These calls need a
 power-of-two block_size of at least 16 (any heads_q / heads_kv) and, over 8-bit
 caches, a head_dim that is a multiple of 16. A query that sees no key gets o = 0
-and lse = -inf.
+and lse = -inf. Infinities and NaN in the cache reach only the queries that see
+their keys.
 """
 import math
 
