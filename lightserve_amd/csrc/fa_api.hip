@@ -782,6 +782,8 @@ static int check_window(const lsfa_window_args* a) {
   if (a->window > 0) keys = std::min(keys, (long long)a->window + a->sinks + a->max_seqlen_q + 96);
   if (a->tokens > (1 << 30) || (keys + 63) / 32 * a->batch > (1LL << 30))
     return fail(LSFA_ERR_UNSUPPORTED, "more than 2^30 tokens, or 2^30 tiles of 32 keys of all sequences (max_seq_len, or the window)");
+  if (q8 && (long long)a->heads_kv * a->block_size >= (1LL << 30))
+    return fail(LSFA_ERR_UNSUPPORTED, "2^30 rows or more of one cache block");
   if (a->batch == 0 || a->tokens == 0 || a->max_seqlen_q == 0) return ok();
   if (!a->q || !a->o || !a->block_tables || !a->seq_lens || ((!a->k_cache || !a->v_cache) && a->num_blocks > 0))
     return fail(LSFA_ERR_INVALID, "q, k_cache, v_cache, o, block_tables and seq_lens must be non-NULL");

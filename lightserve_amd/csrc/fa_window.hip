@@ -735,9 +735,9 @@ __global__ __launch_bounds__(256) void fa_window_combine_kernel(const WindowPara
 // Rows that none of the workgroup's queries sees read as zeros. S^T = K Q^T and
 // O^T += V^T P^T on v_mfma_f32_32x32x16 (fa_common.hpp has the lane layouts), the
 // scores of tile t + 1 beside the softmax of tile t. Bound by the matrix pipe and the
-// exponentials that share its issue slots (batched chunks of 8-bit prompts 327 us, 998 TFLOP/s,
-// where the card's large bf16 product reaches 1265), short ones by their steps' latency (2.7
-// us a tile of 64 keys, and 6 us before the first).
+// exponentials that share its issue slots (batched chunks over 8-bit prefixes 327 to 339
+// us by the card, 960 to 1000 TFLOP/s, where a large bf16 product reaches 1265), short
+// ones by their steps' latency (2.7 us a tile of 64 keys, and 6 us before the first).
 constexpr int kWideTile = 64;  // keys
 
 // The sequence (with its key tiles) and row tile of an item; false past the last. Row

@@ -111,6 +111,8 @@ def test_window_sizes_past_32_bits(built_library):
     assert rc == -2 and "tokens" in msg, (rc, msg)
     assert _lib.window_check(_win(**{**huge, "window": 4096}, batch=65535, tokens=65535)) == (0, "")
     assert _lib.window_check(_win(window=2 ** 31 - 1, workspace_bytes=1 << 40)) == (0, "")
+    rc, msg = _lib.window_check(_win(block_size=1 << 27, max_blocks_per_seq=1))
+    assert rc == -2 and "block" in msg, (rc, msg)
 
 
 def test_struct_sizes_match_the_header(built_library, tmp_path):
