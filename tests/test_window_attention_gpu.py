@@ -293,7 +293,7 @@ def test_nan_of_a_key_reaches_the_rows_that_see_it(gpu):
 
 
 @pytest.mark.parametrize("kind,bad", [("e4m3", math.nan), ("16 bit", math.nan), ("16 bit", math.inf), ("16 bit", -math.inf)])
-@pytest.mark.parametrize("n,heads,d", [(3, 4, 64), (6, 4, 128), (8, 8, 80), (40, 4, 64), (100, 2, 128), (200, 16, 64), (600, 32, 72)])
+@pytest.mark.parametrize("n,heads,d", [(3, 4, 64), (6, 4, 128), (8, 8, 80), (40, 4, 64), (100, 2, 128), (200, 16, 64), (600, 32, 72), (2048, 32, 64)])
 def test_values_not_finite_reach_the_rows_that_see_them_alone(gpu, kind, bad, n, heads, d):
     """V of a key that a chunk's later (or, at the window's start, earlier) queries do not see, in both kernels."""
     print(f"case not finite {kind} {bad} n={n} heads={heads} d={d}", flush=True)
@@ -320,6 +320,9 @@ def test_values_not_finite_reach_the_rows_that_see_them_alone(gpu, kind, bad, n,
         o, lse = paged_prefill(q.cuda(), dev[0], dev[1], table.cuda(), offsets([n]).cuda(),
                                torch.tensor([length], dtype=torch.int32).cuda(), return_lse=True, kv_scales=dev[2],
                                window=window, sinks=sinks)
+        alone = paged_prefill(q.cuda(), dev[0], dev[1], table.cuda(), offsets([n]).cuda(),
+                              torch.tensor([length], dtype=torch.int32).cuda(), kv_scales=dev[2], window=window, sinks=sinks)
+        assert torch.equal(torch.isfinite(alone), torch.isfinite(o)), "without the lse"
         o, ref = o.cpu(), paged8.window_reference(q, *clean, table, offsets([n]), [length], window, sinks)
         for i, j in enumerate(at):
             sees = (j <= p) & ((j > p - window) | (j < sinks) if window is not None else True)
