@@ -511,7 +511,10 @@ typedef struct {
  * as the skinny GEMM's, its first LSFA_GEMV_COUNTER_BYTES hold int32 arrival
  * counters that must be zero on entry and are zero again when the call is done,
  * so calls in stream order (of either kind) can share one workspace; calls that
- * may run at the same time need one each. */
+ * may run at the same time need one each. A call may be two launches, the second
+ * of which merges what the first left in the workspace: host threads that share
+ * one must not launch another call that uses it in between, so they hold a lock
+ * over each call of either kind (or have a workspace each). */
 typedef struct {
   const void* q;
   const void* k_cache;

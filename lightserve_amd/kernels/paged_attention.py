@@ -57,7 +57,7 @@ import torch
 from .. import _lib
 from .flash_attention import SPLIT_MAX_TILES, SPLIT_MIN_KEYS
 from .quantized_kv_cache import check_device, check_quantized
-from .tiled_matmul import _workspace as stream_workspace
+from .tiled_matmul import stream_workspace
 
 
 def _windowed(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens, max_seqlen_q, max_seq_len, causal, sm_scale,
@@ -130,9 +130,12 @@ def _windowed(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens, max_seq
         with _lib.device_guard(device):
             stream = _lib.current_stream(device)
             if nbytes > 0:  # arrival counters, kept at zero from call to call, and partial results
-                ws = stream_workspace(device, stream, nbytes)
+                ws, launching = stream_workspace(device, stream, nbytes)
                 args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
-            _lib.window(args, stream)
+                with launching:
+                    _lib.window(args, stream)
+            else:
+                _lib.window(args, stream)
     return (o, lse) if return_lse else o
 
 

@@ -40,8 +40,11 @@ lsfa_gemv's workspace carries arrival counters (its first
 LSFA_GEMV_COUNTER_BYTES) that must start at zero and that every call leaves
 at zero, so this module keeps one workspace per (device, stream), zeroes its
 counter bytes once when it is created, and reuses it for every call on that
-stream (stream order keeps the calls apart). Workspaces start at 16 MB, so
-they rarely grow. A graph capture gets a workspace of its own, from the
+stream. Stream order keeps the calls apart, as long as nothing is launched
+between the launches of one call: windowed paged attention shares these
+workspaces and may leave partial results there for a second launch, and two
+host threads may use one stream. So each stream has a lock that a call holds
+while it launches. Workspaces start at 16 MB, so they rarely grow. A graph capture gets a workspace of its own, from the
 graph's memory pool, whose fill it records: the graph clears its 256 KB of
 counters before its first product on every replay, whatever ran before it, and
 shares neither counters nor partials with eager calls or with another graph
@@ -94,9 +97,10 @@ MAX_CACHED_STREAMS = 8
 
 
 class _Entry:
-    __slots__ = ("buf", "captured", "graph_buf")
+    __slots__ = ("buf", "captured", "graph_buf", "launching")
 
     def __init__(self):
+        self.launching = threading.Lock()  # held from a call's first launch to its last
         self.buf = None        # the workspace of eager calls
         self.captured = 0      # the last graph capture on the stream (lsfa_capture_id)
         self.graph_buf = None  # its workspace
@@ -110,6 +114,13 @@ _workspaces_lock = threading.Lock()
 def _workspace(device, stream, nbytes):
     with _workspaces_lock:
         return _workspace_locked(device, stream, nbytes)
+
+
+def stream_workspace(device, stream, nbytes):
+    """The stream's workspace, and the lock to hold while a call that uses it is launched."""
+    with _workspaces_lock:
+        buf = _workspace_locked(device, stream, nbytes)
+        return buf, _workspaces[device.index, stream].launching
 
 
 def _workspace_locked(device, stream, nbytes):
@@ -175,9 +186,12 @@ def skinny_matmul(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor = None) ->
     with _lib.device_guard(a.device):
         stream = _lib.current_stream(a.device)
         if nbytes:
-            ws = _workspace(a.device, stream, nbytes)
+            ws, launching = stream_workspace(a.device, stream, nbytes)
             args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
-        _lib.gemv(args, stream)
+            with launching:
+                _lib.gemv(args, stream)
+        else:
+            _lib.gemv(args, stream)
     return out
 
 
@@ -200,9 +214,12 @@ def _run_group(args, device, size=_lib.gemv_group_workspace_size, launch=_lib.ge
     with _lib.device_guard(device):
         stream = _lib.current_stream(device)
         if nbytes:
-            ws = _workspace(device, stream, nbytes)
+            ws, launching = stream_workspace(device, stream, nbytes)
             args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
-        launch(args, stream)
+            with launching:
+                launch(args, stream)
+        else:
+            launch(args, stream)
 
 
 def _empty_outs(a, bs):

@@ -570,3 +570,43 @@ def test_cache_past_32_bits(gpu):
                            offsets([50]).cuda(), torch.tensor([60], dtype=torch.int32).cuda(), return_lse=True, kv_scales=sc)
     ref = paged8.window_reference(q, *paged8.cache_values(*small), torch.arange(4)[None], offsets([50]), [60])
     _assert_close(o, lse.t(), ref, 60, "far blocks, chunk")
+
+
+def test_host_threads_on_one_stream(gpu):
+    """Calls of two launches (key splits of a chunk, long runs of a decode step), calls of one and skinny products from three
+    threads that all use the default stream: every result is the one that the call gives alone."""
+    import threading
+
+    from lightserve_amd.kernels.tiled_matmul import skinny_matmul
+    print("case threads", flush=True)
+    lens = [12000, 9000, 11000]
+    table, pool = tables(lens, 16, 80)
+    cache, _ = _cache("e4m3", torch.bfloat16, pool, 16, 8, 64, 81)
+    bt, sl = table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
+    q, cu = _q(90, 16, 64, torch.bfloat16, 82).cuda(), offsets([30, 20, 40]).cuda()
+    x, w = (torch.randn(n, 4096, generator=torch.Generator().manual_seed(83)).to(torch.bfloat16).cuda() for n in (2, 4096))
+    calls = [lambda: paged_prefill(q, *cache[:2], bt, cu, sl, max_seqlen_q=40, kv_scales=cache[2]),
+             lambda: paged_attention_decode(q[:3], *cache[:2], bt, sl, max_seq_len=12000, kv_scales=cache[2]),
+             lambda: paged_attention_decode(q[3:6], *cache[:2], bt, sl, max_seq_len=12000, kv_scales=cache[2]),
+             lambda: paged_attention_decode(q[:3], *cache[:2], bt, sl, max_seq_len=300, kv_scales=cache[2]),
+             lambda: skinny_matmul(x, w)]
+    want = [f() for f in calls]
+    torch.cuda.synchronize()
+    got, start = [[], [], []], threading.Barrier(3)
+
+    def run(i):
+        start.wait(timeout=60)
+        for turn in range(60):
+            at = (turn + 2 * i) % len(calls)
+            got[i].append((at, calls[at]()))
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for results in got:
+        assert len(results) == 60
+        for at, out in results:
+            assert torch.equal(out, want[at]), f"call {at}"
