@@ -174,7 +174,7 @@ __device__ __forceinline__ f32x4 load_device(const float* from) {
 // and NaN with its weight of zero. The narrow kernel takes such elements of V as zeros where
 // a mask cuts a tile for some of a chunk's rows and, if there were any (ordinary caches have
 // none), adds them to the rows that see their keys before the sums leave the registers; the
-// wide one takes the sums of a wave again, key by key, if they are not finite.
+// wide one takes the sums of a wave again, with them left out, if they are not finite.
 // Ones in the elements of a word of V that are infinite or NaN (e4m3: NaN).
 template <typename T, bool Q8>
 __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
@@ -1216,8 +1216,7 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
   leave();
 
   // Sums that are not finite while V has infinities or NaN in a tile that the mask cuts are
-  // taken again, key by key: a lane holds half of its row of q, and adds each key's V where
-  // the row sees it. (Looking for them in every such tile of the loop, before they are
+  // taken again. (Looking for them in every such tile of the loop, before they are
   // multiplied, made 111 us of 98 of windowed prompts of a 16-bit cache.)
   if (__builtin_expect(__builtin_amdgcn_ballot_w64(!all_finite(acc)) != 0, 0)) {
     auto row_of = [&](const Cache& c, int key, int blk) -> const C* {
@@ -1243,59 +1242,104 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
         }
       }
     }
+    // The wave does so alone, with the offset that its rows ended with, 32 keys at a time
+    // through the part of LDS that O left by. V's infinities and NaN stay out of the products
+    // where the mask cuts the 32 keys and are added to the rows that see them. (8.5 us for 32
+    // keys, of head dim 128: a call over 8192 keys 0.37 -> 2.5 ms, over 32768 1.2 -> 8.8.)
     if (__builtin_amdgcn_ballot_w64(bad) != 0) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
+      LDS_AS char* wb = smem + wave * 32 * DP * 2;
+      int lrow = lane / LPR, lcol = 8 * (lane % LPR);
+      // (LDS is in order within a wave; this keeps the compiler's order)
+      auto in_order = [&]() { asm volatile("" ::: "memory"); };
 #pragma unroll 1
-      for (int i = 0; i < (t_hi - t_lo) * BN; ++i) {
-        const int key = key_of(t_lo + i / BN) + i % BN;
-        if (key > whi_max) continue;
-        const int blk = table[key >> p.block_shift];
-        if ((unsigned)blk >= (unsigned)p.num_blocks) continue;
-        float ks = 1.f, vs = 1.f;
-        if constexpr (Q8) {
-          const uint8_t* e = p.scales + ((((int64_t)blk * p.Hkv + head) << p.block_shift) + (key & ((1 << p.block_shift) - 1))) * 2;
-          ks = fminf(__uint_as_float((uint32_t)e[0] << 23), 0x1p127f);
-          vs = fminf(__uint_as_float((uint32_t)e[1] << 23), 0x1p127f);
-        }
-        const C* row = row_of(K, key, blk);
-        float s = 0.f;
+      for (int i = 0; i < 2 * (t_hi - t_lo); ++i) {
+        const int key0 = key_of(t_lo + (i >> 1)) + 32 * (i & 1);
+        if (key0 > whi_max || (key0 + 31 < wlo_min && key0 >= sinks)) continue;
+        const bool cut = !(key0 + 31 <= whi_min && (key0 >= wlo_max || key0 + 31 < sinks));
+        asm volatile("" : "+v"(koff), "+v"(voff0), "+v"(voff1), "+v"(lrow), "+v"(lcol));  // (nothing made of them stays in registers)
+        uint32_t found = 0;
+        auto to_lds = [&](const Cache& of, int which, bool finite_only) {
+          u32x4 w[32 / RPL];
 #pragma unroll
-        for (int kk = 0; kk < KSTEPS; ++kk)
-          if (16 * kk + 8 * hh < p.D) {
-            X8 k8;
+          for (int j = 0; j < 32 / RPL; ++j) {
+            const int key = key0 + j * RPL + lrow, slot = key & ((1 << p.block_shift) - 1);
+            const bool used = lcol < p.D && key <= whi_max && (key >= wlo_min || key < sinks);
+            const int blk = used ? table[key >> p.block_shift] : -1;
+            w[j] = u32x4{0, 0, 0, 0};
+            if ((unsigned)blk >= (unsigned)p.num_blocks) continue;
+            const C* row = row_of(of, key, blk) + lcol;
             if constexpr (Q8) {
-              const u32x2 w = *(const u32x2*)(row + 16 * kk + 8 * hh);
-              k8 = __builtin_bit_cast(X8, u32x4{codes2<false>(w[0], ks, T()), codes2<true>(w[0], ks, T()), codes2<false>(w[1], ks, T()),
-                                                codes2<true>(w[1], ks, T())});
+              const u32x2 codes = *(const u32x2*)row;
+              w[j] = u32x4{codes[0], codes[1], p.scales[((((int64_t)blk * p.Hkv + head) << p.block_shift) + slot) * 2 + which], 0};
             } else {
-              k8 = __builtin_bit_cast(X8, ldg16((const T*)row + 16 * kk + 8 * hh));
+              w[j] = ldg16((const T*)row);
             }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s = fmaf((float)k8[e], (float)qreg[kk][e], s);
           }
-        s = half_sum(s);
-        const float w = (float)(T)fast_exp2(fmaf(s, sl2, -m_run));
-        if (!(key <= hi && (key >= lo || key < sinks))) continue;
-        const C* vrow = row_of(V, key, blk);
+          in_order();
+#pragma unroll
+          for (int j = 0; j < 32 / RPL; ++j) {
+            u32x4 v = w[j];
+            if (finite_only) {
+#pragma unroll
+              for (int c = 0; c < (Q8 ? 2 : 4); ++c) {
+                const uint32_t x = not_finite<T, Q8>(v[c]);
+                v[c] &= ~x;
+                found |= x;
+              }
+            }
+            if constexpr (Q8) {
+              const float s = fminf(__uint_as_float(w[j][2] << 23), 0x1p127f);
+              v = u32x4{codes2<false>(v[0], s, T()), codes2<true>(v[0], s, T()), codes2<false>(v[1], s, T()), codes2<true>(v[1], s, T())};
+            }
+            *(LDS_AS u32x4*)(wb + swz_off<DP>(j * RPL + lrow, lcol) * 2) = v;
+          }
+          in_order();
+        };
+        to_lds(K, 0, false);
+        f32x16 s = {};
+#pragma unroll
+        for (int kk = 0; kk < KSTEPS; ++kk) s = mfma32(*(const LDS_AS X8*)(wb + (koff ^ (kk << 5))), qreg[kk], s);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const int key = key0 + 4 * hh + 8 * (k >> 2) + (k & 3);
+          s[k] = key <= hi && (key >= lo || key < sinks) ? fast_exp2(fmaf(s[k], sl2, -m_run)) : 0.f;
+        }
+        const X8 pb[2] = {pack8<T>(s, 0), pack8<T>(s, 8)};
+        in_order();
+        to_lds(V, 1, cut);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int d = 32 * dt + 8 * g + 4 * hh;
-            if (d >= p.D) continue;
-            u32x2 v;
-            if constexpr (Q8) {
-              const uint32_t c = *(const uint32_t*)(vrow + d);
-              v = u32x2{codes2<false>(c, vs, T()), codes2<true>(c, vs, T())};
-            } else {
-              v = *(const u32x2*)(vrow + d);
-            }
-            const X4 v4 = __builtin_bit_cast(X4, v);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[dt][4 * g + e] = fmaf(w, (float)v4[e], acc[dt][4 * g + e]);
+          for (int ks = 0; ks < 2; ++ks) {
+            const LDS_AS char* base = wb + ks * 16 * DP * 2;
+            acc[dt] = mfma32(cat4<X8, X4>(lds_read_tr((const LDS_AS T*)(base + (voff0 ^ (dt << 6)))),
+                                          lds_read_tr((const LDS_AS T*)(base + (voff1 ^ (dt << 6))))),
+                             pb[ks], acc[dt]);
           }
+        if (__builtin_amdgcn_ballot_w64(found != 0) == 0) continue;
+#pragma unroll 1
+        for (int key = key0; key < key0 + 32; ++key) {
+          if (key > whi_max || (key < wlo_min && key >= sinks)) continue;
+          const int blk = table[key >> p.block_shift];
+          if ((unsigned)blk >= (unsigned)p.num_blocks || !(key <= hi && (key >= lo || key < sinks))) continue;
+          const C* row = row_of(V, key, blk);
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int d = 32 * dt + 8 * g + 4 * hh;
+              if (d >= p.D) continue;
+              uint32_t w[2] = {*(const uint32_t*)(row + d), 0};
+              if constexpr (!Q8) w[1] = *(const uint32_t*)(row + d + 2);
+              w[0] &= not_finite<T, Q8>(w[0]), w[1] &= not_finite<T, Q8>(w[1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[dt][4 * g + e] += bad_value<T, Q8>(w, e);
+            }
+        }
       }
+      in_order();
       leave();
     }
   }

@@ -610,3 +610,45 @@ def test_host_threads_on_one_stream(gpu):
         assert len(results) == 60
         for at, out in results:
             assert torch.equal(out, want[at]), f"call {at}"
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "16 bit"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_one_value_not_finite_after_a_long_prefix(gpu, kind, d):
+    """A NaN in the diagonal tiles of a long item: the rows that see it alone, the other rows of their wave as without it, and
+    no more than a few times the call's own time (a walk over the keys one by one takes 50 to 100 times as long)."""
+    had, n, hq, hkv, dtype = 8192, 2048, 32, 8, torch.bfloat16
+    print(f"case NaN after a long prefix {kind} d={d}", flush=True)
+    length, at, channel = had + n, had + 700, 9
+    table, pool = tables([length], 16, 84)
+    cache, vals = _cache(kind, dtype, pool, 16, hkv, d, 85)
+    how = dict(max_seqlen_q=n, return_lse=True, kv_scales=cache[2], **({} if kind == "e4m3" else dict(window=length)))
+    q, sl = _q(n, hq, d, dtype, 86), torch.tensor([length], dtype=torch.int32).cuda()
+    bt, cu, qd = table.cuda(), offsets([n]).cuda(), q.cuda()
+
+    def timed():
+        times = []
+        for _ in range(4):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            out = paged_prefill(qd, *cache[:2], bt, cu, sl, **how)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(start.elapsed_time(end))
+        return min(times), out
+
+    clean, _ = timed()
+    bits = cache[1].view(torch.uint8 if kind == "e4m3" else torch.int16)
+    bits[table[0, at // 16], at % 16, :, channel] = 127 if kind == "e4m3" else 0x7fc0
+    dirty, (o, lse) = timed()
+    print(f"[time] clean {1e3 * clean:.0f} us, with a NaN {1e3 * dirty:.0f} us", flush=True)
+    o, lse = o.cpu(), lse.t().cpu()
+    assert torch.isfinite(o[:700]).all() and torch.isnan(o[700:, :, channel]).all()
+    others = torch.arange(d) != channel
+    assert torch.isfinite(o[:, :, others]).all()
+    for first, last in ((0, 20), (680, 720)):  # (the row tile that the NaN cuts, and one before)
+        ref = paged8.window_reference(q[first:last], *vals, table, offsets([last - first]), [had + last])
+        got = o[first:last].clone()
+        got[:, :, channel] = torch.where(torch.isnan(got[:, :, channel]), ref[0][:, :, channel].to(dtype), got[:, :, channel])
+        _assert_close(got, lse[first:last], ref, length, f"rows {first} to {last}")
+    assert dirty <= 25 * clean, "the other rows' sums cost too much"
