@@ -554,5 +554,11 @@ def fast_layout_ok(t):
     return bits & 7 == 0
 
 
+def packed(t):
+    """A packed copy at an address that the kernels take. (contiguous() returns a packed tensor as it is, wherever it begins
+    and whatever the strides of its sizes of one.)"""
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def current_stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)

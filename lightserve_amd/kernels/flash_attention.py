@@ -56,10 +56,9 @@ def as_kernel_layout(t, dp):
         return t
     if t.shape[-1] == dp and _lib.fast_layout_ok(t):
         return t
-    t = t.contiguous()
     if t.shape[-1] != dp:
-        t = F.pad(t, (0, dp - t.shape[-1]))
-    return t
+        return F.pad(t.contiguous(), (0, dp - t.shape[-1]))
+    return _lib.packed(t)
 
 
 def lse_args(lse):

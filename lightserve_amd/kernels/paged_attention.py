@@ -101,7 +101,7 @@ def _windowed(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens, max_seq
     scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
     qs = q.stride()
     if qs[2] != 1 or qs[0] % 8 != 0 or qs[1] % 8 != 0 or q.data_ptr() % 16 != 0:
-        q = q.contiguous()
+        q = _lib.packed(q)
         qs = q.stride()
     bt = block_tables if block_tables.stride(1) == 1 else block_tables.contiguous()
     sl = seq_lens.contiguous()
@@ -170,7 +170,7 @@ def paged_attention_decode(q, k_cache, v_cache, block_tables, seq_lens, *, max_s
     if max_seq_len is None:
         max_seq_len = int(seq_lens.max().item()) if B > 0 else 0
     q_ = q if (q.stride(-1) == 1 and all(s % 8 == 0 for s in q.stride()[:2]) and q.data_ptr() % 16 == 0) \
-        else q.contiguous()
+        else _lib.packed(q)
     bt = block_tables if block_tables.stride(1) == 1 else block_tables.contiguous()
     sl = seq_lens.contiguous()
     o = torch.empty(B, Hq, D, device=q.device, dtype=q.dtype)
@@ -222,7 +222,7 @@ def paged_prefill(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens_k, *
     if max_seqlen_q is None:
         max_seqlen_q = int((cu_seqlens_q[1:] - cu_seqlens_q[:-1]).max().item()) if B > 0 else 0
     q_ = q if (q.stride(-1) == 1 and all(s % 8 == 0 for s in q.stride()[:2]) and q.data_ptr() % 16 == 0) \
-        else q.contiguous()
+        else _lib.packed(q)
     assert k_cache.stride(3) == 1 and v_cache.stride(3) == 1, "the caches' head-dim stride must be 1"
     bt = block_tables if block_tables.stride(1) == 1 else block_tables.contiguous()
     cu, sl = cu_seqlens_q.contiguous(), seq_lens_k.contiguous()  # kept alive until the launch

@@ -116,9 +116,9 @@ def kv_cache_append(k, v, k_cache, v_cache, kv_scales, block_tables, seq_lens, c
     if rows[0] == 0:
         return
     if not _addressable(k):
-        k = k.contiguous()
+        k = _lib.packed(k)
     if not _addressable(v):
-        v = v.contiguous()
+        v = _lib.packed(v)
     _launch(_lib.kv_append, k, v, k_cache, v_cache, kv_scales, shape, block_tables, seq_lens.contiguous(), cu_seqlens)
 
 

@@ -203,3 +203,65 @@ def test_window_arguments(monkeypatch, kw, word):
         paged_prefill(q, kc, vc, bt, cu, sl, max_seqlen_q=1, kv_scales=sc, **kw)
     with pytest.raises(AssertionError, match="causal"):
         paged_prefill(q, kc, vc, bt, cu, sl, max_seqlen_q=1, kv_scales=sc, causal=False, window=3)
+
+
+@pytest.fixture
+def checked(built_library, monkeypatch):
+    """The calls on CPU tensors, each launch replaced by the library's own check of its arguments; the pointers of q (k for the
+    append) that it got."""
+    import contextlib
+    at = []
+
+    def check(name, first):
+        def launch(args, stream):
+            rc, message = getattr(_lib, name + "_check")(args)
+            assert rc == 0, message
+            at.append(getattr(args, first))
+        return launch
+
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(_lib, "device_guard", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(_lib, "current_stream", lambda device: 11)
+    for name, first in (("window", "q"), ("kv_append", "k"), ("decode", "q"), ("prefill_paged", "q")):
+        monkeypatch.setattr(_lib, name, check(name, first))
+    yield at
+    from lightserve_amd.kernels import tiled_matmul
+    tiled_matmul.release_workspaces()
+
+
+def _all_calls(q, k, bt):
+    """The append and the attentions, over 8-bit caches and older ones; a row each."""
+    kc, vc, sc, _, sl, cu = _tensors()
+    half = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
+    sl, cu = sl[:q.shape[0]], cu[:q.shape[0] + 1]
+    return (lambda: kv_cache_append(k, k, kc, vc, sc, bt, sl), lambda: kv_cache_append(k, k, kc, vc, sc, bt, sl, cu),
+            lambda: paged_attention_decode(q, kc, vc, bt, sl, max_seq_len=16, kv_scales=sc),
+            lambda: paged_prefill(q, kc, vc, bt, cu, sl, max_seqlen_q=1, kv_scales=sc),
+            lambda: paged_attention_decode(q, half, half, bt, sl, max_seq_len=16),
+            lambda: paged_prefill(q, half, half, bt, cu, sl, max_seqlen_q=1))
+
+
+def test_packed_rows_at_odd_addresses_are_copied(checked):
+    """Tensors that are contiguous but begin between two 16-byte pieces, and single rows whose strides say nothing."""
+    def shifted(*shape):
+        n = torch.Size(shape).numel()
+        t = torch.zeros(n + 8, dtype=torch.bfloat16)[1:n + 1].view(shape)
+        assert t.is_contiguous() and t.data_ptr() % 16 != 0
+        return t
+
+    single = [torch.zeros(h * 64 + 3, dtype=torch.bfloat16).as_strided((1, h, 64), (h * 64 + 3, 64, 1)) for h in (4, 2)]
+    assert all(t.is_contiguous() and t.stride(0) % 8 != 0 for t in single)
+    bt = torch.zeros(2, 2, dtype=torch.int32)
+    for q, k, table in ((shifted(2, 4, 64), shifted(2, 2, 64), bt), (*single, bt[:1])):
+        for call in _all_calls(q, k, table):
+            call()
+    assert len(checked) == 12 and all(p % 16 == 0 for p in checked)
+
+
+@pytest.mark.parametrize("d", [64, 60])
+def test_the_dense_kernels_layout_of_odd_addresses(d):
+    from lightserve_amd.kernels.flash_attention import as_kernel_layout
+    t = torch.arange(2 * 3 * 5 * d + 1, dtype=torch.float32).to(torch.bfloat16)[1:].view(2, 3, 5, d)
+    got = as_kernel_layout(t, 64)
+    assert _lib.fast_layout_ok(got) and torch.equal(got[..., :d], t) and (got[..., d:] == 0).all()

@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from lightserve_amd.kernels.flash_attention_varlen import flash_attention_varlen_forward
+from lightserve_amd.kernels.paged_attention import paged_attention_decode, paged_prefill
 from lightserve_amd.kernels.quantized_kv_cache import kv_cache_append, kv_cache_read, quantized_kv_cache
 from oracle import paged8
 from tests.paged8_cases import cache8, offsets, tables
@@ -227,3 +228,31 @@ def test_offsets_past_32_bits(gpu):
     gk, gv = kv_cache_read(kc, vc, sc, table.cuda(), cu, total=20, dtype=torch.float32)
     assert torch.equal(gk.cpu().double(), paged8.values(*paged8.quantise_rows(k)))
     assert torch.equal(gv.cpu().double(), paged8.values(*paged8.quantise_rows(v)))
+
+
+def test_rows_at_odd_addresses(gpu):
+    """Packed rows that begin between two 16-byte pieces."""
+    print("case odd addresses", flush=True)
+
+    def shifted(x):
+        t = torch.zeros(x.numel() + 1, dtype=x.dtype, device="cuda")[1:].view(x.shape)
+        assert t.data_ptr() % 16 != 0
+        return t.copy_(x)
+
+    kc, vc, sc = cache8(4, 16, 2, 64, 50)
+    k, v = (_rows(2, 2, 64, torch.bfloat16, s) for s in (51, 52))
+    q = _rows(2, 4, 64, torch.bfloat16, 53, spread=1)
+    for table, lens in ((torch.tensor([[2, 0], [1, 3]], dtype=torch.int32), [18, 20]), (torch.tensor([[3, 1]], dtype=torch.int32), [25])):
+        n = len(lens)
+        sl = torch.tensor(lens, dtype=torch.int32)
+        want = paged8.append_reference(k[:n], v[:n], kc, vc, sc, table, sl)
+        gk, gv, gs = kc.cuda().view(E4M3), vc.cuda().view(E4M3), sc.cuda()
+        dev = table.cuda()
+        kv_cache_append(shifted(k[:n]), shifted(v[:n]), gk, gv, gs, dev, sl.cuda())
+        _same_codes(gk, want[0], "k")
+        _same_codes(gv, want[1], "v")
+        assert torch.equal(gs.cpu(), want[2])
+        cu = offsets([1] * n).cuda()
+        for call in (lambda x, t: paged_attention_decode(x, gk, gv, t, sl.cuda(), kv_scales=gs),
+                     lambda x, t: paged_prefill(x, gk, gv, t, cu, sl.cuda(), kv_scales=gs, window=7)):
+            assert torch.equal(call(shifted(q[:n]), dev), call(q[:n].cuda(), dev))
