@@ -560,5 +560,11 @@ def packed(t):
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def table_rows(block_tables):
+    """A block table with its rows one after another: itself, or a packed copy."""
+    row, column = block_tables.stride()
+    return block_tables if column == 1 and row >= block_tables.shape[1] else packed(block_tables)
+
+
 def current_stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)

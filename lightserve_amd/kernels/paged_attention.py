@@ -103,7 +103,7 @@ def _windowed(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens, max_seq
     if qs[2] != 1 or qs[0] % 8 != 0 or qs[1] % 8 != 0 or q.data_ptr() % 16 != 0:
         q = _lib.packed(q)
         qs = q.stride()
-    bt = block_tables if block_tables.stride(1) == 1 else block_tables.contiguous()
+    bt = _lib.table_rows(block_tables)
     sl = seq_lens.contiguous()
     cu = cu_seqlens_q.contiguous() if cu_seqlens_q is not None else None
     device = q.device
@@ -171,7 +171,7 @@ def paged_attention_decode(q, k_cache, v_cache, block_tables, seq_lens, *, max_s
         max_seq_len = int(seq_lens.max().item()) if B > 0 else 0
     q_ = q if (q.stride(-1) == 1 and all(s % 8 == 0 for s in q.stride()[:2]) and q.data_ptr() % 16 == 0) \
         else _lib.packed(q)
-    bt = block_tables if block_tables.stride(1) == 1 else block_tables.contiguous()
+    bt = _lib.table_rows(block_tables)
     sl = seq_lens.contiguous()
     o = torch.empty(B, Hq, D, device=q.device, dtype=q.dtype)
     lse = torch.empty(B, Hq, device=q.device, dtype=torch.float32) if return_lse else None
@@ -224,7 +224,7 @@ def paged_prefill(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens_k, *
     q_ = q if (q.stride(-1) == 1 and all(s % 8 == 0 for s in q.stride()[:2]) and q.data_ptr() % 16 == 0) \
         else _lib.packed(q)
     assert k_cache.stride(3) == 1 and v_cache.stride(3) == 1, "the caches' head-dim stride must be 1"
-    bt = block_tables if block_tables.stride(1) == 1 else block_tables.contiguous()
+    bt = _lib.table_rows(block_tables)
     cu, sl = cu_seqlens_q.contiguous(), seq_lens_k.contiguous()  # kept alive until the launch
     o = torch.empty(T, Hq, D, device=q.device, dtype=q.dtype)
     lse = torch.empty(Hq, T, device=q.device, dtype=torch.float32) if return_lse else None

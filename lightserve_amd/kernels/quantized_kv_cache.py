@@ -71,7 +71,7 @@ def check_device(named):
 
 def _launch(call, k, v, k_cache, v_cache, kv_scales, shape, block_tables, seq_lens, cu_seqlens):
     """The launch of one of the two calls on checked arguments; k and v are contiguous in head_dim."""
-    bt = block_tables if block_tables.stride(1) == 1 else block_tables.contiguous()
+    bt = _lib.table_rows(block_tables)
     kc, vc = k_cache.stride(), v_cache.stride()
     ks, vs = k.stride(), v.stride()
     rows, max_blocks = bt.shape

@@ -259,6 +259,16 @@ def test_packed_rows_at_odd_addresses_are_copied(checked):
     assert len(checked) == 12 and all(p % 16 == 0 for p in checked)
 
 
+def test_tables_whose_rows_overlap_are_copied(checked):
+    """A table that all sequences share (a row expanded), and one sequence's that was a column."""
+    q, k = torch.zeros(2, 4, 64, dtype=torch.bfloat16), torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    for call in _all_calls(q, k, torch.zeros(2, dtype=torch.int32).expand(2, 2)):
+        call()
+    for call in _all_calls(q[:1], k[:1], torch.zeros(2, 1, dtype=torch.int32).t()):
+        call()
+    assert len(checked) == 12
+
+
 @pytest.mark.parametrize("d", [64, 60])
 def test_the_dense_kernels_layout_of_odd_addresses(d):
     from lightserve_amd.kernels.flash_attention import as_kernel_layout

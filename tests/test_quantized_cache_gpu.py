@@ -230,8 +230,8 @@ def test_offsets_past_32_bits(gpu):
     assert torch.equal(gv.cpu().double(), paged8.values(*paged8.quantise_rows(v)))
 
 
-def test_rows_at_odd_addresses(gpu):
-    """Packed rows that begin between two 16-byte pieces."""
+def test_rows_at_odd_addresses_and_shared_tables(gpu):
+    """Packed rows that begin between two 16-byte pieces; a table that both sequences share; a column as one sequence's table."""
     print("case odd addresses", flush=True)
 
     def shifted(x):
@@ -242,12 +242,14 @@ def test_rows_at_odd_addresses(gpu):
     kc, vc, sc = cache8(4, 16, 2, 64, 50)
     k, v = (_rows(2, 2, 64, torch.bfloat16, s) for s in (51, 52))
     q = _rows(2, 4, 64, torch.bfloat16, 53, spread=1)
-    for table, lens in ((torch.tensor([[2, 0], [1, 3]], dtype=torch.int32), [18, 20]), (torch.tensor([[3, 1]], dtype=torch.int32), [25])):
+    shared = torch.tensor([2, 0], dtype=torch.int32).expand(2, 2)
+    column = torch.tensor([[3], [1]], dtype=torch.int32).t()
+    for table, lens in ((shared, [18, 20]), (column, [25])):
         n = len(lens)
         sl = torch.tensor(lens, dtype=torch.int32)
         want = paged8.append_reference(k[:n], v[:n], kc, vc, sc, table, sl)
         gk, gv, gs = kc.cuda().view(E4M3), vc.cuda().view(E4M3), sc.cuda()
-        dev = table.cuda()
+        dev = shared.cuda()[0].expand(2, 2) if table is shared else table.t().contiguous().cuda().t()
         kv_cache_append(shifted(k[:n]), shifted(v[:n]), gk, gv, gs, dev, sl.cuda())
         _same_codes(gk, want[0], "k")
         _same_codes(gv, want[1], "v")
@@ -255,4 +257,4 @@ def test_rows_at_odd_addresses(gpu):
         cu = offsets([1] * n).cuda()
         for call in (lambda x, t: paged_attention_decode(x, gk, gv, t, sl.cuda(), kv_scales=gs),
                      lambda x, t: paged_prefill(x, gk, gv, t, cu, sl.cuda(), kv_scales=gs, window=7)):
-            assert torch.equal(call(shifted(q[:n]), dev), call(q[:n].cuda(), dev))
+            assert torch.equal(call(shifted(q[:n]), dev), call(q[:n].cuda(), dev.contiguous().clone()))
