@@ -469,7 +469,8 @@ typedef struct {
  *                + i. The read takes positions 0, 1, ...
  * Rows of no sequence, before position 0 or in no block (table entries outside
  * [0, num_blocks)) are not stored; the read writes zeros for them. Two rows of
- * one append must not go to the same slot. */
+ * one append must not go to the same slot. tokens * heads_kv stays below 2^28
+ * (the append; the read and up to head_dim 64 twice that, both four times). */
 typedef struct {
   void* k;
   void* v;

@@ -708,7 +708,10 @@ static int check_kv_cache(const lsfa_kv_cache_args* a, bool append) {
   int rc = check_paged(a->head_dim, 16, a->block_size, a->max_blocks_per_seq, a->k_cache_stride, a->v_cache_stride, 16,
                        a->block_table_stride);
   if (rc) return rc;
-  if ((long long)a->tokens * a->heads_kv > INT32_MAX) return fail(LSFA_ERR_UNSUPPORTED, "more than 2^31 rows in one call");
+  // A launch has fewer than 2^32 threads: 8 or 16 for a row of the append, half as many for one of a large read (launch_kv).
+  const long long rows = (long long)a->tokens * a->heads_kv, threads = rows * (a->head_dim <= 64 ? 8 : 16) / (append ? 1 : 2);
+  if (rows > INT32_MAX || threads > (1LL << 32) - 256)
+    return fail(LSFA_ERR_UNSUPPORTED, "%lld rows in one call, which takes 2^31 - 1 rows and 2^32 threads", rows);
   if (a->tokens == 0) return ok();
   if (!a->k || !a->v || (a->num_blocks > 0 && (!a->kv_scales || !a->k_cache || !a->v_cache)))
     return fail(LSFA_ERR_INVALID, "k, v, k_cache, v_cache and kv_scales must be non-NULL");
@@ -753,6 +756,14 @@ static int run_kv_cache(const lsfa_kv_cache_args* a, bool append, void* stream) 
 int lsfa_kv_append(const lsfa_kv_cache_args* a, void* stream) { return run_kv_cache(a, true, stream); }
 int lsfa_kv_read(const lsfa_kv_cache_args* a, void* stream) { return run_kv_cache(a, false, stream); }
 
+static lsfa::WindowPlan plan_window(const lsfa_window_args* a) {
+  if (a->batch == 0 || a->tokens == 0 || a->max_seqlen_q == 0) return {};
+  return lsfa::window_plan(a->batch, a->tokens, a->heads_kv, a->heads_q / a->heads_kv, a->head_dim,
+                           a->kv_scales != nullptr ? 1 : 2, std::min(a->max_seqlen_q, a->tokens),
+                           std::min<long long>(a->max_seq_len, (long long)a->max_blocks_per_seq * a->block_size), a->window,
+                           a->sinks);
+}
+
 // Checks all but the workspace.
 static int check_window(const lsfa_window_args* a) {
   if (a == nullptr) return fail(LSFA_ERR_INVALID, "args is NULL");
@@ -795,15 +806,10 @@ static int check_window(const lsfa_window_args* a) {
   if (!aligned16(a->q) || !aligned16(a->o) || !aligned16(a->k_cache) || !aligned16(a->v_cache) ||
       (reinterpret_cast<uintptr_t>(a->kv_scales) & 7u) != 0)
     return fail(LSFA_ERR_UNSUPPORTED, "q, o, k_cache and v_cache must be 16-byte aligned, kv_scales 8-byte");
+  const lsfa::WindowPlan w = plan_window(a);
+  if ((long long)w.items * w.waves * 64 > (1LL << 32) - 1 || (long long)a->heads_kv * 256 > (1LL << 32) - 1)
+    return fail(LSFA_ERR_UNSUPPORTED, "rows of q for 2^32 threads or more in one launch (%d tokens, %d heads_q)", a->tokens, a->heads_q);
   return LSFA_OK;
-}
-
-static lsfa::WindowPlan plan_window(const lsfa_window_args* a) {
-  if (a->batch == 0 || a->tokens == 0 || a->max_seqlen_q == 0) return {};
-  return lsfa::window_plan(a->batch, a->tokens, a->heads_kv, a->heads_q / a->heads_kv, a->head_dim,
-                           a->kv_scales != nullptr ? 1 : 2, std::min(a->max_seqlen_q, a->tokens),
-                           std::min<long long>(a->max_seq_len, (long long)a->max_blocks_per_seq * a->block_size), a->window,
-                           a->sinks);
 }
 
 int lsfa_window_check(const lsfa_window_args* a) {

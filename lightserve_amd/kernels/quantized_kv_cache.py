@@ -29,7 +29,8 @@ are cu_seqlens[b] .. cu_seqlens[b+1]-1 (None: one row each, a decode step) and
 its last row goes to position seq_lens[b] - 1 of block_tables int32 [batch,
 max_blocks]. Rows behind the last sequence, before position 0 and in blocks
 outside the cache are not stored; nothing else in the caches changes. Two
-sequences of one call must not write to the same slot. kv_cache_read returns
+sequences of one call must not write to the same slot, and it takes fewer than
+2^28 rows (tokens * heads_kv; 2^29 up to head_dim 64). kv_cache_read returns
 rows 0 .. cu_seqlens[b+1] - cu_seqlens[b] - 1 of each sequence, packed as
 flash_attention_varlen_forward takes them; total is the rows of the result (read
 from cu_seqlens when None, a device sync, so pass it under graph capture), and

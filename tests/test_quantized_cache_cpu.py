@@ -275,3 +275,26 @@ def test_the_dense_kernels_layout_of_odd_addresses(d):
     t = torch.arange(2 * 3 * 5 * d + 1, dtype=torch.float32).to(torch.bfloat16)[1:].view(2, 3, 5, d)
     got = as_kernel_layout(t, 64)
     assert _lib.fast_layout_ok(got) and torch.equal(got[..., :d], t) and (got[..., d:] == 0).all()
+
+
+@pytest.mark.parametrize("d,lanes", [(128, 16), (80, 16), (64, 8), (16, 8)])
+def test_more_rows_than_a_launch_has_threads_for(built_library, d, lanes):
+    """A launch has fewer than 2^32 threads: `lanes` a row for the append, half as many for a large read."""
+    for check, rows in ((_lib.kv_append_check, (1 << 32) // lanes), (_lib.kv_read_check, (1 << 33) // lanes)):
+        most = min(rows - 64, 2 ** 31 - 1)
+        assert check(_kv(heads_kv=1, head_dim=d, tokens=most)) == (0, "")
+        rc, msg = check(_kv(heads_kv=1, head_dim=d, tokens=min(rows, 2 ** 31 - 1)))
+        assert rc == -2 and "rows" in msg, (rc, msg)
+
+
+def test_more_rows_of_queries_than_a_launch_has_threads_for(built_library):
+    """Two threads a (token, query head) row."""
+    big = dict(kv_scales=None, window=0, sinks=0, heads_q=8, heads_kv=1, head_dim=8, batch=8, q_stride=(64, 8), o_stride=(64, 8),
+               max_seqlen_q=1 << 27)
+    assert _lib.window_check(_win(**big, tokens=(1 << 28) - 4096)) == (0, "")
+    for call in (_lib.window_check, lambda a: _lib.window_workspace_size(a)):
+        try:
+            rc, msg = call(_win(**big, tokens=1 << 28))
+        except RuntimeError as e:
+            rc, msg = -2, str(e)
+        assert rc == -2 and "threads" in msg, (rc, msg)

@@ -258,3 +258,21 @@ def test_rows_at_odd_addresses_and_shared_tables(gpu):
         for call in (lambda x, t: paged_attention_decode(x, gk, gv, t, sl.cuda(), kv_scales=gs),
                      lambda x, t: paged_prefill(x, gk, gv, t, cu, sl.cuda(), kv_scales=gs, window=7)):
             assert torch.equal(call(shifted(q[:n]), dev), call(q[:n].cuda(), dev.contiguous().clone()))
+
+
+@pytest.mark.parametrize("d,lanes", [(80, 16), (16, 8)])
+def test_as_many_rows_as_a_launch_has_threads_for(gpu, d, lanes):
+    """The largest append that is not refused, of one row over and over (a stride of 0): its last rows are stored."""
+    rows = (1 << 32) // lanes - 64
+    print(f"case append of {rows} rows d={d}", flush=True)
+    kc, vc, sc = quantized_kv_cache(2, 16, 1, d)
+    k, v = (_rows(1, 1, d, torch.bfloat16, s) for s in (60, 61))
+    table, sl = torch.tensor([[1, 0]], dtype=torch.int32), torch.tensor([20], dtype=torch.int32)
+    cu = torch.tensor([0, rows], dtype=torch.int32)
+    kv_cache_append(k.cuda().expand(rows, 1, d), v.cuda().expand(rows, 1, d), kc, vc, sc, table.cuda(), sl.cuda(), cu.cuda())
+    torch.cuda.synchronize()
+    empty = (torch.zeros(2, 16, 1, d, dtype=torch.uint8), torch.zeros(2, 16, 1, d, dtype=torch.uint8), torch.ones_like(sc.cpu()))
+    want = paged8.append_reference(k.expand(20, 1, d), v.expand(20, 1, d), *empty, table, sl, offsets([20]))
+    _same_codes(kc, want[0], "k")
+    _same_codes(vc, want[1], "v")
+    assert torch.equal(sc.cpu(), want[2])
