@@ -276,3 +276,22 @@ def test_as_many_rows_as_a_launch_has_threads_for(gpu, d, lanes):
     _same_codes(kc, want[0], "k")
     _same_codes(vc, want[1], "v")
     assert torch.equal(sc.cpu(), want[2])
+
+
+def test_the_packed_attention_over_rows_read_back(gpu):
+    """Its output against the oracle's on what the cache stands for. u is half a step of bf16: the weights are rounded to it and
+    their sum with them (2u of sum w |v|), o once more; the scores' fp32 sums add e = (64 + 16) 2^-24 big + 2^-19 twice."""
+    print("case packed attention on rows read back", flush=True)
+    lens = [130, 17, 64]
+    table, pool = tables(lens, 16, 62)
+    cu, sl = offsets(lens).cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
+    k, v = (_rows(sum(lens), 2, 64, torch.bfloat16, s, spread=1).cuda() for s in (63, 64))
+    q = _rows(sum(lens), 4, 64, torch.bfloat16, 65, spread=1)
+    kc, vc, sc = quantized_kv_cache(pool, 16, 2, 64)
+    kv_cache_append(k, v, kc, vc, sc, table.cuda(), sl, cu)
+    o, _ = flash_attention_varlen_forward(q.cuda(), *kv_cache_read(kc, vc, sc, table.cuda(), cu), cu, cu, 130, 130, causal=True)
+    vals = paged8.cache_values(*(t.cpu().view(torch.uint8) for t in (kc, vc, sc)))
+    want, _, a, big = paged8.window_reference(q, *vals, table, offsets(lens), lens)
+    u, e = torch.finfo(torch.bfloat16).eps / 2, 80 * 2.0 ** -24 * big + 2.0 ** -19
+    tol = 1.05 * ((2 * u + 2 * e[..., None] + 130 * 2.0 ** -24) * a + u * want.abs()) + 2.0 ** -24
+    assert ((o.cpu().double() - want).abs() <= tol).all()

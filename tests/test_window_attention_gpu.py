@@ -652,3 +652,116 @@ def test_one_value_not_finite_after_a_long_prefix(gpu, kind, d):
         got[:, :, channel] = torch.where(torch.isnan(got[:, :, channel]), ref[0][:, :, channel].to(dtype), got[:, :, channel])
         _assert_close(got, lse[first:last], ref, length, f"rows {first} to {last}")
     assert dirty <= 25 * clean, "the other rows' sums cost too much"
+
+
+# Chunks for the wide kernel: (queries a sequence, heads, KV heads, head dim): key splits, a head dim with padding, eight waves.
+WIDE = [(40, 4, 2, 64), (200, 4, 2, 80), (64, 16, 8, 128), (1030, 32, 4, 64)]
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("n,hq,hkv,d", WIDE)
+def test_what_no_query_of_a_chunk_sees_is_not_read(gpu, kind, dtype, n, hq, hkv, d):
+    """As test_what_no_query_sees_is_not_read, in the wide kernel: NaN codes, scales of 255, NaN and infinities in K and V and
+    wild table entries between the sinks and the window, behind the sequences and in blocks of nobody."""
+    print(f"case unseen rows of a chunk {kind} {dtype} n={n} hq={hq} d={d}", flush=True)
+    lens, bs, window, sinks = [n + 300, n, n + 150], 16, 40, 5
+    table, pool = tables(lens, bs, 90)
+    q = _q(3 * n, hq, d, dtype, 91)
+    clean = cache8(pool, bs, hkv, d, 92)
+    vals = paged8.cache_values(*clean)
+    if kind == "e4m3":
+        kc, vc, sc = (t.clone() for t in clean)
+        bad_k = bad_v = 127
+    else:
+        kc, vc, sc = vals[0].to(dtype), vals[1].to(dtype), None
+        vals, bad_k, bad_v = (kc.double(), vc.double()), math.nan, math.inf
+        kc, vc = kc.clone(), vc.clone()
+    seen = torch.zeros(pool, bs, dtype=torch.bool)
+    dirty = table.clone()
+    for b, length in enumerate(lens):
+        pos = torch.arange(length)
+        pos = pos[(pos < sinks) | (pos > length - n - window)]
+        seen[table[b, pos // bs].long(), pos % bs] = True
+        for i in set(range(table.shape[1])) - set((pos // bs).tolist()):
+            dirty[b, i] = [-5, 1 << 30, pool, int(table[0, 0])][i % 4]
+    kc[~seen], vc[~seen] = bad_k, bad_v
+    if sc is not None:
+        sc.transpose(1, 2)[~seen] = 255
+    cache = [t.cuda().view(E4M3) if sc is not None else t.cuda() for t in (kc, vc)]
+    sl, cu = torch.tensor(lens, dtype=torch.int32).cuda(), offsets([n] * 3)
+    o, lse = paged_prefill(q.cuda(), *cache, dirty.cuda(), cu.cuda(), sl, max_seqlen_q=n, return_lse=True,
+                           kv_scales=sc.cuda() if sc is not None else None, window=window, sinks=sinks)
+    _assert_close(o, lse.t(), paged8.window_reference(q, *vals, table, cu, lens, window, sinks), max(lens), "wide")
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("n,hq,hkv,d", WIDE)
+def test_nan_of_a_key_and_blocks_outside_in_chunks(gpu, kind, dtype, n, hq, hkv, d):
+    """A NaN in K reaches the rows that see its key, whole, and no other; blocks outside the cache read as zeros."""
+    print(f"case NaN keys of a chunk {kind} {dtype} n={n} hq={hq} d={d}", flush=True)
+    lens, window, sinks = [n + 100, n], 30, 2
+    table, pool = tables(lens, 16, 93)
+    cache, vals = _cache(kind, dtype, pool, 16, hkv, d, 94)
+    at = 100 + n // 2
+    bits = cache[0].view(torch.uint8 if kind == "e4m3" else torch.int16)
+    bits[table[0, at // 16], at % 16, :, d - 3] = 255 if kind == "e4m3" else -1
+    lost = table.clone()
+    lost[0, 97 // 16], lost[1, 0] = pool, -1
+    q = _q(2 * n, hq, d, dtype, 95)
+    cu = offsets([n, n])
+    p = torch.arange(100, 100 + n)
+    for w, s in ((window, sinks), (None, 0)):
+        if w is None and kind != "e4m3":
+            continue
+        o, lse = (t.cpu() for t in paged_prefill(q.cuda(), *cache[:2], lost.cuda(), cu.cuda(),
+                                                 torch.tensor(lens, dtype=torch.int32).cuda(), max_seqlen_q=n, return_lse=True,
+                                                 kv_scales=cache[2], window=w, sinks=s))
+        lse = lse.t().contiguous()
+        sees = (at <= p) & ((at > p - w) if w is not None else True)
+        assert torch.isnan(o[:n][sees]).all() and torch.isnan(lse[:n][sees]).all() and sees.any() and not sees.all()
+        ref = paged8.window_reference(q, *vals, lost, cu, lens, w, s)
+        o[:n][sees], lse[:n][sees] = ref[0][:n][sees].to(dtype), ref[1][:n][sees].float()
+        _assert_close(o, lse, ref, max(lens), f"the others w={w}")
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("hq,hkv,d", [(64, 1, 64), (96, 2, 128), (66, 2, 80), (128, 1, 128)])
+def test_decode_of_many_heads_on_one(gpu, kind, dtype, hq, hkv, d):
+    """More than 32 query heads on a KV head, which go to the wide kernel without offsets: lengths around its tiles, long ones
+    whose keys are split, more sequences than lanes."""
+    print(f"case decode of many heads {kind} {dtype} hq={hq} hkv={hkv} d={d}", flush=True)
+    for lens in ([1, 15, 63, 64, 65, 0, 129, 500], [9000, 3, 2500], [(29 * b * b) % 300 for b in range(70)]):
+        for window, sinks in ((None, 0), (200, 3)):
+            if window is not None or kind == "e4m3":
+                _decode(kind, dtype, lens, hq, hkv, d, 16, hq + d, window, sinks, what=f"{len(lens)} sequences w={window}")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,had,hq,hkv", [(40, 200, 4, 1), (40, 3000, 4, 1), (2048, 150, 32, 2)])
+def test_scores_that_rise_in_chunks(gpu, dtype, n, had, hq, hkv):
+    """Scores near zero in a row's first tile and far above the offset that it set later: the exponentials are taken again and
+    the sums scaled; whole items of four and of eight waves, and splits."""
+    print(f"case rising scores {dtype} n={n} had={had}", flush=True)
+    length, d = n + had, 64
+    table, pool = tables([length], 16, 96)
+    kc, vc, sc = cache8(pool, 16, hkv, d, 97)
+    g = torch.Generator().manual_seed(98)
+    for i in range(-(-length // 16)):  # first tiles of 2^-12, then each 64 keys one of 2^-7 .. 2^-2 of the codes' values
+        e = 115 if i < 4 else int(torch.randint(119, 125, (1,), generator=g))
+        sc[table[0, i], ..., 0] = e
+    vals = paged8.cache_values(kc, vc, sc)
+    q = _q(n, hq, d, dtype, 99)
+    scores = (q[-1, 0].double() @ paged8.rows_of(vals[0], table, 0, length)[:, 0].T) / 8 / math.log(2)
+    assert scores[64:].max() - scores[:64].max() > 20  # past 2^15 of fp16 after the first tile
+    o, lse = paged_prefill(q.cuda(), kc.cuda().view(E4M3), vc.cuda().view(E4M3), table.cuda(), offsets([n]).cuda(),
+                           torch.tensor([length], dtype=torch.int32).cuda(), max_seqlen_q=n, return_lse=True, kv_scales=sc.cuda())
+    want, want_lse, a, big = paged8.window_reference(q, *vals, table, offsets([n]), [length])
+    if dtype == torch.float16:
+        # Scores this far apart bring p into fp16's subnormals, which the bound leaves out: there a p (relative to the row's
+        # offset) is off by at most half of 2^-24. The offset is the largest score of one of the row's tiles, so one p of the row
+        # is at least 1 and their sum l too, and sums under a lower offset are scaled by less than 1 when it rises: o is off by
+        # at most 2^-25 sum |v_j| / l <= 2^-25 sum |v_j| over the keys that the row sees. As 2u a = 2^-10 a, a takes that in as
+        # 2^-15 sum |v_j|.
+        v = paged8.rows_of(vals[1], table, 0, length).abs().cumsum(0)[had:].repeat_interleave(hq // hkv, 1)
+        a = a + 2.0 ** -15 * v
+    _assert_close(o, lse.t(), (want, want_lse, a, big), length, "rising")
