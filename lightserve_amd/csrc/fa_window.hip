@@ -9,9 +9,11 @@
 // Few rows per KV head (decode, and chunks of a few tokens): the narrow kernel.
 // Many: the wide one, further down.
 // The narrow path is bound by HBM (64 sequences of 8192 tokens, 8 KV heads of 128, 8
-// bits: 207 us, 5.2 TB/s; 64 windows of 4096: 116 us, 4.7) or, for one sequence, by
-// latency (1500 tokens 12 us, 32768 30), so it is built around bytes in flight, and
-// each byte of the cache is read once for all query heads that share it:
+// bits: 203 us, 5.3 TB/s; 64 windows of 4096: 112-114 us, 4.8, of 16 bits 193 us, 5.6) or,
+// for one sequence, by latency (1500 tokens 10 us, 32768 27, 131072 64), so it is built
+// around bytes in flight, and each byte of the cache is read once for all query heads that
+// share it. (Where comments below set two variants side by side, both were timed in replayed
+// graphs of a few calls, 2 to 3 us above the kernels' own time.)
 //   rows       (token, query head of the KV head's group) pairs, 16 or 32 to a row
 //              tile, are the columns of S^T = K Q^T and of O^T += V^T P^T on
 //              v_mfma_f32_16x16x32. Q lies in LDS: registers hold loads in flight.
@@ -736,7 +738,8 @@ __global__ __launch_bounds__(256) void fa_window_combine_kernel(const WindowPara
 // O^T += V^T P^T on v_mfma_f32_32x32x16 (fa_common.hpp has the lane layouts), the
 // scores of tile t + 1 beside the softmax of tile t. Bound by the matrix pipe and the
 // exponentials that share its issue slots (batched chunks over 8-bit prefixes 327 to 339
-// us by the card, 960 to 1000 TFLOP/s, where a large bf16 product reaches 1265), short
+// us by the card, 960 to 1000 TFLOP/s, where a large bf16 product of normal operands
+// reaches 1230 to 1330; the first 25 ms after a pause take up to a third longer), short
 // ones by their steps' latency (2.7 us a tile of 64 keys, and 6 us before the first).
 constexpr int kWideTile = 64;  // keys
 

@@ -48,7 +48,8 @@ power-of-two block_size of at least 16 (any heads_q / heads_kv) and, over 8-bit
 caches, a head_dim that is a multiple of 16. A query that sees no key gets o = 0
 and lse = -inf. Infinities and NaN in the cache reach only the queries that see
 their keys. fp16 queries need rows of an 8-bit cache that fp16 holds (those
-appended in fp16 always are; the values are fp16 in the products).
+appended in fp16 always are; the values are fp16 in the products, except that
+a decode step or a chunk of up to 32 rows a KV head multiplies K's scales in fp32).
 """
 import math
 
