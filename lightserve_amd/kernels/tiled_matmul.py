@@ -100,7 +100,7 @@ class _Entry:
     __slots__ = ("buf", "captured", "graph_buf", "launching")
 
     def __init__(self):
-        self.launching = threading.Lock()  # held from a call's first launch to its last
+        self.launching = threading.RLock()  # held from a call's first launch to its last
         self.buf = None        # the workspace of eager calls
         self.captured = 0      # the last graph capture on the stream (lsfa_capture_id)
         self.graph_buf = None  # its workspace
@@ -112,15 +112,13 @@ _workspaces_lock = threading.Lock()
 
 
 def _workspace(device, stream, nbytes):
-    with _workspaces_lock:
-        return _workspace_locked(device, stream, nbytes)
+    return stream_workspace(device, stream, nbytes)[0]
 
 
 def stream_workspace(device, stream, nbytes):
     """The stream's workspace, and the lock to hold while a call that uses it is launched."""
     with _workspaces_lock:
-        buf = _workspace_locked(device, stream, nbytes)
-        return buf, _workspaces[device.index, stream].launching
+        return _workspace_locked(device, stream, nbytes)
 
 
 def _workspace_locked(device, stream, nbytes):
@@ -142,8 +140,8 @@ def _workspace_locked(device, stream, nbytes):
         victim = next((k for k, e in _workspaces.items() if not e.captured), None)
         if victim is None:
             break
-        del _workspaces[victim]
-    return buf
+        del _workspaces[victim]  # (this call's own, where all others have captures)
+    return buf, entry.launching
 
 
 def release_workspaces():

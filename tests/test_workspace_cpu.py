@@ -130,3 +130,17 @@ def test_threads_on_streams_of_their_own_do_not_wait(played):
     for t in threads:
         t.join()
     assert len(set(met)) == 2
+
+
+def test_a_workspace_that_the_cache_has_no_room_for(capture):
+    """More streams with a captured graph than the cache keeps: an eager call on another stream still gets a workspace and its
+    lock, which it can take twice (a finalizer or signal handler may make a call of its own)."""
+    for n in range(tm.MAX_CACHED_STREAMS):
+        capture(n + 1)
+        tm._workspace(CPU, 100 + n, 1 << 20)
+    capture(0)
+    first, launching = tm.stream_workspace(CPU, STREAM, 1 << 20)
+    again, other = tm.stream_workspace(CPU, STREAM, 1 << 20)
+    assert _clean(first) and _clean(again) and (first is again) == (launching is other)
+    with launching, launching:
+        pass
