@@ -97,8 +97,8 @@ def draw(rng):
     most = 200_000_000 // (c["sequences"] * c["layers"] * row)
     if op == "keep":
         c["nodes_longest"] = _spread(rng, 1, max(1, min(4096, most)))
-        c |= dict(nodes_shortest=rng.randint(0, c["nodes_longest"]), kept_percent=rng.randint(1, 100), cached=rng.choice([0, rng.randint(1, 200)]))
-        return c
+        return c | dict(nodes_shortest=rng.randint(0, c["nodes_longest"]), kept_percent=rng.randint(1, 100),
+                        cached=rng.choice([0, rng.randint(1, 200)]))
     c["beams"] = _spread(rng, 1, min(32, max(1, most // 200)))
     c["longest"] = _spread(rng, 1, max(70, min(8192, (most - c["beams"] * c["block"]) // 2)))
     return c | dict(shortest=rng.randint(0, c["longest"]))
@@ -229,7 +229,8 @@ def _prepare_accept(case, gen, host, seed):
     logits = (torch.randn(total, vocab, generator=gen, device="cuda") * 2.5).to(DTYPES[case["dtype"]])
     # Drafts guess well: a node's token is the choice after its parent two times in three.
     first = [c for c, p in zip(cu.tolist(), parents) for _ in p]
-    parent = torch.tensor([first[t] + max(p, 0) for t, p in enumerate(p for tree in parents for p in tree)], dtype=torch.long).cuda()
+    flat = [p for tree in parents for p in tree]
+    parent = torch.tensor([at + max(p, 0) for at, p in zip(first, flat)], dtype=torch.long).cuda()
     guess = torch.randint(0, vocab, (total,), generator=gen, device="cuda")
     good = torch.rand(total, generator=gen, device="cuda") < 0.67
     choice = logits.float().argmax(1) if total else guess
@@ -238,7 +239,7 @@ def _prepare_accept(case, gen, host, seed):
 
 
 def _caches(case, gen, blocks):
-    """K and V of all layers, and an 8-bit cache's scales, each [layers, ...]."""
+    """K and V of all layers, and an 8-bit cache's scales, each one tensor [layers, ...]."""
     shape = (case["layers"], blocks, case["block"], case["kv_heads"], case["dim"])
     if case["cache"] != "e4m3":
         return (*(torch.randn(shape, generator=gen, device="cuda", dtype=DTYPES[case["cache"]]) for _ in range(2)), None)
@@ -293,8 +294,6 @@ def prepare(case, seed):
     s = {"tree": _prepare_tree, "accept": _prepare_accept, "keep": _prepare_keep, "select": _prepare_select,
          "reorder": _prepare_reorder}[case["op"]](case, gen, host, seed)
     s["case"] = case
-    if "k" in s:  # a program holds a cache for each layer
-        s["layers"] = [None if s[name] is None else list(s[name].unbind(0)) for name in ("k", "v", "scales")]
     return s
 
 
@@ -453,11 +452,10 @@ def run(s):
                               seq_lens=s["seq_lens"]), s["seq_lens"]
     if op == "select":
         return beam_search_select(s["logits"], s["scores"], s["case"]["number"])
-    k, v, scales = s["layers"]
     if op == "keep":
-        kv_cache_keep(k, v, s["block_tables"], s["seq_lens"], s["keep"], s["counts"], kv_scales=scales)
+        kv_cache_keep(s["k"], s["v"], s["block_tables"], s["seq_lens"], s["keep"], s["counts"], kv_scales=s["scales"])
         return s["k"], s["v"], s["scales"]
-    kv_cache_reorder(k, v, s["block_tables"], s["seq_lens"], s["parents"], kv_scales=scales)
+    kv_cache_reorder(s["k"], s["v"], s["block_tables"], s["seq_lens"], s["parents"], kv_scales=s["scales"])
     return s["k"], s["v"], s["scales"], s["block_tables"]
 
 
