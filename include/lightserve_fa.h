@@ -447,6 +447,109 @@ typedef struct {
   int32_t reserved;
 } lsfa_greedy_args;
 
+/* The drafted tokens of a tree that the model itself would have chosen (no
+ * reference counterpart). Sequence b's nodes are rows cu_seqlens[b] ..
+ * cu_seqlens[b+1]-1 of logits (the model's after each node), tokens and
+ * tree_mask (at most max_nodes <= LSFA_TREE_MAX_NODES of them), bit j of a
+ * node's mask saying that it sees node j of its sequence. a_i is the argmax
+ * of node i's logits (as lsfa_greedy takes it). The path begins at node 0 and goes
+ * from node i to the lowest j > i with mask_j = mask_i | bit j and token_j = a_i.
+ *   path int32 [batch, max_nodes]: its nodes, -1 behind them; counts int32
+ *   [batch]; next_tokens int64 [batch]: a of the path's last node (a sequence
+ *   without nodes: count 0, next token -1); seq_lens (optional) += counts
+ *   workspace: lsfa_accept_workspace_size() bytes, 256-byte aligned, with
+ *   counters ahead of partial results as lsfa_gemv_args has them */
+#define LSFA_TREE_MAX_NODES 256
+typedef struct {
+  const void* logits;
+  const int64_t* tokens;
+  const int64_t* tree_mask;
+  const int32_t* cu_seqlens;
+  int32_t* seq_lens;
+  int32_t* path;
+  int32_t* counts;
+  int64_t* next_tokens;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t logits_stride;
+  int64_t mask_stride;
+  int32_t dtype;
+  int32_t rows;
+  int32_t cols;
+  int32_t batch;
+  int32_t mask_words;
+  int32_t max_nodes;
+} lsfa_accept_args;
+
+/* Beam search's selection (no reference counterpart): the num best of
+ * scores[b, k] + log_softmax(logits[b * beams + k])[v] over a sequence's beams k
+ * and the vocabulary v, best first, the lower k * cols + v of equals. Ranked
+ * in 64 bits. A row that holds NaN or +inf, or nothing above -inf, offers no
+ * candidates, nor does a beam whose score is NaN or -inf; where fewer than num
+ * candidates are above -inf the rest of the outputs are score -inf, beam 0, token 0.
+ *   logits [batch * beams, cols] fp32/fp16/bf16, columns contiguous; scores fp32
+ *   [batch, beams]; outputs [batch, num] (fp32, int32, int64); beams <=
+ *   LSFA_BEAMS_MAX, num <= LSFA_BEAMS_NUM_MAX
+ *   workspace: lsfa_beam_workspace_size() bytes, as lsfa_accept_args */
+#define LSFA_BEAMS_MAX 64
+#define LSFA_BEAMS_NUM_MAX 64
+typedef struct {
+  const void* logits;
+  const float* scores;
+  float* out_scores;
+  int32_t* out_beams;
+  int64_t* out_tokens;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t logits_stride;
+  int32_t dtype;
+  int32_t batch;
+  int32_t beams;
+  int32_t cols;
+  int32_t num;
+  int32_t reserved;
+} lsfa_beam_args;
+
+/* Rows moved inside a paged KV cache, in all layers by one launch (no reference
+ * counterpart). Caches [layers][num_blocks, block_size, heads_kv, head_dim] of
+ * elements of elem_bytes (kv_scales non-NULL: e4m3 codes with the scales of
+ * lsfa_kv_cache_args, elem_bytes 1), strides in elements (layer, block, slot,
+ * head); a head's row is a multiple of 16 bytes.
+ * lsfa_kv_keep: row start + index[b, i] of sequence b becomes its row start + i, for
+ *   i < counts[b] <= width, start = seq_lens[b] - counts[b] (seq_lens counts the
+ *   rows once they are kept). Entries of at most their own place i, and those
+ *   whose rows the cache does not have, are left alone.
+ * lsfa_kv_reorder: sequence b's beams are rows b * width .. of block_tables and
+ *   seq_lens (the first one's length counts for all). Beam k goes on from
+ *   beam index[b, k] (none of 0 .. width-1: itself): the block-table entries of
+ *   complete blocks become its parent's, and the rows of the last, incomplete block are
+ *   copied into the block that the beam's own entry names, which no other
+ *   beam's may. width <= LSFA_BEAMS_MAX. */
+typedef struct {
+  void* k_cache;
+  void* v_cache;
+  uint8_t* kv_scales;
+  int32_t* block_tables;
+  const int32_t* seq_lens;
+  const int32_t* index;
+  const int32_t* counts;
+  int64_t k_stride[4];
+  int64_t v_stride[4];
+  int64_t scale_layer_stride;
+  int64_t block_table_stride;
+  int64_t index_stride;
+  int32_t elem_bytes;
+  int32_t layers;
+  int32_t batch;
+  int32_t heads_kv;
+  int32_t head_dim;
+  int32_t block_size;
+  int32_t num_blocks;
+  int32_t max_blocks_per_seq;
+  int32_t width;
+  int32_t reserved;
+} lsfa_kv_rows_args;
+
 /* 8-bit paged KV cache: append (quantise on write) and read back. No
  * counterpart in the reference, whose caches hold the model's own type
  * (engine/config.py:5-7).
@@ -552,6 +655,22 @@ typedef struct {
   int32_t reserved;
 } lsfa_window_args;
 
+/* The same for a tree of drafted tokens per sequence (no reference counterpart): the
+ * queries are the sequence's last n cached tokens, n <= LSFA_TREE_MAX_NODES. Query i
+ * sees the tokens before them (of those, under a window, the ones that a query at
+ * position seq_len - n + (drafts that it sees) - 1 sees) and the drafts j whose bit its
+ * mask has, the window apart. window.cu_seqlens_q must be non-NULL;
+ * window.causal is not read.
+ *   tree_mask [tokens, mask_words] words of 64 bits, mask_stride words apart;
+ *   bit j of the row: word j / 64, bit j % 64. Bits past the n drafts are not read. */
+typedef struct {
+  lsfa_window_args window;
+  const int64_t* tree_mask;
+  int64_t mask_stride;
+  int32_t mask_words;
+  int32_t reserved;
+} lsfa_tree_args;
+
 /* ABI version of the loaded library (LSFA_ABI_VERSION). */
 int lsfa_abi_version(void);
 
@@ -639,6 +758,27 @@ int lsfa_window_workspace_size(const lsfa_window_args* args, uint64_t* bytes);
 /* Attention over a paged cache of 8 or 16 bits with an optional window and
  * sinks (see lsfa_window_args). Deterministic. */
 int lsfa_window(const lsfa_window_args* args, void* stream);
+
+/* Attention of draft trees over a paged cache (see lsfa_tree_args): validation,
+ * workspace size, launch. Deterministic. */
+int lsfa_tree_check(const lsfa_tree_args* args);
+int lsfa_tree_workspace_size(const lsfa_tree_args* args, uint64_t* bytes);
+int lsfa_tree(const lsfa_tree_args* args, void* stream);
+
+/* Acceptance of drafted tokens and beam search's selection (see lsfa_accept_args and
+ * lsfa_beam_args): validation, workspace size, launch (one). Deterministic. */
+int lsfa_accept_check(const lsfa_accept_args* args);
+int lsfa_accept_workspace_size(const lsfa_accept_args* args, uint64_t* bytes);
+int lsfa_accept(const lsfa_accept_args* args, void* stream);
+int lsfa_beam_check(const lsfa_beam_args* args);
+int lsfa_beam_workspace_size(const lsfa_beam_args* args, uint64_t* bytes);
+int lsfa_beam(const lsfa_beam_args* args, void* stream);
+
+/* Rows moved inside a paged KV cache (see lsfa_kv_rows_args): validation and launch (one). */
+int lsfa_kv_keep_check(const lsfa_kv_rows_args* args);
+int lsfa_kv_keep(const lsfa_kv_rows_args* args, void* stream);
+int lsfa_kv_reorder_check(const lsfa_kv_rows_args* args);
+int lsfa_kv_reorder(const lsfa_kv_rows_args* args, void* stream);
 
 /* Host-only validation of RoPE arguments; never touches the GPU. */
 int lsfa_rope_check(const lsfa_rope_args* args);

@@ -36,7 +36,11 @@ EXPORTED_SYMBOLS = ("lsfa_abi_version", "lsfa_last_error", "lsfa_fwd_check", "ls
                     "lsfa_gemm_group_check", "lsfa_gemm_group_workspace_size", "lsfa_gemm_group",
                     "lsfa_greedy_check", "lsfa_greedy",
                     "lsfa_kv_append_check", "lsfa_kv_append", "lsfa_kv_read_check", "lsfa_kv_read",
-                    "lsfa_window_check", "lsfa_window_workspace_size", "lsfa_window")
+                    "lsfa_window_check", "lsfa_window_workspace_size", "lsfa_window",
+                    "lsfa_tree_check", "lsfa_tree_workspace_size", "lsfa_tree",
+                    "lsfa_accept_check", "lsfa_accept_workspace_size", "lsfa_accept",
+                    "lsfa_beam_check", "lsfa_beam_workspace_size", "lsfa_beam",
+                    "lsfa_kv_keep_check", "lsfa_kv_keep", "lsfa_kv_reorder_check", "lsfa_kv_reorder")
 
 _i64x4 = ctypes.c_int64 * 4
 _i64x3 = ctypes.c_int64 * 3
@@ -210,6 +214,51 @@ class WindowArgs(ctypes.Structure):
     ]
 
 
+class TreeArgs(ctypes.Structure):
+    """Mirror of lsfa_tree_args, the fields of its lsfa_window_args among its own."""
+    _fields_ = [
+        *WindowArgs._fields_, ("tree_mask", ctypes.c_void_p), ("mask_stride", ctypes.c_int64),
+        ("mask_words", ctypes.c_int32), ("tree_reserved", ctypes.c_int32),
+    ]
+
+
+class AcceptArgs(ctypes.Structure):
+    """Mirror of lsfa_accept_args."""
+    _fields_ = [
+        ("logits", ctypes.c_void_p), ("tokens", ctypes.c_void_p), ("tree_mask", ctypes.c_void_p),
+        ("cu_seqlens", ctypes.c_void_p), ("seq_lens", ctypes.c_void_p), ("path", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p), ("next_tokens", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
+        ("logits_stride", ctypes.c_int64), ("mask_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("rows", ctypes.c_int32), ("cols", ctypes.c_int32), ("batch", ctypes.c_int32),
+        ("mask_words", ctypes.c_int32), ("max_nodes", ctypes.c_int32),
+    ]
+
+
+class BeamArgs(ctypes.Structure):
+    """Mirror of lsfa_beam_args."""
+    _fields_ = [
+        ("logits", ctypes.c_void_p), ("scores", ctypes.c_void_p), ("out_scores", ctypes.c_void_p),
+        ("out_beams", ctypes.c_void_p), ("out_tokens", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64), ("logits_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("batch", ctypes.c_int32), ("beams", ctypes.c_int32), ("cols", ctypes.c_int32),
+        ("num", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
+class KvRowsArgs(ctypes.Structure):
+    """Mirror of lsfa_kv_rows_args."""
+    _fields_ = [
+        ("k_cache", ctypes.c_void_p), ("v_cache", ctypes.c_void_p), ("kv_scales", ctypes.c_void_p),
+        ("block_tables", ctypes.c_void_p), ("seq_lens", ctypes.c_void_p), ("index", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p), ("k_stride", _i64x4), ("v_stride", _i64x4),
+        ("scale_layer_stride", ctypes.c_int64), ("block_table_stride", ctypes.c_int64), ("index_stride", ctypes.c_int64),
+        ("elem_bytes", ctypes.c_int32), ("layers", ctypes.c_int32), ("batch", ctypes.c_int32), ("heads_kv", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("block_size", ctypes.c_int32), ("num_blocks", ctypes.c_int32),
+        ("max_blocks_per_seq", ctypes.c_int32), ("width", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
 # Packed forms of the argument structs: filling one from Python costs a call
 # per field and per stride array (7.8 us for lsfa_fwd_args), packing the same
 # fields in one call and copying the bytes 2.7 us. "=" is the structs' own
@@ -219,7 +268,8 @@ _PACK = {cls: struct.Struct(fmt) for cls, fmt in (
     (FwdArgs, "=5Q19q2Q8ifi"), (BwdArgs, "=10QQ35q2Q8ifi"), (DecodeArgs, "=8QQ17q9if"),
     (PrefillPagedArgs, "=8Q13q10ifi"), (GemvGroupArgs, "=3QqQq4Q4Q4q4q4i4i3Q2qfi"),
     (RmsNormArgs, "=5Q4q3if"), (RopeArgs, "=6Q9q8i4Q7qQq2i"),
-    (KvCacheArgs, "=8Q11q8i"), (WindowArgs, "=11Q13q14ifi"))}
+    (KvCacheArgs, "=8Q11q8i"), (WindowArgs, "=11Q13q14ifi"), (TreeArgs, "=11Q13q14ifiQq2i"),
+    (AcceptArgs, "=9QQ2q6i"), (BeamArgs, "=6QQq6i"), (KvRowsArgs, "=7Q11q10i"))}
 
 
 def pack(cls, *fields):
@@ -274,7 +324,10 @@ def load():
                              ("lsfa_gemv_check", GemvArgs), ("lsfa_gemv_group_check", GemvGroupArgs),
                              ("lsfa_gemm_group_check", GemvGroupArgs),
                              ("lsfa_greedy_check", GreedyArgs), ("lsfa_kv_append_check", KvCacheArgs),
-                             ("lsfa_kv_read_check", KvCacheArgs), ("lsfa_window_check", WindowArgs)):
+                             ("lsfa_kv_read_check", KvCacheArgs), ("lsfa_window_check", WindowArgs),
+                             ("lsfa_tree_check", TreeArgs), ("lsfa_accept_check", AcceptArgs),
+                             ("lsfa_beam_check", BeamArgs), ("lsfa_kv_keep_check", KvRowsArgs),
+                             ("lsfa_kv_reorder_check", KvRowsArgs)):
             fn = getattr(lib, name)
             fn.restype = ctypes.c_int
             fn.argtypes = [ctypes.POINTER(struct)]
@@ -284,7 +337,9 @@ def load():
                              ("lsfa_prefill_paged", PrefillPagedArgs), ("lsfa_gemv", GemvArgs),
                              ("lsfa_gemv_group", GemvGroupArgs), ("lsfa_gemm_group", GemvGroupArgs),
                              ("lsfa_greedy", GreedyArgs), ("lsfa_kv_append", KvCacheArgs),
-                             ("lsfa_kv_read", KvCacheArgs), ("lsfa_window", WindowArgs)):
+                             ("lsfa_kv_read", KvCacheArgs), ("lsfa_window", WindowArgs), ("lsfa_tree", TreeArgs),
+                             ("lsfa_accept", AcceptArgs), ("lsfa_beam", BeamArgs), ("lsfa_kv_keep", KvRowsArgs),
+                             ("lsfa_kv_reorder", KvRowsArgs)):
             fn = getattr(lib, name)
             fn.restype = ctypes.c_int
             fn.argtypes = [ctypes.POINTER(struct), ctypes.c_void_p]
@@ -304,8 +359,11 @@ def load():
         lib.lsfa_gemv_workspace_size.argtypes = [ctypes.POINTER(GemvArgs), ctypes.POINTER(ctypes.c_uint64)]
         lib.lsfa_decode_workspace_size.restype = ctypes.c_int
         lib.lsfa_decode_workspace_size.argtypes = [ctypes.POINTER(DecodeArgs), ctypes.POINTER(ctypes.c_uint64)]
-        lib.lsfa_window_workspace_size.restype = ctypes.c_int
-        lib.lsfa_window_workspace_size.argtypes = [ctypes.POINTER(WindowArgs), ctypes.POINTER(ctypes.c_uint64)]
+        for name, struct in (("lsfa_window", WindowArgs), ("lsfa_tree", TreeArgs), ("lsfa_accept", AcceptArgs),
+                             ("lsfa_beam", BeamArgs)):
+            size = getattr(lib, name + "_workspace_size")
+            size.restype = ctypes.c_int
+            size.argtypes = [ctypes.POINTER(struct), ctypes.POINTER(ctypes.c_uint64)]
         version = lib.lsfa_abi_version()
         if version != ABI_VERSION:
             raise RuntimeError(f"{_LIB_NAME} has ABI version {version}, expected {ABI_VERSION}")
@@ -482,6 +540,77 @@ def window_workspace_size(args):
 
 def window(args, stream):
     _raise_on(load().lsfa_window(ctypes.byref(args), stream), "lsfa_window")
+
+
+def tree_check(args):
+    """Host-only validation (no GPU access); returns (status, message)."""
+    rc = load().lsfa_tree_check(ctypes.byref(args))
+    return rc, load().lsfa_last_error().decode(errors="replace")
+
+
+def tree_workspace_size(args):
+    """Bytes of device workspace lsfa_tree needs (host only; 0 when no sequence is shared out)."""
+    n = ctypes.c_uint64(0)
+    _raise_on(load().lsfa_tree_workspace_size(ctypes.byref(args), ctypes.byref(n)), "lsfa_tree_workspace_size")
+    return n.value
+
+
+def tree(args, stream):
+    _raise_on(load().lsfa_tree(ctypes.byref(args), stream), "lsfa_tree")
+
+
+def accept_check(args):
+    """Host-only validation (no GPU access); returns (status, message)."""
+    rc = load().lsfa_accept_check(ctypes.byref(args))
+    return rc, load().lsfa_last_error().decode(errors="replace")
+
+
+def accept_workspace_size(args):
+    """Bytes of device workspace lsfa_accept needs (host only)."""
+    n = ctypes.c_uint64(0)
+    _raise_on(load().lsfa_accept_workspace_size(ctypes.byref(args), ctypes.byref(n)), "lsfa_accept_workspace_size")
+    return n.value
+
+
+def accept(args, stream):
+    _raise_on(load().lsfa_accept(ctypes.byref(args), stream), "lsfa_accept")
+
+
+def beam_check(args):
+    """Host-only validation (no GPU access); returns (status, message)."""
+    rc = load().lsfa_beam_check(ctypes.byref(args))
+    return rc, load().lsfa_last_error().decode(errors="replace")
+
+
+def beam_workspace_size(args):
+    """Bytes of device workspace lsfa_beam needs (host only)."""
+    n = ctypes.c_uint64(0)
+    _raise_on(load().lsfa_beam_workspace_size(ctypes.byref(args), ctypes.byref(n)), "lsfa_beam_workspace_size")
+    return n.value
+
+
+def beam(args, stream):
+    _raise_on(load().lsfa_beam(ctypes.byref(args), stream), "lsfa_beam")
+
+
+def kv_keep_check(args):
+    """Host-only validation (no GPU access); returns (status, message)."""
+    rc = load().lsfa_kv_keep_check(ctypes.byref(args))
+    return rc, load().lsfa_last_error().decode(errors="replace")
+
+
+def kv_keep(args, stream):
+    _raise_on(load().lsfa_kv_keep(ctypes.byref(args), stream), "lsfa_kv_keep")
+
+
+def kv_reorder_check(args):
+    """Host-only validation (no GPU access); returns (status, message)."""
+    rc = load().lsfa_kv_reorder_check(ctypes.byref(args))
+    return rc, load().lsfa_last_error().decode(errors="replace")
+
+
+def kv_reorder(args, stream):
+    _raise_on(load().lsfa_kv_reorder(ctypes.byref(args), stream), "lsfa_kv_reorder")
 
 
 def rope_check(args):

@@ -28,6 +28,11 @@ hipError_t add_rmsnorm(const NormParams& p, int dtype, bool vec, hipStream_t s);
 hipError_t gemv(const GemvParams& p, bool is_bf16, hipStream_t s);
 hipError_t gemv_mfma(const GemvParams& p, bool is_bf16, hipStream_t s);
 int gemv_capacity(int m);
+SelectPlan select_plan(long long rows, int cols, int dtype);
+hipError_t accept_drafts(const AcceptParams& p, int dtype, int loads, hipStream_t s);
+hipError_t beam_select(const BeamParams& p, int dtype, int loads, hipStream_t s);
+hipError_t kv_keep(const KvRowsParams& p, hipStream_t s);
+hipError_t kv_reorder(const KvRowsParams& p, hipStream_t s);
 hipError_t greedy(const void* logits, int64_t stride, int dtype, int rows, int cols, int64_t* tokens,
                   int32_t* seq_lens, hipStream_t s);
 }  // namespace lsfa
@@ -812,19 +817,22 @@ static int check_window(const lsfa_window_args* a) {
   return LSFA_OK;
 }
 
-int lsfa_window_check(const lsfa_window_args* a) {
-  const int rc = check_window(a);
-  if (rc) return rc;
-  const uint64_t need = plan_window(a).part_bytes;
+static int check_workspace(const char* size_call, const void* workspace, uint64_t bytes, uint64_t need) {
   if (need > 0) {
-    if (!a->workspace) return fail(LSFA_ERR_INVALID, "workspace must be non-NULL");
-    if (a->workspace_bytes < need)
-      return fail(LSFA_ERR_INVALID, "workspace_bytes %llu is below the %llu bytes lsfa_window_workspace_size asks for",
-                  (unsigned long long)a->workspace_bytes, (unsigned long long)need);
-    if ((reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0)
+    if (!workspace) return fail(LSFA_ERR_INVALID, "workspace must be non-NULL");
+    if (bytes < need)
+      return fail(LSFA_ERR_INVALID, "workspace_bytes %llu is below the %llu bytes %s asks for", (unsigned long long)bytes,
+                  (unsigned long long)need, size_call);
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
       return fail(LSFA_ERR_INVALID, "workspace is not 256-byte aligned");
   }
   return ok();
+}
+
+int lsfa_window_check(const lsfa_window_args* a) {
+  const int rc = check_window(a);
+  if (rc) return rc;
+  return check_workspace("lsfa_window_workspace_size", a->workspace, a->workspace_bytes, plan_window(a).part_bytes);
 }
 
 int lsfa_window_workspace_size(const lsfa_window_args* a, uint64_t* bytes) {
@@ -835,9 +843,7 @@ int lsfa_window_workspace_size(const lsfa_window_args* a, uint64_t* bytes) {
   return ok();
 }
 
-int lsfa_window(const lsfa_window_args* a, void* stream) {
-  const int rc = lsfa_window_check(a);
-  if (rc) return rc;
+static int run_window(const lsfa_window_args* a, const lsfa_tree_args* tree, void* stream) {
   if (a->batch == 0 || a->tokens == 0 || a->max_seqlen_q == 0) return ok();
   lsfa::WindowParams p;
   memset(&p, 0, sizeof(p));
@@ -863,9 +869,59 @@ int lsfa_window(const lsfa_window_args* a, void* stream) {
   p.sinks = a->sinks;
   p.scale_log2 = a->sm_scale * 1.4426950408889634f;
   p.scale_abs = fmaxf(fabsf(p.scale_log2), 1e-30f);
+  if (tree != nullptr) {
+    p.tree = reinterpret_cast<const uint32_t*>(tree->tree_mask);
+    p.tree_stride = 2 * tree->mask_stride;
+    p.tree_words = 2 * tree->mask_words;
+  }
   hipError_t e = lsfa::window_attention(p, plan_window(a), a->dtype == LSFA_DTYPE_BF16, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(LSFA_ERR_LAUNCH, "windowed paged attention launch failed: %s", hipGetErrorString(e));
   return ok();
+}
+
+int lsfa_window(const lsfa_window_args* a, void* stream) {
+  const int rc = lsfa_window_check(a);
+  return rc ? rc : run_window(a, nullptr, stream);
+}
+
+static int check_tree(const lsfa_tree_args* a) {
+  if (a == nullptr) return fail(LSFA_ERR_INVALID, "args is NULL");
+  const lsfa_window_args* w = &a->window;
+  lsfa_window_args as = *w;
+  as.causal = 1;
+  const int rc = check_window(&as);
+  if (rc) return rc;
+  if (!w->cu_seqlens_q) return fail(LSFA_ERR_INVALID, "a tree needs cu_seqlens_q");
+  if (w->max_seqlen_q > LSFA_TREE_MAX_NODES)
+    return fail(LSFA_ERR_UNSUPPORTED, "at most %d drafts of a sequence (max_seqlen_q=%d)", LSFA_TREE_MAX_NODES, w->max_seqlen_q);
+  if (a->mask_words < 1 || a->mask_words > LSFA_TREE_MAX_NODES / 64 || a->mask_words * 64 < w->max_seqlen_q)
+    return fail(LSFA_ERR_INVALID, "mask_words (%d) must be 1 .. %d and hold a bit for each of %d drafts", a->mask_words,
+                LSFA_TREE_MAX_NODES / 64, w->max_seqlen_q);
+  if (a->mask_stride < a->mask_words) return fail(LSFA_ERR_INVALID, "mask_stride must be >= mask_words");
+  if (w->batch == 0 || w->tokens == 0 || w->max_seqlen_q == 0) return ok();
+  if (!a->tree_mask || (reinterpret_cast<uintptr_t>(a->tree_mask) & 7u) != 0)
+    return fail(LSFA_ERR_INVALID, "tree_mask must be non-NULL and 8-byte aligned");
+  return ok();
+}
+
+int lsfa_tree_check(const lsfa_tree_args* a) {
+  const int rc = check_tree(a);
+  if (rc) return rc;
+  return check_workspace("lsfa_tree_workspace_size", a->window.workspace, a->window.workspace_bytes,
+                         plan_window(&a->window).part_bytes);
+}
+
+int lsfa_tree_workspace_size(const lsfa_tree_args* a, uint64_t* bytes) {
+  if (bytes == nullptr) return fail(LSFA_ERR_INVALID, "bytes is NULL");
+  const int rc = check_tree(a);
+  if (rc) return rc;
+  *bytes = align256(plan_window(&a->window).part_bytes);
+  return ok();
+}
+
+int lsfa_tree(const lsfa_tree_args* a, void* stream) {
+  const int rc = lsfa_tree_check(a);
+  return rc ? rc : run_window(&a->window, a, stream);
 }
 
 static int prefill_split_count(const lsfa_prefill_paged_args* a, int* least_tiles) {
@@ -1249,6 +1305,203 @@ int lsfa_greedy(const lsfa_greedy_args* a, void* stream) {
   if (e != hipSuccess) return fail(LSFA_ERR_LAUNCH, "greedy launch failed: %s", hipGetErrorString(e));
   return ok();
 }
+
+static int check_logits(const void* logits, int64_t stride, int dtype, long long rows, int cols) {
+  if (dtype != LSFA_DTYPE_FP32 && dtype != LSFA_DTYPE_FP16 && dtype != LSFA_DTYPE_BF16)
+    return fail(LSFA_ERR_INVALID, "unknown dtype %d", dtype);
+  if (rows < 0 || cols < 0) return fail(LSFA_ERR_INVALID, "negative size (rows=%lld cols=%d)", rows, cols);
+  if (rows == 0) return LSFA_OK;
+  if (cols == 0) return fail(LSFA_ERR_INVALID, "choice from an empty row");
+  if (!logits) return fail(LSFA_ERR_INVALID, "logits must be non-NULL");
+  if (stride < cols) return fail(LSFA_ERR_INVALID, "logits_stride must be >= cols");
+  if ((reinterpret_cast<uintptr_t>(logits) & (dtype == LSFA_DTYPE_FP32 ? 3u : 1u)) != 0)
+    return fail(LSFA_ERR_INVALID, "logits are not aligned to their type");
+  if (rows > (1 << 20) || cols > (1 << 20) || rows * lsfa::select_plan(rows, cols, dtype).chunks >= (1LL << 23))
+    return fail(LSFA_ERR_UNSUPPORTED, "more than 2^20 rows or columns, or 2^23 chunks of rows (rows=%lld cols=%d)", rows, cols);
+  return LSFA_OK;
+}
+
+static uint64_t accept_bytes(const lsfa_accept_args* a) {
+  return a->rows == 0 ? 0
+                      : align256(LSFA_GEMV_COUNTER_BYTES + (uint64_t)a->rows * lsfa::select_plan(a->rows, a->cols, a->dtype).chunks * 8);
+}
+
+static int check_accept(const lsfa_accept_args* a) {
+  if (a == nullptr) return fail(LSFA_ERR_INVALID, "args is NULL");
+  if (a->batch < 0 || a->max_nodes < 0) return fail(LSFA_ERR_INVALID, "negative size (batch=%d max_nodes=%d)", a->batch, a->max_nodes);
+  const int rc = check_logits(a->logits, a->logits_stride, a->dtype, a->rows, a->cols);
+  if (rc) return rc;
+  if (a->batch > LSFA_GEMV_COUNTER_BYTES / 4) return fail(LSFA_ERR_UNSUPPORTED, "more than 65536 sequences (batch=%d)", a->batch);
+  if (a->max_nodes > LSFA_TREE_MAX_NODES)
+    return fail(LSFA_ERR_UNSUPPORTED, "at most %d drafts of a sequence (max_nodes=%d)", LSFA_TREE_MAX_NODES, a->max_nodes);
+  if (a->mask_words < 1 || a->mask_words > LSFA_TREE_MAX_NODES / 64 || a->mask_words * 64 < a->max_nodes)
+    return fail(LSFA_ERR_INVALID, "mask_words (%d) must be 1 .. %d and hold a bit for each of %d nodes", a->mask_words,
+                LSFA_TREE_MAX_NODES / 64, a->max_nodes);
+  if (a->mask_stride < a->mask_words) return fail(LSFA_ERR_INVALID, "mask_stride must be >= mask_words");
+  if (a->batch == 0) return LSFA_OK;
+  if (!a->cu_seqlens || !a->counts || !a->next_tokens || (a->max_nodes > 0 && !a->path) || (a->rows > 0 && (!a->tokens || !a->tree_mask)))
+    return fail(LSFA_ERR_INVALID, "tokens, tree_mask, cu_seqlens, path, counts and next_tokens must be non-NULL");
+  return LSFA_OK;
+}
+
+int lsfa_accept_check(const lsfa_accept_args* a) {
+  const int rc = check_accept(a);
+  if (rc) return rc;
+  return check_workspace("lsfa_accept_workspace_size", a->workspace, a->workspace_bytes, a->batch == 0 ? 0 : accept_bytes(a));
+}
+
+int lsfa_accept_workspace_size(const lsfa_accept_args* a, uint64_t* bytes) {
+  if (bytes == nullptr) return fail(LSFA_ERR_INVALID, "bytes is NULL");
+  const int rc = check_accept(a);
+  if (rc) return rc;
+  *bytes = accept_bytes(a);
+  return ok();
+}
+
+int lsfa_accept(const lsfa_accept_args* a, void* stream) {
+  const int rc = lsfa_accept_check(a);
+  if (rc) return rc;
+  if (a->batch == 0) return ok();
+  lsfa::AcceptParams p;
+  memset(&p, 0, sizeof(p));
+  p.logits = a->logits; p.tokens = a->tokens; p.mask = reinterpret_cast<const uint64_t*>(a->tree_mask);
+  p.cu = a->cu_seqlens; p.seq_lens = a->seq_lens; p.path = a->path; p.counts = a->counts; p.next = a->next_tokens;
+  p.counters = static_cast<int*>(a->workspace);
+  p.part = reinterpret_cast<uint64_t*>(static_cast<char*>(a->workspace) + LSFA_GEMV_COUNTER_BYTES);
+  p.stride = a->logits_stride; p.mask_stride = a->mask_stride;
+  p.rows = a->rows; p.cols = a->cols; p.B = a->batch; p.mask_words = a->mask_words; p.max_nodes = a->max_nodes;
+  const lsfa::SelectPlan plan = lsfa::select_plan(a->rows, std::max(a->cols, 1), a->dtype);
+  p.chunks = plan.chunks;
+  hipError_t e = lsfa::accept_drafts(p, a->dtype, plan.loads, reinterpret_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(LSFA_ERR_LAUNCH, "accept launch failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+static uint64_t beam_bytes(const lsfa_beam_args* a) {
+  const uint64_t rows = (uint64_t)a->batch * a->beams;
+  return align256(LSFA_GEMV_COUNTER_BYTES + rows * lsfa::select_plan(rows, a->cols, a->dtype).chunks * (a->num + 2) * 8);
+}
+
+static int check_beam(const lsfa_beam_args* a) {
+  if (a == nullptr) return fail(LSFA_ERR_INVALID, "args is NULL");
+  if (a->batch < 0) return fail(LSFA_ERR_INVALID, "negative size (batch=%d)", a->batch);
+  if (a->beams < 1 || a->beams > LSFA_BEAMS_MAX || a->num < 1 || a->num > LSFA_BEAMS_NUM_MAX)
+    return fail(LSFA_ERR_UNSUPPORTED, "1 .. %d beams and 1 .. %d candidates of a sequence (beams=%d num=%d)", LSFA_BEAMS_MAX,
+                LSFA_BEAMS_NUM_MAX, a->beams, a->num);
+  const long long rows = (long long)a->batch * a->beams;
+  const int rc = check_logits(a->logits, a->logits_stride, a->dtype, rows, a->cols);
+  if (rc) return rc;
+  if (rows == 0) return LSFA_OK;
+  if (a->batch > LSFA_GEMV_COUNTER_BYTES / 4) return fail(LSFA_ERR_UNSUPPORTED, "more than 65536 sequences (batch=%d)", a->batch);
+  // (the lists that meet lie in LDS)
+  if ((long long)a->beams * lsfa::select_plan(rows, a->cols, a->dtype).chunks > 2048)
+    return fail(LSFA_ERR_UNSUPPORTED, "more than 2048 chunks of one sequence's rows (beams=%d cols=%d)", a->beams, a->cols);
+  if (!a->scores || !a->out_scores || !a->out_beams || !a->out_tokens)
+    return fail(LSFA_ERR_INVALID, "scores and the outputs must be non-NULL");
+  return LSFA_OK;
+}
+
+int lsfa_beam_check(const lsfa_beam_args* a) {
+  const int rc = check_beam(a);
+  if (rc) return rc;
+  return check_workspace("lsfa_beam_workspace_size", a->workspace, a->workspace_bytes, a->batch == 0 ? 0 : beam_bytes(a));
+}
+
+int lsfa_beam_workspace_size(const lsfa_beam_args* a, uint64_t* bytes) {
+  if (bytes == nullptr) return fail(LSFA_ERR_INVALID, "bytes is NULL");
+  const int rc = check_beam(a);
+  if (rc) return rc;
+  *bytes = a->batch == 0 ? 0 : beam_bytes(a);
+  return ok();
+}
+
+int lsfa_beam(const lsfa_beam_args* a, void* stream) {
+  const int rc = lsfa_beam_check(a);
+  if (rc) return rc;
+  if (a->batch == 0) return ok();
+  lsfa::BeamParams p;
+  memset(&p, 0, sizeof(p));
+  p.logits = a->logits; p.scores = a->scores;
+  p.out_scores = a->out_scores; p.out_beams = a->out_beams; p.out_tokens = a->out_tokens;
+  p.stride = a->logits_stride;
+  p.B = a->batch; p.K = a->beams; p.cols = a->cols; p.num = a->num;
+  const lsfa::SelectPlan plan = lsfa::select_plan((long long)a->batch * a->beams, a->cols, a->dtype);
+  p.chunks = plan.chunks;
+  p.counters = static_cast<int*>(a->workspace);
+  p.lists = reinterpret_cast<uint64_t*>(static_cast<char*>(a->workspace) + LSFA_GEMV_COUNTER_BYTES);
+  p.sums = p.lists + (int64_t)a->batch * a->beams * p.chunks * a->num;
+  hipError_t e = lsfa::beam_select(p, a->dtype, plan.loads, reinterpret_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(LSFA_ERR_LAUNCH, "beam selection launch failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+static int check_kv_rows(const lsfa_kv_rows_args* a, bool reorder) {
+  if (a == nullptr) return fail(LSFA_ERR_INVALID, "args is NULL");
+  if (a->elem_bytes != 1 && a->elem_bytes != 2 && a->elem_bytes != 4)
+    return fail(LSFA_ERR_INVALID, "elements of 1, 2 or 4 bytes (elem_bytes=%d)", a->elem_bytes);
+  if (a->layers < 0 || a->batch < 0 || a->heads_kv <= 0 || a->head_dim <= 0 || a->num_blocks < 0 || a->max_blocks_per_seq < 0 || a->width < 0)
+    return fail(LSFA_ERR_INVALID, "negative size or no heads (layers=%d batch=%d heads_kv=%d head_dim=%d num_blocks=%d "
+                "max_blocks_per_seq=%d width=%d)", a->layers, a->batch, a->heads_kv, a->head_dim, a->num_blocks, a->max_blocks_per_seq,
+                a->width);
+  const int per = 16 / a->elem_bytes;
+  if (a->head_dim % per != 0 || a->head_dim > 1024)
+    return fail(LSFA_ERR_UNSUPPORTED, "head_dim must be a multiple of %d up to 1024 (got %d)", per, a->head_dim);
+  if (a->block_size <= 0 || (a->block_size & (a->block_size - 1)) != 0 || a->block_size > (1 << 14))
+    return fail(LSFA_ERR_UNSUPPORTED, "block_size must be a power of two up to 2^14 (got %d)", a->block_size);
+  for (int i = 0; i < 4; ++i)
+    if (a->k_stride[i] % per != 0 || a->v_stride[i] % per != 0 || a->k_stride[i] < 0 || a->v_stride[i] < 0)
+      return fail(LSFA_ERR_UNSUPPORTED, "the caches' strides must be multiples of 16 bytes and not negative");
+  if (!aligned16(a->k_cache) || !aligned16(a->v_cache)) return fail(LSFA_ERR_UNSUPPORTED, "the caches must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(a->kv_scales) & 1u) != 0 || a->scale_layer_stride % 2 != 0)
+    return fail(LSFA_ERR_UNSUPPORTED, "kv_scales and their layer stride must be even");
+  if (a->block_table_stride < a->max_blocks_per_seq || a->index_stride < a->width)
+    return fail(LSFA_ERR_INVALID, "block_table_stride and index_stride must cover a row");
+  if (a->batch > 65535 || a->layers > 65535 || (long long)a->heads_kv * a->head_dim > (1 << 24) ||
+      (long long)a->max_blocks_per_seq * a->block_size > (1LL << 30))
+    return fail(LSFA_ERR_UNSUPPORTED, "more than 65535 sequences or layers, 2^24 elements of a token or 2^30 tokens of a sequence");
+  if (reorder) {
+    if (a->width > LSFA_BEAMS_MAX) return fail(LSFA_ERR_UNSUPPORTED, "at most %d beams of a sequence (width=%d)", LSFA_BEAMS_MAX, a->width);
+    if ((long long)a->layers * a->block_size > 65534)
+      return fail(LSFA_ERR_UNSUPPORTED, "more than 65534 rows of one block in all layers (layers=%d block_size=%d)", a->layers, a->block_size);
+  }
+  if (a->layers == 0 || a->batch == 0 || a->width == 0) return LSFA_OK;
+  if (!a->block_tables || !a->seq_lens || !a->index || (!reorder && !a->counts) || ((!a->k_cache || !a->v_cache) && a->num_blocks > 0))
+    return fail(LSFA_ERR_INVALID, "k_cache, v_cache, block_tables, seq_lens, index and (to keep rows) counts must be non-NULL");
+  return LSFA_OK;
+}
+
+static int run_kv_rows(const lsfa_kv_rows_args* a, bool reorder, void* stream) {
+  const int rc = check_kv_rows(a, reorder);
+  if (rc) return rc;
+  if (a->layers == 0 || a->batch == 0 || a->width == 0) return ok();
+  lsfa::KvRowsParams p;
+  memset(&p, 0, sizeof(p));
+  p.k = a->k_cache; p.v = a->v_cache; p.scales = a->kv_scales;
+  p.tables = a->block_tables; p.tables_out = a->block_tables;
+  p.seq_lens = a->seq_lens; p.index = a->index; p.counts = a->counts;
+  for (int i = 0; i < 4; ++i) {
+    p.sk[i] = a->k_stride[i] * a->elem_bytes;
+    p.sv[i] = a->v_stride[i] * a->elem_bytes;
+  }
+  p.scale_layer = a->scale_layer_stride; p.sbt = a->block_table_stride; p.si = a->index_stride;
+  p.layers = a->layers; p.B = a->batch; p.Hkv = a->heads_kv; p.row_bytes = a->head_dim * a->elem_bytes;
+  p.block_shift = log2_exact(a->block_size);
+  p.max_blocks = a->max_blocks_per_seq; p.num_blocks = a->num_blocks; p.width = a->width;
+  hipError_t e = reorder ? lsfa::kv_reorder(p, reinterpret_cast<hipStream_t>(stream)) : lsfa::kv_keep(p, reinterpret_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(LSFA_ERR_LAUNCH, "KV row move launch failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+int lsfa_kv_keep_check(const lsfa_kv_rows_args* a) {
+  const int rc = check_kv_rows(a, false);
+  return rc ? rc : ok();
+}
+int lsfa_kv_keep(const lsfa_kv_rows_args* a, void* stream) { return run_kv_rows(a, false, stream); }
+int lsfa_kv_reorder_check(const lsfa_kv_rows_args* a) {
+  const int rc = check_kv_rows(a, true);
+  return rc ? rc : ok();
+}
+int lsfa_kv_reorder(const lsfa_kv_rows_args* a, void* stream) { return run_kv_rows(a, true, stream); }
 
 int lsfa_rope_check(const lsfa_rope_args* a) {
   if (a == nullptr) return fail(LSFA_ERR_INVALID, "args is NULL");

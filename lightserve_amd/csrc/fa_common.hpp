@@ -371,6 +371,11 @@ struct WindowParams {
   int runs, long_run, part_rows, splits;  // WindowPlan's
   float scale_log2;        // sm_scale * log2(e)
   float scale_abs;         // |scale_log2|, at least 1e-30
+  // Draft trees (the TREE instances): a sequence's queries are drafted tokens, its last cached ones, and
+  // bit j of a query's mask says that it sees draft j.
+  const uint32_t* tree;    // [tokens][tree_stride] words of 32 bits
+  int64_t tree_stride;
+  int tree_words;          // words of a mask
 };
 struct WindowPlan {
   int runs, columns;    // narrow kernel: runs that the key tiles are shared out over, column blocks of 16 rows
@@ -379,6 +384,53 @@ struct WindowPlan {
   int items, waves;     // wide kernel (items > 0): row tiles at most, waves of a workgroup
   int splits;           // workgroups that an item's key tiles are shared out over
   uint64_t part_bytes;  // workspace: arrival counters and partial results, 0 where nothing is shared out
+};
+
+// Choices among a step's logits (fa_select.hip): chunks of a row, and 16-byte loads of a thread per chunk.
+struct SelectPlan {
+  int chunks, loads;
+};
+struct AcceptParams {
+  const void* logits;     // [rows, cols]
+  const int64_t* tokens;  // [rows]
+  const uint64_t* mask;   // [rows][mask_stride] words
+  const int32_t* cu;      // [B + 1]
+  int32_t* seq_lens;      // [B] or null
+  int32_t* path;          // [B, max_nodes]
+  int32_t* counts;        // [B]
+  int64_t* next;          // [B]
+  int* counters;          // [B] arrivals, zero on entry and on exit
+  uint64_t* part;         // [rows, chunks]
+  int64_t stride, mask_stride;
+  int rows, cols, B, mask_words, max_nodes, chunks;
+};
+struct BeamParams {
+  const void* logits;   // [B * K, cols]
+  const float* scores;  // [B, K]
+  float* out_scores;    // [B, num]
+  int32_t* out_beams;
+  int64_t* out_tokens;
+  int* counters;        // [B] arrivals, zero on entry and on exit
+  uint64_t* lists;      // [B * K, chunks, num]: keys and indices of a chunk's largest values
+  uint64_t* sums;       // [B * K, chunks, 2]: its maximum and sum of exponentials
+  int64_t stride;
+  int B, K, cols, num, chunks;
+};
+
+// Rows moved inside a paged KV cache (fa_kvrows.hip); byte strides.
+struct KvRowsParams {
+  void* k;
+  void* v;
+  void* scales;  // of 8-bit caches [layers][num_blocks, Hkv, block_size, 2], or null
+  const int32_t* tables;
+  int32_t* tables_out;  // the same, where the call writes it
+  const int32_t* seq_lens;
+  const int32_t* index;   // [B, width]: rows to keep, or parents
+  const int32_t* counts;  // [B] (keep)
+  int64_t sk[4], sv[4];   // layer, block, slot, head
+  int64_t scale_layer, sbt, si;
+  int layers, B, Hkv, row_bytes;  // bytes of one head's row
+  int block_shift, max_blocks, num_blocks, width;
 };
 
 // Fused residual add + RMSNorm over rows of a [rows, cols] matrix (column

@@ -5,6 +5,8 @@
 // w tokens with s sinks, j > p - w or j < s. Sequence b's queries are the last
 // n of its seq_lens[b] cached tokens (one for a decode step). An 8-bit cache
 // holds e4m3 codes and one power-of-two scale for each row (fa_kvq.hip).
+// In a tree of drafted tokens (the TREE instances) the n queries see the tokens
+// before them and, of one another, those that their masks name.
 //
 // Few rows per KV head (decode, and chunks of a few tokens): the narrow kernel.
 // Many: the wide one, further down.
@@ -201,11 +203,29 @@ __device__ __forceinline__ float bad_value(const uint32_t* w, int k) {
   return (float)__builtin_bit_cast(T, (uint16_t)(w[k / 2] >> (16 * (k & 1))));
 }
 
+// Draft trees: bits at .. at + 31 of the mask of query `row`, of n drafts (bits at the number of
+// the tile's first key, which may lie before the drafts).
+__device__ __forceinline__ uint32_t draft_bits(const WindowParams& p, int64_t row, int n, int at) {
+  const int i = at >> 5;
+  const uint32_t* m = p.tree + row * p.tree_stride;
+  const uint32_t w0 = (unsigned)i < (unsigned)p.tree_words ? m[i] : 0u;
+  const uint32_t w1 = (unsigned)(i + 1) < (unsigned)p.tree_words ? m[i + 1] : 0u;
+  const uint32_t bits = __builtin_amdgcn_alignbit(w1, w0, at & 31);
+  const int left = n - at;  // drafts from bit 0 on
+  return left >= 32 ? bits : left > 0 ? bits & ((1u << left) - 1) : 0u;
+}
+// Position of a query: as many tokens after the last certain one as it sees drafts besides itself.
+__device__ __forceinline__ int draft_position(const WindowParams& p, int64_t row, int n, int base) {
+  int seen = 0;
+  for (int i = 0; i < p.tree_words; ++i) seen += __builtin_popcount(draft_bits(p, row, n, 32 * i));
+  return base + max(seen, 1) - 1;
+}
+
 constexpr int kRowTile = 16;  // rows of a column block; a row tile has one or two
 
 // NC column blocks of 16 rows share the tile's K and V operands. ONE: of a decode step, whose
-// rows all see the same keys.
-template <typename T, typename C, int DP, int NC, bool ONE>
+// rows all see the same keys. TREE: of draft trees.
+template <typename T, typename C, int DP, int NC, bool ONE, bool TREE>
 __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowParams p) {
   using X8 = typename VecT<T>::x8;
   constexpr bool Q8 = sizeof(C) == 1;
@@ -321,15 +341,21 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
     int hi[NC], lo[NC];
 #pragma unroll
     for (int x = 0; x < NC; ++x) {
-      const int pos = p.causal ? seq - n + (rt * RT + 16 * x + c) / G : seq - 1;
-      hi[x] = 16 * x + c < nrows ? pos : -1;
+      const bool row_ok = 16 * x + c < nrows;
+      int pos = p.causal ? seq - n + (rt * RT + 16 * x + c) / G : seq - 1;
+      if constexpr (TREE) pos = row_ok && p.window > 0 ? draft_position(p, tok0 + (rt * RT + 16 * x + c) / G, n, seq - n) : 0;
+      hi[x] = row_ok ? (TREE ? seq - n - 1 : pos) : -1;  // (TREE: beside the drafts of its mask)
       lo[x] = p.window > 0 ? pos - p.window + 1 : 0;
     }
+    // TREE: drafts that the lane's row of column block x sees among the 32 keys from key0 on.
+    auto drafts = [&](int x, int key0) -> uint32_t {
+      return 16 * x + c < nrows ? draft_bits(p, tok0 + (rt * RT + 16 * x + c) / G, n, key0 - (seq - n)) : 0u;
+    };
     // The same of the tile's first and last rows.
     const int t0 = rt * RT / G, t1 = (rt * RT + min(nrows, RT) - 1) / G;
-    const int hi_min = __builtin_amdgcn_readfirstlane(p.causal ? seq - n + t0 : seq - 1);
-    const int hi_max = __builtin_amdgcn_readfirstlane(p.causal ? seq - n + t1 : seq - 1);
-    const int lo_min = p.window > 0 ? hi_min - p.window + 1 : 0, lo_max = p.window > 0 ? hi_max - p.window + 1 : 0;
+    const int hi_min = __builtin_amdgcn_readfirstlane(TREE ? seq - n - 1 : p.causal ? seq - n + t0 : seq - 1);
+    const int hi_max = __builtin_amdgcn_readfirstlane(!TREE && p.causal ? seq - n + t1 : seq - 1);
+    const int lo_min = p.window > 0 ? hi_min + TREE - p.window + 1 : 0, lo_max = p.window > 0 ? hi_max - p.window + 1 : 0;
 
     // Of the run's tiles ta .. tb - 1 of this sequence those that the row tile sees,
     // u = 0 .. nt - 1: n1 with sinks (numbered by their keys) from tile ta on, then
@@ -447,7 +473,9 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
         }
       load_s(t, c0, 0), load_s(t, c1, 1);
       if (!whole(key0)) {
-        uint32_t found = 0;
+        uint32_t found = 0, tree[NC];
+#pragma unroll
+        for (int x = 0; x < NC; ++x) tree[x] = TREE ? drafts(x, key0) >> (4 * g) : 0u;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -455,7 +483,7 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
             const int key = key0 + 16 * h + 4 * g + i;
 #pragma unroll
             for (int x = 0; x < NC; ++x)
-              if (!(key <= hi[x] && (key >= lo[x] || key < sinks))) s[x][h][i] = -INFINITY;
+              if (!(key <= hi[x] && (key >= lo[x] || key < sinks)) && !(TREE && (tree[x] >> (16 * h + i) & 1))) s[x][h][i] = -INFINITY;
             // Rows of V that no query sees are not read as numbers (0 * NaN is NaN).
             const bool used = key <= hi_max && (key >= lo_min || key < sinks);
             if (!used) vs[h][i] = 1.f;
@@ -547,7 +575,7 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
             for (int w = 0; w < VW; ++w) v[w] &= not_finite<T, Q8>(v[w]);
 #pragma unroll
             for (int x = 0; x < NC; ++x)
-              if (key <= hi[x] && (key >= lo[x] || key < sinks)) {
+              if ((key <= hi[x] && (key >= lo[x] || key < sinks)) || (TREE && (drafts(x, key) & 1))) {
 #pragma unroll
                 for (int j = 0; j < VJ; ++j) acc[x][j][i] += bad_value<T, Q8>(v, j);
               }
@@ -746,7 +774,7 @@ constexpr int kWideTile = 64;  // keys
 // The sequence (with its key tiles) and row tile of an item; false past the last. Row
 // tiles go longest first (ranked_item) where their lengths differ: up to 64 sequences
 // without a window. Else they go in order, the last of a sequence first.
-template <int BM>
+template <int BM, bool TREE>
 __device__ __forceinline__ bool wide_item(const WindowParams& p, int item, int lane, int& b, int& rt, KeyTiles& kt) {
   const int G = p.Hq / p.Hkv;
   auto tiles_of = [&](const KeyTiles& t) -> int { return (int)(((int64_t)min(t.n, p.max_n) * G + BM - 1) / BM); };
@@ -759,7 +787,7 @@ __device__ __forceinline__ bool wide_item(const WindowParams& p, int item, int l
     auto above = [&](int x) -> int {
       if (x < 0) return tq;
       if (tq == 0 || nk <= kWideTile * x) return 0;
-      if (!p.causal) return tq;
+      if (TREE || !p.causal) return tq;
       const long long y = ((long long)kWideTile * x - off) * G;  // row tile t ends past key 64 x iff t >= y / BM
       return y < 0 ? tq : 1 + (int)max(0LL, tq - 1 - y / BM);
     };
@@ -805,12 +833,12 @@ struct WideSpan {
   int sink, first, count;
   int hi_max, lo_min;  // keys past hi_max, or before lo_min and no sinks, are seen by no row
 };
-template <int BM>
+template <int BM, bool TREE>
 __device__ __forceinline__ WideSpan wide_span(const WindowParams& p, const KeyTiles& kt, int rt) {
   const int G = p.Hq / p.Hkv, rows = kt.n * G;
-  const int t0 = rt * BM / G, t1 = (min(rows, (rt + 1) * BM) - 1) / G;
+  const int t0 = TREE ? 0 : rt * BM / G, t1 = (min(rows, (rt + 1) * BM) - 1) / G;
   WideSpan s;
-  s.hi_max = p.causal ? kt.seq - kt.n + t1 : kt.seq - 1;
+  s.hi_max = !TREE && p.causal ? kt.seq - kt.n + t1 : kt.seq - 1;
   s.lo_min = p.window > 0 ? kt.seq - kt.n + t0 - p.window + 1 : 0;
   const int end = max(s.hi_max + 1, 0);
   s.first = min(max(s.lo_min, 0), end) / kWideTile;
@@ -832,7 +860,7 @@ template <int BM, int DP> constexpr int kWidePart = BM * 4 + BM * DP;
 template <typename T> constexpr float kWideMaxLog2P = 64.0f;
 template <> constexpr float kWideMaxLog2P<_Float16> = 15.0f;
 
-template <typename T, typename C, int DP, int NW, bool LSE, bool SPLIT>
+template <typename T, typename C, int DP, int NW, bool LSE, bool SPLIT, bool TREE>
 __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(const WindowParams p) {
   using X8 = typename VecT<T>::x8;
   using X4 = typename VecT<T>::x4;
@@ -856,10 +884,10 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
   const int G = p.Hq / p.Hkv;
   int b, rt;
   KeyTiles kt;
-  if (!wide_item<BM>(p, blockIdx.x / p.Hkv, lane, b, rt, kt)) return;  // uniform, before any barrier
+  if (!wide_item<BM, TREE>(p, blockIdx.x / p.Hkv, lane, b, rt, kt)) return;  // uniform, before any barrier
   const int head = wide_head(p, b);
   const int64_t tok0 = kt.tok0;
-  WideSpan sp = wide_span<BM>(p, kt, rt);
+  WideSpan sp = wide_span<BM, TREE>(p, kt, rt);
   const int sink = __builtin_amdgcn_readfirstlane(sp.sink), first = __builtin_amdgcn_readfirstlane(sp.first);
   const int hi_max = __builtin_amdgcn_readfirstlane(sp.hi_max), lo_min = __builtin_amdgcn_readfirstlane(sp.lo_min);
   int t_lo = 0, t_hi = __builtin_amdgcn_readfirstlane(sp.count);
@@ -878,11 +906,12 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
   // The lane's row and what it sees, and the same over the wave's rows.
   const int r0 = rt * BM + wave * 32, r = r0 + l32, tok = r / G, hq = head * G + (r - tok * G);
   const bool row_ok = r < nrows;
-  const int pos = p.causal ? seq - kt.n + tok : seq - 1;
-  const int hi = row_ok ? pos : -1, lo = p.window > 0 ? pos - p.window + 1 : 0;
-  const int w0 = seq - kt.n + r0 / G, w1 = seq - kt.n + (min(r0 + 32, nrows) - 1) / G;
-  const int whi_min = __builtin_amdgcn_readfirstlane(p.causal ? w0 : seq - 1);
-  const int whi_max = __builtin_amdgcn_readfirstlane(r0 >= nrows ? -1 : p.causal ? w1 : seq - 1);
+  int pos = p.causal ? seq - kt.n + tok : seq - 1;
+  if constexpr (TREE) pos = row_ok && p.window > 0 ? draft_position(p, tok0 + tok, kt.n, seq - kt.n) : 0;
+  const int hi = row_ok ? (TREE ? seq - kt.n - 1 : pos) : -1, lo = p.window > 0 ? pos - p.window + 1 : 0;
+  const int w0 = seq - kt.n + (TREE ? 0 : r0 / G), w1 = TREE ? seq - 1 : seq - kt.n + (min(r0 + 32, nrows) - 1) / G;
+  const int whi_min = __builtin_amdgcn_readfirstlane(TREE ? seq - kt.n - 1 : p.causal ? w0 : seq - 1);
+  const int whi_max = __builtin_amdgcn_readfirstlane(r0 >= nrows ? -1 : !TREE && p.causal ? w1 : seq - 1);
   const int wlo_min = __builtin_amdgcn_readfirstlane(p.window > 0 ? w0 - p.window + 1 : 0);
   const int wlo_max = __builtin_amdgcn_readfirstlane(p.window > 0 ? w1 - p.window + 1 : 0);
 
@@ -999,17 +1028,23 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
     }
     __builtin_amdgcn_sched_barrier(0);
   };
+  // TREE: drafts that the lane's row sees among the 32 keys from key0 on.
+  auto drafts = [&](int key0) -> uint32_t { return row_ok ? draft_bits(p, tok0 + tok, kt.n, key0 - (seq - kt.n)) : 0u; };
   auto mask = [&](int t, f32x16* s) {
     const int key0 = key_of(t);
     if (!(key0 + BN - 1 <= whi_min && (key0 >= wlo_max || key0 + BN - 1 < sinks))) {
       asm volatile("" ::: "memory");  // stays a branch
       const int up = hi - key0 - 4 * hh, dn = lo - key0 - 4 * hh, sk = sinks - key0 - 4 * hh;
+      uint32_t tree[KB];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) tree[kb] = TREE ? drafts(key0 + 32 * kb) >> (4 * hh) : 0u;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int k = 32 * kb + 8 * (i >> 2) + (i & 3);
-          s[kb][i] = k <= up && (k >= dn || k < sk) ? s[kb][i] : -INFINITY;
+          const bool seen = k <= up && (k >= dn || k < sk);
+          s[kb][i] = seen || (TREE && (tree[kb] >> (k & 31) & 1)) ? s[kb][i] : -INFINITY;
         }
     }
   };
@@ -1302,12 +1337,14 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
         };
         to_lds(K, 0, false);
         f32x16 s = {};
+        const uint32_t tree = TREE ? drafts(key0) >> (4 * hh) : 0u;
 #pragma unroll
         for (int kk = 0; kk < KSTEPS; ++kk) s = mfma32(*(const LDS_AS X8*)(wb + (koff ^ (kk << 5))), qreg[kk], s);
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           const int key = key0 + 4 * hh + 8 * (k >> 2) + (k & 3);
-          s[k] = key <= hi && (key >= lo || key < sinks) ? fast_exp2(fmaf(s[k], sl2, -m_run)) : 0.f;
+          const bool seen = (key <= hi && (key >= lo || key < sinks)) || (TREE && (tree >> (8 * (k >> 2) + (k & 3)) & 1));
+          s[k] = seen ? fast_exp2(fmaf(s[k], sl2, -m_run)) : 0.f;
         }
         const X8 pb[2] = {pack8<T>(s, 0), pack8<T>(s, 8)};
         in_order();
@@ -1326,7 +1363,8 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
         for (int key = key0; key < key0 + 32; ++key) {
           if (key > whi_max || (key < wlo_min && key >= sinks)) continue;
           const int blk = table[key >> p.block_shift];
-          if ((unsigned)blk >= (unsigned)p.num_blocks || !(key <= hi && (key >= lo || key < sinks))) continue;
+          const bool seen = (key <= hi && (key >= lo || key < sinks)) || (TREE && (drafts(key) & 1));
+          if ((unsigned)blk >= (unsigned)p.num_blocks || !seen) continue;
           const C* row = row_of(V, key, blk);
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt)
@@ -1350,7 +1388,7 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
 
 // Merges the key splits of fa_window_wide_kernel<..., SPLIT>: workgroup (item,
 // dt) combines 32 channels of the item's rows in the accumulators' order.
-template <typename T, int DP, int NW>
+template <typename T, int DP, int NW, bool TREE>
 __global__ __launch_bounds__(NW * 64) void fa_window_wide_combine_kernel(const WindowParams p) {
   using X4 = typename VecT<T>::x4;
   constexpr int BM = NW * 32, DT = DP / 32;
@@ -1358,9 +1396,9 @@ __global__ __launch_bounds__(NW * 64) void fa_window_wide_combine_kernel(const W
   const int l32 = lane & 31, hh = lane >> 5, G = p.Hq / p.Hkv;
   int b, rt;
   KeyTiles kt;
-  if (!wide_item<BM>(p, blockIdx.x / p.Hkv, lane, b, rt, kt)) return;
+  if (!wide_item<BM, TREE>(p, blockIdx.x / p.Hkv, lane, b, rt, kt)) return;
   const int head = wide_head(p, b);
-  const int count = wide_span<BM>(p, kt, rt).count, share = split_share(count, p.splits);
+  const int count = wide_span<BM, TREE>(p, kt, rt).count, share = split_share(count, p.splits);
   if (count <= share) return;  // already in o
   const int n = (count + share - 1) / share;
   const int r = rt * BM + wave * 32 + l32, nrows = min(kt.n, p.max_n) * G;
@@ -1443,11 +1481,13 @@ WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int eb, int max
   return w;
 }
 
-template <typename T, typename C, int DP, int NC>
+template <typename T, typename C, int DP, int NC, bool TREE>
 static hipError_t launch_narrow(const WindowParams& p, const WindowPlan& w, hipStream_t s) {
   const int rt = kRowTile * NC, tiles = (p.max_n * (p.Hq / p.Hkv) + rt - 1) / rt;
-  if (p.max_n == 1) hipLaunchKernelGGL((fa_window_narrow_kernel<T, C, DP, NC, true>), dim3(p.Hkv * tiles, p.runs), dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((fa_window_narrow_kernel<T, C, DP, NC, false>), dim3(p.Hkv * tiles, p.runs), dim3(256), 0, s, p);
+  if (!TREE && p.max_n == 1)
+    hipLaunchKernelGGL((fa_window_narrow_kernel<T, C, DP, NC, !TREE, false>), dim3(p.Hkv * tiles, p.runs), dim3(256), 0, s, p);
+  else
+    hipLaunchKernelGGL((fa_window_narrow_kernel<T, C, DP, NC, false, TREE>), dim3(p.Hkv * tiles, p.runs), dim3(256), 0, s, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || w.long_run == 0) return e;
   const dim3 parts(p.Hkv * tiles, p.B, DP / 32);
@@ -1457,28 +1497,32 @@ static hipError_t launch_narrow(const WindowParams& p, const WindowPlan& w, hipS
     hipLaunchKernelGGL((fa_window_combine_kernel<T, DP, NC, 32>), parts, dim3(256), 0, s, p);
   return hipGetLastError();
 }
-template <typename T, typename C, int DP>
+template <typename T, typename C, int DP, bool TREE>
 static hipError_t launch_wide(const WindowParams& p, const WindowPlan& w, hipStream_t s) {
   if (w.splits > 1) {
-    hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 4, true, true>), dim3(w.items, w.splits), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 4, true, true, TREE>), dim3(w.items, w.splits), dim3(256), 0, s, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((fa_window_wide_combine_kernel<T, DP, 4>), dim3(w.items, DP / 32), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((fa_window_wide_combine_kernel<T, DP, 4, TREE>), dim3(w.items, DP / 32), dim3(256), 0, s, p);
     return hipGetLastError();
   }
   if (w.waves == 8) {
-    if (p.lse != nullptr) hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 8, true, false>), dim3(w.items), dim3(512), 0, s, p);
-    else hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 8, false, false>), dim3(w.items), dim3(512), 0, s, p);
+    if (TREE || p.lse != nullptr) hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 8, true, false, TREE>), dim3(w.items), dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 8, TREE, false, TREE>), dim3(w.items), dim3(512), 0, s, p);
   } else {
-    if (p.lse != nullptr) hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 4, true, false>), dim3(w.items), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 4, false, false>), dim3(w.items), dim3(256), 0, s, p);
+    if (TREE || p.lse != nullptr) hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 4, true, false, TREE>), dim3(w.items), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 4, TREE, false, TREE>), dim3(w.items), dim3(256), 0, s, p);
   }
   return hipGetLastError();
 }
+template <typename T, typename C, int DP, bool TREE>
+static hipError_t launch_rows(const WindowParams& p, const WindowPlan& w, hipStream_t s) {
+  if (w.items > 0) return launch_wide<T, C, DP, TREE>(p, w, s);
+  return w.columns == 1 ? launch_narrow<T, C, DP, 1, TREE>(p, w, s) : launch_narrow<T, C, DP, 2, TREE>(p, w, s);
+}
 template <typename T, typename C, int DP>
 static hipError_t launch_window(const WindowParams& p, const WindowPlan& w, hipStream_t s) {
-  if (w.items > 0) return launch_wide<T, C, DP>(p, w, s);
-  return w.columns == 1 ? launch_narrow<T, C, DP, 1>(p, w, s) : launch_narrow<T, C, DP, 2>(p, w, s);
+  return p.tree != nullptr ? launch_rows<T, C, DP, true>(p, w, s) : launch_rows<T, C, DP, false>(p, w, s);
 }
 template <typename T>
 static hipError_t dispatch_window(const WindowParams& p, const WindowPlan& w, hipStream_t s) {

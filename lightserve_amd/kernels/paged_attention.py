@@ -61,9 +61,10 @@ from .quantized_kv_cache import check_device, check_quantized
 from .tiled_matmul import stream_workspace
 
 
-def _windowed(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens, max_seqlen_q, max_seq_len, causal, sm_scale,
-              return_lse, kv_scales, window, sinks):
-    """Attention over an 8-bit cache or under a window (lsfa_window); the lse is [tokens, heads_q]."""
+def windowed_attention(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens, max_seqlen_q, max_seq_len, causal, sm_scale,
+                       return_lse, kv_scales, window, sinks, tree_mask=None):
+    """Attention over an 8-bit cache or under a window (lsfa_window), or of draft trees (lsfa_tree, with a checked
+    tree_mask); the lse is [tokens, heads_q]."""
     rows, dtype = q.shape, q.dtype
     assert len(rows) == 3, "q must be [tokens, heads_q, head_dim]"
     assert dtype == torch.bfloat16 or dtype == torch.float16, "windowed paged attention supports bf16 and fp16"
@@ -90,10 +91,11 @@ def _windowed(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens, max_seq
     on = q.get_device()
     if not (on >= 0 and on == k_cache.get_device() == v_cache.get_device() == block_tables.get_device()
             == seq_lens.get_device() and (cu_seqlens_q is None or cu_seqlens_q.get_device() == on)
-            and (kv_scales is None or kv_scales.get_device() == on)):
+            and (kv_scales is None or kv_scales.get_device() == on) and (tree_mask is None or tree_mask.get_device() == on)):
         check_device((("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables),
                       ("seq_lens", seq_lens), *((("cu_seqlens_q", cu_seqlens_q),) if cu_seqlens_q is not None else ()),
-                      *((("kv_scales", kv_scales),) if kv_scales is not None else ())))
+                      *((("kv_scales", kv_scales),) if kv_scales is not None else ()),
+                      *((("tree_mask", tree_mask),) if tree_mask is not None else ())))
     if window is None:
         assert sinks == 0, "sinks need a window"
     else:
@@ -118,8 +120,8 @@ def _windowed(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens, max_seq
     if T > 0:
         keys = min(int(max_seq_len), max_blocks * block_size)
         ks, vs = k_cache.stride(), v_cache.stride()
-        args = _lib.pack(
-            _lib.WindowArgs, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(),
+        fields = (
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(),
             lse.data_ptr() if return_lse else 0, kv_scales.data_ptr() if kv_scales is not None else 0,
             cu.data_ptr() if cu is not None else 0, sl.data_ptr(), bt.data_ptr(), 0, 0,  # the workspace follows
             qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], Hq * D, D, ls[0], ls[1], bt.stride(0),
@@ -127,16 +129,23 @@ def _windowed(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens, max_seq
             bool(causal),
             # a window or sinks past the longest sequence say no more than its length
             0 if window is None else min(int(window), keys + 1), min(int(sinks), keys), scale, 0)
-        nbytes = _lib.window_workspace_size(args)
+        if tree_mask is None:
+            args = _lib.pack(_lib.WindowArgs, *fields)
+            size, launch = _lib.window_workspace_size, _lib.window
+        else:
+            args = _lib.pack(_lib.TreeArgs, *fields, tree_mask.data_ptr(), max(tree_mask.stride(0), tree_mask.shape[1]),
+                             tree_mask.shape[1], 0)
+            size, launch = _lib.tree_workspace_size, _lib.tree
+        nbytes = size(args)
         with _lib.device_guard(device):
             stream = _lib.current_stream(device)
             if nbytes > 0:  # arrival counters, kept at zero from call to call, and partial results
                 ws, launching = stream_workspace(device, stream, nbytes)
                 args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
                 with launching:
-                    _lib.window(args, stream)
+                    launch(args, stream)
             else:
-                _lib.window(args, stream)
+                launch(args, stream)
     return (o, lse) if return_lse else o
 
 
@@ -162,7 +171,7 @@ def paged_attention_decode(q, k_cache, v_cache, block_tables, seq_lens, *, max_s
     if kv_scales is not None or window is not None or sinks != 0:
         if max_seq_len is None:
             max_seq_len = int(seq_lens.max().item()) if seq_lens.numel() > 0 else 0
-        return _windowed(q, k_cache, v_cache, block_tables, None, seq_lens, 1, max_seq_len, True, sm_scale, return_lse,
+        return windowed_attention(q, k_cache, v_cache, block_tables, None, seq_lens, 1, max_seq_len, True, sm_scale, return_lse,
                          kv_scales, window, sinks)
     _check(q, k_cache, v_cache, block_tables, seq_lens)
     B, Hq, D = q.shape
@@ -198,7 +207,7 @@ def paged_prefill(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens_k, *
         if max_seqlen_q is None:
             max_seqlen_q = int((cu_seqlens_q[1:] - cu_seqlens_q[:-1]).max().item()) if cu_seqlens_q.numel() > 1 else 0
         most = block_tables.shape[-1] * k_cache.shape[1]
-        got = _windowed(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens_k, max_seqlen_q, most, causal, sm_scale,
+        got = windowed_attention(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens_k, max_seqlen_q, most, causal, sm_scale,
                         return_lse, kv_scales, window, sinks)
         return (got[0], got[1].t()) if return_lse else got
     assert q.dim() == 3, "q must be packed [total_q, heads_q, head_dim]"
