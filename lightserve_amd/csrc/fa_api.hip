@@ -28,7 +28,7 @@ hipError_t add_rmsnorm(const NormParams& p, int dtype, bool vec, hipStream_t s);
 hipError_t gemv(const GemvParams& p, bool is_bf16, hipStream_t s);
 hipError_t gemv_mfma(const GemvParams& p, bool is_bf16, hipStream_t s);
 int gemv_capacity(int m);
-SelectPlan select_plan(long long rows, int cols, int dtype);
+SelectPlan select_plan(long long rows, int cols, int dtype, bool beams);
 hipError_t accept_drafts(const AcceptParams& p, int dtype, int loads, hipStream_t s);
 hipError_t beam_select(const BeamParams& p, int dtype, int loads, hipStream_t s);
 hipError_t kv_keep(const KvRowsParams& p, hipStream_t s);
@@ -1306,7 +1306,7 @@ int lsfa_greedy(const lsfa_greedy_args* a, void* stream) {
   return ok();
 }
 
-static int check_logits(const void* logits, int64_t stride, int dtype, long long rows, int cols) {
+static int check_logits(const void* logits, int64_t stride, int dtype, long long rows, int cols, bool beams) {
   if (dtype != LSFA_DTYPE_FP32 && dtype != LSFA_DTYPE_FP16 && dtype != LSFA_DTYPE_BF16)
     return fail(LSFA_ERR_INVALID, "unknown dtype %d", dtype);
   if (rows < 0 || cols < 0) return fail(LSFA_ERR_INVALID, "negative size (rows=%lld cols=%d)", rows, cols);
@@ -1316,20 +1316,20 @@ static int check_logits(const void* logits, int64_t stride, int dtype, long long
   if (stride < cols) return fail(LSFA_ERR_INVALID, "logits_stride must be >= cols");
   if ((reinterpret_cast<uintptr_t>(logits) & (dtype == LSFA_DTYPE_FP32 ? 3u : 1u)) != 0)
     return fail(LSFA_ERR_INVALID, "logits are not aligned to their type");
-  if (rows > (1 << 20) || cols > (1 << 20) || rows * lsfa::select_plan(rows, cols, dtype).chunks >= (1LL << 23))
+  if (rows > (1 << 20) || cols > (1 << 20) || rows * lsfa::select_plan(rows, cols, dtype, beams).chunks >= (1LL << 23))
     return fail(LSFA_ERR_UNSUPPORTED, "more than 2^20 rows or columns, or 2^23 chunks of rows (rows=%lld cols=%d)", rows, cols);
   return LSFA_OK;
 }
 
 static uint64_t accept_bytes(const lsfa_accept_args* a) {
   return a->rows == 0 ? 0
-                      : align256(LSFA_GEMV_COUNTER_BYTES + (uint64_t)a->rows * lsfa::select_plan(a->rows, a->cols, a->dtype).chunks * 8);
+                      : align256(LSFA_GEMV_COUNTER_BYTES + (uint64_t)a->rows * lsfa::select_plan(a->rows, a->cols, a->dtype, false).parts * 8);
 }
 
 static int check_accept(const lsfa_accept_args* a) {
   if (a == nullptr) return fail(LSFA_ERR_INVALID, "args is NULL");
   if (a->batch < 0 || a->max_nodes < 0) return fail(LSFA_ERR_INVALID, "negative size (batch=%d max_nodes=%d)", a->batch, a->max_nodes);
-  const int rc = check_logits(a->logits, a->logits_stride, a->dtype, a->rows, a->cols);
+  const int rc = check_logits(a->logits, a->logits_stride, a->dtype, a->rows, a->cols, false);
   if (rc) return rc;
   if (a->batch > LSFA_GEMV_COUNTER_BYTES / 4) return fail(LSFA_ERR_UNSUPPORTED, "more than 65536 sequences (batch=%d)", a->batch);
   if (a->max_nodes > LSFA_TREE_MAX_NODES)
@@ -1370,8 +1370,8 @@ int lsfa_accept(const lsfa_accept_args* a, void* stream) {
   p.part = reinterpret_cast<uint64_t*>(static_cast<char*>(a->workspace) + LSFA_GEMV_COUNTER_BYTES);
   p.stride = a->logits_stride; p.mask_stride = a->mask_stride;
   p.rows = a->rows; p.cols = a->cols; p.B = a->batch; p.mask_words = a->mask_words; p.max_nodes = a->max_nodes;
-  const lsfa::SelectPlan plan = lsfa::select_plan(a->rows, std::max(a->cols, 1), a->dtype);
-  p.chunks = plan.chunks;
+  const lsfa::SelectPlan plan = lsfa::select_plan(a->rows, std::max(a->cols, 1), a->dtype, false);
+  p.chunks = plan.chunks; p.per = plan.per; p.parts = plan.parts;
   hipError_t e = lsfa::accept_drafts(p, a->dtype, plan.loads, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(LSFA_ERR_LAUNCH, "accept launch failed: %s", hipGetErrorString(e));
   return ok();
@@ -1379,7 +1379,7 @@ int lsfa_accept(const lsfa_accept_args* a, void* stream) {
 
 static uint64_t beam_bytes(const lsfa_beam_args* a) {
   const uint64_t rows = (uint64_t)a->batch * a->beams;
-  return align256(LSFA_GEMV_COUNTER_BYTES + rows * lsfa::select_plan(rows, a->cols, a->dtype).chunks * (a->num + 2) * 8);
+  return align256(LSFA_GEMV_COUNTER_BYTES + rows * lsfa::select_plan(rows, a->cols, a->dtype, true).chunks * (a->num + 2) * 8);
 }
 
 static int check_beam(const lsfa_beam_args* a) {
@@ -1389,12 +1389,12 @@ static int check_beam(const lsfa_beam_args* a) {
     return fail(LSFA_ERR_UNSUPPORTED, "1 .. %d beams and 1 .. %d candidates of a sequence (beams=%d num=%d)", LSFA_BEAMS_MAX,
                 LSFA_BEAMS_NUM_MAX, a->beams, a->num);
   const long long rows = (long long)a->batch * a->beams;
-  const int rc = check_logits(a->logits, a->logits_stride, a->dtype, rows, a->cols);
+  const int rc = check_logits(a->logits, a->logits_stride, a->dtype, rows, a->cols, true);
   if (rc) return rc;
   if (rows == 0) return LSFA_OK;
   if (a->batch > LSFA_GEMV_COUNTER_BYTES / 4) return fail(LSFA_ERR_UNSUPPORTED, "more than 65536 sequences (batch=%d)", a->batch);
   // (the lists that meet lie in LDS)
-  if ((long long)a->beams * lsfa::select_plan(rows, a->cols, a->dtype).chunks > 2048)
+  if ((long long)a->beams * lsfa::select_plan(rows, a->cols, a->dtype, true).chunks > 2048)
     return fail(LSFA_ERR_UNSUPPORTED, "more than 2048 chunks of one sequence's rows (beams=%d cols=%d)", a->beams, a->cols);
   if (!a->scores || !a->out_scores || !a->out_beams || !a->out_tokens)
     return fail(LSFA_ERR_INVALID, "scores and the outputs must be non-NULL");
@@ -1425,7 +1425,7 @@ int lsfa_beam(const lsfa_beam_args* a, void* stream) {
   p.out_scores = a->out_scores; p.out_beams = a->out_beams; p.out_tokens = a->out_tokens;
   p.stride = a->logits_stride;
   p.B = a->batch; p.K = a->beams; p.cols = a->cols; p.num = a->num;
-  const lsfa::SelectPlan plan = lsfa::select_plan((long long)a->batch * a->beams, a->cols, a->dtype);
+  const lsfa::SelectPlan plan = lsfa::select_plan((long long)a->batch * a->beams, a->cols, a->dtype, true);
   p.chunks = plan.chunks;
   p.counters = static_cast<int*>(a->workspace);
   p.lists = reinterpret_cast<uint64_t*>(static_cast<char*>(a->workspace) + LSFA_GEMV_COUNTER_BYTES);

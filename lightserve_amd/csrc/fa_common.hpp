@@ -386,9 +386,10 @@ struct WindowPlan {
   uint64_t part_bytes;  // workspace: arrival counters and partial results, 0 where nothing is shared out
 };
 
-// Choices among a step's logits (fa_select.hip): chunks of a row, and 16-byte loads of a thread per chunk.
+// Choices among a step's logits (fa_select.hip): chunks of a row, 16-byte loads of a thread per chunk, chunks of a
+// workgroup and workgroups of a row.
 struct SelectPlan {
-  int chunks, loads;
+  int chunks, loads, per, parts;
 };
 struct AcceptParams {
   const void* logits;     // [rows, cols]
@@ -400,9 +401,9 @@ struct AcceptParams {
   int32_t* counts;        // [B]
   int64_t* next;          // [B]
   int* counters;          // [B] arrivals, zero on entry and on exit
-  uint64_t* part;         // [rows, chunks]
+  uint64_t* part;         // [rows, parts]
   int64_t stride, mask_stride;
-  int rows, cols, B, mask_words, max_nodes, chunks;
+  int rows, cols, B, mask_words, max_nodes, chunks, per, parts;
 };
 struct BeamParams {
   const void* logits;   // [B * K, cols]

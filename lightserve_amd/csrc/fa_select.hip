@@ -20,6 +20,7 @@
 #include "../../include/lightserve_fa.h"
 #include "fa_common.hpp"
 
+#include <cfloat>
 #include <algorithm>
 #include <type_traits>
 
@@ -34,41 +35,43 @@ __device__ __forceinline__ uint64_t load_agent(const uint64_t* from) {
   return __hip_atomic_load((uint64_t*)from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// Whole numbers in the order of the values; 0 is below all of them.
-template <typename T> struct Order;
-template <> struct Order<float> {
-  using Raw = uint32_t;
-  static __device__ __forceinline__ uint32_t key(uint32_t u) {
-    u = u == 0x80000000u ? 0u : u;
-    const uint32_t k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-    return (u & 0x7fffffffu) > 0x7f800000u ? 0xffffffffu : k;
-  }
-  static __device__ __forceinline__ float value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
-};
-template <typename T> struct Order16 {
-  using Raw = uint16_t;
-  static constexpr uint32_t kInf = __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
-  static __device__ __forceinline__ uint32_t key(uint32_t u) {
-    u = u == 0x8000u ? 0u : u;
-    const uint32_t k = (u & 0x8000u) ? (~u & 0xffffu) : (u | 0x8000u);
-    return (u & 0x7fffu) > kInf ? 0xffffu : k;
-  }
-  static __device__ __forceinline__ float value(uint32_t k) {
-    return (float)__builtin_bit_cast(T, (uint16_t)((k & 0x8000u) ? k ^ 0x8000u : ~k));
-  }
-};
-template <> struct Order<_Float16> : Order16<_Float16> {};
-template <> struct Order<__bf16> : Order16<__bf16> {};
-
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-  for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
-  return v;
+// Whole numbers in the order of values that are no NaN (-0 as +0), and back.
+__device__ __forceinline__ uint32_t key_of(float f) {
+  const uint32_t u = __float_as_uint(f + 0.f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
-__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint64_t w = __shfl_xor((unsigned long long)v, o);
-    v = w > v ? w : v;
-  }
+__device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
+constexpr uint32_t kKeyNan = 0xffffffffu, kKeyLow = 0x007fffffu;  // above all numbers; of -inf, below them
+
+// Largest of two, NaN where one is (one instruction for three of them).
+__device__ __forceinline__ float nan_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// All lanes' values by one operation, in every lane. The steps within and across rows of 16 lanes leave
+// the result in the last one.
+template <typename F>
+__device__ __forceinline__ float wave_all(float v, F f) {
+#define LSFA_STEP(ctrl, rows) \
+  v = f(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp((int)__float_as_uint(v), (int)__float_as_uint(v), ctrl, rows, 0xf, false)))
+  LSFA_STEP(0x111, 0xf);  // row_shr 1, 2, 4, 8
+  LSFA_STEP(0x112, 0xf);
+  LSFA_STEP(0x114, 0xf);
+  LSFA_STEP(0x118, 0xf);
+  LSFA_STEP(0x142, 0xa);  // row_bcast 15, 31
+  LSFA_STEP(0x143, 0xc);
+#undef LSFA_STEP
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  return wave_all(v, [](float a, float b) { return nan_max(a, b); });
+}
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ int lanes_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
   return v;
 }
 
@@ -76,15 +79,9 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
 // words of memory (a row may begin anywhere: chunks count from the word that it begins in).
 template <typename T, int U>
 struct Chunk {
-  using O = Order<T>;
   static constexpr int EPV = 16 / sizeof(T), E = EPV * U;  // values of a load, of a thread
   static constexpr int C = kThreads * E;
-  // A value's key above its position in the chunk, inverted.
-  using Comp = std::conditional_t<sizeof(T) == 2, uint32_t, uint64_t>;
-  static constexpr int kShift = sizeof(T) == 2 ? 16 : 32;
-  static constexpr int kBits = sizeof(T) == 2 ? 32 : 64;
   static_assert(C <= 65536, "positions have 16 bits");
-
   u32x4 v[U];
   int lo, hi;  // positions of the row's values in the chunk
   int first;   // index in the row of position 0
@@ -103,29 +100,40 @@ struct Chunk {
     first = (int)(start - skip);
   }
   __device__ __forceinline__ int pos(int i) const { return (i / EPV * kThreads + (int)threadIdx.x) * EPV + i % EPV; }
-  __device__ __forceinline__ uint32_t raw(int i) const {
-    const int e = i % EPV;
-    if constexpr (sizeof(T) == 4) return v[i / EPV][e];
-    else return e & 1 ? v[i / EPV][e / 2] >> 16 : v[i / EPV][e / 2] & 0xffffu;
-  }
-  __device__ __forceinline__ bool has(int i) const { return pos(i) >= lo && pos(i) < hi; }
-  // Value i of the thread; 0 where the row has none.
-  __device__ __forceinline__ Comp comp(int i) const {
-    return has(i) ? ((Comp)O::key(raw(i)) << kShift) | (Comp)(65535 - pos(i)) : (Comp)0;
+  // -inf in the places of the first and last chunk that the row does not have.
+  __device__ __forceinline__ void cut() {
+    if (lo <= 0 && hi >= C) return;  // uniform
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      if (pos(i) >= lo && pos(i) < hi) continue;
+      const int e = i % EPV;
+      const int j = sizeof(T) == 4 ? e : e / 2;
+      uint32_t w = v[i / EPV][j];
+      if constexpr (sizeof(T) == 4) w = 0xff800000u;
+      else {
+        constexpr uint32_t low = __is_same(T, _Float16) ? 0xfc00u : 0xff80u;
+        w = e & 1 ? (w & 0xffffu) | low << 16 : (w & 0xffff0000u) | low;
+      }
+      v[i / EPV][j] = w;
+    }
   }
   __device__ __forceinline__ float value(int i) const {
-    if constexpr (sizeof(T) == 4) return __uint_as_float(raw(i));
-    else return (float)__builtin_bit_cast(T, (uint16_t)raw(i));
+    const int e = i % EPV;
+    const uint32_t w = v[i / EPV][sizeof(T) == 4 ? e : e / 2];
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+    else if constexpr (__is_same(T, _Float16)) return (float)__builtin_bit_cast(_Float16, (uint16_t)(e & 1 ? w >> 16 : w));
+    else return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
   }
-  // The same with the index in the row below the key: comparable over a row's chunks.
-  __device__ __forceinline__ uint64_t global(Comp c) const {
-    if (c == 0) return 0;
-    const uint32_t index = (uint32_t)(first + 65535 - (int)(c & 0xffffu));
-    return (uint64_t)(uint32_t)(c >> kShift) << 32 | (uint32_t)~index;
+  __device__ __forceinline__ float largest() const {
+    float m[2] = {value(0), value(1)};
+#pragma unroll
+    for (int i = 2; i < E; i += 2) m[i / 2 & 1] = nan_max(nan_max(m[i / 2 & 1], value(i)), value(i + 1));
+    return nan_max(m[0], m[1]);
   }
 };
+// A key above an index, inverted: of equal keys the lower index is the larger.
+__device__ __forceinline__ uint64_t entry_of(uint32_t key, int index) { return (uint64_t)key << 32 | (uint32_t)~index; }
 __device__ __forceinline__ int index_of(uint64_t g) { return (int)~(uint32_t)g; }
-template <typename T> __device__ __forceinline__ float value_of(uint64_t g) { return Order<T>::value((uint32_t)(g >> 32)); }
 
 // Whether this workgroup is the last of `all` that arrive at the counter, whose partial
 // results are then there to be read with load_agent. (Stores of the others have left for device
@@ -149,18 +157,22 @@ __device__ __forceinline__ void nodes_of(const AcceptParams& p, int b, int& tok0
   n = min(max(min(p.cu[b + 1], p.rows) - tok0, 0), p.max_nodes);
 }
 
+// A workgroup takes p.per chunks of a row, one in flight while it looks at the one before, and leaves
+// the largest value and its index.
 template <typename T, int U>
 __global__ __launch_bounds__(kThreads) void fa_accept_kernel(const AcceptParams p) {
   using Ch = Chunk<T, U>;
-  __shared__ uint64_t st_best[kWaves];
+  __shared__ float st_m[kWaves];
+  __shared__ int st_k[kWaves], st_at;
   __shared__ int st_last;
+  __shared__ unsigned long long st_best[LSFA_TREE_MAX_NODES];
   __shared__ uint64_t st_mask[LSFA_TREE_MAX_NODES][LSFA_TREE_MAX_NODES / 64];
   __shared__ int64_t st_token[LSFA_TREE_MAX_NODES];
-  __shared__ int st_choice[LSFA_TREE_MAX_NODES], st_path[LSFA_TREE_MAX_NODES];
+  __shared__ int st_path[LSFA_TREE_MAX_NODES];
   __shared__ int st_count;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  if (blockIdx.x == (unsigned)(p.rows * p.chunks)) {  // sequences without nodes
+  if (blockIdx.x == (unsigned)(p.rows * p.parts)) {  // sequences without nodes
     for (int b = 0; b < p.B; ++b) {
       int tok0, n;
       nodes_of(p, b, tok0, n);
@@ -170,20 +182,16 @@ __global__ __launch_bounds__(kThreads) void fa_accept_kernel(const AcceptParams 
     }
     return;
   }
-  const int chunk = (int)(blockIdx.x % (unsigned)p.chunks);
+  const int part = (int)(blockIdx.x % (unsigned)p.parts);
   // The nodes of all sequences are numbered one after another; a workgroup takes those p.rows apart
   // (one, unless offsets that are none let sequences share rows).
-  for (int64_t id = blockIdx.x / (unsigned)p.chunks;; id += p.rows) {
+  for (int64_t id = blockIdx.x / (unsigned)p.parts;; id += p.rows) {
     int b = -1, tok0 = 0, n = 0, node = 0;
     int64_t at = 0;
     for (int j = 0; j < p.B && b < 0; j += 64) {
       int t = 0, c = 0;
       if (j + lane < p.B) nodes_of(p, j + lane, t, c);
-      int upto = c;
-      for (int o = 1; o < 64; o <<= 1) {
-        const int w = __shfl_up(upto, o);
-        if (lane >= o) upto += w;
-      }
+      const int upto = lanes_sum(c);
       const unsigned long long hit = __ballot(at + upto > id);
       if (hit != 0) {
         const int src = __builtin_ctzll(hit);
@@ -196,42 +204,75 @@ __global__ __launch_bounds__(kThreads) void fa_accept_kernel(const AcceptParams 
     }
     if (b < 0) return;  // uniform
 
-    Ch x;
-    x.load(p.logits, tok0 + node, p.stride, p.cols, chunk);
-    typename Ch::Comp m = 0;
-#pragma unroll
-    for (int i = 0; i < Ch::E; ++i) {
-      const typename Ch::Comp c = x.comp(i);
-      m = c > m ? c : m;
+    const int k0 = part * p.per, k1 = min(k0 + p.per, p.chunks);
+    const int64_t row = tok0 + node;
+    Ch x, ahead;
+    x.load(p.logits, row, p.stride, p.cols, k0);
+    float best = -INFINITY;  // the thread's, and the first chunk that has it
+    int best_k = k0;
+    for (int k = k0; k < k1; ++k) {
+      if (k + 1 < k1) ahead.load(p.logits, row, p.stride, p.cols, k + 1);
+      x.cut();
+      const float m = x.largest();
+      if (m > best || (m != m && best == best)) best = m, best_k = k;
+      if (k + 1 < k1) x = ahead;
     }
-    m = wave_max(m);
-    if (lane == 0) st_best[wave] = x.global(m);
+    // Of equal ones the lowest chunk, then the lowest position in it.
+    auto same = [](float a, float b) -> bool { return a == b || (a != a && b != b); };
+    const float wm = wave_max(best);
+    int wk = same(best, wm) ? best_k : 0x7fffffff;
+    for (int o = 32; o > 0; o >>= 1) wk = min(wk, __shfl_xor(wk, o));
+    if (lane == 0) st_m[wave] = wm, st_k[wave] = wk;
+    if (tid == 0) st_at = 0x7fffffff;
     __syncthreads();
-    if (tid == 0) {
-      uint64_t best = st_best[0];
-      for (int w = 1; w < kWaves; ++w) best = st_best[w] > best ? st_best[w] : best;
-      store_agent(p.part + (int64_t)(tok0 + node) * p.chunks + chunk, best);
+    float top = st_m[0];
+    for (int w = 1; w < kWaves; ++w) top = nan_max(top, st_m[w]);
+    int k = 0x7fffffff;
+    for (int w = 0; w < kWaves; ++w)
+      if (same(st_m[w], top)) k = min(k, st_k[w]);
+    if (p.per > 1) {
+      x.load(p.logits, row, p.stride, p.cols, k);
+      x.cut();
     }
-    if (!last_to_arrive(p.counters + b, n * p.chunks, &st_last)) continue;
+    if (same(wm, top) && wk == k) {  // (a wave without it there has nothing to look for)
+      int found = 0x7fffffff;
+#pragma unroll
+      for (int i = Ch::E - 1; i >= 0; --i) found = same(x.value(i), top) ? x.pos(i) : found;
+      if (found != 0x7fffffff) atomicMin(&st_at, found);
+    }
+    __syncthreads();
+    if (tid == 0)
+      store_agent(p.part + row * p.parts + part, entry_of(top != top ? kKeyNan : key_of(top), x.first + st_at));
+    if (!last_to_arrive(p.counters + b, n * p.parts, &st_last)) continue;
 
     const int words = p.mask_words;
     for (int i = tid; i < n; i += kThreads) {
-      uint64_t best = 0;
-#pragma unroll 8
-      for (int s = 0; s < p.chunks; ++s) {
-        const uint64_t g = load_agent(p.part + (int64_t)(tok0 + i) * p.chunks + s);
-        best = g > best ? g : best;
-      }
-      st_choice[i] = index_of(best);
+      st_best[i] = 0;
       st_token[i] = p.tokens[tok0 + i];
       for (int w = 0; w < words; ++w) st_mask[i][w] = p.mask[(int64_t)(tok0 + i) * p.mask_stride + w];
     }
     __syncthreads();
+    for (int t0 = 0; t0 < n * p.parts; t0 += 4 * kThreads) {
+      uint64_t g[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int t = t0 + u * kThreads + tid;
+        g[u] = t < n * p.parts ? load_agent(p.part + (int64_t)tok0 * p.parts + t) : 0;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int t = t0 + u * kThreads + tid;
+        if (t < n * p.parts) atomicMax(&st_best[t / p.parts], (unsigned long long)g[u]);
+      }
+    }
+    __syncthreads();
+    // (a row of -inf only: its first value)
+    auto choice = [&](int i) -> int { return (uint32_t)(st_best[i] >> 32) == kKeyLow ? 0 : index_of(st_best[i]); };
     if (wave == 0) {
       int cur = 0, count = 1;
       if (lane == 0) st_path[0] = 0;
       while (true) {
-        const int64_t want = st_choice[cur];
+        const int64_t want = choice(cur);
         int next = -1;
         for (int j0 = 0; j0 < n && next < 0; j0 += 64) {
           const int j = j0 + lane;
@@ -249,7 +290,7 @@ __global__ __launch_bounds__(kThreads) void fa_accept_kernel(const AcceptParams 
       if (lane == 0) {
         st_count = count;
         p.counts[b] = count;
-        p.next[b] = st_choice[cur];
+        p.next[b] = choice(cur);
         if (p.seq_lens != nullptr) p.seq_lens[b] += count;
       }
     }
@@ -260,18 +301,19 @@ __global__ __launch_bounds__(kThreads) void fa_accept_kernel(const AcceptParams 
 }
 
 // ------------------------------------------------------------------- beams
-// exp(t) of a difference t <= 0 in 32 bits, the argument's rounding put back.
+// exp(t) of a difference t <= 0 in 32 bits (0 below exp(-100), whose sum no logarithm shows), with the rounding of the
+// argument put back: exp2 of t log2(e) rounded, and the part of t that it left out.
 __device__ __forceinline__ float exp_near(float t) {
-  constexpr float kLog2e = 1.44269502162933349609375f, kRest = 1.925963033500011079e-8f, kLn2 = 0.6931471805599453f;
-  const float y = t * kLog2e, low = fmaf(t, kRest, fmaf(t, kLog2e, -y));
+  constexpr float kLog2e = 1.44269502162933349609375f, kLn2 = 0.693147182464599609375f, kLn2Rest = -1.904654323148236e-9f;
+  const float c = fmaxf(t, -100.f), y = c * kLog2e;
+  const float left = fmaf(-y, kLn2Rest, fmaf(-y, kLn2, c));
   const float e = fast_exp2(y);
-  return e == 0.f ? 0.f : fmaf(e, low * kLn2, e);
+  return fmaf(e, left, e);
 }
 
 template <typename T, int U>
 __global__ __launch_bounds__(kThreads) void fa_beams_kernel(const BeamParams p) {
   using Ch = Chunk<T, U>;
-  using Comp = typename Ch::Comp;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ float st_m[kWaves];
   __shared__ double st_l[kWaves];
@@ -284,105 +326,77 @@ __global__ __launch_bounds__(kThreads) void fa_beams_kernel(const BeamParams p) 
 
   Ch x;
   x.load(p.logits, row, p.stride, p.cols, chunk);
-  Comp m = 0;
-#pragma unroll
-  for (int i = 0; i < Ch::E; ++i) {
-    const Comp c = x.comp(i);
-    m = c > m ? c : m;
-  }
-  const Comp wm = wave_max(m);
-  // The wave's sum of exponentials: NaN where it has a NaN or +inf.
-  const float top = wm == 0 ? -INFINITY : Order<T>::value((uint32_t)(wm >> Ch::kShift));
+  x.cut();
+  const float mine = x.largest(), top = wave_max(mine);  // NaN where there is one
   double l = 0.;
-  if (top != -INFINITY) {
+  if (top > -INFINITY) {
 #pragma unroll
-    for (int i = 0; i < Ch::E; ++i)
-      if (x.has(i)) l += (double)exp_near(x.value(i) - top);
+    for (int i = 0; i < Ch::E; ++i) l += (double)exp_near(x.value(i) - top);
   }
   for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
   if (lane == 0) st_m[wave] = top, st_l[wave] = l;
 
-  // The wave's N largest: those from the Nth largest of its lanes' largest on hold them all, the
-  // few more that there are go by a second search (no two values are equal).
-  auto nth_largest = [&](auto count_from) -> Comp {  // the largest c with count_from(c) >= N, or 1
-    Comp c = 0;
-    for (int bit = Ch::kBits - 1; bit >= 0; --bit) {
-      const Comp t = c | (Comp)1 << bit;
-      const int n = count_from(t);
-      if (n >= N) c = t;
-      if (n == N) break;
-    }
-    return c == 0 ? (Comp)1 : c;
-  };
-  const Comp from = nth_largest([&](Comp t) -> int { return __builtin_popcountll(__ballot(m >= t)); });
-  Comp* mine = (Comp*)lds + wave * (64 * Ch::E);
-  int hits = 0;
-#pragma unroll
-  for (int i = 0; i < Ch::E; ++i) hits += x.comp(i) >= from;
-  int upto = hits;
-  for (int o = 1; o < 64; o <<= 1) {
-    const int w = __shfl_up(upto, o);
-    if (lane >= o) upto += w;
+  // The wave's N largest are at or above the Nth largest of its lanes' largest, and little else is
+  // (finite values: -inf is no candidate, and a row with NaN has none).
+  const uint32_t mk = mine > -INFINITY ? key_of(mine) : 0u;
+  uint32_t from = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t t = from | 1u << bit;
+    const int n = __builtin_popcountll(__ballot(mk >= t));
+    if (n >= N) from = t;
+    if (n == N) break;
   }
-  int n = __builtin_amdgcn_readlane(upto, 63), put = upto - hits;
+  const float least = from == 0 ? -FLT_MAX : fmaxf(value_of(from), -FLT_MAX);
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < Ch::E; ++i) n += __builtin_popcountll(__ballot(x.value(i) >= least));
+  auto entry = [&](int i) -> uint64_t { return entry_of(key_of(x.value(i)), x.first + x.pos(i)); };
+  // More than a place for each lane (many equal ones, or a large N): the entry that exactly N are at or above.
+  uint64_t exact = 0;
+  if (n > 64) {
+    for (int bit = 63; bit >= 0; --bit) {
+      const uint64_t t = exact | 1ull << bit;
+      int k = 0;
+#pragma unroll
+      for (int i = 0; i < Ch::E; ++i) k += __builtin_popcountll(__ballot(x.value(i) >= least && entry(i) >= t));
+      if (k >= N) exact = t;
+      if (k == N) break;
+    }
+    n = N;
+  }
+  uint64_t* pool = (uint64_t*)lds;  // [4 * 64]
+  int put = 0;
 #pragma unroll
   for (int i = 0; i < Ch::E; ++i) {
-    const Comp c = x.comp(i);
-    if (c >= from) mine[put++] = c;
-  }
-  asm volatile("" ::: "memory");
-  Comp cand = lane < n ? mine[lane] : (Comp)0;
-  if (n > 64) {  // uniform over the wave
-    const Comp least = nth_largest([&](Comp t) -> int {
-      int k = 0;
-      for (int j = 0; j < n; j += 64) k += __builtin_popcountll(__ballot(j + lane < n && mine[j + lane] >= t));
-      return k;
-    });
-    int kept = 0;
-    cand = 0;
-    for (int j = 0; j < n; j += 64) {
-      const Comp c = j + lane < n ? mine[j + lane] : (Comp)0;
-      const bool in = c >= least;
-      const unsigned long long ones = __ballot(in);
-      // (at most N <= 64 of them: a slot for each, in places that the loop has read)
-      asm volatile("" ::: "memory");
-      if (in) mine[kept + __builtin_popcountll(ones & ((1ull << lane) - 1))] = c;
-      kept += __builtin_popcountll(ones);
-    }
-    asm volatile("" ::: "memory");
-    n = kept;
-    cand = lane < n ? mine[lane] : (Comp)0;
+    bool in = x.value(i) >= least;
+    if (exact != 0) in = in && entry(i) >= exact;
+    const unsigned long long ones = __ballot(in);
+    if (ones == 0) continue;
+    if (in) pool[wave * 64 + put + __builtin_amdgcn_mbcnt_hi((uint32_t)(ones >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ones, 0))] = entry(i);
+    put += __builtin_popcountll(ones);
   }
   if (lane == 0) st_n[wave] = n;
   __syncthreads();
-  // The workgroup's, one after another, each at its rank.
-  int base = 0, all = 0;
-  for (int w = 0; w < kWaves; ++w) {
-    base += w < wave ? st_n[w] : 0;
-    all += st_n[w];
-  }
-  Comp* pool = (Comp*)lds;
-  __syncthreads();  // (the waves' own parts are in registers)
-  if (lane < n) pool[base + lane] = cand;
-  __syncthreads();
+  // The workgroup's, each at its rank.
   uint64_t* out = p.lists + list * N;
-  if (lane < n) {
-    int rank = 0;
-    for (int j = 0; j < all; ++j) rank += pool[j] > cand;
-    if (rank < N) store_agent(out + rank, x.global(cand));
+  const uint64_t cand = lane < n ? pool[wave * 64 + lane] : 0;
+  int rank = 0, all = 0;
+  for (int w = 0; w < kWaves; ++w) {
+    const int have = st_n[w];
+    all += have;
+#pragma unroll 4
+    for (int j = 0; j < have; ++j) rank += pool[w * 64 + j] > cand;
   }
+  if (lane < n && rank < N) store_agent(out + rank, cand);
   for (int j = all + tid; j < N; j += kThreads) store_agent(out + j, 0);
   if (tid == 0) {
     float M = st_m[0];
-    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, st_m[w]);
+    for (int w = 1; w < kWaves; ++w) M = nan_max(M, st_m[w]);
     double L = 0.;
-    bool nan = false;
-    for (int w = 0; w < kWaves; ++w) {
-      nan |= !(st_l[w] < (double)INFINITY) || st_m[w] != st_m[w];
+    for (int w = 0; w < kWaves; ++w)
       if (st_m[w] > -INFINITY) L += st_l[w] * exp((double)st_m[w] - (double)M);
-    }
     store_agent(p.sums + 2 * list, __float_as_uint(M));
-    store_agent(p.sums + 2 * list + 1, (uint64_t)__double_as_longlong(nan ? (double)NAN : L));
+    store_agent(p.sums + 2 * list + 1, (uint64_t)__double_as_longlong(L));
   }
   if (!last_to_arrive(p.counters + b, p.K * S, &st_last)) return;
 
@@ -400,20 +414,22 @@ __global__ __launch_bounds__(kThreads) void fa_beams_kernel(const BeamParams p) 
   for (int t = tid; t < lists; t += kThreads) {
     const int k0 = t / S * S;
     float M = lmax[k0];
-    for (int s = 1; s < S; ++s) M = fmaxf(M, lmax[k0 + s]);
+#pragma unroll 4
+    for (int s = 1; s < S; ++s) M = nan_max(M, lmax[k0 + s]);
     if (lmax[t] > -INFINITY) sum[t] *= exp((double)lmax[t] - (double)M);
     if (t == k0) st_lse[t / S] = M;  // (K <= LSFA_BEAMS_MAX)
   }
   __syncthreads();
   for (int k = tid; k < p.K; k += kThreads) {
     double L = 0.;
+#pragma unroll 4
     for (int s = 0; s < S; ++s) L += sum[k * S + s];
     const double lse = st_lse[k] + log(L);
     st_lse[k] = lse > -(double)INFINITY && lse < (double)INFINITY ? lse : (double)NAN;  // a row without lse offers nothing
   }
   __syncthreads();
   auto score = [&](int k, uint64_t g) -> double {
-    const double sc = (double)p.scores[(int64_t)b * p.K + k] + ((double)value_of<T>(g) - st_lse[k]);
+    const double sc = (double)p.scores[(int64_t)b * p.K + k] + ((double)value_of((uint32_t)(g >> 32)) - st_lse[k]);
     return g != 0 && sc > -(double)INFINITY ? sc : -(double)INFINITY;
   };
   for (int t = tid; t < lists; t += kThreads) sum[t] = score(t / S, load_agent(p.lists + (list0 + t) * N));
@@ -423,6 +439,7 @@ __global__ __launch_bounds__(kThreads) void fa_beams_kernel(const BeamParams p) 
   for (int t = tid, i = 0; t < lists; t += kThreads, ++i) {
     const double h = sum[t];
     int rank = 0;
+#pragma unroll 4
     for (int j = 0; j < lists; ++j) rank += sum[j] > h || (sum[j] == h && j < t);
     if (rank < N && h > -(double)INFINITY) chosen |= 1u << i;
     if (rank == N - 1) st_floor = h;
@@ -430,13 +447,13 @@ __global__ __launch_bounds__(kThreads) void fa_beams_kernel(const BeamParams p) 
   __syncthreads();
   double* cs = (double*)lds;       // [N * N]
   int* ci = (int*)(cs + N * N);    // k V + v
-  const double least = st_floor;
+  const double floor = st_floor;
   for (int t = tid, i = 0; t < lists; t += kThreads, ++i) {
     if (!(chosen >> i & 1)) continue;
     for (int j = 0; j < N; ++j) {
       const uint64_t g = load_agent(p.lists + (list0 + t) * N + j);
       const double sc = score(t / S, g);
-      if (!(sc >= least) || sc == -(double)INFINITY) break;
+      if (!(sc >= floor) || sc == -(double)INFINITY) break;
       const int at = atomicAdd(&st_found, 1);
       cs[at] = sc;
       ci[at] = t / S * p.cols + index_of(g);
@@ -470,24 +487,25 @@ static int chunks_of(int cols, int size, int U) {
   const int epv = 16 / size, c = kThreads * epv * U;
   return (int)(((long long)cols + epv - 1 + c - 1) / c);
 }
-SelectPlan select_plan(long long rows, int cols, int dtype) {
+SelectPlan select_plan(long long rows, int cols, int dtype, bool beams) {
   const int size = dtype == 0 ? 4 : 2;
   SelectPlan s;
-  s.loads = 4;
+  s.loads = beams && size == 4 ? 8 : 4;
   while (s.loads > 1 && rows * chunks_of(cols, size, s.loads) < 512) s.loads /= 2;
   s.chunks = chunks_of(cols, size, s.loads);
+  s.per = beams ? 1 : (int)std::max(1LL, std::min<long long>(s.chunks, rows * s.chunks / 2048));
+  s.parts = (s.chunks + s.per - 1) / s.per;
   return s;
 }
 
 template <typename T, int U>
 static void launch_accept(const AcceptParams& p, hipStream_t s) {
-  hipLaunchKernelGGL((fa_accept_kernel<T, U>), dim3((unsigned)(p.rows * p.chunks + 1)), dim3(kThreads), 0, s, p);
+  hipLaunchKernelGGL((fa_accept_kernel<T, U>), dim3((unsigned)(p.rows * p.parts + 1)), dim3(kThreads), 0, s, p);
 }
 template <typename T, int U>
 static void launch_beams(const BeamParams& p, hipStream_t s) {
-  using Ch = Chunk<T, U>;
   const size_t lists = (size_t)p.K * p.chunks;
-  const size_t lds = std::max({sizeof(typename Ch::Comp) * kWaves * 64 * Ch::E, lists * 12, (size_t)p.num * p.num * 12});
+  const size_t lds = std::max({(size_t)kWaves * 64 * 8, lists * 12, (size_t)p.num * p.num * 12});
   hipLaunchKernelGGL((fa_beams_kernel<T, U>), dim3((unsigned)(p.B * p.K * p.chunks)), dim3(kThreads), lds, s, p);
 }
 template <typename T>
@@ -498,11 +516,12 @@ static void by_loads(const AcceptParams& p, int loads, hipStream_t s) {
 }
 template <typename T>
 static void by_loads(const BeamParams& p, int loads, hipStream_t s) {
+  if constexpr (sizeof(T) == 4)
+    if (loads == 8) return launch_beams<T, 8>(p, s);
   if (loads == 4) launch_beams<T, 4>(p, s);
   else if (loads == 2) launch_beams<T, 2>(p, s);
   else launch_beams<T, 1>(p, s);
 }
-
 // Host entries used by the C ABI layer (arguments validated there).
 hipError_t accept_drafts(const AcceptParams& p, int dtype, int loads, hipStream_t s) {
   if (dtype == 0) by_loads<float>(p, loads, s);
