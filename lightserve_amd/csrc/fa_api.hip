@@ -21,7 +21,7 @@ hipError_t fwd_f32(const FwdParams& p, int dp, bool causal, bool varlen, float s
 hipError_t bwd_f32(const BwdParams& p, int dp, bool causal, hipStream_t s);
 hipError_t decode_gqa(const DecodeParams& p, bool is_bf16, int dp, hipStream_t s);
 hipError_t kv_cache_move(const KvCacheParams& p, int dtype, bool append, hipStream_t s);
-WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int eb, int max_n, long long max_keys, int window, int sinks);
+WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int eb, int max_n, long long max_keys, int window, int sinks, bool tree);
 hipError_t window_attention(WindowParams p, const WindowPlan& w, bool is_bf16, hipStream_t s);
 hipError_t rope_inplace(const RopeParams& p, int dtype, hipStream_t s);
 hipError_t add_rmsnorm(const NormParams& p, int dtype, bool vec, hipStream_t s);
@@ -761,16 +761,16 @@ static int run_kv_cache(const lsfa_kv_cache_args* a, bool append, void* stream) 
 int lsfa_kv_append(const lsfa_kv_cache_args* a, void* stream) { return run_kv_cache(a, true, stream); }
 int lsfa_kv_read(const lsfa_kv_cache_args* a, void* stream) { return run_kv_cache(a, false, stream); }
 
-static lsfa::WindowPlan plan_window(const lsfa_window_args* a) {
+static lsfa::WindowPlan plan_window(const lsfa_window_args* a, bool tree = false) {
   if (a->batch == 0 || a->tokens == 0 || a->max_seqlen_q == 0) return {};
   return lsfa::window_plan(a->batch, a->tokens, a->heads_kv, a->heads_q / a->heads_kv, a->head_dim,
                            a->kv_scales != nullptr ? 1 : 2, std::min(a->max_seqlen_q, a->tokens),
                            std::min<long long>(a->max_seq_len, (long long)a->max_blocks_per_seq * a->block_size), a->window,
-                           a->sinks);
+                           a->sinks, tree);
 }
 
 // Checks all but the workspace.
-static int check_window(const lsfa_window_args* a) {
+static int check_window(const lsfa_window_args* a, bool tree = false) {
   if (a == nullptr) return fail(LSFA_ERR_INVALID, "args is NULL");
   if (a->dtype != LSFA_DTYPE_FP16 && a->dtype != LSFA_DTYPE_BF16)
     return fail(a->dtype == LSFA_DTYPE_FP32 ? LSFA_ERR_UNSUPPORTED : LSFA_ERR_INVALID,
@@ -811,7 +811,7 @@ static int check_window(const lsfa_window_args* a) {
   if (!aligned16(a->q) || !aligned16(a->o) || !aligned16(a->k_cache) || !aligned16(a->v_cache) ||
       (reinterpret_cast<uintptr_t>(a->kv_scales) & 7u) != 0)
     return fail(LSFA_ERR_UNSUPPORTED, "q, o, k_cache and v_cache must be 16-byte aligned, kv_scales 8-byte");
-  const lsfa::WindowPlan w = plan_window(a);
+  const lsfa::WindowPlan w = plan_window(a, tree);
   if ((long long)w.items * w.waves * 64 > (1LL << 32) - 1 || (long long)a->heads_kv * 256 > (1LL << 32) - 1)
     return fail(LSFA_ERR_UNSUPPORTED, "rows of q for 2^32 threads or more in one launch (%d tokens, %d heads_q)", a->tokens, a->heads_q);
   return LSFA_OK;
@@ -873,8 +873,9 @@ static int run_window(const lsfa_window_args* a, const lsfa_tree_args* tree, voi
     p.tree = reinterpret_cast<const uint32_t*>(tree->tree_mask);
     p.tree_stride = 2 * tree->mask_stride;
     p.tree_words = 2 * tree->mask_words;
+    p.causal = 0;
   }
-  hipError_t e = lsfa::window_attention(p, plan_window(a), a->dtype == LSFA_DTYPE_BF16, reinterpret_cast<hipStream_t>(stream));
+  hipError_t e = lsfa::window_attention(p, plan_window(a, tree != nullptr), a->dtype == LSFA_DTYPE_BF16, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(LSFA_ERR_LAUNCH, "windowed paged attention launch failed: %s", hipGetErrorString(e));
   return ok();
 }
@@ -889,8 +890,12 @@ static int check_tree(const lsfa_tree_args* a) {
   const lsfa_window_args* w = &a->window;
   lsfa_window_args as = *w;
   as.causal = 1;
-  const int rc = check_window(&as);
+  const int rc = check_window(&as, true);
   if (rc) return rc;
+  const lsfa::WindowPlan plan = plan_window(w, true);
+  const long long all = ((long long)std::min<long long>(w->max_seq_len, (long long)w->max_blocks_per_seq * w->block_size) + 127) / 64;
+  if (plan.items > 0 && all * plan.items >= (1LL << 31))
+    return fail(LSFA_ERR_UNSUPPORTED, "2^31 key tiles or more of all sequences, row tiles and KV heads");
   if (!w->cu_seqlens_q) return fail(LSFA_ERR_INVALID, "a tree needs cu_seqlens_q");
   if (w->max_seqlen_q > LSFA_TREE_MAX_NODES)
     return fail(LSFA_ERR_UNSUPPORTED, "at most %d drafts of a sequence (max_seqlen_q=%d)", LSFA_TREE_MAX_NODES, w->max_seqlen_q);
@@ -908,14 +913,14 @@ int lsfa_tree_check(const lsfa_tree_args* a) {
   const int rc = check_tree(a);
   if (rc) return rc;
   return check_workspace("lsfa_tree_workspace_size", a->window.workspace, a->window.workspace_bytes,
-                         plan_window(&a->window).part_bytes);
+                         plan_window(&a->window, true).part_bytes);
 }
 
 int lsfa_tree_workspace_size(const lsfa_tree_args* a, uint64_t* bytes) {
   if (bytes == nullptr) return fail(LSFA_ERR_INVALID, "bytes is NULL");
   const int rc = check_tree(a);
   if (rc) return rc;
-  *bytes = align256(plan_window(&a->window).part_bytes);
+  *bytes = align256(plan_window(&a->window, true).part_bytes);
   return ok();
 }
 

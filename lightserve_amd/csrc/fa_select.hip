@@ -64,17 +64,6 @@ __device__ __forceinline__ float wave_all(float v, F f) {
 __device__ __forceinline__ float wave_max(float v) {
   return wave_all(v, [](float a, float b) { return nan_max(a, b); });
 }
-// Inclusive sum over the wave's lanes.
-__device__ __forceinline__ int lanes_sum(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
-  return v;
-}
-
 // One chunk of a row in a workgroup's registers: U 16-byte loads a thread, of whole 16-byte
 // words of memory (a row may begin anywhere: chunks count from the word that it begins in).
 template <typename T, int U>

@@ -5,8 +5,8 @@
 // w tokens with s sinks, j > p - w or j < s. Sequence b's queries are the last
 // n of its seq_lens[b] cached tokens (one for a decode step). An 8-bit cache
 // holds e4m3 codes and one power-of-two scale for each row (fa_kvq.hip).
-// In a tree of drafted tokens (the TREE instances) the n queries see the tokens
-// before them and, of one another, those that their masks name.
+// In a tree of drafted tokens (TREE) the n queries see the tokens before them and, of
+// one another, those that their masks name; trees of many rows are fa_tree.hip's.
 //
 // Few rows per KV head (decode, and chunks of a few tokens): the narrow kernel.
 // Many: the wide one, further down.
@@ -41,76 +41,18 @@
 // long runs, the last run to arrive those of short ones, whose launches are a few
 // microseconds. Either way they are added in the runs' order, whichever ends first.
 #include "../../include/lightserve_fa.h"
-#include "fa_common.hpp"
+#include "fa_paged.hpp"
 
 #include <algorithm>
 #include <type_traits>
 
 namespace lsfa {
 
-constexpr float kWinLn2 = 0.6931471805599453f;
-
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-// Two e4m3 codes (the low or the high half of w) times a power of two.
-template <bool HI>
-__device__ __forceinline__ uint32_t codes2(uint32_t w, float scale, __bf16) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
-}
-template <bool HI>
-__device__ __forceinline__ uint32_t codes2(uint32_t w, float scale, _Float16) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
-}
-
-// A sequence's keys, queries and first row of q, and its key tiles of 32: those
-// with sinks that its window's tiles do not hold, then the window's from `first` on.
-struct KeyTiles {
-  int seq, n, tok0;
-  int sink, first;
-  int count;         // all of them; 1 where queries see no key, 0 without queries
-};
-__device__ __forceinline__ KeyTiles key_tiles_of(const WindowParams& p, int seq, int n, int tok0) {
-  KeyTiles t;
-  t.seq = seq, t.n = n, t.tok0 = tok0;
-  t.first = t.sink = 0;
-  if (p.window > 0) {
-    t.first = max(seq - n - p.window + 1, 0) >> 5;
-    t.sink = min((min(p.sinks, seq) + 31) >> 5, t.first);
-  }
-  t.count = n > 0 ? max(t.sink + ((seq + 31) >> 5) - t.first, 1) : 0;
-  return t;
-}
-__device__ __forceinline__ KeyTiles key_tiles(const WindowParams& p, int b) {
-  int n = 1, tok0 = b;
-  if (p.cu_q != nullptr) {  // (no row outside q, whatever the offsets)
-    tok0 = min(max(p.cu_q[b], 0), p.tokens);
-    n = max(min(p.cu_q[b + 1], p.tokens) - tok0, 0);
-  }
-  return key_tiles_of(p, min(max(p.seq_lens[b], 0), min(p.max_seq_len, p.max_blocks << p.block_shift)), n, tok0);
-}
-
-// The kernel's arguments, read again. What only the beginning and the end of a run or item
-// need is taken from here: kept in scalar registers through the loop it would push the
-// loop's own ones out of them (the wide kernel's reads of LDS then all wait for each other).
-__device__ __forceinline__ const __attribute__((address_space(4))) WindowParams* arguments() {
-  auto a = (const __attribute__((address_space(4))) WindowParams*)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(a));
-  return a;
-}
-
-// Inclusive sum over the wave's lanes.
-__device__ __forceinline__ int lanes_sum(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15, rows 1 and 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31, rows 2 and 3
-  return v;
 }
 // Tiles of a run: the tiles there are over the runs there are, no less than one for each wave.
 __device__ __forceinline__ int run_tiles(int all, int runs) {
@@ -172,53 +114,6 @@ __device__ __forceinline__ f32x4 load_device(const float* from) {
   const uint64_t b = __hip_atomic_load((uint64_t*)from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   return f32x4{__uint_as_float((uint32_t)a), __uint_as_float((uint32_t)(a >> 32)), __uint_as_float((uint32_t)b),
                __uint_as_float((uint32_t)(b >> 32))};
-}
-
-// 0 * infinity is NaN, so a row that does not see a key must not add that key's infinities
-// and NaN with its weight of zero. The narrow kernel takes such elements of V as zeros where
-// a mask cuts a tile for some of a chunk's rows and, if there were any (ordinary caches have
-// none), adds them to the rows that see their keys before the sums leave the registers; the
-// wide one takes the sums of a wave again, with them left out, if they are not finite.
-// Ones in the elements of a word of V that are infinite or NaN (e4m3: NaN).
-template <typename T, bool Q8>
-__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
-  if constexpr (Q8) return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
-  constexpr uint32_t e = __is_same(T, _Float16) ? 0x7c007c00u : 0x7f807f80u;  // exponents of ones
-  const uint32_t x = w & e;
-  return ((x & 0xffffu) == (e & 0xffffu) ? 0xffffu : 0u) | ((x & 0xffff0000u) == (e & 0xffff0000u) ? 0xffff0000u : 0u);
-}
-template <int N, typename A>
-__device__ __forceinline__ bool all_finite(const A (&acc)[N]) {
-  float s = 0.f;
-#pragma unroll
-  for (int j = 0; j < N; ++j)
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof(A) / 4); ++i) s = fmaf(acc[j][i], 0.f, s);
-  return s == 0.f;
-}
-// Element k of words of V, infinite or NaN, or zero.
-template <typename T, bool Q8>
-__device__ __forceinline__ float bad_value(const uint32_t* w, int k) {
-  if constexpr (Q8) return (w[k / 4] >> (8 * (k & 3)) & 0xff) != 0 ? __builtin_nanf("") : 0.f;
-  return (float)__builtin_bit_cast(T, (uint16_t)(w[k / 2] >> (16 * (k & 1))));
-}
-
-// Draft trees: bits at .. at + 31 of the mask of query `row`, of n drafts (bits at the number of
-// the tile's first key, which may lie before the drafts).
-__device__ __forceinline__ uint32_t draft_bits(const WindowParams& p, int64_t row, int n, int at) {
-  const int i = at >> 5;
-  const uint32_t* m = p.tree + row * p.tree_stride;
-  const uint32_t w0 = (unsigned)i < (unsigned)p.tree_words ? m[i] : 0u;
-  const uint32_t w1 = (unsigned)(i + 1) < (unsigned)p.tree_words ? m[i + 1] : 0u;
-  const uint32_t bits = __builtin_amdgcn_alignbit(w1, w0, at & 31);
-  const int left = n - at;  // drafts from bit 0 on
-  return left >= 32 ? bits : left > 0 ? bits & ((1u << left) - 1) : 0u;
-}
-// Position of a query: as many tokens after the last certain one as it sees drafts besides itself.
-__device__ __forceinline__ int draft_position(const WindowParams& p, int64_t row, int n, int base) {
-  int seen = 0;
-  for (int i = 0; i < p.tree_words; ++i) seen += __builtin_popcount(draft_bits(p, row, n, 32 * i));
-  return base + max(seen, 1) - 1;
 }
 
 constexpr int kRowTile = 16;  // rows of a column block; a row tile has one or two
@@ -774,7 +669,7 @@ constexpr int kWideTile = 64;  // keys
 // The sequence (with its key tiles) and row tile of an item; false past the last. Row
 // tiles go longest first (ranked_item) where their lengths differ: up to 64 sequences
 // without a window. Else they go in order, the last of a sequence first.
-template <int BM, bool TREE>
+template <int BM>
 __device__ __forceinline__ bool wide_item(const WindowParams& p, int item, int lane, int& b, int& rt, KeyTiles& kt) {
   const int G = p.Hq / p.Hkv;
   auto tiles_of = [&](const KeyTiles& t) -> int { return (int)(((int64_t)min(t.n, p.max_n) * G + BM - 1) / BM); };
@@ -787,7 +682,7 @@ __device__ __forceinline__ bool wide_item(const WindowParams& p, int item, int l
     auto above = [&](int x) -> int {
       if (x < 0) return tq;
       if (tq == 0 || nk <= kWideTile * x) return 0;
-      if (TREE || !p.causal) return tq;
+      if (!p.causal) return tq;
       const long long y = ((long long)kWideTile * x - off) * G;  // row tile t ends past key 64 x iff t >= y / BM
       return y < 0 ? tq : 1 + (int)max(0LL, tq - 1 - y / BM);
     };
@@ -833,12 +728,12 @@ struct WideSpan {
   int sink, first, count;
   int hi_max, lo_min;  // keys past hi_max, or before lo_min and no sinks, are seen by no row
 };
-template <int BM, bool TREE>
+template <int BM>
 __device__ __forceinline__ WideSpan wide_span(const WindowParams& p, const KeyTiles& kt, int rt) {
   const int G = p.Hq / p.Hkv, rows = kt.n * G;
-  const int t0 = TREE ? 0 : rt * BM / G, t1 = (min(rows, (rt + 1) * BM) - 1) / G;
+  const int t0 = rt * BM / G, t1 = (min(rows, (rt + 1) * BM) - 1) / G;
   WideSpan s;
-  s.hi_max = !TREE && p.causal ? kt.seq - kt.n + t1 : kt.seq - 1;
+  s.hi_max = p.causal ? kt.seq - kt.n + t1 : kt.seq - 1;
   s.lo_min = p.window > 0 ? kt.seq - kt.n + t0 - p.window + 1 : 0;
   const int end = max(s.hi_max + 1, 0);
   s.first = min(max(s.lo_min, 0), end) / kWideTile;
@@ -860,7 +755,7 @@ template <int BM, int DP> constexpr int kWidePart = BM * 4 + BM * DP;
 template <typename T> constexpr float kWideMaxLog2P = 64.0f;
 template <> constexpr float kWideMaxLog2P<_Float16> = 15.0f;
 
-template <typename T, typename C, int DP, int NW, bool LSE, bool SPLIT, bool TREE>
+template <typename T, typename C, int DP, int NW, bool LSE, bool SPLIT>
 __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(const WindowParams p) {
   using X8 = typename VecT<T>::x8;
   using X4 = typename VecT<T>::x4;
@@ -884,10 +779,10 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
   const int G = p.Hq / p.Hkv;
   int b, rt;
   KeyTiles kt;
-  if (!wide_item<BM, TREE>(p, blockIdx.x / p.Hkv, lane, b, rt, kt)) return;  // uniform, before any barrier
+  if (!wide_item<BM>(p, blockIdx.x / p.Hkv, lane, b, rt, kt)) return;  // uniform, before any barrier
   const int head = wide_head(p, b);
   const int64_t tok0 = kt.tok0;
-  WideSpan sp = wide_span<BM, TREE>(p, kt, rt);
+  WideSpan sp = wide_span<BM>(p, kt, rt);
   const int sink = __builtin_amdgcn_readfirstlane(sp.sink), first = __builtin_amdgcn_readfirstlane(sp.first);
   const int hi_max = __builtin_amdgcn_readfirstlane(sp.hi_max), lo_min = __builtin_amdgcn_readfirstlane(sp.lo_min);
   int t_lo = 0, t_hi = __builtin_amdgcn_readfirstlane(sp.count);
@@ -906,12 +801,11 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
   // The lane's row and what it sees, and the same over the wave's rows.
   const int r0 = rt * BM + wave * 32, r = r0 + l32, tok = r / G, hq = head * G + (r - tok * G);
   const bool row_ok = r < nrows;
-  int pos = p.causal ? seq - kt.n + tok : seq - 1;
-  if constexpr (TREE) pos = row_ok && p.window > 0 ? draft_position(p, tok0 + tok, kt.n, seq - kt.n) : 0;
-  const int hi = row_ok ? (TREE ? seq - kt.n - 1 : pos) : -1, lo = p.window > 0 ? pos - p.window + 1 : 0;
-  const int w0 = seq - kt.n + (TREE ? 0 : r0 / G), w1 = TREE ? seq - 1 : seq - kt.n + (min(r0 + 32, nrows) - 1) / G;
-  const int whi_min = __builtin_amdgcn_readfirstlane(TREE ? seq - kt.n - 1 : p.causal ? w0 : seq - 1);
-  const int whi_max = __builtin_amdgcn_readfirstlane(r0 >= nrows ? -1 : !TREE && p.causal ? w1 : seq - 1);
+  const int pos = p.causal ? seq - kt.n + tok : seq - 1;
+  const int hi = row_ok ? pos : -1, lo = p.window > 0 ? pos - p.window + 1 : 0;
+  const int w0 = seq - kt.n + r0 / G, w1 = seq - kt.n + (min(r0 + 32, nrows) - 1) / G;
+  const int whi_min = __builtin_amdgcn_readfirstlane(p.causal ? w0 : seq - 1);
+  const int whi_max = __builtin_amdgcn_readfirstlane(r0 >= nrows ? -1 : p.causal ? w1 : seq - 1);
   const int wlo_min = __builtin_amdgcn_readfirstlane(p.window > 0 ? w0 - p.window + 1 : 0);
   const int wlo_max = __builtin_amdgcn_readfirstlane(p.window > 0 ? w1 - p.window + 1 : 0);
 
@@ -1028,23 +922,17 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
     }
     __builtin_amdgcn_sched_barrier(0);
   };
-  // TREE: drafts that the lane's row sees among the 32 keys from key0 on.
-  auto drafts = [&](int key0) -> uint32_t { return row_ok ? draft_bits(p, tok0 + tok, kt.n, key0 - (seq - kt.n)) : 0u; };
   auto mask = [&](int t, f32x16* s) {
     const int key0 = key_of(t);
     if (!(key0 + BN - 1 <= whi_min && (key0 >= wlo_max || key0 + BN - 1 < sinks))) {
       asm volatile("" ::: "memory");  // stays a branch
       const int up = hi - key0 - 4 * hh, dn = lo - key0 - 4 * hh, sk = sinks - key0 - 4 * hh;
-      uint32_t tree[KB];
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) tree[kb] = TREE ? drafts(key0 + 32 * kb) >> (4 * hh) : 0u;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int k = 32 * kb + 8 * (i >> 2) + (i & 3);
-          const bool seen = k <= up && (k >= dn || k < sk);
-          s[kb][i] = seen || (TREE && (tree[kb] >> (k & 31) & 1)) ? s[kb][i] : -INFINITY;
+          s[kb][i] = k <= up && (k >= dn || k < sk) ? s[kb][i] : -INFINITY;
         }
     }
   };
@@ -1337,14 +1225,12 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
         };
         to_lds(K, 0, false);
         f32x16 s = {};
-        const uint32_t tree = TREE ? drafts(key0) >> (4 * hh) : 0u;
 #pragma unroll
         for (int kk = 0; kk < KSTEPS; ++kk) s = mfma32(*(const LDS_AS X8*)(wb + (koff ^ (kk << 5))), qreg[kk], s);
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           const int key = key0 + 4 * hh + 8 * (k >> 2) + (k & 3);
-          const bool seen = (key <= hi && (key >= lo || key < sinks)) || (TREE && (tree >> (8 * (k >> 2) + (k & 3)) & 1));
-          s[k] = seen ? fast_exp2(fmaf(s[k], sl2, -m_run)) : 0.f;
+          s[k] = key <= hi && (key >= lo || key < sinks) ? fast_exp2(fmaf(s[k], sl2, -m_run)) : 0.f;
         }
         const X8 pb[2] = {pack8<T>(s, 0), pack8<T>(s, 8)};
         in_order();
@@ -1363,8 +1249,7 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
         for (int key = key0; key < key0 + 32; ++key) {
           if (key > whi_max || (key < wlo_min && key >= sinks)) continue;
           const int blk = table[key >> p.block_shift];
-          const bool seen = (key <= hi && (key >= lo || key < sinks)) || (TREE && (drafts(key) & 1));
-          if ((unsigned)blk >= (unsigned)p.num_blocks || !seen) continue;
+          if ((unsigned)blk >= (unsigned)p.num_blocks || !(key <= hi && (key >= lo || key < sinks))) continue;
           const C* row = row_of(V, key, blk);
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt)
@@ -1388,7 +1273,7 @@ __global__ __launch_bounds__((NW * 64), (8 / NW)) void fa_window_wide_kernel(con
 
 // Merges the key splits of fa_window_wide_kernel<..., SPLIT>: workgroup (item,
 // dt) combines 32 channels of the item's rows in the accumulators' order.
-template <typename T, int DP, int NW, bool TREE>
+template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64) void fa_window_wide_combine_kernel(const WindowParams p) {
   using X4 = typename VecT<T>::x4;
   constexpr int BM = NW * 32, DT = DP / 32;
@@ -1396,9 +1281,9 @@ __global__ __launch_bounds__(NW * 64) void fa_window_wide_combine_kernel(const W
   const int l32 = lane & 31, hh = lane >> 5, G = p.Hq / p.Hkv;
   int b, rt;
   KeyTiles kt;
-  if (!wide_item<BM, TREE>(p, blockIdx.x / p.Hkv, lane, b, rt, kt)) return;
+  if (!wide_item<BM>(p, blockIdx.x / p.Hkv, lane, b, rt, kt)) return;
   const int head = wide_head(p, b);
-  const int count = wide_span<BM, TREE>(p, kt, rt).count, share = split_share(count, p.splits);
+  const int count = wide_span<BM>(p, kt, rt).count, share = split_share(count, p.splits);
   if (count <= share) return;  // already in o
   const int n = (count + share - 1) / share;
   const int r = rt * BM + wave * 32 + l32, nrows = min(kt.n, p.max_n) * G;
@@ -1436,8 +1321,11 @@ __global__ __launch_bounds__(NW * 64) void fa_window_wide_combine_kernel(const W
 // rows), take 66 us there and 88 in the wide one, 4 chunks of 64 tokens (256 rows) 73 and 46.
 constexpr long long kNarrowRows = 32;
 
+WindowPlan tree_plan(int B, int tokens, int Hkv, int G, int dp, int max_n, long long seen);  // fa_tree.hip
+hipError_t tree_attention(const WindowParams& p, const WindowPlan& w, bool is_bf16, hipStream_t s);
+
 // How a launch goes, from what the host knows (sizes and bounds, not lengths).
-WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int eb, int max_n, long long max_keys, int window, int sinks) {
+WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int eb, int max_n, long long max_keys, int window, int sinks, bool tree) {
   WindowPlan w = {};
   const int dp = D <= 64 ? 64 : 128;
   const long long rows = (long long)max_n * G;
@@ -1462,6 +1350,7 @@ WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int eb, int max
       w.part_bytes = LSFA_GEMV_COUNTER_BYTES + (uint64_t)tiles * 2 * w.runs * (w.long_run > 0 ? 4 : 1) * part_bytes;
     return w;
   }
+  if (tree) return tree_plan(B, tokens, Hkv, G, dp, max_n, seen);
   auto items = [&](int bm) {
     return Hkv * std::min((long long)tokens * G / bm + B, (rows + bm - 1) / bm * B);
   };
@@ -1497,32 +1386,29 @@ static hipError_t launch_narrow(const WindowParams& p, const WindowPlan& w, hipS
     hipLaunchKernelGGL((fa_window_combine_kernel<T, DP, NC, 32>), parts, dim3(256), 0, s, p);
   return hipGetLastError();
 }
-template <typename T, typename C, int DP, bool TREE>
+template <typename T, typename C, int DP>
 static hipError_t launch_wide(const WindowParams& p, const WindowPlan& w, hipStream_t s) {
   if (w.splits > 1) {
-    hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 4, true, true, TREE>), dim3(w.items, w.splits), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 4, true, true>), dim3(w.items, w.splits), dim3(256), 0, s, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((fa_window_wide_combine_kernel<T, DP, 4, TREE>), dim3(w.items, DP / 32), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((fa_window_wide_combine_kernel<T, DP, 4>), dim3(w.items, DP / 32), dim3(256), 0, s, p);
     return hipGetLastError();
   }
   if (w.waves == 8) {
-    if (TREE || p.lse != nullptr) hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 8, true, false, TREE>), dim3(w.items), dim3(512), 0, s, p);
-    else hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 8, TREE, false, TREE>), dim3(w.items), dim3(512), 0, s, p);
+    if (p.lse != nullptr) hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 8, true, false>), dim3(w.items), dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 8, false, false>), dim3(w.items), dim3(512), 0, s, p);
   } else {
-    if (TREE || p.lse != nullptr) hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 4, true, false, TREE>), dim3(w.items), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 4, TREE, false, TREE>), dim3(w.items), dim3(256), 0, s, p);
+    if (p.lse != nullptr) hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 4, true, false>), dim3(w.items), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((fa_window_wide_kernel<T, C, DP, 4, false, false>), dim3(w.items), dim3(256), 0, s, p);
   }
   return hipGetLastError();
 }
-template <typename T, typename C, int DP, bool TREE>
-static hipError_t launch_rows(const WindowParams& p, const WindowPlan& w, hipStream_t s) {
-  if (w.items > 0) return launch_wide<T, C, DP, TREE>(p, w, s);
-  return w.columns == 1 ? launch_narrow<T, C, DP, 1, TREE>(p, w, s) : launch_narrow<T, C, DP, 2, TREE>(p, w, s);
-}
 template <typename T, typename C, int DP>
 static hipError_t launch_window(const WindowParams& p, const WindowPlan& w, hipStream_t s) {
-  return p.tree != nullptr ? launch_rows<T, C, DP, true>(p, w, s) : launch_rows<T, C, DP, false>(p, w, s);
+  if (p.tree != nullptr) return w.columns == 1 ? launch_narrow<T, C, DP, 1, true>(p, w, s) : launch_narrow<T, C, DP, 2, true>(p, w, s);
+  if (w.items > 0) return launch_wide<T, C, DP>(p, w, s);
+  return w.columns == 1 ? launch_narrow<T, C, DP, 1, false>(p, w, s) : launch_narrow<T, C, DP, 2, false>(p, w, s);
 }
 template <typename T>
 static hipError_t dispatch_window(const WindowParams& p, const WindowPlan& w, hipStream_t s) {
@@ -1536,6 +1422,7 @@ hipError_t window_attention(WindowParams p, const WindowPlan& w, bool is_bf16, h
   p.part_rows = w.part_rows;
   p.long_run = w.long_run;
   p.splits = w.splits;
+  if (p.tree != nullptr && w.items > 0) return tree_attention(p, w, is_bf16, s);
   return is_bf16 ? dispatch_window<__bf16>(p, w, s) : dispatch_window<_Float16>(p, w, s);
 }
 
