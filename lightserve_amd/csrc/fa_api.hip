@@ -893,7 +893,7 @@ static int check_tree(const lsfa_tree_args* a) {
   const int rc = check_window(&as, true);
   if (rc) return rc;
   const lsfa::WindowPlan plan = plan_window(w, true);
-  const long long all = ((long long)std::min<long long>(w->max_seq_len, (long long)w->max_blocks_per_seq * w->block_size) + 127) / 64;
+  const long long all = ((long long)std::min<long long>(w->max_seq_len, (long long)w->max_blocks_per_seq * w->block_size) + 63) / 32;
   if (plan.items > 0 && all * plan.items >= (1LL << 31))
     return fail(LSFA_ERR_UNSUPPORTED, "2^31 key tiles or more of all sequences, row tiles and KV heads");
   if (!w->cu_seqlens_q) return fail(LSFA_ERR_INVALID, "a tree needs cu_seqlens_q");

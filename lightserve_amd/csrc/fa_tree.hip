@@ -1,11 +1,11 @@
 // Attention of draft trees over paged KV caches, where a KV head's group has more than
-// 32 rows (nodes times query heads), for gfx950. Fewer are fa_window.hip's narrow kernel's.
+// 16 rows (nodes times query heads), for gfx950. Fewer are fa_window.hip's narrow kernel's.
 //
 // A tree's nodes all see the sequence's earlier tokens (under a window its last ones and the
 // sinks) and, of one another, those that their masks name: all but the last key tiles are
 // whole, and every row tile of a sequence has the same ones. So a workgroup of NW waves takes
-// 32 NW (node, query head) rows of a sequence and KV head, wave w rows 32 w .. 32 w + 31, as many
-// as the trees of the launch need, up to 256, and each byte of the cache is read once for them.
+// 32 NW (node, query head) rows of a sequence and KV head, wave w rows 32 w .. 32 w + 31: up to 256,
+// as the trees and the work of the launch have it (tree_plan), and reads a byte of the cache once for them.
 //   key tiles  of BN keys lie in LDS in q's type. 16-bit rows go there by direct loads, two
 //              tiles ahead of the one in use; 8-bit ones by way of registers one tile ahead,
 //              their scales applied once for all rows.
@@ -49,40 +49,44 @@ __device__ __forceinline__ TreeSequence<BM, BN> tree_sequence(const P& p, int b)
   t.n = n;
   return t;
 }
-// The key tiles of all items.
-template <int BM, int BN>
-__device__ __forceinline__ int tree_tiles(const WindowParams& p, int lane) {
-  int all = 0;
-  for (int j = 0; j < p.B; j += 64) {
-    TreeSequence<BM, BN> t = {};
-    if (j + lane < p.B) t = tree_sequence<BM, BN>(p, j + lane);
-    all += __builtin_amdgcn_readlane(lanes_sum(t.items * t.count), 63);
-  }
-  return all;
-}
-// The sequence that holds tile (ITEMS: item) number `at`; the numbers of its first tile and item.
+// All items' key tiles in runs: tiles of a run, and the sequence that holds the first tile of run (ITEMS: item) number `id`
+// with the numbers of its own first tile and item; p.B past the last.
+constexpr int kRunLeast = 2;  // tiles
+struct TreePlace {
+  int per, all, b, tile0, item0;
+};
 template <int BM, int BN, bool ITEMS>
-__device__ __forceinline__ int tree_find(const WindowParams& p, int at, int lane, int& tile0, int& item0) {
-  tile0 = item0 = 0;
+__device__ __forceinline__ TreePlace tree_place(const WindowParams& p, int id, int lane) {
+  TreePlace w = {0, 0, p.B, 0, 0};
+  TreeSequence<BM, BN> t = {};
+  if (lane < p.B) t = tree_sequence<BM, BN>(p, lane);
+  int tiles = lanes_sum(t.items * t.count), items = lanes_sum(t.items);  // up to 64 sequences lie in the lanes
+  w.all = __builtin_amdgcn_readlane(tiles, 63);
+  for (int j = 64; j < p.B; j += 64) {
+    TreeSequence<BM, BN> more = {};
+    if (j + lane < p.B) more = tree_sequence<BM, BN>(p, j + lane);
+    w.all += __builtin_amdgcn_readlane(lanes_sum(more.items * more.count), 63);
+  }
+  w.per = __builtin_amdgcn_readfirstlane(max((w.all + p.splits - 1) / p.splits, kRunLeast));
+  const int64_t at = ITEMS ? (int64_t)id : (int64_t)id * w.per;
   for (int j = 0; j < p.B; j += 64) {
-    TreeSequence<BM, BN> t = {};
-    if (j + lane < p.B) t = tree_sequence<BM, BN>(p, j + lane);
-    const int tiles = lanes_sum(t.items * t.count), items = lanes_sum(t.items);
-    const unsigned long long hit = __ballot(ITEMS ? item0 + items > at : tile0 + tiles > at);
+    if (j > 0) {
+      t = {};
+      if (j + lane < p.B) t = tree_sequence<BM, BN>(p, j + lane);
+      tiles = lanes_sum(t.items * t.count), items = lanes_sum(t.items);
+    }
+    const unsigned long long hit = __ballot(ITEMS ? w.item0 + items > at : w.tile0 + tiles > at);
     if (hit != 0) {
       const int src = __builtin_ctzll(hit);
-      tile0 += __builtin_amdgcn_readlane(tiles - t.items * t.count, src);
-      item0 += __builtin_amdgcn_readlane(items - t.items, src);
-      return j + src;
+      w.tile0 += __builtin_amdgcn_readlane(tiles - t.items * t.count, src);
+      w.item0 += __builtin_amdgcn_readlane(items - t.items, src);
+      w.b = j + src;
+      return w;
     }
-    tile0 += __builtin_amdgcn_readlane(tiles, 63);
-    item0 += __builtin_amdgcn_readlane(items, 63);
+    w.tile0 += __builtin_amdgcn_readlane(tiles, 63);
+    w.item0 += __builtin_amdgcn_readlane(items, 63);
   }
-  return p.B;
-}
-constexpr int kRunLeast = 4;  // tiles
-__device__ __forceinline__ int tree_run(const WindowParams& p, int all) {
-  return __builtin_amdgcn_readfirstlane(max((all + p.splits - 1) / p.splits, kRunLeast));
+  return w;
 }
 // Row tile and KV head of item v of sequence b. (The row tiles of a head follow one another; heads are turned from
 // sequence to sequence, so that an XCD reads all channels of its L2.)
@@ -125,12 +129,11 @@ __global__ __launch_bounds__((NW * 64), (NW == 8 ? 1 : 2)) void fa_tree_kernel(c
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hh = lane >> 5;
-  const int all = tree_tiles<BM, BN>(params, lane), per = tree_run(params, all);
-  if ((int64_t)blockIdx.x * per >= all) return;  // uniform, before any barrier
-  int at = blockIdx.x * per;
-  const int end = min(all, at + per);
-  int tile0, item0;
-  int b = __builtin_amdgcn_readfirstlane(tree_find<BM, BN, false>(params, at, lane, tile0, item0));
+  const TreePlace place = tree_place<BM, BN, false>(params, blockIdx.x, lane);
+  int b = __builtin_amdgcn_readfirstlane(place.b), tile0 = place.tile0;
+  if (b >= params.B) return;  // uniform, before any barrier
+  int at = blockIdx.x * place.per;
+  const int end = min(place.all, at + place.per);
 
 #pragma unroll 1
   do {
@@ -165,18 +168,13 @@ __global__ __launch_bounds__((NW * 64), (NW == 8 ? 1 : 2)) void fa_tree_kernel(c
     if (window > 0) lo = (row_ok ? draft_position(p, tok0 + tok, n, base) : base) - window + 1;
     const int lo_min = window > 0 ? base - window + 1 : 0, lo_max = window > 0 ? seq - window : 0;  // of any row
 
-    X8 q[KSTEPS];  // the B operand of S^T: row l32, columns 16 kk + 8 hh .. + 7
+    u32x4 qraw[KSTEPS];  // the B operand of S^T: row l32, columns 16 kk + 8 hh .. + 7
 #pragma unroll
     for (int kk = 0; kk < KSTEPS; ++kk) {
       const int col = 16 * kk + 8 * hh;
-      u32x4 raw = {0, 0, 0, 0};
-      if (row_ok && col < p.D) raw = ldg16((const T*)p.q + (tok0 + tok) * p.sqt + (int64_t)hq * p.sqh + col);
-      if (p.scale_log2 < 0.f) raw ^= 0x80008000u;
-      q[kk] = __builtin_bit_cast(X8, raw);
+      qraw[kk] = u32x4{0, 0, 0, 0};
+      if (row_ok && col < p.D) qraw[kk] = ldg16((const T*)p.q + (tok0 + tok) * p.sqt + (int64_t)hq * p.sqh + col);
     }
-
-    // (Q is waited for here: with its loads pending, the compiler would wait for all others in every tile.)
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
 
     // Loads of the wave's RPW rows of a tile, 8 elements a lane. 8-bit: row (l / LPR) NL + i in
     // instruction i, so that a lane's rows have adjacent scales; 16-bit: what the direct load's linear
@@ -267,6 +265,28 @@ __global__ __launch_bounds__((NW * 64), (NW == 8 ? 1 : 2)) void fa_tree_kernel(c
     // sums. Sums that are not finite are therefore taken again, with such values left out of the products and
     // added to the rows that see them (ordinary caches have none).
     bool careful = false;
+    Codes c;
+    Where w2;
+    auto load_first = [&]() {
+      const Where w1 = where(t_lo + 1);
+      w2 = where(t_lo + 2);
+      if constexpr (Q8) {
+        load_codes(c, where(t_lo));
+      } else {
+        load_direct(where(t_lo), 0);
+        load_direct(w1, 1);
+      }
+    };
+    load_first();
+    // (Q is waited for behind the first tiles' loads, and ahead of the tiles' loop)
+    X8 q[KSTEPS];
+    const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int kk = 0; kk < KSTEPS; ++kk) {
+      qraw[kk] ^= flip;
+      asm volatile("" : "+v"(qraw[kk]));
+      q[kk] = __builtin_bit_cast(X8, qraw[kk]);
+    }
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
@@ -274,15 +294,9 @@ __global__ __launch_bounds__((NW * 64), (NW == 8 ? 1 : 2)) void fa_tree_kernel(c
       m_run = -1e30f, l_run = 0.f, l_lse = 0.f;
       bool begun = false;
       if (tid == 0) *st_bad = 0;
-      Codes c;
-      Where w1 = where(t_lo + 1), w2 = where(t_lo + 2);
       if constexpr (Q8) {
-        load_codes(c, where(t_lo));
         write_codes(c, 0);
-        load_codes(c, w1);
-      } else {
-        load_direct(where(t_lo), 0);
-        load_direct(w1, 1);
+        load_codes(c, where(t_lo + 1));
       }
       int buf = 0;
 #pragma unroll 1
@@ -468,6 +482,7 @@ __global__ __launch_bounds__((NW * 64), (NW == 8 ? 1 : 2)) void fa_tree_kernel(c
       __syncthreads();
       if (*st_bad == 0) break;
       careful = true;
+      load_first();
       __syncthreads();  // before the flag is cleared
     }
 
@@ -518,50 +533,66 @@ __global__ __launch_bounds__((NW * 64), (NW == 8 ? 1 : 2)) void fa_tree_kernel(c
 }
 
 // Merges the partial results of items in several runs: workgroup (item, dt) combines 32 channels of the item's
-// rows in the accumulators' order, in the order of the runs.
+// rows in the accumulators' order. NG groups of waves take every NG-th run and meet in LDS (a sequence of 8000 tokens alone
+// lies in some 80 runs, whose results one wave after another would wait for).
+template <int NW> constexpr int kGroups = 8 / NW;
 template <typename T, int DP, int NW, int BN>
-__global__ __launch_bounds__(NW * 64) void fa_tree_combine_kernel(const WindowParams p) {
+__global__ __launch_bounds__((NW * kGroups<NW> * 64)) void fa_tree_combine_kernel(const WindowParams p) {
   using X4 = typename VecT<T>::x4;
-  constexpr int BM = NW * 32, DT = DP / 32, U = 4;  // U: results in flight
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, dt = blockIdx.y;
+  constexpr int BM = NW * 32, DT = DP / 32, NG = kGroups<NW>, U = 8;  // U: results in flight
+  __shared__ f32x4 meet[NG > 1 ? NG - 1 : 1][5][NW * 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) % NW, dt = blockIdx.y;
+  const int group = __builtin_amdgcn_readfirstlane(tid / (NW * 64));
   const int l32 = lane & 31, hh = lane >> 5, G = p.Hq / p.Hkv;
-  const int per = tree_run(p, tree_tiles<BM, BN>(p, lane));
-  int tile0, item0;
-  const int b = __builtin_amdgcn_readfirstlane(tree_find<BM, BN, true>(p, blockIdx.x, lane, tile0, item0));
+  const TreePlace place = tree_place<BM, BN, true>(p, blockIdx.x, lane);
+  const int b = __builtin_amdgcn_readfirstlane(place.b), per = place.per;
   if (b >= p.B) return;
   const TreeSequence<BM, BN> sq = tree_sequence<BM, BN>(p, b);
-  const int v = (int)blockIdx.x - item0, at = tile0 + v * sq.count;
+  const int v = (int)blockIdx.x - place.item0, at = place.tile0 + v * sq.count;
   const int first = __builtin_amdgcn_readfirstlane(at / per), n = __builtin_amdgcn_readfirstlane((at + sq.count - 1) / per) - first + 1;
   if (n <= 1) return;  // already in o
   int rt, head;
   tree_item(v, sq.items, p.Hkv, b, rt, head);
   const int r = rt * BM + wave * 32 + l32, nrows = min(sq.n, p.max_n) * G;
-  if (rt * BM + wave * 32 >= nrows) return;
   float M = -1e30f, L = 0.f, E = 0.f;
   f32x4 O[4] = {};
-  for (int i = 0; i < n; i += U) {
-    f32x4 st[U], o[U][4];
+  auto take = [&](const f32x4& st, const f32x4 (&o)[4]) {
+    const float m = fmaxf(M, st[0]), a = fast_exp2(M - m), w = fast_exp2(st[0] - m);
+    L = a * L + w * st[1];
+    E = a * E + w * st[2];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = min(i + u, n - 1);
-      const float* part = p.part + (2 * (int64_t)(first + k) + (k == 0)) * kTreePart<BM, DP>;
-      st[u] = *(const f32x4*)(part + (wave * 32 + l32) * 4);
-      const f32x4* po = (const f32x4*)(part + BM * 4) + (wave * DT + dt) * 4 * 64 + lane;
+    for (int g = 0; g < 4; ++g) O[g] = a * O[g] + w * o[g];
+    M = m;
+  };
+  if (rt * BM + wave * 32 < nrows) {
+    for (int i = group; i < n; i += NG * U) {
+      f32x4 st[U], o[U][4];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) o[u][g] = po[g * 64];
-    }
+      for (int u = 0; u < U; ++u) {
+        const int k = min(i + NG * u, n - 1);
+        const float* part = p.part + (2 * (int64_t)(first + k) + (k == 0)) * kTreePart<BM, DP>;
+        st[u] = *(const f32x4*)(part + (wave * 32 + l32) * 4);
+        const f32x4* po = (const f32x4*)(part + BM * 4) + (wave * DT + dt) * 4 * 64 + lane;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i + u >= n) break;
-      const float m = fmaxf(M, st[u][0]), a = fast_exp2(M - m), w = fast_exp2(st[u][0] - m);
-      L = a * L + w * st[u][1];
-      E = a * E + w * st[u][2];
+        for (int g = 0; g < 4; ++g) o[u][g] = po[g * 64];
+      }
 #pragma unroll
-      for (int g = 0; g < 4; ++g) O[g] = a * O[g] + w * o[u][g];
-      M = m;
+      for (int u = 0; u < U; ++u)
+        if (i + NG * u < n) take(st[u], o[u]);
     }
   }
-  if (r >= nrows) return;
+  if (group > 0) {
+    meet[group - 1][0][wave * 64 + lane] = f32x4{M, L, E, 0.f};
+#pragma unroll
+    for (int g = 0; g < 4; ++g) meet[group - 1][1 + g][wave * 64 + lane] = O[g];
+  }
+  __syncthreads();
+  if (group > 0 || r >= nrows) return;
+#pragma unroll 1
+  for (int k = 0; k < min(n, NG) - 1; ++k) {
+    const f32x4 o[4] = {meet[k][1][wave * 64 + lane], meet[k][2][wave * 64 + lane], meet[k][3][wave * 64 + lane], meet[k][4][wave * 64 + lane]};
+    take(meet[k][0][wave * 64 + lane], o);
+  }
   const int tok = r / G, hq = head * G + (r - tok * G);
   const float inv = L == 0.f ? 0.f : 1.f / L;
   T* o = (T*)p.o + ((int64_t)sq.tok0 + tok) * p.sot + (int64_t)hq * p.soh;
@@ -584,12 +615,19 @@ constexpr int tree_keys(int waves) { return waves == 8 ? 64 : 32; }
 WindowPlan tree_plan(int B, int tokens, int Hkv, int G, int dp, int max_n, long long seen) {
   WindowPlan w = {};
   const long long rows = (long long)max_n * G;
-  w.waves = rows > 128 ? 8 : rows > 64 ? 4 : 2;
-  const long long bm = w.waves * 32, bn = tree_keys(w.waves);
-  w.items = (int)(Hkv * std::min((long long)tokens * G / bm + B, (rows + bm - 1) / bm * B));
-  // As many runs as workgroups are resident, of at least kRunLeast tiles.
-  const long long slots = w.waves == 8 ? 256 : w.waves == 4 ? 512 : 768, tiles = ((seen + bn - 1) / bn + 1) * w.items;
-  w.splits = (int)std::max(1LL, std::min(slots, (tiles + kRunLeast - 1) / kRunLeast));
+  // More waves read a key tile for more rows and keep fewer workgroups resident: eight pay from eight tiles a resident
+  // workgroup, four from five. Waves 2, 4 and 8 on 32 query heads over 8 of 128 (us): 64 nodes after 1500 keys 27, 30, 33,
+  // after 8000 42, 38, 46; four trees of 64 after 1500 keys 43, 33, 38, after 4000 67, 45, 44; 16 after 6000 287, 169, 148.
+  for (w.waves = 8;; w.waves /= 2) {
+    const long long bm = w.waves * 32, bn = tree_keys(w.waves), slots = w.waves == 8 ? 256 : w.waves == 4 ? 512 : 768;
+    w.items = (int)(Hkv * std::min((long long)tokens * G / bm + B, (rows + bm - 1) / bm * B));
+    const long long tiles = ((seen + bn - 1) / bn + 1) * w.items;
+    if (w.waves > 2 && (rows <= bm / 2 || tiles < slots * (w.waves == 8 ? 8 : 5))) continue;
+    // As many runs as workgroups are resident, of at least kRunLeast tiles.
+    w.splits = (int)std::max(1LL, std::min(slots, (tiles + kRunLeast - 1) / kRunLeast));
+    break;
+  }
+  const long long bm = w.waves * 32;
   w.part_bytes = LSFA_GEMV_COUNTER_BYTES + (uint64_t)w.splits * 2 * (bm * (4 + dp)) * 4;
   return w;
 }
@@ -599,7 +637,7 @@ static hipError_t launch_tree(const WindowParams& p, const WindowPlan& w, hipStr
   hipLaunchKernelGGL((fa_tree_kernel<T, C, DP, NW, tree_keys(NW)>), dim3(w.splits), dim3(NW * 64), 0, s, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((fa_tree_combine_kernel<T, DP, NW, tree_keys(NW)>), dim3(w.items, DP / 32), dim3(NW * 64), 0, s, p);
+  hipLaunchKernelGGL((fa_tree_combine_kernel<T, DP, NW, tree_keys(NW)>), dim3(w.items, DP / 32), dim3(NW * kGroups<NW> * 64), 0, s, p);
   return hipGetLastError();
 }
 template <typename T, typename C, int DP>

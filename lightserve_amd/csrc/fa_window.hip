@@ -1330,7 +1330,7 @@ WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int eb, int max
   const int dp = D <= 64 ? 64 : 128;
   const long long rows = (long long)max_n * G;
   const long long seen = window > 0 ? std::min(max_keys, (long long)window + max_n + sinks + 96) : max_keys;
-  if (rows <= kNarrowRows) {
+  if (rows <= (tree ? kRowTile : kNarrowRows)) {
     w.columns = rows > kRowTile ? 2 : 1;
     const int rt = kRowTile * w.columns;
     w.part_rows = (int)std::min<long long>(rows, rt);
@@ -1406,7 +1406,7 @@ static hipError_t launch_wide(const WindowParams& p, const WindowPlan& w, hipStr
 }
 template <typename T, typename C, int DP>
 static hipError_t launch_window(const WindowParams& p, const WindowPlan& w, hipStream_t s) {
-  if (p.tree != nullptr) return w.columns == 1 ? launch_narrow<T, C, DP, 1, true>(p, w, s) : launch_narrow<T, C, DP, 2, true>(p, w, s);
+  if (p.tree != nullptr) return launch_narrow<T, C, DP, 1, true>(p, w, s);
   if (w.items > 0) return launch_wide<T, C, DP>(p, w, s);
   return w.columns == 1 ? launch_narrow<T, C, DP, 1, false>(p, w, s) : launch_narrow<T, C, DP, 2, false>(p, w, s);
 }
