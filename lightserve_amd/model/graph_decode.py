@@ -19,6 +19,11 @@ Two decode loops:
            bytes that a step reads of it), --window W [--sinks S] attends to
            the last W tokens and the first S only.
 
+With --drafts N [--branches W] or --beams K the command times that loop with
+several candidates per sequence instead (candidates.py): a step takes W drafted
+continuations of N tokens and keeps what the greedy choice agrees with, or K
+beams and keeps the K best of their continuations; each is one graph replay.
+
     python -m lightserve_amd.model.graph_decode [--mode full|kvcache|both] [--n-layers 4] ...
 
 Per-step latencies are HIP-event timed around each step with a synchronize
@@ -32,6 +37,8 @@ import statistics
 import torch
 import torch.nn.functional as F
 
+from ..kernels.beam_search import MAX_BEAMS
+from ..kernels.draft_tree import MAX_NODES, accept_drafts, kv_cache_keep, paged_tree_attention
 from ..kernels.paged_attention import paged_attention_decode, paged_prefill
 from ..kernels.quantized_kv_cache import kv_cache_append, quantized_kv_cache
 from ..kernels.rope import apply_rope_
@@ -121,6 +128,9 @@ class KVCacheDecoder:
     cached so far), k/v caches per layer and the block tables. step() issues
     only device work of static shape, so it can be captured and replayed;
     prefill() caches a prompt chunk by chunk before the decode steps.
+    draft_step() and accept() are a step's two halves where it takes a tree of
+    drafted tokens per sequence. caches holds all layers' K, V and scales (None
+    at 16 bits) as [layers, ...]; k_cache, v_cache and kv_scales are its layers.
 
     kv_e4m3 keeps K and V in 8 bits (quantized_kv_cache); window and sinks
     limit what a token attends to (paged_attention.py)."""
@@ -136,17 +146,25 @@ class KVCacheDecoder:
             else torch.arange(n_blocks)
         self.block_tables = order.to(torch.int32).view(batch_size, self.max_blocks).to(device)
         shape = (n_blocks, block_size, nkv, hd)
-        self.kv_scales = [None for _ in weights.layers]
+        layers = len(weights.layers)
         if kv_e4m3:
-            caches = [quantized_kv_cache(*shape, device=device) for _ in weights.layers]
-            self.k_cache, self.v_cache, self.kv_scales = ([c[i] for c in caches] for i in range(3))
+            k, v, sc = quantized_kv_cache(layers * n_blocks, *shape[1:], device=device)
+            self.caches = k.view(layers, *shape), v.view(layers, *shape), sc.view(layers, n_blocks, *sc.shape[1:])
         else:
-            self.k_cache = [torch.zeros(shape, dtype=config.dtype, device=device) for _ in weights.layers]
-            self.v_cache = [torch.zeros(shape, dtype=config.dtype, device=device) for _ in weights.layers]
+            self.caches = (*(torch.zeros(layers, *shape, dtype=config.dtype, device=device) for _ in range(2)), None)
+        self.k_cache, self.v_cache, self.kv_scales = (
+            [None] * layers if c is None else list(c.unbind(0)) for c in self.caches)
         self.attention = dict(window=window, sinks=sinks)
         self.seq_lens = torch.zeros(batch_size, dtype=torch.int32, device=device)
         self.tokens = torch.full((batch_size,), SEED_TOKEN_ID, dtype=torch.long, device=device)
+        self.own_tables = self.block_tables.clone()
         self.cos, self.sin = precompute_rope(config, device)
+
+    def reset(self):
+        """Back to the seed token, in place: a captured graph holds the tensors' addresses."""
+        self.seq_lens.zero_()
+        self.tokens.fill_(SEED_TOKEN_ID)
+        self.block_tables.copy_(self.own_tables)  # (a beam search shares blocks)
 
     def rotate_and_append(self, i, q, k, v, positions, lens, cu=None, **where):
         """RoPE of q and k [B, n, heads, head_dim] in place and K/V into layer i's cache: one launch, or for an 8-bit
@@ -162,25 +180,63 @@ class KVCacheDecoder:
 
     def step(self):
         """Logits [B, vocab] of the current tokens; appends their K/V."""
-        cfg, B = self.cfg, self.B
+        lens = self.seq_lens + 1
+
+        def attend(i, q):
+            return paged_attention_decode(q, self.k_cache[i], self.v_cache[i], self.block_tables, lens,
+                                          max_seq_len=self.cfg.max_seq_len, kv_scales=self.kv_scales[i], **self.attention)
+        # the slot of a K/V row is the one its block table gives for the position
+        return self._rows(self.tokens, self.seq_lens, lens, None, attend, block_tables=self.block_tables)
+
+    def draft_step(self, tokens, tree_mask, depth):
+        """Logits [B * n, vocab] of trees of n nodes: tokens int64 [B, n], tree_mask int64 [B * n, words] and depth int32 [B, n]
+        (draft_tree.py; node 0 is the current token). Appends their K/V behind the cached rows and leaves seq_lens as
+        it is: accept() says which of them stay. Rows past the block table are not stored."""
+        B, n = tokens.shape
+        assert B == self.B and depth.shape == (B, n), "tokens and depth must be [batch, nodes]"
+        pos = self.seq_lens.view(B, 1)
+        rows = torch.arange(n, device=pos.device)
+        lens = self.seq_lens + n
+        cu = torch.arange(0, (B + 1) * n, n, device=pos.device, dtype=torch.int32)
+        where = {}
+        if self.caches[2] is None:  # (kv_cache_append finds the slots of an 8-bit cache by itself)
+            at = pos + rows  # [B, n], int64
+            blocks = self.block_tables.gather(1, (at // self.bs).clamp(max=self.max_blocks - 1)).long()
+            where["slots"] = torch.where(at < self.max_blocks * self.bs, blocks * self.bs + at % self.bs, -1).view(-1)
+
+        def attend(i, q):
+            return paged_tree_attention(q, self.k_cache[i], self.v_cache[i], self.block_tables, cu, lens, tree_mask, max_nodes=n,
+                                        kv_scales=self.kv_scales[i], **self.attention)
+        return self._rows(tokens.reshape(-1), (pos + depth).view(-1), lens, cu, attend, **where)
+
+    def accept(self, logits, tokens, tree_mask):
+        """What accept_drafts returns for draft_step's logits; the path's rows become the sequence's last, seq_lens grows by
+        them and the choice after them is the next current token."""
+        B, n = tokens.shape
+        cu = torch.arange(0, (B + 1) * n, n, device=tokens.device, dtype=torch.int32)
+        path, counts, following = accept_drafts(logits, tokens.reshape(-1), tree_mask, cu, max_nodes=n, seq_lens=self.seq_lens)
+        kv_cache_keep(*self.caches[:2], self.block_tables, self.seq_lens, path, counts, kv_scales=self.caches[2])
+        self.tokens.copy_(following)
+        return path, counts, following
+
+    def _rows(self, tokens, positions, lens, cu, attend, **where):
+        """Logits of the rows `tokens` at `positions`, their K/V cached; attend(layer, q) is the attention over the cache. The
+        rest are rotate_and_append's."""
+        cfg, R = self.cfg, tokens.shape[0]
         nh, nkv, hd = cfg.n_heads, cfg.kv_heads, cfg.head_dim
-        pos = self.seq_lens
-        lens = pos + 1
-        residual = F.embedding(self.tokens, self.w.embed_tokens)  # [B, H]
+        residual = F.embedding(tokens, self.w.embed_tokens)  # [R, H]
         pending = None
         for i, layer in enumerate(self.w.layers):
             # residual add + RMSNorm folded into the q/k/v launch (the first layer's input is the embedding)
             x_in, r_in = (residual, None) if pending is None else (pending, residual)
             (q, k, v), residual = add_rmsnorm_matmul_shared_input(
                 x_in, r_in, layer.input_layernorm_weight, cfg.rms_eps, (layer.q_proj, layer.k_proj, layer.v_proj))
-            # RoPE at each sequence's position; the same launch stores the rotated k and v rows at the slot
-            # its block table gives for that position
-            self.rotate_and_append(i, q.view(B, 1, nh, hd), k.view(B, 1, nkv, hd), v.view(B, 1, nkv, hd), pos, lens,
-                                   block_tables=self.block_tables)
-            o = paged_attention_decode(q.view(B, nh, hd), self.k_cache[i], self.v_cache[i], self.block_tables,
-                                       lens, max_seq_len=cfg.max_seq_len, kv_scales=self.kv_scales[i], **self.attention)
+            # RoPE at each row's position; for a 16-bit cache the same launch stores the rotated k and v rows
+            self.rotate_and_append(i, q.view(R, 1, nh, hd), k.view(R, 1, nkv, hd), v.view(R, 1, nkv, hd), positions, lens, cu,
+                                   **where)
+            o = attend(i, q.view(R, nh, hd))
             (gate, up), residual = add_rmsnorm_matmul_shared_input(
-                matmul(o.view(B, nh * hd), layer.o_proj), residual, layer.post_attention_layernorm_weight,
+                matmul(o.view(R, nh * hd), layer.o_proj), residual, layer.post_attention_layernorm_weight,
                 cfg.rms_eps, (layer.gate_proj, layer.up_proj))
             pending = swiglu_matmul(gate, up, layer.down_proj)
         (logits,), _ = add_rmsnorm_matmul_shared_input(pending, residual, self.w.norm_weight, cfg.rms_eps,
@@ -279,9 +335,38 @@ def reset(dec, config, args):
         dec.ids.copy_(make_seeded_buffer(args.batch_size, config.max_seq_len, dec.ids.device))
         dec.cur_len = 1
     else:
-        dec.seq_lens.zero_()
-        dec.tokens.fill_(SEED_TOKEN_ID)
+        dec.reset()
     return dec
+
+
+def candidates_main(args):
+    """Times steps with drafts or beams (candidates.py) eagerly and as graph replays, each from the seed token, and counts the
+    tokens that a step yields."""
+    from .candidates import BeamSearch, LookupDrafts
+    B = args.batch_size
+    config = llama3_8b_shape(n_layers=args.n_layers, max_seq_len=args.max_seq_len, gqa=args.gqa)
+    most = 1 if args.beams else args.drafts + 1  # tokens of a step
+    needed = (args.warmup_steps + args.num_steps + 1) * most + (0 if args.beams else args.drafts * args.branches + 1)
+    assert needed < config.max_seq_len, f"--max-seq-len {config.max_seq_len} too small, {needed + 1} do"
+    weights = init_weights(config, device="cuda", seed=args.seed)
+    dec = KVCacheDecoder(weights, config, B * (args.beams or 1), block_size=args.block_size, **cache_options(args))
+    loop = BeamSearch(dec, args.beams) if args.beams else LookupDrafts(dec, args.drafts, args.branches)
+    res = {"beams": args.beams, "drafts": args.drafts, "branches": args.branches, "batch_size": B, "n_layers": config.n_layers,
+           "n_kv_heads": config.kv_heads}
+    for kind in ("eager", "graph"):
+        step = loop.step
+        if kind == "graph":
+            step = capture(loop.step)[0].replay
+        loop.reset()
+        res[kind] = summarize(time_steps(step, args.num_steps, args.warmup_steps))
+        res["tokens_per_step"] = (dec.seq_lens.sum().item() / dec.B) / (args.num_steps + args.warmup_steps)
+        print(f"{kind:<6} median {res[kind]['median_ms']:.3f} ms a step, {res['tokens_per_step']:.2f} tokens of each sequence",
+              flush=True)
+    print(json.dumps(res), flush=True)
+    if args.out:
+        with open(args.out, "w") as f:
+            json.dump(res, f, indent=2)
+    return res
 
 
 def prefill_main(args):
@@ -335,10 +420,25 @@ def main(argv=None):
     ap.add_argument("--kv-e4m3", action="store_true", help="8-bit KV cache (kvcache mode and --prefill)")
     ap.add_argument("--window", type=int, default=None, metavar="W", help="sliding window of W tokens (as --kv-e4m3)")
     ap.add_argument("--sinks", type=int, default=0, metavar="S", help="first tokens that stay visible under --window")
+    ap.add_argument("--drafts", type=int, default=0, metavar="N",
+                    help="instead: steps that verify drafted continuations of N tokens, looked up in the text so far")
+    ap.add_argument("--branches", type=int, default=1, metavar="W", help="continuations a step (--drafts)")
+    ap.add_argument("--beams", type=int, default=0, metavar="K", help="instead: steps of a beam search with K beams a sequence")
     args = ap.parse_args(argv)
+    for name in ("drafts", "beams", "prefill"):
+        if getattr(args, name) < 0:
+            ap.error(f"--{name} must not be negative")
+    if bool(args.prefill) + bool(args.drafts) + bool(args.beams) > 1:
+        ap.error("give one of --prefill, --drafts and --beams")
+    if args.branches < 1 or args.drafts * args.branches > MAX_NODES - 1:
+        ap.error(f"--branches must be positive, and --drafts times it at most {MAX_NODES - 1}")
+    if args.beams > MAX_BEAMS:
+        ap.error(f"--beams takes at most {MAX_BEAMS}")
     assert torch.cuda.is_available(), "needs a GPU"
     if args.prefill:
         return prefill_main(args)
+    if args.drafts or args.beams:
+        return candidates_main(args)
     config = llama3_8b_shape(n_layers=args.n_layers, max_seq_len=args.max_seq_len, gqa=args.gqa)
     needed = args.warmup_steps + args.num_steps + 3
     assert needed < config.max_seq_len, f"--max-seq-len {config.max_seq_len} too small for {needed} decode steps"
