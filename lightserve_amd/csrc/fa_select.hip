@@ -124,6 +124,10 @@ struct Chunk {
 __device__ __forceinline__ uint64_t entry_of(uint32_t key, int index) { return (uint64_t)key << 32 | (uint32_t)~index; }
 __device__ __forceinline__ int index_of(uint64_t g) { return (int)~(uint32_t)g; }
 
+// Where sequence b's counter lies: arrivals at one cache line wait for one another (32 sequences' next to
+// each other cost 1792 workgroups 8 us), so up to 1024 sequences have lines of their own.
+__device__ __forceinline__ int counter_of(int b, int B) { return B <= LSFA_GEMV_COUNTER_BYTES / 256 ? b * 64 : b; }
+
 // Whether this workgroup is the last of `all` that arrive at the counter, whose partial
 // results are then there to be read with load_agent. (Stores of the others have left for device
 // scope before they arrive; the counter is left at zero.)
@@ -232,7 +236,7 @@ __global__ __launch_bounds__(kThreads) void fa_accept_kernel(const AcceptParams 
     __syncthreads();
     if (tid == 0)
       store_agent(p.part + row * p.parts + part, entry_of(top != top ? kKeyNan : key_of(top), x.first + st_at));
-    if (!last_to_arrive(p.counters + b, n * p.parts, &st_last)) continue;
+    if (!last_to_arrive(p.counters + counter_of(b, p.B), n * p.parts, &st_last)) continue;
 
     const int words = p.mask_words;
     for (int i = tid; i < n; i += kThreads) {
@@ -300,14 +304,36 @@ __device__ __forceinline__ float exp_near(float t) {
   return fmaf(e, left, e);
 }
 
+// The Nth largest of all threads' keys (0 where fewer are above 0): at least N values are at or above it where each is its
+// thread's largest, and few more.
+__device__ __forceinline__ uint32_t nth_of_threads(uint32_t key, int N, uint32_t* st_key) {
+  __syncthreads();
+  st_key[threadIdx.x] = key;
+  __syncthreads();
+  uint32_t k[kWaves], from = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) k[w] = st_key[w * 64 + (threadIdx.x & 63)];
+#pragma unroll 1
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t t = from | 1u << bit;
+    int c = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) c += __builtin_popcountll(__ballot(k[w] >= t));
+    if (c >= N) from = t;
+    if (c == N) break;
+  }
+  return from;
+}
+
 template <typename T, int U>
 __global__ __launch_bounds__(kThreads) void fa_beams_kernel(const BeamParams p) {
   using Ch = Chunk<T, U>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ float st_m[kWaves];
   __shared__ double st_l[kWaves];
-  __shared__ int st_n[kWaves], st_last, st_found;
-  __shared__ double st_lse[LSFA_BEAMS_MAX], st_floor;
+  __shared__ uint32_t st_key[kThreads];
+  __shared__ int st_n[kWaves], st_put, st_last, st_found, st_kept, st_chosen[LSFA_BEAMS_NUM_MAX];
+  __shared__ double st_lse[LSFA_BEAMS_MAX], st_score[LSFA_BEAMS_MAX], st_floor;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int N = p.num, S = p.chunks;
   const int chunk = (int)(blockIdx.x % (unsigned)S), row = (int)(blockIdx.x / (unsigned)S), b = row / p.K;
@@ -324,25 +350,31 @@ __global__ __launch_bounds__(kThreads) void fa_beams_kernel(const BeamParams p) 
   }
   for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
   if (lane == 0) st_m[wave] = top, st_l[wave] = l;
+  if (tid == 0) st_put = 0;
 
-  // The wave's N largest are at or above the Nth largest of its lanes' largest, and little else is
+  // The chunk's N largest are at or above the Nth largest of its threads' largest, and little else is
   // (finite values: -inf is no candidate, and a row with NaN has none).
-  const uint32_t mk = mine > -INFINITY ? key_of(mine) : 0u;
-  uint32_t from = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t t = from | 1u << bit;
-    const int n = __builtin_popcountll(__ballot(mk >= t));
-    if (n >= N) from = t;
-    if (n == N) break;
-  }
+  const uint32_t from = nth_of_threads(mine > -INFINITY ? key_of(mine) : 0u, N, st_key);
   const float least = from == 0 ? -FLT_MAX : fmaxf(value_of(from), -FLT_MAX);
-  int n = 0;
-#pragma unroll
-  for (int i = 0; i < Ch::E; ++i) n += __builtin_popcountll(__ballot(x.value(i) >= least));
   auto entry = [&](int i) -> uint64_t { return entry_of(key_of(x.value(i)), x.first + x.pos(i)); };
-  // More than a place for each lane (many equal ones, or a large N): the entry that exactly N are at or above.
-  uint64_t exact = 0;
-  if (n > 64) {
+  uint64_t* pool = (uint64_t*)lds;  // [kThreads]
+  int c = 0;
+#pragma unroll
+  for (int i = 0; i < Ch::E; ++i) c += x.value(i) >= least;
+  const int upto = lanes_sum(c), n = __builtin_amdgcn_readlane(upto, 63);
+  int at = 0;
+  if (lane == 0) at = atomicAdd(&st_put, n);
+  at = __builtin_amdgcn_readfirstlane(at) + upto - c;
+#pragma unroll
+  for (int i = 0; i < Ch::E; ++i)
+    if (x.value(i) >= least) {
+      if (at < kThreads) pool[at] = entry(i);
+      ++at;
+    }
+  __syncthreads();
+  int all = st_put, have = all;
+  if (all > kThreads) {  // (many equal ones): of each wave the entries that exactly N are at or above, or all
+    uint64_t exact = 0;
     for (int bit = 63; bit >= 0; --bit) {
       const uint64_t t = exact | 1ull << bit;
       int k = 0;
@@ -351,33 +383,30 @@ __global__ __launch_bounds__(kThreads) void fa_beams_kernel(const BeamParams p) 
       if (k >= N) exact = t;
       if (k == N) break;
     }
-    n = N;
-  }
-  uint64_t* pool = (uint64_t*)lds;  // [4 * 64]
-  int put = 0;
+    pool[tid] = 0;
+    c = 0;
 #pragma unroll
-  for (int i = 0; i < Ch::E; ++i) {
-    bool in = x.value(i) >= least;
-    if (exact != 0) in = in && entry(i) >= exact;
-    const unsigned long long ones = __ballot(in);
-    if (ones == 0) continue;
-    if (in) pool[wave * 64 + put + __builtin_amdgcn_mbcnt_hi((uint32_t)(ones >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ones, 0))] = entry(i);
-    put += __builtin_popcountll(ones);
+    for (int i = 0; i < Ch::E; ++i) c += x.value(i) >= least && entry(i) >= exact;
+    at = wave * 64 + lanes_sum(c) - c;
+#pragma unroll
+    for (int i = 0; i < Ch::E; ++i)
+      if (x.value(i) >= least && entry(i) >= exact) pool[at++] = entry(i);
+    if (lane == 0) st_n[wave] = min(n, N);
+    __syncthreads();
+    all = kThreads;
+    have = 0;
+    for (int w = 0; w < kWaves; ++w) have += st_n[w];
   }
-  if (lane == 0) st_n[wave] = n;
-  __syncthreads();
-  // The workgroup's, each at its rank.
+  // Each at its rank.
   uint64_t* out = p.lists + list * N;
-  const uint64_t cand = lane < n ? pool[wave * 64 + lane] : 0;
-  int rank = 0, all = 0;
-  for (int w = 0; w < kWaves; ++w) {
-    const int have = st_n[w];
-    all += have;
+  const uint64_t cand = tid < all ? pool[tid] : 0;
+  int rank = 0;
+  if (cand != 0) {
 #pragma unroll 4
-    for (int j = 0; j < have; ++j) rank += pool[w * 64 + j] > cand;
+    for (int j = 0; j < all; ++j) rank += pool[j] > cand;
+    if (rank < N) store_agent(out + rank, cand);
   }
-  if (lane < n && rank < N) store_agent(out + rank, cand);
-  for (int j = all + tid; j < N; j += kThreads) store_agent(out + j, 0);
+  for (int j = have + tid; j < N; j += kThreads) store_agent(out + j, 0);
   if (tid == 0) {
     float M = st_m[0];
     for (int w = 1; w < kWaves; ++w) M = nan_max(M, st_m[w]);
@@ -387,18 +416,24 @@ __global__ __launch_bounds__(kThreads) void fa_beams_kernel(const BeamParams p) 
     store_agent(p.sums + 2 * list, __float_as_uint(M));
     store_agent(p.sums + 2 * list + 1, (uint64_t)__double_as_longlong(L));
   }
-  if (!last_to_arrive(p.counters + b, p.K * S, &st_last)) return;
+  if (!last_to_arrive(p.counters + counter_of(b, p.B), p.K * S, &st_last)) return;
 
-  // The sequence's lists meet: K S of them, in the order of k V + v.
+  // The sequence's lists meet: K S of them, in the order of k V + v. What is read was written elsewhere and
+  // takes a microsecond to come: all of it is asked for at once, then the N lists with the best first entries.
   const int lists = p.K * S;
   const int64_t list0 = (int64_t)b * lists;
-  double* sum = (double*)lds;               // [lists]; then the scores of their first entries
-  float* lmax = (float*)(sum + lists);      // [lists]
+  double* sum = (double*)lds;                 // [lists]; then the scores of their first entries
+  uint64_t* firsts = (uint64_t*)(sum + lists);  // [lists]
+  float* lmax = (float*)(firsts + lists);     // [lists]
   for (int t = tid; t < lists; t += kThreads) {
-    lmax[t] = __uint_as_float((uint32_t)load_agent(p.sums + 2 * (list0 + t)));
-    sum[t] = __longlong_as_double((long long)load_agent(p.sums + 2 * (list0 + t) + 1));
+    const uint64_t m = load_agent(p.sums + 2 * (list0 + t)), l2 = load_agent(p.sums + 2 * (list0 + t) + 1);
+    firsts[t] = load_agent(p.lists + (list0 + t) * N);
+    lmax[t] = __uint_as_float((uint32_t)m);
+    sum[t] = __longlong_as_double((long long)l2);
   }
-  if (tid == 0) st_found = 0, st_floor = -(double)INFINITY;
+  const double own = tid < p.K ? (double)p.scores[(int64_t)b * p.K + tid] : 0.;
+  if (tid < N) st_chosen[tid] = -1;
+  if (tid == 0) st_found = st_kept = 0, st_floor = -(double)INFINITY;
   __syncthreads();
   for (int t = tid; t < lists; t += kThreads) {
     const int k0 = t / S * S;
@@ -409,46 +444,85 @@ __global__ __launch_bounds__(kThreads) void fa_beams_kernel(const BeamParams p) 
     if (t == k0) st_lse[t / S] = M;  // (K <= LSFA_BEAMS_MAX)
   }
   __syncthreads();
-  for (int k = tid; k < p.K; k += kThreads) {
+  if (tid < p.K) {
     double L = 0.;
 #pragma unroll 4
-    for (int s = 0; s < S; ++s) L += sum[k * S + s];
-    const double lse = st_lse[k] + log(L);
-    st_lse[k] = lse > -(double)INFINITY && lse < (double)INFINITY ? lse : (double)NAN;  // a row without lse offers nothing
+    for (int s = 0; s < S; ++s) L += sum[tid * S + s];
+    const double lse = st_lse[tid] + log(L);
+    st_lse[tid] = lse > -(double)INFINITY && lse < (double)INFINITY ? lse : (double)NAN;  // a row without lse offers nothing
+    st_score[tid] = own;
   }
   __syncthreads();
   auto score = [&](int k, uint64_t g) -> double {
-    const double sc = (double)p.scores[(int64_t)b * p.K + k] + ((double)value_of((uint32_t)(g >> 32)) - st_lse[k]);
+    const double sc = st_score[k] + ((double)value_of((uint32_t)(g >> 32)) - st_lse[k]);
     return g != 0 && sc > -(double)INFINITY ? sc : -(double)INFINITY;
   };
-  for (int t = tid; t < lists; t += kThreads) sum[t] = score(t / S, load_agent(p.lists + (list0 + t) * N));
-  __syncthreads();
-  // The N best lie in the N lists with the best first entries, at or above the Nth of those.
-  uint32_t chosen = 0;  // of the thread's lists (t = tid + 256 i)
-  for (int t = tid, i = 0; t < lists; t += kThreads, ++i) {
+  // The N best lie in the N lists with the best first entries, at or above the Nth of those. First the Nth largest
+  // of the threads' best, in 32 bits: few lists are at or above it, and only those are ranked.
+  float best = -INFINITY;
+  for (int t = tid; t < lists; t += kThreads) {
+    sum[t] = score(t / S, firsts[t]);
+    best = fmaxf(best, (float)sum[t]);
+  }
+  uint32_t low = nth_of_threads(best > -INFINITY ? key_of(best) : 0u, N, st_key);
+  double* ks = (double*)firsts;  // [lists]: the scores of those, and in lmax their numbers
+  int* kt = (int*)lmax;
+  for (int t = tid; t < lists; t += kThreads) {
     const double h = sum[t];
+    if (!(h > -(double)INFINITY) || key_of((float)h) < low) continue;
+    const int at = atomicAdd(&st_kept, 1);
+    ks[at] = h;
+    kt[at] = t;
+  }
+  __syncthreads();
+  const int kept = st_kept;
+  for (int i = tid; i < kept; i += kThreads) {
+    const double h = ks[i];
+    const int t = kt[i];
     int rank = 0;
 #pragma unroll 4
-    for (int j = 0; j < lists; ++j) rank += sum[j] > h || (sum[j] == h && j < t);
-    if (rank < N && h > -(double)INFINITY) chosen |= 1u << i;
+    for (int j = 0; j < kept; ++j) rank += ks[j] > h || (ks[j] == h && kt[j] < t);
+    if (rank < N) st_chosen[rank] = t;
     if (rank == N - 1) st_floor = h;
   }
   __syncthreads();
   double* cs = (double*)lds;       // [N * N]
   int* ci = (int*)(cs + N * N);    // k V + v
   const double floor = st_floor;
-  for (int t = tid, i = 0; t < lists; t += kThreads, ++i) {
-    if (!(chosen >> i & 1)) continue;
-    for (int j = 0; j < N; ++j) {
-      const uint64_t g = load_agent(p.lists + (list0 + t) * N + j);
-      const double sc = score(t / S, g);
-      if (!(sc >= floor) || sc == -(double)INFINITY) break;
-      const int at = atomicAdd(&st_found, 1);
-      cs[at] = sc;
-      ci[at] = t / S * p.cols + index_of(g);
+  best = -INFINITY;
+  for (int e0 = tid; e0 < N * N; e0 += 4 * kThreads) {
+    uint64_t g[4];
+    int of[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int e = e0 + u * kThreads;
+      of[u] = e < N * N ? st_chosen[e / N] : -1;
+      g[u] = of[u] >= 0 ? load_agent(p.lists + (list0 + of[u]) * N + e % N) : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int e = e0 + u * kThreads;
+      const double sc = g[u] != 0 ? score(of[u] / S, g[u]) : -(double)INFINITY;
+      if (e >= N * N) break;
+      cs[e] = sc >= floor ? sc : -(double)INFINITY;
+      ci[e] = of[u] / S * p.cols + index_of(g[u]);
+      best = fmaxf(best, (float)cs[e]);
     }
   }
-  __syncthreads();
+  // Once more the few that can be among the N best, moved to the front: no more than have been read.
+  low = nth_of_threads(best > -INFINITY ? key_of(best) : 0u, N, st_key);
+  for (int e0 = 0; e0 < N * N; e0 += kThreads) {
+    const int e = e0 + tid;
+    const double sc = e < N * N ? cs[e] : -(double)INFINITY;
+    const int id = e < N * N ? ci[e] : 0;
+    __syncthreads();
+    if (sc > -(double)INFINITY && key_of((float)sc) >= low) {
+      const int to = atomicAdd(&st_found, 1);
+      cs[to] = sc;
+      ci[to] = id;
+    }
+    __syncthreads();
+  }
   const int found = st_found;
   for (int i = tid; i < found; i += kThreads) {
     const double sc = cs[i];
@@ -480,7 +554,7 @@ SelectPlan select_plan(long long rows, int cols, int dtype, bool beams) {
   const int size = dtype == 0 ? 4 : 2;
   SelectPlan s;
   s.loads = beams && size == 4 ? 8 : 4;
-  while (s.loads > 1 && rows * chunks_of(cols, size, s.loads) < 512) s.loads /= 2;
+  while (s.loads > 1 && rows * chunks_of(cols, size, s.loads) < (beams ? 256 : 512)) s.loads /= 2;
   s.chunks = chunks_of(cols, size, s.loads);
   s.per = beams ? 1 : (int)std::max(1LL, std::min<long long>(s.chunks, rows * s.chunks / 2048));
   s.parts = (s.chunks + s.per - 1) / s.per;
@@ -494,7 +568,7 @@ static void launch_accept(const AcceptParams& p, hipStream_t s) {
 template <typename T, int U>
 static void launch_beams(const BeamParams& p, hipStream_t s) {
   const size_t lists = (size_t)p.K * p.chunks;
-  const size_t lds = std::max({(size_t)kWaves * 64 * 8, lists * 12, (size_t)p.num * p.num * 12});
+  const size_t lds = std::max({(size_t)kThreads * 8, lists * 20, (size_t)p.num * p.num * 12});
   hipLaunchKernelGGL((fa_beams_kernel<T, U>), dim3((unsigned)(p.B * p.K * p.chunks)), dim3(kThreads), lds, s, p);
 }
 template <typename T>
