@@ -569,7 +569,8 @@ __global__ __launch_bounds__((NW * kGroups<NW> * 64)) void fa_tree_combine_kerne
       f32x4 st[U], o[U][4];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int k = min(i + NG * u, n - 1);
+        const int k = i + NG * u;
+        if (k >= n) break;  // (uniform)
         const float* part = p.part + (2 * (int64_t)(first + k) + (k == 0)) * kTreePart<BM, DP>;
         st[u] = *(const f32x4*)(part + (wave * 32 + l32) * 4);
         const f32x4* po = (const f32x4*)(part + BM * 4) + (wave * DT + dt) * 4 * 64 + lane;
