@@ -42,11 +42,12 @@ def beam_search_select(logits, scores, num=None):
     num = beams if num is None else num
     assert 1 <= beams <= MAX_BEAMS and 1 <= num <= MAX_CANDIDATES, f"1 to {MAX_BEAMS} beams and {MAX_CANDIDATES} candidates"
     assert rows == 0 or vocab > 0, "the vocabulary must not be empty"
-    check_device((("logits", logits), ("scores", scores)))
+    if not logits.get_device() == scores.get_device() >= 0:
+        check_device((("logits", logits), ("scores", scores)))
     if rows and (logits.stride(1) != 1 or logits.stride(0) < vocab):
         logits = _lib.packed(logits)
     device = logits.device
-    out = torch.empty((batch, num), dtype=torch.float32, device=device)
+    out = scores.new_empty((batch, num))
     parents = torch.empty((batch, num), dtype=torch.int32, device=device)
     tokens = torch.empty((batch, num), dtype=torch.int64, device=device)
     if batch > 0:

@@ -115,17 +115,18 @@ def accept_drafts(logits, tokens, tree_mask, cu_seqlens, *, max_nodes=None, seq_
         assert seq_lens.dtype == _I32 and seq_lens.shape == (batch,) and (batch == 0 or seq_lens.is_contiguous()), \
             "seq_lens must be contiguous int32 [batch]"
     assert total == 0 or vocab > 0, "the vocabulary must not be empty"
-    check_device((("logits", logits), ("tokens", tokens), ("tree_mask", tree_mask), ("cu_seqlens", cu_seqlens),
-                  *((("seq_lens", seq_lens),) if seq_lens is not None else ())))
+    on = logits.get_device()
+    if not (on >= 0 and on == tokens.get_device() == tree_mask.get_device() == cu_seqlens.get_device()
+            and (seq_lens is None or seq_lens.get_device() == on)):
+        check_device((("logits", logits), ("tokens", tokens), ("tree_mask", tree_mask), ("cu_seqlens", cu_seqlens),
+                      *((("seq_lens", seq_lens),) if seq_lens is not None else ())))
     if max_nodes is None:
         max_nodes = _longest(cu_seqlens)
     _check_nodes(max_nodes, tree_mask)
     if total and (logits.stride(1) != 1 or logits.stride(0) < vocab):
         logits = _lib.packed(logits)
     device = logits.device
-    path = torch.empty((batch, max_nodes), dtype=_I32, device=device)
-    counts = torch.empty(batch, dtype=_I32, device=device)
-    following = torch.empty(batch, dtype=_I64, device=device)
+    path, counts, following = cu_seqlens.new_empty((batch, max_nodes)), cu_seqlens.new_empty(batch), tokens.new_empty(batch)
     if batch > 0:
         tokens, cu = tokens.contiguous(), cu_seqlens.contiguous()
         args = _lib.pack(
@@ -147,7 +148,7 @@ def cache_rows(call, k_cache, v_cache, kv_scales, block_tables, seq_lens, index,
     L, (n, bs, h, d) = shape[0] if layers else 1, shape[-4:]
     assert strides[0][-1] == 1 and strides[1][-1] == 1, "the caches' head-dim stride must be 1"
     for s in strides:
-        assert all(x > 0 or m == 1 for x, m in zip(s, shape)), "rows of the caches must not share memory"
+        assert min(s) > 0 or all(x > 0 or m == 1 for x, m in zip(s, shape)), "rows of the caches must not share memory"
     assert (kv_scales is None) == (k_cache.dtype != torch.float8_e4m3fn), "an 8-bit cache, and no other, has kv_scales"
     scale_layer = 0
     if kv_scales is not None:
