@@ -27,7 +27,7 @@ behind the path), counts int32 [batch] and next_tokens int64 [batch], the choice
 nodes has count 0 and next token -1. seq_lens, when given, grows by counts in the same launch.
 
 kv_cache_keep moves rows inside the cache: row start + keep[b, i] becomes row start + i for i < counts[b], start = seq_lens[b] -
-counts[b] (seq_lens counts what is cached once the rows are kept, as accept_drafts leaves it). Entries with keep[b, i] <= i stay where they
+counts[b] (seq_lens counts what is cached once the rows are kept, as accept_drafts leaves it; counts are held to 0 .. keep's width). Entries with keep[b, i] <= i stay where they
 are, and so do rows that the block table or the cache does not have. keep may have any width and need not be a path: with
 it a sequence drops rows from its middle, too. Caches are [num_blocks, block_size, heads_kv, head_dim] in any of fp32, bf16,
 fp16 or 8 bits with kv_scales (quantized_kv_cache.py), or the same for all layers as one tensor [layers, ...]: one launch. Sequences must not share

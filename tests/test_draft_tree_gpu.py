@@ -15,6 +15,7 @@ import threading
 import pytest
 import torch
 
+from lightserve_amd.kernels.beam_search import kv_cache_reorder
 from lightserve_amd.kernels.draft_tree import accept_drafts, draft_tree, kv_cache_keep, paged_tree_attention
 from lightserve_amd.kernels.paged_attention import paged_prefill
 from oracle import candidates, paged8
@@ -128,6 +129,57 @@ def test_tree_any_mask(gpu):
         _attend(kind, dtype, nodes, had, 4, 2, 64, 16, 22, 30, 2, mask=mask, what="any, window")
     wide = torch.randint(-2 ** 62, 2 ** 62, (sum(nodes), 4), generator=g)
     _attend("16 bit", torch.bfloat16, nodes, had, 12, 2, 64, 16, 23, mask=wide, words=4, what="wider than needed")
+
+
+def test_tree_of_more_nodes_than_keys(gpu):
+    """Lengths below the number of nodes: the first nodes' own keys lie before the sequence, and nobody sees them."""
+    print("case tree lengths below nodes", flush=True)
+    for kind, dtype in KINDS:
+        _attend(kind, dtype, [9, 12, 3, 2], [-4, -11, -3, 5], 4, 2, 64, 16, 31, what="few rows")
+        _attend(kind, dtype, [40, 100, 70], [-7, -99, -70], 8, 2, 64, 16, 32, what="many rows")
+        _attend(kind, dtype, [40, 100, 70], [-7, -99, 3], 8, 2, 64, 16, 33, 5, 2, what="window")
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "16 bit"])
+@pytest.mark.parametrize("n", [3, 40])
+def test_tree_far_blocks(gpu, kind, n):
+    """Blocks whose offsets in the cache, in elements, pass 32 bits give what the same rows give near its beginning; and so do
+    rows moved there."""
+    print(f"case tree far {kind} n={n}", flush=True)
+    nodes, had, hkv, d, bs = [n, n + 2], [50, 200], 2, 128, 16
+    lens = [a + b for a, b in zip(nodes, had)]
+    table, pool = tables(lens, bs, 3)
+    (k, v, sc), _ = _cache(kind, torch.bfloat16, pool, bs, hkv, d, 4)
+    blocks = 2 ** 32 // (bs * hkv * d) + pool + 5
+    far = blocks - pool
+    big = [torch.empty(blocks, *c.shape[1:], dtype=torch.uint8, device="cuda").view(c.dtype) if c.dtype == E4M3 else
+           torch.empty(blocks, *c.shape[1:], dtype=c.dtype, device="cuda") for c in (k, v)]
+    for c, small in zip(big, (k, v)):
+        raw_bytes = c.view(torch.uint8) if c.dtype == E4M3 else c
+        raw_bytes[far:] = small.view(torch.uint8) if c.dtype == E4M3 else small
+    scales = None
+    if sc is not None:
+        scales = torch.zeros(blocks, hkv, bs, 2, dtype=torch.uint8, device="cuda")
+        scales[far:] = sc
+    q = torch.randn(sum(nodes), 8, d, generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
+    _, mask, cu = forest(nodes, 6)
+    near_table, far_table = table.cuda(), torch.where(table >= 0, table + far, -1).cuda()
+    rest = (cu.cuda(), _i32(lens).cuda(), mask.cuda())
+    a = paged_tree_attention(q, k, v, near_table, *rest, kv_scales=sc)
+    b = paged_tree_attention(q, *big, far_table, *rest, kv_scales=scales)
+    assert torch.equal(a, b)
+    keep, counts = _i32([[0, 2, -1], [1, 4, 4]]).cuda(), _i32([2, 3]).cuda()
+    kept = _i32([h + c for h, c in zip(had, [2, 3])]).cuda()
+    kv_cache_keep(k, v, near_table, kept, keep, counts, kv_scales=sc)
+    kv_cache_keep(*big, far_table, kept, keep, counts, kv_scales=scales)
+    parents, two = _i32([[1, 0]]).cuda(), _i32([60, 60]).cuda()
+    kv_cache_reorder(k, v, near_table, two, parents, kv_scales=sc)
+    kv_cache_reorder(*big, far_table, two, parents, kv_scales=scales)
+    torch.cuda.synchronize()
+    assert torch.equal(torch.where(near_table >= 0, near_table + far, -1), far_table)
+    for c, small in zip(big, (k, v)):
+        assert torch.equal(raw(c[far:].contiguous()), raw(small))
+    assert sc is None or torch.equal(scales[far:], sc)
 
 
 @pytest.mark.parametrize("sm_scale", [0.0, -0.2, 3.0])
