@@ -1,5 +1,6 @@
 // Attention of draft trees over paged KV caches, where a KV head's group has more than
-// 16 rows (nodes times query heads), for gfx950. Fewer are fa_window.hip's narrow kernel's.
+// 16 rows (nodes times query heads), or a few long sequences, for gfx950. The others are fa_window.hip's
+// narrow kernel's (its window_plan says which).
 //
 // A tree's nodes all see the sequence's earlier tokens (under a window its last ones and the
 // sinks) and, of one another, those that their masks name: all but the last key tiles are

@@ -6,7 +6,7 @@
 // n of its seq_lens[b] cached tokens (one for a decode step). An 8-bit cache
 // holds e4m3 codes and one power-of-two scale for each row (fa_kvq.hip).
 // In a tree of drafted tokens (TREE) the n queries see the tokens before them and, of
-// one another, those that their masks name; trees of many rows are fa_tree.hip's.
+// one another, those that their masks name; trees of more rows are fa_tree.hip's (window_plan).
 //
 // Few rows per KV head (decode, and chunks of a few tokens): the narrow kernel.
 // Many: the wide one, further down.
@@ -1320,6 +1320,11 @@ __global__ __launch_bounds__(NW * 64) void fa_window_wide_combine_kernel(const W
 // Most rows of a sequence and KV head in the narrow kernel: 16 chunks of 8 tokens, group 4 (32
 // rows), take 66 us there and 88 in the wide one, 4 chunks of 64 tokens (256 rows) 73 and 46.
 constexpr long long kNarrowRows = 32;
+// Trees of more than 16 rows go to the tile kernel (8 nodes of group 4 after 1500 keys 16 us there, 25 here), and
+// of fewer where a sequence's runs leave more rows of partial results than this to the one that merges them, of up to 8 rows and
+// of more (trees of 2 nodes after 4500 keys 20.8 us here and 21.7 there, after 8000 28.6 and 24.7; of 4 nodes after 1500
+// 16.7 and 17.4, after 2200 20.8 and 18.3, four of them after 2000 29.6 and 19.6, 64 after 4000 211 and 225).
+constexpr long long kTreeMerge[2] = {400, 200};
 
 WindowPlan tree_plan(int B, int tokens, int Hkv, int G, int dp, int max_n, long long seen);  // fa_tree.hip
 hipError_t tree_attention(const WindowParams& p, const WindowPlan& w, bool is_bf16, hipStream_t s);
@@ -1330,7 +1335,9 @@ WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int eb, int max
   const int dp = D <= 64 ? 64 : 128;
   const long long rows = (long long)max_n * G;
   const long long seen = window > 0 ? std::min(max_keys, (long long)window + max_n + sinks + 96) : max_keys;
-  if (rows <= (tree ? kRowTile : kNarrowRows)) {
+  const long long narrow_runs = std::min(std::max(512 / (long long)Hkv, 1LL), std::max(1LL, ((seen + 31) / 32 * B + 3) / 4));
+  if (tree && (rows > kRowTile || rows * (narrow_runs / B) > kTreeMerge[rows > 8])) return tree_plan(B, tokens, Hkv, G, dp, max_n, seen);
+  if (rows <= kNarrowRows) {
     w.columns = rows > kRowTile ? 2 : 1;
     const int rt = kRowTile * w.columns;
     w.part_rows = (int)std::min<long long>(rows, rt);
@@ -1350,7 +1357,6 @@ WindowPlan window_plan(int B, int tokens, int Hkv, int G, int D, int eb, int max
       w.part_bytes = LSFA_GEMV_COUNTER_BYTES + (uint64_t)tiles * 2 * w.runs * (w.long_run > 0 ? 4 : 1) * part_bytes;
     return w;
   }
-  if (tree) return tree_plan(B, tokens, Hkv, G, dp, max_n, seen);
   auto items = [&](int bm) {
     return Hkv * std::min((long long)tokens * G / bm + B, (rows + bm - 1) / bm * B);
   };
