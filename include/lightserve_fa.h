@@ -489,7 +489,8 @@ typedef struct {
  * candidates are above -inf the rest of the outputs are score -inf, beam 0, token 0.
  *   logits [batch * beams, cols] fp32/fp16/bf16, columns contiguous; scores fp32
  *   [batch, beams]; outputs [batch, num] (fp32, int32, int64); beams <=
- *   LSFA_BEAMS_MAX, num <= LSFA_BEAMS_NUM_MAX
+ *   LSFA_BEAMS_MAX, num <= LSFA_BEAMS_NUM_MAX, and at most 2560 chunks of 8192
+ *   logits of one sequence's beams
  *   workspace: lsfa_beam_workspace_size() bytes, as lsfa_accept_args */
 #define LSFA_BEAMS_MAX 64
 #define LSFA_BEAMS_NUM_MAX 64

@@ -1398,9 +1398,9 @@ static int check_beam(const lsfa_beam_args* a) {
   if (rc) return rc;
   if (rows == 0) return LSFA_OK;
   if (a->batch > LSFA_GEMV_COUNTER_BYTES / 4) return fail(LSFA_ERR_UNSUPPORTED, "more than 65536 sequences (batch=%d)", a->batch);
-  // (the lists that meet lie in LDS)
-  if ((long long)a->beams * lsfa::select_plan(rows, a->cols, a->dtype, true).chunks > 2048)
-    return fail(LSFA_ERR_UNSUPPORTED, "more than 2048 chunks of one sequence's rows (beams=%d cols=%d)", a->beams, a->cols);
+  // (what is known of the lists that meet lies in LDS, 20 bytes of each)
+  if ((long long)a->beams * lsfa::select_plan(rows, a->cols, a->dtype, true).chunks > 2560)
+    return fail(LSFA_ERR_UNSUPPORTED, "more than 2560 chunks of one sequence's rows (beams=%d cols=%d)", a->beams, a->cols);
   if (!a->scores || !a->out_scores || !a->out_beams || !a->out_tokens)
     return fail(LSFA_ERR_INVALID, "scores and the outputs must be non-NULL");
   return LSFA_OK;

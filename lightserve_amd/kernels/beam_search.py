@@ -13,8 +13,8 @@ and tokens int64 (the v), all [batch, num]. Equal ones go to the lower k, then t
 computed and candidates are compared in 64 bits (sums of different beams are often nearer to each other than 32 bits
 tell), the scores rounded once. A row of logits with NaN or +inf, or nothing above -inf, offers no candidates, nor
 does a beam with a score of NaN or -inf; where fewer than num candidates are above -inf, the rest have score -inf, beam 0
-and token 0. Up to 64 beams, 64 candidates and 2^20 tokens of a vocabulary, and 2048 chunks of 8192 tokens (4096 in fp32) of one
-sequence's beams.
+and token 0. Up to 64 beams, 64 candidates and 2^20 tokens of a vocabulary, and 2560 chunks of 8192 tokens of one
+sequence's beams (64 of 2^18 tokens, 19 of 2^20).
 
 kv_cache_reorder lets beam k of sequence b go on from beam parents[b, k] (int32 [batch, K]; any other number: from itself). Beams b * K ..
 b * K + K - 1 are the sequence's rows of block_tables int32 [batch * K, max_blocks] and seq_lens int32 [batch * K]; they have one length, which the

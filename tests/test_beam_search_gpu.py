@@ -58,6 +58,24 @@ def test_select_many_beams(gpu, dtype):
     _select(_logits(200, 60, dtype, 4), _scores(100, 2, 4), 4, "100 sequences")
 
 
+def test_select_the_most_chunks(gpu):
+    """64 beams of a vocabulary of 2^18, most of it masked: the largest number of chunks that one sequence's beams have."""
+    print("case select most", flush=True)
+    x = torch.full((64, 2 ** 18), -math.inf, dtype=torch.bfloat16)
+    at = torch.randint(0, 2 ** 18, (64, 40), generator=torch.Generator().manual_seed(9))
+    x.scatter_(1, at, _logits(64, 40, torch.bfloat16, 10, 1.0))
+    x[:, -1] = 3.0
+    scores = torch.full((1, 64), -10.0) - torch.arange(64) / 8
+    got = beam_search_select(x.cuda(), scores.cuda(), 64)
+    # (the oracle's definition on the few finite logits)
+    keep = [(float(scores[0, k]) + (x[k, v].double().item() - x[k].double().logsumexp(0).item()), k, v)
+            for k in range(64) for v in sorted(set(at[k].tolist() + [2 ** 18 - 1]))]
+    want = sorted(keep, key=lambda c: (-c[0], c[1], c[2]))[:64]
+    gaps = [a[0] - b[0] for a, b in zip(want, want[1:]) if a[1] != b[1]]
+    assert min(gaps) > 1e-6
+    assert got[1][0].tolist() == [w[1] for w in want] and got[2][0].tolist() == [w[2] for w in want]
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_select_ties(gpu, dtype):
     """Equal candidates go to the lower beam, then the lower token: equal logits, equal beams, and both."""
