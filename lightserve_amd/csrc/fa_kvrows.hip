@@ -12,7 +12,9 @@
 //            own one. A thread reads its column of one row of that block for all beams before it
 //            writes any, so that parents may be permuted at will.
 //
-// Both are bound by HBM, or for few rows by the chain of their loads (index, table entry, row).
+// Both are bound by HBM (half of 2500..4001 rows of 7 sequences in 4 layers of 8 bits 37 us, a copy's rate; the last
+// blocks of 8-bit beams, rows of 128 bytes, 117 us, 4.1 TB/s), or for few rows by the chain of their loads (index, table
+// entry, row; 3.6 us in 32 layers).
 #include "fa_common.hpp"
 
 #include <algorithm>
