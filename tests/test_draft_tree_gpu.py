@@ -459,6 +459,16 @@ def test_keep_many(gpu, kind, n, kept):
     _keep(kind, double, [kept, 10], [kept, 10], [kept + 5, 20], 16, 2, 64, 4, what="the same row twice")
 
 
+def test_keep_wide_launches(gpu):
+    """Many layers (a wave by itself goes through long lists), and few (16 waves together, at both widths of columns)."""
+    print("case keep launches", flush=True)
+    g = torch.Generator().manual_seed(2)
+    for layers, sequences, n, kept in ((300, 2, 90, 60), (2, 1, 90, 60), (1, 2, 1200, 600), (2, 1, 600, 513)):
+        keep = torch.stack([torch.randperm(n, generator=g)[:kept].sort().values for _ in range(sequences)]).int()
+        _keep(torch.bfloat16, keep, [kept] * sequences, [kept + 5] * sequences, [n + 9] * sequences, 16, 2, 64, 7, layers=layers,
+              what=f"{layers} layers, {kept} of {n}")
+
+
 def test_keep_outside(gpu):
     """Rows that the table, the cache or the sequence does not have are not moved; counts past the width are held to it."""
     print("case keep outside", flush=True)
