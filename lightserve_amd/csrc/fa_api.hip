@@ -1321,8 +1321,8 @@ static int check_logits(const void* logits, int64_t stride, int dtype, long long
   if (stride < cols) return fail(LSFA_ERR_INVALID, "logits_stride must be >= cols");
   if ((reinterpret_cast<uintptr_t>(logits) & (dtype == LSFA_DTYPE_FP32 ? 3u : 1u)) != 0)
     return fail(LSFA_ERR_INVALID, "logits are not aligned to their type");
-  if (rows > (1 << 20) || cols > (1 << 20) || rows * lsfa::select_plan(rows, cols, dtype, beams).chunks >= (1LL << 23))
-    return fail(LSFA_ERR_UNSUPPORTED, "more than 2^20 rows or columns, or 2^23 chunks of rows (rows=%lld cols=%d)", rows, cols);
+  if (rows > (1 << 20) || cols > (1 << 20) || rows * lsfa::select_plan(rows, cols, dtype, beams).parts >= (1LL << 23))
+    return fail(LSFA_ERR_UNSUPPORTED, "more than 2^20 rows or columns, or 2^23 workgroups for them (rows=%lld cols=%d)", rows, cols);
   return LSFA_OK;
 }
 

@@ -8,8 +8,8 @@
 //   beams    The `num` best of s_k + x_kv - lse_k over a sequence's beams k and the vocabulary v, with
 //            lse_k = log sum_v exp x_kv; the first k V + v of equals.
 //
-// Both read each logit once (that and, for few rows, latency is what bounds them; 556 rows of 128256 in bf16 34 us, 4.1
-// TB/s, 8 of them 9.3; eight beams of 32 sequences over 50257 in fp32 27 us, 18 of them the reading): a workgroup takes a
+// Both read each logit once (that and, for few rows, latency is what bounds them; 556 rows of 128256 in bf16 29 us, 4.8
+// TB/s, 8 of them 10; eight beams of 32 sequences over 50257 in fp32 27 us, 18 of them the reading): a workgroup takes a
 // chunk of a row into registers and leaves the chunk's largest value, or its sorted `num`
 // largest with the chunk's maximum and sum of exponentials; the last workgroup of a sequence to
 // arrive does the rest. Values are compared as integers whose order is the floats' (the sign bit
@@ -573,13 +573,19 @@ static int chunks_of(int cols, int size, int U) {
 SelectPlan select_plan(long long rows, int cols, int dtype, bool beams) {
   const int size = dtype == 0 ? 4 : 2;
   SelectPlan s;
-  s.loads = beams && size == 4 ? 8 : 4;
+  // Beams: chunks of 8192 values (half of that 30.5 us for 28.3, 256 rows of 50257 in fp32, and 33.3 for 29.8 in bf16).
+  // Acceptance reads ahead: 4096 (2048 in fp32; 556 rows of 128256 29.3 us, with twice of that 31).
+  s.loads = !beams ? 2 : size == 4 ? 8 : 4;
   // Smaller chunks where there are few of them. (Not for the sake of more CUs: all that arrive at a sequence's counter wait
   // for one another, and their partial results for the last one. 512 chunks of 8 rows of 128256 12.7 us, 128 9.6; 252 of
   // four beams 16.4, 64 14.6.)
   while (s.loads > 1 && rows * chunks_of(cols, size, s.loads) < 64) s.loads /= 2;
   s.chunks = chunks_of(cols, size, s.loads);
-  s.per = beams ? 1 : (int)std::max(1LL, std::min<long long>(s.chunks, rows * s.chunks / 2048));
+  // Acceptance: as many chunks to a workgroup as leave 256 of them or one for each row. (556 rows of 128256 29.3 us; one
+  // chunk to a workgroup 76 us for 512 rows, 2048 workgroups 33, 256 27. 32 rows: 512 workgroups 13.7, 256 11.1.) Beams: one chunk,
+  // since the selection of a chunk has waits that only another workgroup fills (32 x 8 beams of 50257 in fp32: 28.3 us,
+  // several chunks with the best so far as a floor 31 at best).
+  s.per = beams ? 1 : (int)std::max(1LL, std::min<long long>(s.chunks, (rows * s.chunks + 255) / 256));
   s.parts = (s.chunks + s.per - 1) / s.per;
   return s;
 }
@@ -596,8 +602,7 @@ static void launch_beams(const BeamParams& p, hipStream_t s) {
 }
 template <typename T>
 static void by_loads(const AcceptParams& p, int loads, hipStream_t s) {
-  if (loads == 4) launch_accept<T, 4>(p, s);
-  else if (loads == 2) launch_accept<T, 2>(p, s);
+  if (loads == 2) launch_accept<T, 2>(p, s);
   else launch_accept<T, 1>(p, s);
 }
 template <typename T>
