@@ -151,8 +151,8 @@ __device__ __forceinline__ void nodes_of(const AcceptParams& p, int b, int& tok0
   n = min(max(min(p.cu[b + 1], p.rows) - tok0, 0), p.max_nodes);
 }
 
-// A workgroup takes p.per chunks of a row, one in flight while it looks at the one before, and leaves
-// the largest value and its index.
+// A workgroup takes p.per chunks of a row, the next one in flight while it looks at one, and leaves the
+// largest value and its index.
 template <typename T, int U>
 __global__ __launch_bounds__(kThreads) void fa_accept_kernel(const AcceptParams p) {
   using Ch = Chunk<T, U>;
@@ -200,17 +200,25 @@ __global__ __launch_bounds__(kThreads) void fa_accept_kernel(const AcceptParams 
 
     const int k0 = part * p.per, k1 = min(k0 + p.per, p.chunks);
     const int64_t row = tok0 + node;
-    Ch x, ahead;
-    x.load(p.logits, row, p.stride, p.cols, k0);
+    constexpr int AHEAD = 2;  // chunks in registers (three 34.5 us for 33.5, 556 rows of 128256 that no cache holds)
+    Ch ring[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (k0 + j < k1) ring[j].load(p.logits, row, p.stride, p.cols, k0 + j);
     float best = -INFINITY;  // the thread's, and the first chunk that has it
     int best_k = k0;
-    for (int k = k0; k < k1; ++k) {
-      if (k + 1 < k1) ahead.load(p.logits, row, p.stride, p.cols, k + 1);
-      x.cut();
-      const float m = x.largest();
-      if (m > best || (m != m && best == best)) best = m, best_k = k;
-      if (k + 1 < k1) x = ahead;
+    for (int k = k0; k < k1; k += AHEAD) {
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        if (k + j >= k1) break;
+        Ch& x = ring[j];
+        x.cut();
+        const float m = x.largest();
+        if (m > best || (m != m && best == best)) best = m, best_k = k + j;
+        if (k + j + AHEAD < k1) x.load(p.logits, row, p.stride, p.cols, k + j + AHEAD);
+      }
     }
+    Ch& x = ring[0];  // (a single chunk's still)
     // Of equal ones the lowest chunk, then the lowest position in it.
     auto same = [](float a, float b) -> bool { return a == b || (a != a && b != b); };
     const float wm = wave_max(best);
