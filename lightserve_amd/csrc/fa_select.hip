@@ -334,6 +334,10 @@ __device__ __forceinline__ uint32_t nth_of_threads(uint32_t key, int N, uint32_t
   return from;
 }
 
+// Most entries of a sequence's lists that its merging takes whole (eight beams of 128256, the best 16: 2048 entries 16.8 us,
+// in two steps 18.9; 16 x 16 of 32000, the best 32 26.0 and 30.2; 56 lists of 16 27.4 and 29.7).
+constexpr int kFew = 8 * kThreads;
+
 template <typename T, int U>
 __global__ __launch_bounds__(kThreads) void fa_beams_kernel(const BeamParams p) {
   using Ch = Chunk<T, U>;
@@ -428,15 +432,24 @@ __global__ __launch_bounds__(kThreads) void fa_beams_kernel(const BeamParams p) 
   if (!last_to_arrive(p.counters + counter_of(b, p.B), p.K * S, &st_last)) return;
 
   // The sequence's lists meet: K S of them, in the order of k V + v. What is read was written elsewhere and
-  // takes a microsecond to come: all of it is asked for at once, then the N lists with the best first entries.
+  // takes a microsecond to come: all of it is asked for at once, or of many entries the lists' first ones, then the N lists
+  // with the best of them.
   const int lists = p.K * S;
   const int64_t list0 = (int64_t)b * lists;
   double* sum = (double*)lds;                 // [lists]; then the scores of their first entries
   uint64_t* firsts = (uint64_t*)(sum + lists);  // [lists]
   float* lmax = (float*)(firsts + lists);     // [lists]
+  const int entries = lists * N;
+  const bool few = entries <= kFew;
+  uint64_t mine_of[kFew / kThreads];  // few: the thread's entries
+  if (few) {
+#pragma unroll
+    for (int u = 0; u < kFew / kThreads; ++u)
+      mine_of[u] = u * kThreads + tid < entries ? load_agent(p.lists + list0 * N + u * kThreads + tid) : 0;
+  }
   for (int t = tid; t < lists; t += kThreads) {
     const uint64_t m = load_agent(p.sums + 2 * (list0 + t)), l2 = load_agent(p.sums + 2 * (list0 + t) + 1);
-    firsts[t] = load_agent(p.lists + (list0 + t) * N);
+    if (!few) firsts[t] = load_agent(p.lists + (list0 + t) * N);
     lmax[t] = __uint_as_float((uint32_t)m);
     sum[t] = __longlong_as_double((long long)l2);
   }
@@ -466,32 +479,34 @@ __global__ __launch_bounds__(kThreads) void fa_beams_kernel(const BeamParams p) 
     const double sc = st_score[k] + ((double)value_of((uint32_t)(g >> 32)) - st_lse[k]);
     return g != 0 && sc > -(double)INFINITY ? sc : -(double)INFINITY;
   };
-  // The N best lie in the N lists with the best first entries, at or above the Nth of those. More than 64 lists are not
-  // all ranked: few are at or above the Nth largest, in 32 bits, of the threads' best ones (56 lists 28.3 us so and 29.7 in
-  // that way, 252 20.6 and 16.3).
+  // What is at or above the Nth largest, in 32 bits, of the threads' best candidates is ranked: the N best and few others.
+  double* cs = (double*)lds;                       // [entries or N * N] of those
+  int* ci = (int*)(cs + (few ? entries : N * N));  // k V + v
   float best = -INFINITY;
-  for (int t = tid; t < lists; t += kThreads) {
-    sum[t] = score(t / S, firsts[t]);
-    best = fmaxf(best, (float)sum[t]);
-  }
-  auto choose = [&](int t, double h, int rank) {
-    if (!(h > -(double)INFINITY)) return;
-    if (rank < N) st_chosen[rank] = t;
-    if (rank == N - 1) st_floor = h;
-  };
-  uint32_t low = 0;
-  if (lists <= 64) {
-    __syncthreads();
-    if (tid < lists) {
-      const double h = sum[tid];
-      int rank = 0;
-#pragma unroll 8
-      for (int j = 0; j < lists; ++j) rank += sum[j] > h || (sum[j] == h && j < tid);
-      choose(tid, h, rank);
+  if (few) {
+    double sc[kFew / kThreads];
+#pragma unroll
+    for (int u = 0; u < kFew / kThreads; ++u) {
+      sc[u] = mine_of[u] != 0 ? score((u * kThreads + tid) / N / S, mine_of[u]) : -(double)INFINITY;
+      best = fmaxf(best, (float)sc[u]);
     }
+    const uint32_t low = nth_of_threads(best > -INFINITY ? key_of(best) : 0u, N, st_key);
+#pragma unroll
+    for (int u = 0; u < kFew / kThreads; ++u) {
+      if (!(sc[u] > -(double)INFINITY) || key_of((float)sc[u]) < low) continue;
+      const int to = atomicAdd(&st_found, 1);
+      cs[to] = sc[u];
+      ci[to] = (u * kThreads + tid) / N / S * p.cols + index_of(mine_of[u]);
+    }
+    __syncthreads();
   } else {
-    low = nth_of_threads(best > -INFINITY ? key_of(best) : 0u, N, st_key);
-    double* ks = (double*)firsts;  // [lists]: the scores of those, and in lmax their numbers
+    // The N best lie in the N lists with the best first entries, at or above the Nth of those.
+    for (int t = tid; t < lists; t += kThreads) {
+      sum[t] = score(t / S, firsts[t]);
+      best = fmaxf(best, (float)sum[t]);
+    }
+    uint32_t low = nth_of_threads(best > -INFINITY ? key_of(best) : 0u, N, st_key);
+    double* ks = (double*)firsts;  // [lists]: the scores of those lists that may be, and in lmax their numbers
     int* kt = (int*)lmax;
     for (int t = tid; t < lists; t += kThreads) {
       const double h = sum[t];
@@ -508,48 +523,45 @@ __global__ __launch_bounds__(kThreads) void fa_beams_kernel(const BeamParams p) 
       int rank = 0;
 #pragma unroll 4
       for (int j = 0; j < kept; ++j) rank += ks[j] > h || (ks[j] == h && kt[j] < t);
-      choose(t, h, rank);
-    }
-  }
-  __syncthreads();
-  double* cs = (double*)lds;       // [N * N]
-  int* ci = (int*)(cs + N * N);    // k V + v
-  const double floor = st_floor;
-  best = -INFINITY;
-  for (int e0 = tid; e0 < N * N; e0 += 4 * kThreads) {
-    uint64_t g[4];
-    int of[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int e = e0 + u * kThreads;
-      of[u] = e < N * N ? st_chosen[e / N] : -1;
-      g[u] = of[u] >= 0 ? load_agent(p.lists + (list0 + of[u]) * N + e % N) : 0;
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int e = e0 + u * kThreads;
-      const double sc = g[u] != 0 ? score(of[u] / S, g[u]) : -(double)INFINITY;
-      if (e >= N * N) break;
-      cs[e] = sc >= floor ? sc : -(double)INFINITY;
-      ci[e] = of[u] / S * p.cols + index_of(g[u]);
-      best = fmaxf(best, (float)cs[e]);
-    }
-  }
-  // Those that are left, moved to the front: no more than have been read. Of more than 64 once more the few that can be
-  // among the N best: with values of 16 bits many are equal (N = 16 29.7 us for 41; N = 8 46.3 for 45.4 without).
-  low = 0;
-  if (N * N > 64) low = nth_of_threads(best > -INFINITY ? key_of(best) : 0u, N, st_key);
-  for (int e0 = 0; e0 < N * N; e0 += kThreads) {
-    const int e = e0 + tid;
-    const double sc = e < N * N ? cs[e] : -(double)INFINITY;
-    const int id = e < N * N ? ci[e] : 0;
-    __syncthreads();
-    if (sc > -(double)INFINITY && key_of((float)sc) >= low) {
-      const int to = atomicAdd(&st_found, 1);
-      cs[to] = sc;
-      ci[to] = id;
+      if (rank < N) st_chosen[rank] = t;
+      if (rank == N - 1) st_floor = h;
     }
     __syncthreads();
+    const double floor = st_floor;
+    best = -INFINITY;
+    for (int e0 = tid; e0 < N * N; e0 += 4 * kThreads) {
+      uint64_t g[4];
+      int of[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int e = e0 + u * kThreads;
+        of[u] = e < N * N ? st_chosen[e / N] : -1;
+        g[u] = of[u] >= 0 ? load_agent(p.lists + (list0 + of[u]) * N + e % N) : 0;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int e = e0 + u * kThreads;
+        const double sc = g[u] != 0 ? score(of[u] / S, g[u]) : -(double)INFINITY;
+        if (e >= N * N) break;
+        cs[e] = sc >= floor ? sc : -(double)INFINITY;
+        ci[e] = of[u] / S * p.cols + index_of(g[u]);
+        best = fmaxf(best, (float)cs[e]);
+      }
+    }
+    // Moved to the front: no more than have been read.
+    low = nth_of_threads(best > -INFINITY ? key_of(best) : 0u, N, st_key);
+    for (int e0 = 0; e0 < N * N; e0 += kThreads) {
+      const int e = e0 + tid;
+      const double sc = e < N * N ? cs[e] : -(double)INFINITY;
+      const int id = e < N * N ? ci[e] : 0;
+      __syncthreads();
+      if (sc > -(double)INFINITY && key_of((float)sc) >= low) {
+        const int to = atomicAdd(&st_found, 1);
+        cs[to] = sc;
+        ci[to] = id;
+      }
+      __syncthreads();
+    }
   }
   const int found = st_found;
   for (int i = tid; i < found; i += kThreads) {
@@ -605,7 +617,8 @@ static void launch_accept(const AcceptParams& p, hipStream_t s) {
 template <typename T, int U>
 static void launch_beams(const BeamParams& p, hipStream_t s) {
   const size_t lists = (size_t)p.K * p.chunks;
-  const size_t lds = std::max({(size_t)kThreads * 8, lists * 20, (size_t)p.num * p.num * 12});
+  const size_t lds = std::max({(size_t)kThreads * 8, lists * 20,
+                               12 * (lists * p.num <= (size_t)kFew ? lists * p.num : (size_t)p.num * p.num)});
   hipLaunchKernelGGL((fa_beams_kernel<T, U>), dim3((unsigned)(p.B * p.K * p.chunks)), dim3(kThreads), lds, s, p);
 }
 template <typename T>
