@@ -17,7 +17,8 @@ paged_tree_attention takes the arguments of paged_prefill (paged_attention.py): 
 keys with its n nodes, which are the last n. A node sees all keys before those, under a window the ones that a query
 at position seq_len - n + (nodes it sees) - 1 sees, and the nodes of its mask, whatever the window. Any mask does; a node that
 sees nothing gets o = 0 and lse = -inf. Sequences may have 0 to 256 nodes each; max_nodes bounds them (read from cu_seqlens_q
-when None, a device sync, so pass it under graph capture). 8- and 16-bit caches, bf16 and fp16, head dims that are multiples of
+when None, a device sync, so pass it under graph capture); o's rows behind the last sequence, and of nodes past max_nodes, are
+not written. 8- and 16-bit caches, bf16 and fp16, head dims that are multiples of
 16 (8 over 16-bit caches) up to 128, power-of-two block sizes of at least 16.
 
 accept_drafts takes the logits [total, vocab] (fp32, fp16 or bf16) and the tokens int64 [total] of all nodes. The path of a sequence begins at its
