@@ -661,7 +661,8 @@ typedef struct {
  * sees the tokens before them (of those, under a window, the ones that a query at
  * position seq_len - n + (drafts that it sees) - 1 sees) and the drafts j whose bit its
  * mask has, the window apart. window.cu_seqlens_q must be non-NULL;
- * window.causal is not read.
+ * window.causal is not read. seq_lens may pass what the block table (or max_seq_len)
+ * holds: the drafts stand where the length says, and keys that are not held are seen by none.
  *   tree_mask [tokens, mask_words] words of 64 bits, mask_stride words apart;
  *   bit j of the row: word j / 64, bit j % 64. Bits past the n drafts are not read. */
 typedef struct {

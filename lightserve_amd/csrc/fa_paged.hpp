@@ -18,29 +18,38 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w, float scale, _Float16) {
 
 // A sequence's keys, queries and first row of q, and its key tiles of 32: those
 // with sinks that its window's tiles do not hold, then the window's from `first` on.
+// Keys are those that the block table holds. Draft trees stand at the end of the length itself, which may
+// pass the table: there only what is read is held to it, not where the tree begins.
 struct KeyTiles {
-  int seq, n, tok0;
+  int len, seq, n, tok0;
   int sink, first;
   int count;         // all of them; 1 where queries see no key, 0 without queries
 };
-__device__ __forceinline__ KeyTiles key_tiles_of(const WindowParams& p, int seq, int n, int tok0) {
+__device__ __forceinline__ int table_keys(const WindowParams& p) { return min(p.max_seq_len, p.max_blocks << p.block_shift); }
+template <bool TREE>
+__device__ __forceinline__ KeyTiles key_tiles_of(const WindowParams& p, int len, int n, int tok0) {
   KeyTiles t;
-  t.seq = seq, t.n = n, t.tok0 = tok0;
+  t.seq = TREE ? min(len, table_keys(p)) : len;
+  t.len = len, t.n = n, t.tok0 = tok0;
   t.first = t.sink = 0;
   if (p.window > 0) {
-    t.first = max(seq - n - p.window + 1, 0) >> 5;
-    t.sink = min((min(p.sinks, seq) + 31) >> 5, t.first);
+    t.first = max(len - n - p.window + 1, 0);
+    if (TREE) t.first = min(t.first, t.seq);
+    t.first >>= 5;
+    t.sink = min((min(p.sinks, t.seq) + 31) >> 5, t.first);
   }
-  t.count = n > 0 ? max(t.sink + ((seq + 31) >> 5) - t.first, 1) : 0;
+  t.count = n > 0 ? max(t.sink + ((t.seq + 31) >> 5) - t.first, 1) : 0;
   return t;
 }
+template <bool TREE>
 __device__ __forceinline__ KeyTiles key_tiles(const WindowParams& p, int b) {
   int n = 1, tok0 = b;
   if (p.cu_q != nullptr) {  // (no row outside q, whatever the offsets)
     tok0 = min(max(p.cu_q[b], 0), p.tokens);
     n = max(min(p.cu_q[b + 1], p.tokens) - tok0, 0);
   }
-  return key_tiles_of(p, min(max(p.seq_lens[b], 0), min(p.max_seq_len, p.max_blocks << p.block_shift)), n, tok0);
+  const int len = max(p.seq_lens[b], 0);
+  return key_tiles_of<TREE>(p, TREE ? len : min(len, table_keys(p)), n, tok0);
 }
 
 // The kernel's arguments, read again. What only the beginning and the end of a run or item
@@ -82,7 +91,7 @@ __device__ __forceinline__ float bad_value(const uint32_t* w, int k) {
 }
 
 // Draft trees: bits at .. at + 31 of the mask of query `row`, of n drafts (bits at the number of
-// the tile's first key, which may lie before the drafts).
+// the tile's first key, which may lie before the drafts). Where keys are meant, n is the drafts that the table holds.
 template <typename P>
 __device__ __forceinline__ uint32_t draft_bits(const P& p, int64_t row, int n, int at) {
   const int i = at >> 5;

@@ -28,11 +28,11 @@
 
 namespace lsfa {
 
-// A sequence's keys, nodes and first row of q, and the key tiles that its items have: `sink` from key 0 on, then those from
-// tile `first` on (at least one in all, where it has nodes).
+// A sequence's length, keys that the block table holds, nodes and first row of q, and the key tiles that its items have: `sink`
+// from key 0 on, then those from tile `first` on (at least one in all, where it has nodes).
 template <int BM, int BN>
 struct TreeSequence {
-  int seq, n, tok0;
+  int len, seq, n, tok0;
   int items;  // row tiles times KV heads
   int sink, first, count;
 };
@@ -43,11 +43,12 @@ __device__ __forceinline__ TreeSequence<BM, BN> tree_sequence(const P& p, int b)
   t.n = min(max(min(p.cu_q[b + 1], p.tokens) - t.tok0, 0), p.max_n);
   // (nodes past max_n are left out at the end of the sequence's rows, not of its keys)
   const int n = max(min(p.cu_q[b + 1], p.tokens) - t.tok0, 0);
-  t.seq = min(max(p.seq_lens[b], 0), min(p.max_seq_len, p.max_blocks << p.block_shift));
+  t.len = max(p.seq_lens[b], 0);
+  t.seq = min(t.len, min(p.max_seq_len, p.max_blocks << p.block_shift));
   t.items = (int)(((int64_t)t.n * (p.Hq / p.Hkv) + BM - 1) / BM) * p.Hkv;
   t.first = t.sink = 0;
   if (p.window > 0) {
-    t.first = min(max(t.seq - n - p.window + 1, 0), t.seq) / BN;
+    t.first = min(max(t.len - n - p.window + 1, 0), t.seq) / BN;
     t.sink = min((min(p.sinks, t.seq) + BN - 1) / BN, t.first);
   }
   t.count = t.items > 0 ? max(t.sink + (t.seq + BN - 1) / BN - t.first, 1) : 0;
@@ -162,16 +163,18 @@ __global__ __launch_bounds__((NW * 64), (NW == 8 ? 1 : 2)) void fa_tree_kernel(c
     int rt, head;
     tree_item(v, sq.items, p.Hkv, b, rt, head);
     rt = __builtin_amdgcn_readfirstlane(rt), head = __builtin_amdgcn_readfirstlane(head);
-    const int G = p.Hq / p.Hkv, base = seq - n, nrows = min(n, p.max_n) * G;
+    const int len = __builtin_amdgcn_readfirstlane(sq.len);
+    const int G = p.Hq / p.Hkv, base = len - n, nrows = min(n, p.max_n) * G;
+    const int certain = min(base, seq), drafts = min(n, seq - base);  // keys before the drafts, and drafts, that are there
     const int window = p.window, sinks = window > 0 ? p.sinks : 0;
     const float sl2 = p.scale_abs;
 
-    // The lane's row: it sees keys lo .. base - 1 (and the sinks) and the drafts of its mask.
+    // The lane's row: it sees keys lo .. certain - 1 (and the sinks) and the drafts of its mask.
     const int r0 = rt * BM + wave * 32, r = r0 + l32, tok = r / G, hq = head * G + (r - tok * G);
     const bool row_ok = r < nrows, live = r0 < nrows;  // live: the wave has rows
     int lo = 0;
     if (window > 0) lo = (row_ok ? draft_position(p, tok0 + tok, n, base) : base) - window + 1;
-    const int lo_min = window > 0 ? base - window + 1 : 0, lo_max = window > 0 ? seq - window : 0;  // of any row
+    const int lo_min = window > 0 ? base - window + 1 : 0, lo_max = window > 0 ? len - window : 0;  // of any row
 
     u32x4 qraw[KSTEPS];  // the B operand of S^T: row l32, columns 16 kk + 8 hh .. + 7
 #pragma unroll
@@ -368,12 +371,12 @@ __global__ __launch_bounds__((NW * 64), (NW == 8 ? 1 : 2)) void fa_tree_kernel(c
             }
             __builtin_amdgcn_sched_barrier(0);
           }
-          if (!(key0 + BN <= base && (key0 >= lo_max || key0 + BN <= sinks))) {
+          if (!(key0 + BN <= certain && (key0 >= lo_max || key0 + BN <= sinks))) {
             asm volatile("" ::: "memory");  // stays a branch
-            const int up = row_ok ? base - key0 - 4 * hh : 0, dn = lo - key0 - 4 * hh, sk = sinks - key0 - 4 * hh;
+            const int up = row_ok ? certain - key0 - 4 * hh : 0, dn = lo - key0 - 4 * hh, sk = sinks - key0 - 4 * hh;
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
-              const uint32_t tree = row_ok ? draft_bits(p, tok0 + tok, n, key0 + 32 * kb - base) >> (4 * hh) : 0u;
+              const uint32_t tree = row_ok ? draft_bits(p, tok0 + tok, drafts, key0 + 32 * kb - base) >> (4 * hh) : 0u;
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
                 const int k = 32 * kb + 8 * (i >> 2) + (i & 3);
@@ -463,7 +466,7 @@ __global__ __launch_bounds__((NW * 64), (NW == 8 ? 1 : 2)) void fa_tree_kernel(c
               asm volatile("" : "+v"(d0), "+s"(most));
               const int key = key0 + __builtin_ctzll(left);
               const int blk = table[key >> block_shift];
-              const bool sees = row_ok && ((key < base && (key >= lo || key < sinks)) || (draft_bits(p, tok0 + tok, n, key - base) & 1));
+              const bool sees = row_ok && ((key < certain && (key >= lo || key < sinks)) || (draft_bits(p, tok0 + tok, drafts, key - base) & 1));
               if ((unsigned)blk >= (unsigned)num_blocks || !sees) continue;
               const C* from = (const C*)(vbase + (uint64_t)blk * vblock + (uint64_t)(key & ((1 << block_shift) - 1)) * vslot);
 #pragma unroll

@@ -147,10 +147,10 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
   // The runs' tiles, this run's, the sequence that holds its first one, and the number of
   // that sequence's first tile. (Up to 64 sequences lie in the lanes.)
   KeyTiles mine = {};
-  if (lane < p.B) mine = key_tiles(p, lane);
+  if (lane < p.B) mine = key_tiles<TREE>(p, lane);
   int upto = lanes_sum(mine.count), all = __builtin_amdgcn_readlane(upto, 63);
   for (int j = 64; j < p.B; j += 64) {
-    const int more = j + lane < p.B ? key_tiles(p, j + lane).count : 0;
+    const int more = j + lane < p.B ? key_tiles<TREE>(p, j + lane).count : 0;
     all += __builtin_amdgcn_readlane(lanes_sum(more), 63);
   }
   // Adjacent heads' rows of a token are adjacent in the cache: read by one workgroup
@@ -171,7 +171,7 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
   int b = 0, at = 0, have = mine.count;
   for (int j = 0; j < p.B; j += 64) {
     if (j > 0) {
-      have = j + lane < p.B ? key_tiles(p, j + lane).count : 0;
+      have = j + lane < p.B ? key_tiles<TREE>(p, j + lane).count : 0;
       upto = lanes_sum(have);
     }
     const unsigned long long hit = __ballot(at + upto > start);
@@ -207,14 +207,15 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
   for (; b < p.B && at < end; ++b) {
     KeyTiles kt;
     if (p.B <= 64) {
-      kt = key_tiles_of(p, __builtin_amdgcn_readlane(mine.seq, b), __builtin_amdgcn_readlane(mine.n, b),
+      kt = key_tiles_of<TREE>(p, __builtin_amdgcn_readlane(mine.len, b), __builtin_amdgcn_readlane(mine.n, b),
                         __builtin_amdgcn_readlane(mine.tok0, b));
     } else {
-      kt = key_tiles(p, b);
-      kt = key_tiles_of(p, __builtin_amdgcn_readfirstlane(kt.seq), __builtin_amdgcn_readfirstlane(kt.n),
+      kt = key_tiles<TREE>(p, b);
+      kt = key_tiles_of<TREE>(p, __builtin_amdgcn_readfirstlane(kt.len), __builtin_amdgcn_readfirstlane(kt.n),
                         __builtin_amdgcn_readfirstlane(kt.tok0));
     }
     const int count = kt.count, seq = kt.seq, n = kt.n, sink = kt.sink, first = kt.first, head0 = at;
+    const int base = kt.len - n;  // TREE: the first draft's key
     if (count == 0) continue;
     const int ta = max(start - at, 0), tb = min(count, end - at);
     at += count;
@@ -238,19 +239,20 @@ __global__ __launch_bounds__(256, 2) void fa_window_narrow_kernel(const WindowPa
     for (int x = 0; x < NC; ++x) {
       const bool row_ok = 16 * x + c < nrows;
       int pos = p.causal ? seq - n + (rt * RT + 16 * x + c) / G : seq - 1;
-      if constexpr (TREE) pos = row_ok && p.window > 0 ? draft_position(p, tok0 + (rt * RT + 16 * x + c) / G, n, seq - n) : 0;
-      hi[x] = row_ok ? (TREE ? seq - n - 1 : pos) : -1;  // (TREE: beside the drafts of its mask)
+      if constexpr (TREE) pos = row_ok && p.window > 0 ? draft_position(p, tok0 + (rt * RT + 16 * x + c) / G, n, base) : 0;
+      hi[x] = row_ok ? (TREE ? min(base, seq) - 1 : pos) : -1;  // (TREE: beside the drafts of its mask)
       lo[x] = p.window > 0 ? pos - p.window + 1 : 0;
     }
     // TREE: drafts that the lane's row of column block x sees among the 32 keys from key0 on.
     auto drafts = [&](int x, int key0) -> uint32_t {
-      return 16 * x + c < nrows ? draft_bits(p, tok0 + (rt * RT + 16 * x + c) / G, n, key0 - (seq - n)) : 0u;
+      return 16 * x + c < nrows ? draft_bits(p, tok0 + (rt * RT + 16 * x + c) / G, min(n, seq - base), key0 - base) : 0u;
     };
     // The same of the tile's first and last rows.
     const int t0 = rt * RT / G, t1 = (rt * RT + min(nrows, RT) - 1) / G;
-    const int hi_min = __builtin_amdgcn_readfirstlane(TREE ? seq - n - 1 : p.causal ? seq - n + t0 : seq - 1);
+    const int hi_min = __builtin_amdgcn_readfirstlane(TREE ? min(base, seq) - 1 : p.causal ? seq - n + t0 : seq - 1);
     const int hi_max = __builtin_amdgcn_readfirstlane(!TREE && p.causal ? seq - n + t1 : seq - 1);
-    const int lo_min = p.window > 0 ? hi_min + TREE - p.window + 1 : 0, lo_max = p.window > 0 ? hi_max - p.window + 1 : 0;
+    const int lo_min = p.window > 0 ? (TREE ? min(base - p.window + 1, seq) : hi_min - p.window + 1) : 0;
+    const int lo_max = p.window > 0 ? (TREE ? kt.len - 1 : hi_max) - p.window + 1 : 0;
 
     // Of the run's tiles ta .. tb - 1 of this sequence those that the row tile sees,
     // u = 0 .. nt - 1: n1 with sinks (numbered by their keys) from tile ta on, then
@@ -604,7 +606,7 @@ __global__ __launch_bounds__(256) void fa_window_combine_kernel(const WindowPara
   int all = 0, at = 0, tok0 = 0, count = 0, nrows = 0;  // tiles of all sequences, tiles before b's; b's
   for (int j = 0; j < p.B; j += 64) {
     KeyTiles mine = {};
-    if (j + lane < p.B) mine = key_tiles(p, j + lane);
+    if (j + lane < p.B) mine = p.tree != nullptr ? key_tiles<true>(p, j + lane) : key_tiles<false>(p, j + lane);
     const int upto = lanes_sum(mine.count);
     if (j <= b && b < j + 64) {
       at = all + __builtin_amdgcn_readlane(upto - mine.count, b - j);
@@ -674,7 +676,7 @@ __device__ __forceinline__ bool wide_item(const WindowParams& p, int item, int l
   const int G = p.Hq / p.Hkv;
   auto tiles_of = [&](const KeyTiles& t) -> int { return (int)(((int64_t)min(t.n, p.max_n) * G + BM - 1) / BM); };
   KeyTiles mine = {};
-  if (lane < p.B) mine = key_tiles(p, lane);
+  if (lane < p.B) mine = key_tiles<false>(p, lane);
   int tq = tiles_of(mine);
   bool found = false;
   if (p.B > 1 && p.B <= 64 && p.window == 0) {
@@ -695,7 +697,7 @@ __device__ __forceinline__ bool wide_item(const WindowParams& p, int item, int l
     for (int j = 0; j < p.B && !found; j += 64) {
       if (j > 0) {
         mine = {};
-        if (j + lane < p.B) mine = key_tiles(p, j + lane);
+        if (j + lane < p.B) mine = key_tiles<false>(p, j + lane);
         tq = tiles_of(mine);
       }
       const int upto = lanes_sum(tq);
@@ -711,7 +713,7 @@ __device__ __forceinline__ bool wide_item(const WindowParams& p, int item, int l
   }
   if (!found) return false;
   const int src = b & 63;
-  kt = key_tiles_of(p, __builtin_amdgcn_readlane(mine.seq, src), __builtin_amdgcn_readlane(mine.n, src),
+  kt = key_tiles_of<false>(p, __builtin_amdgcn_readlane(mine.len, src), __builtin_amdgcn_readlane(mine.n, src),
                     __builtin_amdgcn_readlane(mine.tok0, src));
   return true;
 }

@@ -16,7 +16,9 @@ tree_mask is int64 [total_q, words]: bit j of a row (word j // 64, bit j % 64) s
 paged_tree_attention takes the arguments of paged_prefill (paged_attention.py): seq_lens_k counts each sequence's cached
 keys with its n nodes, which are the last n. A node sees all keys before those, under a window the ones that a query
 at position seq_len - n + (nodes it sees) - 1 sees, and the nodes of its mask, whatever the window. Any mask does; a node that
-sees nothing gets o = 0 and lse = -inf. Sequences may have 0 to 256 nodes each; max_nodes bounds them (read from cu_seqlens_q
+sees nothing gets o = 0 and lse = -inf. A length may pass the block table, as where a tree is longer than what is left of a cache: the
+nodes stand where the length says, and nobody sees the rows that the table does not have, so that a node's o is right as long as its
+own row and its ancestors' are cached. Sequences may have 0 to 256 nodes each; max_nodes bounds them (read from cu_seqlens_q
 when None, a device sync, so pass it under graph capture); o's rows behind the last sequence, and of nodes past max_nodes, are
 not written. 8- and 16-bit caches, bf16 and fp16, head dims that are multiples of
 16 (8 over 16-bit caches) up to 128, power-of-two block sizes of at least 16.

@@ -24,7 +24,8 @@ def _place(table, num_blocks, bs, b, pos):
 
 
 def tree_reference(q, k, v, table, cu, seq_lens, mask, window=None, sinks=0, sm_scale=None):
-    """q [T, Hq, D], caches float64 [blocks, bs, Hkv, D] -> o, lse [T, Hq], sum w |v|, the largest sum |q k| |scale|, and sum |v|."""
+    """q [T, Hq, D], caches float64 [blocks, bs, Hkv, D] -> o, lse [T, Hq], sum w |v|, the largest sum |q k| |scale|, and sum |v|.
+    Nobody sees what lies past the table."""
     T, hq, d = q.shape
     n_blocks, bs, hkv, _ = k.shape
     scale = 1 / math.sqrt(d) if sm_scale is None else sm_scale
@@ -32,7 +33,7 @@ def tree_reference(q, k, v, table, cu, seq_lens, mask, window=None, sinks=0, sm_
     lse, big = torch.full((T, hq), -math.inf, dtype=torch.double), torch.zeros(T, hq, dtype=torch.double)
     for b, length in enumerate(int(x) for x in seq_lens):
         t0, n = int(cu[b]), int(cu[b + 1] - cu[b])
-        base = length - n
+        base, held = length - n, min(length, table.shape[1] * bs)
         rows = torch.zeros(max(length, 1), 2, hkv, d, dtype=torch.double)  # what no block holds reads as zeros
         for j in range(length):
             at = _place(table, n_blocks, bs, b, j)
@@ -43,6 +44,7 @@ def tree_reference(q, k, v, table, cu, seq_lens, mask, window=None, sinks=0, sm_
             pos = base + max(bin(m).count("1"), 1) - 1
             sees = [j for j in range(max(base, 0)) if window is None or j > pos - window or j < sinks]
             sees += [base + j for j in range(n) if m >> j & 1 and base + j >= 0]
+            sees = [j for j in sees if j < held]
             if not sees:
                 continue
             kk, vv = rows[sees, 0].repeat_interleave(hq // hkv, 1), rows[sees, 1].repeat_interleave(hq // hkv, 1)
