@@ -27,7 +27,8 @@ accept_drafts takes the logits [total, vocab] (fp32, fp16 or bf16) and the token
 node 0 and goes on, from node i, to the lowest node j > i that sees what i sees and itself and whose token is i's greedy
 choice (greedy_next_token's: NaN above all, ties to the lower index). It returns path int32 [batch, max_nodes] (-1
 behind the path), counts int32 [batch] and next_tokens int64 [batch], the choice after the path's last node. A sequence without
-nodes has count 0 and next token -1. seq_lens, when given, grows by counts in the same launch.
+nodes has count 0 and next token -1. A node whose mask is 0 follows no other: so drafts whose rows the cache does not hold, whose logits mean
+nothing, are kept off the paths. seq_lens, when given, grows by counts in the same launch.
 
 kv_cache_keep moves rows inside the cache: row start + keep[b, i] becomes row start + i for i < counts[b], start = seq_lens[b] -
 counts[b] (seq_lens counts what is cached once the rows are kept, as accept_drafts leaves it; counts are held to 0 .. keep's width). Entries with keep[b, i] <= i stay where they

@@ -191,7 +191,8 @@ class KVCacheDecoder:
     def draft_step(self, tokens, tree_mask, depth):
         """Logits [B * n, vocab] of trees of n nodes: tokens int64 [B, n], tree_mask int64 [B * n, words] and depth int32 [B, n]
         (draft_tree.py; node 0 is the current token). Appends their K/V behind the cached rows and leaves seq_lens as
-        it is: accept() says which of them stay. Rows past the block table are not stored."""
+        it is: accept() says which of them stay. Rows past the block table are not stored; their nodes' logits mean nothing, and
+        accept() takes none of them."""
         B, n = tokens.shape
         assert B == self.B and depth.shape == (B, n), "tokens and depth must be [batch, nodes]"
         pos = self.seq_lens.view(B, 1)
@@ -211,8 +212,11 @@ class KVCacheDecoder:
 
     def accept(self, logits, tokens, tree_mask):
         """What accept_drafts returns for draft_step's logits; the path's rows become the sequence's last, seq_lens grows by
-        them and the choice after them is the next current token."""
+        them and the choice after them is the next current token. Drafts at or past max_seq_len are not accepted: a path ends
+        where the cache does."""
         B, n = tokens.shape
+        fits = self.seq_lens.view(B, 1) + torch.arange(n, device=tokens.device, dtype=torch.int32) < self.cfg.max_seq_len
+        tree_mask = torch.where(fits.view(-1, 1), tree_mask, 0)  # (a node that sees nothing is no node's child)
         cu = torch.arange(0, (B + 1) * n, n, device=tokens.device, dtype=torch.int32)
         path, counts, following = accept_drafts(logits, tokens.reshape(-1), tree_mask, cu, max_nodes=n, seq_lens=self.seq_lens)
         kv_cache_keep(*self.caches[:2], self.block_tables, self.seq_lens, path, counts, kv_scales=self.caches[2])
