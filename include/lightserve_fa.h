@@ -660,7 +660,8 @@ typedef struct {
  * queries are the sequence's last n cached tokens, n <= LSFA_TREE_MAX_NODES. Query i
  * sees the tokens before them (of those, under a window, the ones that a query at
  * position seq_len - n + (drafts that it sees) - 1 sees) and the drafts j whose bit its
- * mask has, the window apart. window.cu_seqlens_q must be non-NULL;
+ * mask has, the window apart (in a tree as deep as the window a node sees ancestors
+ * that a token by itself would not). window.cu_seqlens_q must be non-NULL;
  * window.causal is not read. seq_lens may pass what the block table (or max_seq_len)
  * holds: the drafts stand where the length says, and keys that are not held are seen by none.
  *   tree_mask [tokens, mask_words] words of 64 bits, mask_stride words apart;

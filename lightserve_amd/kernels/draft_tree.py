@@ -15,7 +15,8 @@ or apply_rope_ store a chunk's), at the rotary positions of their depth, and the
 tree_mask is int64 [total_q, words]: bit j of a row (word j // 64, bit j % 64) says that the node sees node j of its sequence.
 paged_tree_attention takes the arguments of paged_prefill (paged_attention.py): seq_lens_k counts each sequence's cached
 keys with its n nodes, which are the last n. A node sees all keys before those, under a window the ones that a query
-at position seq_len - n + (nodes it sees) - 1 sees, and the nodes of its mask, whatever the window. Any mask does; a node that
+at position seq_len - n + (nodes it sees) - 1 sees, and the nodes of its mask, whatever the window: a tree less deep than the window is
+what its tokens are one by one, while in a deeper one nodes see ancestors that a single token's window would leave out. Any mask does; a node that
 sees nothing gets o = 0 and lse = -inf. A length may pass the block table, as where a tree is longer than what is left of a cache: the
 nodes stand where the length says, and nobody sees the rows that the table does not have, so that a node's o is right as long as its
 own row and its ancestors' are cached. Sequences may have 0 to 256 nodes each; max_nodes bounds them (read from cu_seqlens_q

@@ -21,13 +21,16 @@ BUCKETS = 1 << 16  # of LookupDrafts' index: pairs of tokens that fall together 
 
 class LookupDrafts:
     """Greedy decoding with drafts from the text itself: the continuations of the `branches` latest earlier places where its
-    last two tokens stand. Where there are fewer, any other draft costs its rows of the step and nothing else.
+    last two tokens stand. Where there are fewer, any other draft costs its rows of the step and nothing else. Under a window
+    drafts must be fewer than its tokens (KVCacheDecoder.draft_step).
 
     text int64 [B, max_seq_len + 1]: each sequence's tokens, the current one last, at seq_lens (the last column is scratch, and
     so is what follows once the cache is full)."""
 
     def __init__(self, dec, drafts, branches=1):
         assert drafts >= 1 and branches >= 1, "at least one draft"
+        window = dec.attention["window"]
+        assert window is None or drafts < window, f"drafts must be fewer than the window's tokens ({drafts} of {window})"
         self.dec, self.drafts, self.branches = dec, drafts, branches
         self.n = 1 + drafts * branches
         # node 0, then one chain after another, each from node 0 on
@@ -84,7 +87,7 @@ class LookupDrafts:
     def step(self):
         dec, last = self.dec, self._last()
         tokens = self.propose()
-        path, counts, following = dec.accept(dec.draft_step(tokens, self.mask, self.depth), tokens, self.mask)
+        path, counts, following = dec.accept(dec.draft_step(tokens, self.mask, self.depth, self.drafts), tokens, self.mask)
         # the path's tokens after node 0, then the choice after them, go behind the current token
         i, counts = torch.arange(self.n, device=tokens.device), counts.view(-1, 1)
         taken = tokens.gather(1, path.roll(-1, 1).clamp(min=0).long())

@@ -188,13 +188,18 @@ class KVCacheDecoder:
         # the slot of a K/V row is the one its block table gives for the position
         return self._rows(self.tokens, self.seq_lens, lens, None, attend, block_tables=self.block_tables)
 
-    def draft_step(self, tokens, tree_mask, depth):
+    def draft_step(self, tokens, tree_mask, depth, deepest=None):
         """Logits [B * n, vocab] of trees of n nodes: tokens int64 [B, n], tree_mask int64 [B * n, words] and depth int32 [B, n]
         (draft_tree.py; node 0 is the current token). Appends their K/V behind the cached rows and leaves seq_lens as
         it is: accept() says which of them stay. Rows past the block table are not stored; their nodes' logits mean nothing, and
-        accept() takes none of them."""
+        accept() takes none of them.
+
+        deepest (default: a chain's, n - 1) is at least the largest depth. Under a window it must be below the window: a node sees
+        all of its ancestors, where a token by itself would not see those a window back."""
         B, n = tokens.shape
         assert B == self.B and depth.shape == (B, n), "tokens and depth must be [batch, nodes]"
+        deepest, window = n - 1 if deepest is None else deepest, self.attention["window"]
+        assert window is None or deepest < window, f"a tree must be less deep than the window ({deepest} of {window})"
         pos = self.seq_lens.view(B, 1)
         rows = torch.arange(n, device=pos.device)
         lens = self.seq_lens + n
@@ -436,6 +441,8 @@ def main(argv=None):
         ap.error("give one of --prefill, --drafts and --beams")
     if args.branches < 1 or args.drafts * args.branches > MAX_NODES - 1:
         ap.error(f"--branches must be positive, and --drafts times it at most {MAX_NODES - 1}")
+    if args.window is not None and args.drafts >= args.window > 0:
+        ap.error("--drafts must be below --window")
     if args.beams > MAX_BEAMS:
         ap.error(f"--beams takes at most {MAX_BEAMS}")
     assert torch.cuda.is_available(), "needs a GPU"

@@ -126,3 +126,25 @@ def test_lookup_drafts_to_the_end(gpu, kv_e4m3, drafts, branches):
             short = exact[p - 1].max() - exact[p - 1, eager.text[b, p]]
             assert short <= 2 * bound[p - 1], (b, p, short, bound[p - 1])
     assert all(torch.equal(raw(f.contiguous()), w) for f, w in zip(fences, had)), "blocks of no table were written"
+
+
+@pytest.mark.parametrize("drafts,branches,window,sinks", [(3, 2, 4, 0), (3, 5, 4, 2), (7, 1, 8, 1)])
+def test_lookup_drafts_under_a_short_window(gpu, drafts, branches, window, sinks):
+    """As many drafts as a window allows: the tokens are the windowed choices."""
+    print(f"case lookup window={window} drafts={drafts}", flush=True)
+    config, weights = _model()
+    loop = LookupDrafts(KVCacheDecoder(weights, config, 2, window=window, sinks=sinks), drafts, branches)
+    prompt = torch.randint(0, config.vocab_size, (2, 6), generator=torch.Generator().manual_seed(5)).repeat(1, 4).cuda()
+    loop.start(prompt, 16)
+    for _ in range(12):
+        loop.step()
+    lens = loop.dec.seq_lens.tolist()
+    for b in range(2):
+        ids = loop.text[b:b + 1, :lens[b]]
+        held = [tuple(c.unsqueeze(0) for c in layer) for layer in _held(loop.dec, b, lens[b])]
+        exact = windowed_llama_forward(weights, config, ids, window, sinks, held)[0]
+        plain = windowed_llama_forward(weights, config, ids)[0]
+        bound = 2 * (reference_llama_forward(weights, config, ids).double().cpu()[0] - plain).abs().amax(-1)
+        for p in range(24, lens[b]):
+            short = exact[p - 1].max() - exact[p - 1, loop.text[b, p]]
+            assert short <= 2 * bound[p - 1], (b, p, short, bound[p - 1])

@@ -1,8 +1,14 @@
 """Decoding with several candidates per sequence where a cache ends, on the CPU: the oracle, and checks of calls that reach past
 what a cache or a launch has."""
+from types import SimpleNamespace
+
+import pytest
 import torch
 
 from lightserve_amd.kernels.draft_tree import draft_tree
+from lightserve_amd.model.candidates import LookupDrafts
+from lightserve_amd.model.graph_decode import KVCacheDecoder, main
+from lightserve_amd.model.minimal_llama import TOY_CONFIG
 from oracle import candidates, paged8
 from tests.paged8_cases import tables
 
@@ -20,3 +26,39 @@ def test_oracle_tree_past_the_table():
         length = min(had + i + 1, end)
         want = paged8.window_reference(q[i:i + 1], k, v, table, torch.tensor([0, 1], dtype=torch.int32), [length], None, 0)
         assert torch.allclose(o[i], want[0][0], atol=1e-12) and torch.allclose(lse[i], want[1][0], atol=1e-12), i
+
+
+def _decoder(window, sinks=0):
+    return KVCacheDecoder(SimpleNamespace(layers=[None]), TOY_CONFIG, 2, device="cpu", window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("window,sinks", [(4, 0), (4, 2)])
+def test_oracle_tree_under_a_window(window, sinks):
+    """Nodes less deep than the window are one-token steps; deeper ones see all of their ancestors, and are not."""
+    n, had = 9, 30
+    table, pool = tables([had + n], 16, 1)
+    g = torch.Generator().manual_seed(2)
+    k, v = (torch.randn(pool, 16, 2, 8, generator=g).double() for _ in range(2))
+    q = torch.randn(n, 4, 8, generator=g)
+    o = candidates.tree_reference(q, k, v, table, [0, n], [had + n], draft_tree(range(-1, n - 1))[0], window, sinks)[0]
+    want = paged8.window_reference(q, k, v, table, torch.tensor([0, n], dtype=torch.int32), [had + n], window, sinks)[0]
+    same = [torch.allclose(o[i], want[i], atol=1e-12) for i in range(n)]
+    assert same == [i < window for i in range(n)]
+
+
+def test_refuses_trees_deeper_than_the_window():
+    for window in (1, 4):
+        with pytest.raises(AssertionError, match="window"):
+            LookupDrafts(_decoder(window), window, 2)
+    LookupDrafts(_decoder(4), 3, 20)
+    LookupDrafts(_decoder(None), 30)
+    dec = _decoder(4, 2)
+    step = (torch.zeros(2, 5, dtype=torch.long), torch.ones(10, 1, dtype=torch.int64), torch.zeros(2, 5, dtype=torch.int32))
+    for deepest in (None, 4, 100):
+        with pytest.raises(AssertionError, match="window"):
+            dec.draft_step(*step, deepest=deepest)
+    with pytest.raises(AttributeError):  # (past the checks: the decoder has no weights)
+        dec.draft_step(*step, deepest=3)
+    for words in (["--drafts", "4", "--window", "4"], ["--drafts", "9", "--window", "4", "--branches", "2"]):
+        with pytest.raises(SystemExit):
+            main(words)
