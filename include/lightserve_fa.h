@@ -483,8 +483,9 @@ typedef struct {
 
 /* Beam search's selection (no reference counterpart): the num best of
  * scores[b, k] + log_softmax(logits[b * beams + k])[v] over a sequence's beams k
- * and the vocabulary v, best first, the lower k * cols + v of equals. Ranked
- * in 64 bits. A row that holds NaN or +inf, or nothing above -inf, offers no
+ * and the vocabulary v, best first, the lower k * cols + v of equals. Scores are
+ * ranked in 64 bits; a row's log-sum, of 32-bit exponentials, is off by up to 2^-23.
+ * A row that holds NaN or +inf, or nothing above -inf, offers no
  * candidates, nor does a beam whose score is NaN or -inf; where fewer than num
  * candidates are above -inf the rest of the outputs are score -inf, beam 0, token 0.
  *   logits [batch * beams, cols] fp32/fp16/bf16, columns contiguous; scores fp32

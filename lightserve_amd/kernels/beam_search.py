@@ -9,9 +9,11 @@ candidates per sequence, each a row of its own in the block tables:
 beam_search_select takes the logits [batch * K, vocab] (fp32, fp16 or bf16) of a step and the beams' scores fp32 [batch, K] (sums of log
 probabilities; -inf for a beam that takes no part, as all but the first in a search's first step) and
 returns the num (default K) best of scores[b, k] + log_softmax(logits[b * K + k])[v] of each sequence, best first: scores fp32, beams int32 (the k)
-and tokens int64 (the v), all [batch, num]. Equal ones go to the lower k, then the lower v. The softmax is
-computed and candidates are compared in 64 bits (sums of different beams are often nearer to each other than 32 bits
-tell), the scores rounded once. A row of logits with NaN or +inf, or nothing above -inf, offers no candidates, nor
+and tokens int64 (the v), all [batch, num]. Equal ones go to the lower k, then the lower v. Sums and scores are held and
+compared in 64 bits (sums of different beams are often nearer to each other than 32 bits tell) and rounded once at the end; the
+exponentials are 32-bit ones, so that a beam's log-sum is off by up to 2^-23 and candidates of different beams that are nearer
+than 2^-22 may stand either way. (So may different logits of one beam whose sums 64 bits round to one number, as beside
+a score of -1e30.) A row of logits with NaN or +inf, or nothing above -inf, offers no candidates, nor
 does a beam with a score of NaN or -inf; where fewer than num candidates are above -inf, the rest have score -inf, beam 0
 and token 0. Up to 64 beams, 64 candidates and 2^20 tokens of a vocabulary, and 2560 chunks of 8192 tokens of one
 sequence's beams (64 of 2^18 tokens, 19 of 2^20).
