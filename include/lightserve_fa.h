@@ -453,7 +453,8 @@ typedef struct {
  * tree_mask (at most max_nodes <= LSFA_TREE_MAX_NODES of them), bit j of a
  * node's mask saying that it sees node j of its sequence. a_i is the argmax
  * of node i's logits (as lsfa_greedy takes it). The path begins at node 0 and goes
- * from node i to the lowest j > i with mask_j = mask_i | bit j and token_j = a_i.
+ * from node i to the lowest j > i with mask_j = mask_i | bit j and token_j = a_i (bits
+ * past the sequence's nodes are not read).
  *   path int32 [batch, max_nodes]: its nodes, -1 behind them; counts int32
  *   [batch]; next_tokens int64 [batch]: a of the path's last node (a sequence
  *   without nodes: count 0, next token -1); seq_lens (optional) += counts

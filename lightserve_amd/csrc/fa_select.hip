@@ -248,11 +248,16 @@ __global__ __launch_bounds__(kThreads) void fa_accept_kernel(const AcceptParams 
       store_agent(p.part + row * p.parts + part, entry_of(top != top ? kKeyNan : key_of(top), x.first + st_at));
     if (!last_to_arrive(p.counters + counter_of(b, p.B), n * p.parts, &st_last)) continue;
 
-    const int words = p.mask_words;
+    // (bits past the sequence's nodes say nothing, as in the attention)
+    const int words = p.mask_words, nodes = min(p.cu[b + 1], p.rows) - tok0;
     for (int i = tid; i < n; i += kThreads) {
       st_best[i] = 0;
       st_token[i] = p.tokens[tok0 + i];
-      for (int w = 0; w < words; ++w) st_mask[i][w] = p.mask[(int64_t)(tok0 + i) * p.mask_stride + w];
+      for (int w = 0; w < words; ++w) {
+        const int bits = nodes - 64 * w;
+        const uint64_t m = p.mask[(int64_t)(tok0 + i) * p.mask_stride + w];
+        st_mask[i][w] = bits >= 64 ? m : bits > 0 ? m & ((1ull << bits) - 1) : 0;
+      }
     }
     __syncthreads();
     for (int t0 = 0; t0 < n * p.parts; t0 += 4 * kThreads) {

@@ -12,7 +12,8 @@ or apply_rope_ store a chunk's), at the rotary positions of their depth, and the
     path, counts, next_tokens = accept_drafts(logits, tokens, tree_mask, cu_seqlens, *, max_nodes=None, seq_lens=None)
     kv_cache_keep(k_cache, v_cache, block_tables, seq_lens, path, counts, *, kv_scales=None)
 
-tree_mask is int64 [total_q, words]: bit j of a row (word j // 64, bit j % 64) says that the node sees node j of its sequence.
+tree_mask is int64 [total_q, words]: bit j of a row (word j // 64, bit j % 64) says that the node sees node j of its sequence;
+bits past the sequence's nodes say nothing.
 paged_tree_attention takes the arguments of paged_prefill (paged_attention.py): seq_lens_k counts each sequence's cached
 keys with its n nodes, which are the last n. A node sees all keys before those, under a window the ones that a query
 at position seq_len - n + (nodes it sees) - 1 sees, and the nodes of its mask, whatever the window: a tree less deep than the window is

@@ -72,7 +72,8 @@ def accept_reference(logits, tokens, mask, cu, max_nodes):
     """path [B, max_nodes], counts [B], next tokens [B] (lists)."""
     paths, counts, following = [], [], []
     for b in range(len(cu) - 1):
-        t0, n = int(cu[b]), min(int(cu[b + 1] - cu[b]), max_nodes)
+        t0, nodes = int(cu[b]), int(cu[b + 1] - cu[b])
+        n, known = min(nodes, max_nodes), (1 << nodes) - 1  # (bits past the nodes say nothing)
         path, nxt = [], -1
         if n > 0:
             path = [0]
@@ -80,7 +81,7 @@ def accept_reference(logits, tokens, mask, cu, max_nodes):
                 cur = path[-1]
                 nxt = first_largest(logits[t0 + cur].double())
                 child = next((j for j in range(cur + 1, n) if int(tokens[t0 + j]) == nxt
-                              and bits_of(mask[t0 + j]) == bits_of(mask[t0 + cur]) | 1 << j), None)
+                              and bits_of(mask[t0 + j]) & known == bits_of(mask[t0 + cur]) & known | 1 << j), None)
                 if child is None:
                     break
                 path.append(child)

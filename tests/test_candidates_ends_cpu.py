@@ -62,3 +62,14 @@ def test_refuses_trees_deeper_than_the_window():
     for words in (["--drafts", "4", "--window", "4"], ["--drafts", "9", "--window", "4", "--branches", "2"]):
         with pytest.raises(SystemExit):
             main(words)
+
+
+def test_oracle_accept_reads_no_bits_past_the_nodes():
+    logits = torch.eye(4)[[2, 1, 3, 0, 2]]
+    mask, cu, tokens = draft_tree([-1, 0, 0, 2, 3])[0], torch.tensor([0, 5]), [0, 1, 2, 3, 0]
+    want = candidates.accept_reference(logits, tokens, mask, cu, 5)
+    assert want == ([[0, 2, 3, 4, -1]], [4], [2])
+    for bits in (1 << 5, 1 << 62, -1 << 5):
+        dirty = mask.clone()
+        dirty[::2] |= bits
+        assert candidates.accept_reference(logits, tokens, dirty, cu, 5) == want
