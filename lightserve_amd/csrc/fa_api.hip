@@ -812,7 +812,8 @@ static int check_window(const lsfa_window_args* a, bool tree = false) {
       (reinterpret_cast<uintptr_t>(a->kv_scales) & 7u) != 0)
     return fail(LSFA_ERR_UNSUPPORTED, "q, o, k_cache and v_cache must be 16-byte aligned, kv_scales 8-byte");
   const lsfa::WindowPlan w = plan_window(a, tree);
-  if ((long long)w.items * w.waves * 64 > (1LL << 32) - 1 || (long long)a->heads_kv * 256 > (1LL << 32) - 1)
+  // (a tree's merging launch has eight waves an item, whatever the first one has)
+  if ((long long)w.items * (tree ? 8 : w.waves) * 64 > (1LL << 32) - 1 || (long long)a->heads_kv * 256 > (1LL << 32) - 1)
     return fail(LSFA_ERR_UNSUPPORTED, "rows of q for 2^32 threads or more in one launch (%d tokens, %d heads_q)", a->tokens, a->heads_q);
   return LSFA_OK;
 }

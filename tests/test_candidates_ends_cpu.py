@@ -5,12 +5,14 @@ from types import SimpleNamespace
 import pytest
 import torch
 
+from lightserve_amd import _lib
 from lightserve_amd.kernels.draft_tree import draft_tree
 from lightserve_amd.model.candidates import LookupDrafts
 from lightserve_amd.model.graph_decode import KVCacheDecoder, main
 from lightserve_amd.model.minimal_llama import TOY_CONFIG
 from oracle import candidates, paged8
 from tests.paged8_cases import tables
+from tests.test_candidates_cpu import WINDOW, _set
 
 
 def test_oracle_tree_past_the_table():
@@ -73,3 +75,16 @@ def test_oracle_accept_reads_no_bits_past_the_nodes():
         dirty = mask.clone()
         dirty[::2] |= bits
         assert candidates.accept_reference(logits, tokens, dirty, cu, 5) == want
+
+
+def test_tree_check_counts_the_merging_launch(built_library):
+    """The launch that merges partial results has 512 threads for each row tile and KV head, more than the first one where two or
+    four waves take a tile: 2^23 of them are refused by the check, not by the launch."""
+    def check(heads_kv, nodes, **kw):
+        return _lib.tree_check(_set(_lib.TreeArgs, WINDOW, dict(
+            tree_mask=4096, mask_stride=1, mask_words=1, batch=65535, tokens=65535 * nodes, max_seqlen_q=nodes, heads_kv=heads_kv, heads_q=heads_kv,
+            max_seq_len=64, max_blocks_per_seq=4, workspace_bytes=1 << 60) | kw))
+    assert check(127, 20)[0] == 0
+    for heads_kv, nodes in ((129, 20), (129, 65), (400, 33)):
+        rc, msg = check(heads_kv, nodes, mask_words=2, mask_stride=2)
+        assert rc == -2 and "threads" in msg, (heads_kv, nodes, rc, msg)
