@@ -895,8 +895,12 @@ static int check_tree(const lsfa_tree_args* a) {
   if (rc) return rc;
   const lsfa::WindowPlan plan = plan_window(w, true);
   const long long all = ((long long)std::min<long long>(w->max_seq_len, (long long)w->max_blocks_per_seq * w->block_size) + 63) / 32;
-  if (plan.items > 0 && all * plan.items > (1LL << 30))
-    return fail(LSFA_ERR_UNSUPPORTED, "more than 2^30 key tiles of all sequences, row tiles and KV heads");
+  if (plan.items > 0) {
+    // (their numbers are 32-bit; offsets that are none may give every sequence max_seqlen_q rows, more than `items` counts)
+    const long long bm = 32 * plan.waves, tiles = ((long long)std::min(w->max_seqlen_q, w->tokens) * (w->heads_q / w->heads_kv) + bm - 1) / bm;
+    if (all * plan.items > (1LL << 30) || all * w->heads_kv * w->batch > ((1LL << 31) - 1) / tiles)
+      return fail(LSFA_ERR_UNSUPPORTED, "more than 2^30 key tiles of all sequences, row tiles and KV heads");
+  }
   if (!w->cu_seqlens_q) return fail(LSFA_ERR_INVALID, "a tree needs cu_seqlens_q");
   if (w->max_seqlen_q > LSFA_TREE_MAX_NODES)
     return fail(LSFA_ERR_UNSUPPORTED, "at most %d drafts of a sequence (max_seqlen_q=%d)", LSFA_TREE_MAX_NODES, w->max_seqlen_q);

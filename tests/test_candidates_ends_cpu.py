@@ -88,3 +88,16 @@ def test_tree_check_counts_the_merging_launch(built_library):
     for heads_kv, nodes in ((129, 20), (129, 65), (400, 33)):
         rc, msg = check(heads_kv, nodes, mask_words=2, mask_stride=2)
         assert rc == -2 and "threads" in msg, (heads_kv, nodes, rc, msg)
+
+
+def test_tree_check_counts_whatever_the_offsets(built_library):
+    """Offsets are the device's to read: with some that let sequences share rows, every one of 65535 may have 256 nodes, and the numbers
+    of their key tiles have to stay below 2^31."""
+    def check(tokens, batch, **kw):
+        return _lib.tree_check(_set(_lib.TreeArgs, WINDOW, dict(
+            tree_mask=4096, mask_stride=4, mask_words=4, batch=batch, tokens=tokens, max_seqlen_q=256, heads_kv=8, heads_q=256, max_seq_len=16384,
+            max_blocks_per_seq=1024, block_table_stride=1024, workspace_bytes=1 << 60) | kw))
+    rc, msg = check(256, 65535)
+    assert rc == -2 and "tiles" in msg
+    assert check(256, 4096)[0] == 0 and check(256 * 4096, 4096)[0] == 0
+    assert check(3, 65535)[0] == 0  # (three rows of q: no sequence has more)
