@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from lightserve_amd.kernels.draft_tree import draft_tree
-from lightserve_amd.model.candidates import LookupDrafts
+from lightserve_amd.model.candidates import BeamSearch, LookupDrafts
 from lightserve_amd.model.graph_decode import KVCacheDecoder, capture
 from oracle import candidates
 from oracle.model import reference_llama_forward, windowed_llama_forward
@@ -148,3 +148,33 @@ def test_lookup_drafts_under_a_short_window(gpu, drafts, branches, window, sinks
         for p in range(24, lens[b]):
             short = exact[p - 1].max() - exact[p - 1, loop.text[b, p]]
             assert short <= 2 * bound[p - 1], (b, p, short, bound[p - 1])
+
+
+@pytest.mark.parametrize("kv_e4m3", [False, True])
+def test_beam_search_to_the_end(gpu, kv_e4m3):
+    """Beams that fill the cache to its last row have the sums of their tokens' log probabilities as scores (bounds as in
+    test_candidate_decoding_gpu.py), and steps past it write nothing outside the cache."""
+    print(f"case beams to the end e4m3={kv_e4m3}", flush=True)
+    config, weights = _model()
+    sequences, beams, P, end = 2, 3, 45, config.max_seq_len
+    loop = BeamSearch(KVCacheDecoder(weights, config, sequences * beams, kv_e4m3=kv_e4m3), beams)
+    fences, had = _fenced(loop.dec)
+    prompt = torch.randint(0, config.vocab_size, (sequences, P), generator=torch.Generator().manual_seed(6)).cuda()
+    loop.start(prompt, 16)
+    for _ in range(end - P):
+        loop.step()
+    assert loop.dec.seq_lens.tolist() == [end] * (sequences * beams)
+    for b in range(sequences):
+        for k in range(beams):
+            ids = loop.text[b, k, :end].view(1, -1)
+            held = [tuple(c.unsqueeze(0) for c in layer) for layer in _held(loop.dec, b * beams + k, end)]
+            plain = windowed_llama_forward(weights, config, ids)
+            bound = 4 * (reference_llama_forward(weights, config, ids).double().cpu() - plain)[0, P - 1:].abs().amax(-1).sum().item()
+            p = windowed_llama_forward(weights, config, ids, None, 0, held).double().log_softmax(-1)[0, P - 1:]
+            off = abs(p.gather(1, loop.text[b, k, P:end + 1].cpu().view(-1, 1)).sum().item() - loop.scores[b, k].item())
+            print(f"[beams] {b} {k}: {off:.3f} of {bound:.3f}", flush=True)
+            assert off <= bound
+    for _ in range(4):
+        loop.step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(raw(f.contiguous()), w) for f, w in zip(fences, had)), "blocks of no table were written"
