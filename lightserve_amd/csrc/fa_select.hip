@@ -9,7 +9,7 @@
 //            lse_k = log sum_v exp x_kv; the first k V + v of equals.
 //
 // Both read each logit once (that and, for few rows, latency is what bounds them; 556 rows of 128256 in bf16 29 us, 4.8
-// TB/s, 8 of them 10; eight beams of 32 sequences over 50257 in fp32 27 us, 18 of them the reading): a workgroup takes a
+// TB/s, 8 of them 10; eight beams of 32 sequences over 50257 in fp32 28 us, some 20 of them the chunks): a workgroup takes a
 // chunk of a row into registers and leaves the chunk's largest value, or its sorted `num`
 // largest with the chunk's maximum and sum of exponentials; the last workgroup of a sequence to
 // arrive does the rest. Values are compared as integers whose order is the floats' (the sign bit

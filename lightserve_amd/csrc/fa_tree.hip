@@ -17,8 +17,8 @@
 //              inside an item or hold several: workgroups end together whatever the lengths. An
 //              item in several runs leaves fp32 partial results that a second launch merges.
 //
-// 32 query heads over 8 KV heads of 128: 16 trees of up to 16 nodes after 1024..8192 keys of 16 bits 70 us, bound
-// by memory (4.1 TB/s with the merging); 16 of 64 nodes over 8 bits 116, where products, softmax, conversions and
+// 32 query heads over 8 KV heads of 128: 16 trees of up to 16 nodes after 512..8192 keys of 16 bits 70 us, bound
+// by memory (4.1 TB/s with the merging); 16 of 64 nodes after 1024..8192 of 8 bits 117, where products, softmax, conversions and
 // partial results (14 us to merge, 10 to write) share the time (0.67 PFLOP/s); one of 8 nodes after 1500 15, latency.
 #include "../../include/lightserve_fa.h"
 #include "fa_paged.hpp"
