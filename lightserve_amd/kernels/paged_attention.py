@@ -127,8 +127,8 @@ def windowed_attention(q, k_cache, v_cache, block_tables, cu_seqlens_q, seq_lens
             qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], Hq * D, D, ls[0], ls[1], bt.stride(0),
             _lib.TORCH_TO_LSFA[dtype], B, T, Hq, Hkv, D, block_size, num_blocks, max_blocks, int(max_seqlen_q), keys,
             bool(causal),
-            # a window or sinks past the longest sequence say no more than its length
-            0 if window is None else min(int(window), keys + 1), min(int(sinks), keys), scale, 0)
+            # a window or sinks past the longest sequence say no more than its length (a tree's length may pass the table's keys)
+            0 if window is None else min(int(window), keys + 1 if tree_mask is None else 1 << 30), min(int(sinks), keys), scale, 0)
         if tree_mask is None:
             args = _lib.pack(_lib.WindowArgs, *fields)
             size, launch = _lib.window_workspace_size, _lib.window

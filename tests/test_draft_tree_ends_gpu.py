@@ -30,7 +30,7 @@ def _past(kind, dtype, nodes, had, blocks, hq, hkv, d, bs, seed, window=None, si
 
 @pytest.mark.parametrize("kind,dtype", KINDS)
 @pytest.mark.parametrize("hq,hkv", [(2, 2), (8, 2)])
-@pytest.mark.parametrize("window,sinks", [(None, 0), (20, 3), (6, 0), (300, 70)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (20, 3), (6, 0), (300, 70), (90, 0), (300, 2)])
 def test_tree_past_the_table(gpu, kind, dtype, hq, hkv, window, sinks):
     """Every number of rows past the table, tables that end inside a key tile, and lengths far behind them."""
     print(f"case past {kind} {dtype} {hq} {hkv} window={window} sinks={sinks}", flush=True)
