@@ -4,6 +4,8 @@ As in test_candidate_decoding_gpu.py logits are held to float64 forwards of each
 holds them, by twice the reference's bf16 forward's mean distance from float64 on the same tokens; paths, tokens and rows are
 exact given the logits.
 """
+from dataclasses import replace
+
 import pytest
 import torch
 
@@ -90,15 +92,17 @@ def test_draft_steps_at_the_end(gpu, kv_e4m3, window, sinks, room):
 
 @pytest.mark.parametrize("kv_e4m3", [False, True])
 @pytest.mark.parametrize("drafts,branches", [(3, 3), (8, 1), (20, 12)])
-def test_lookup_drafts_to_the_end(gpu, kv_e4m3, drafts, branches):
+@pytest.mark.parametrize("end,block_size", [(64, 16), (59, 32)])
+def test_lookup_drafts_to_the_end(gpu, kv_e4m3, drafts, branches, end, block_size):
     """Every token up to the cache's end is the choice of the logits before it, eagerly and in replays, for sequences that get there
     one after another; steps past the end write nothing outside the cache."""
-    print(f"case lookup to the end e4m3={kv_e4m3} drafts={drafts} branches={branches}", flush=True)
+    print(f"case lookup to the end e4m3={kv_e4m3} drafts={drafts} branches={branches} end={end}", flush=True)
     config, weights = _model()
-    eager, graphed = (LookupDrafts(KVCacheDecoder(weights, config, 3, kv_e4m3=kv_e4m3), drafts, branches) for _ in range(2))
+    config = replace(config, max_seq_len=end)
+    eager, graphed = (LookupDrafts(KVCacheDecoder(weights, config, 3, block_size, kv_e4m3=kv_e4m3), drafts, branches) for _ in range(2))
     fences, had = _fenced(eager.dec)
     graph, _ = capture(graphed.step)
-    end, P = config.max_seq_len, 49
+    P = 49
     prompt = torch.randint(0, config.vocab_size, (3, 7), generator=torch.Generator().manual_seed(5)).repeat(1, 7).cuda()
     for loop in (eager, graphed):
         loop.start(prompt, 16)
